@@ -285,7 +285,7 @@ def _run_attend(s):
     if own:
         import izwi_amd
         return izwi_amd.shared_prefix_attention(s["q"], s["cache"], s["lens"], prefix=s["prefix"], prefix_lens=s["prefix_lens"],
-                                                lineage=s["lineage"], scale=s["scale"])
+                                                lineage=s["lineage"], beams=s["case"]["width"], scale=s["scale"])
     case = s["case"]
     prompts, width, kv, d = case["prompts"], case["width"], case["kv"], case["d"]
     group = case["heads"] // kv
