@@ -1,6 +1,7 @@
 /*
  * izwi_decode_ops — the decode-step neighbours of the quantized projections: RMSNorm, the
- * q/k head norm, rotary embedding and single-token grouped-query attention, f32 and f16.
+ * q/k head norm, rotary embedding and single-token grouped-query attention, f32 and f16; for several
+ * continuations of one prompt a quantized key / value cache, the attention over it and beam search's selection.
  *
  * Each entry point is the device side of one of the reference's fused-kernel hooks
  * (crates/izwi-core/src/kernels/mod.rs:109-225), which today dispatch to Metal only
@@ -123,6 +124,89 @@ int izwi_decode_gqa_attention_f32(const float* q, const float* k, const float* v
  * index of the row's maximum (ties go to the smaller index, as a left-to-right scan keeps the
  * first; a NaN is never the maximum; a row of NaNs gives 0). */
 int izwi_argmax_f32(const float* logits, int64_t rows, int64_t n, uint32_t* out, int mem_space, void* stream);
+
+/* ---- several continuations of one prompt -----------------------------------------------------------------------
+ *
+ * Sequences that decode together from a quantized cache: `prompts` prompts of `beams` sequences each (sequence b
+ * belongs to prompt b / beams; one beam per prompt is ordinary batched decoding, one prompt a batch behind a common
+ * system prompt).  What the sequences of a prompt share stands once, in a cache with a slot per prompt; what each of
+ * them adds stands in a cache with a slot per sequence.  Lengths are device arrays, so that a captured step can be
+ * replayed while they grow.  Device pointers only throughout. */
+
+/* Cache formats, by their ggml ids: blocks of 32 values along a head's row, an f16 scale and 8 or 4 bits a value.
+ * Blocks of equal bits to the GGUF formats' (izwi_qmm_quantize_weights_f32 makes the same Q8_0 ones); a block that
+ * holds an infinity or NaN, or whose scale has no f16, reads as NaN, one whose scale is zero as zeros. */
+enum { IZWI_KV_Q4_0 = 2, IZWI_KV_Q8_0 = 8 };
+
+/* Bytes of a cache of `slots` slots, each of kv_capacity positions (rounded up to 32) of num_kv_heads key and value
+ * rows; head_dim 64, 128 or 256.  0 for a shape that cannot be (the message says why).  The layout is the library's
+ * own; the buffer needs no clearing. */
+uint64_t izwi_decode_kv_cache_bytes(int type, int64_t slots, int64_t num_kv_heads, int64_t kv_capacity, int64_t head_dim);
+
+/* Quantizes the rows of `batch` sequences of up to `tokens` tokens into slots first_slot, first_slot + 1, ..: row
+ * (b, t) of k and v holds num_kv_heads heads of head_dim values, k_stride (v_stride) elements behind row (b, t) - 1,
+ * and goes to position starts[b] + t, for t < counts[b] (counts NULL: all).  Rows outside the capacity are left out;
+ * positions that no row goes to stay as they were. */
+int izwi_decode_kv_append_f32(int type, const float* k, const float* v, int64_t k_stride, int64_t v_stride,
+                              const int32_t* starts, const int32_t* counts, int64_t batch, int64_t tokens,
+                              int64_t first_slot, int64_t slots, int64_t num_kv_heads, int64_t kv_capacity,
+                              int64_t head_dim, void* cache, void* stream);
+int izwi_decode_kv_append_f16(int type, const uint16_t* k, const uint16_t* v, int64_t k_stride, int64_t v_stride,
+                              const int32_t* starts, const int32_t* counts, int64_t batch, int64_t tokens,
+                              int64_t first_slot, int64_t slots, int64_t num_kv_heads, int64_t kv_capacity,
+                              int64_t head_dim, void* cache, void* stream);
+
+/* The values that positions starts[b] .. starts[b] + tokens - 1 of those slots stand for, into contiguous k and v
+ * `[batch, tokens, num_kv_heads, head_dim]`; zeros from counts[b] tokens on and outside the capacity.  With `lineage`
+ * (below) position p of slot s is read from the slot of beam lineage[s][p] of the same prompt (`beams` slots a prompt, at
+ * most 255; zeros where there is no such beam): a beam's history in one piece. */
+int izwi_decode_kv_read_f32(int type, const void* cache, int64_t slots, int64_t num_kv_heads, int64_t kv_capacity,
+                            int64_t head_dim, const uint8_t* lineage, int64_t beams, const int32_t* starts,
+                            const int32_t* counts, int64_t batch, int64_t tokens, int64_t first_slot, float* k, float* v,
+                            void* stream);
+int izwi_decode_kv_read_f16(int type, const void* cache, int64_t slots, int64_t num_kv_heads, int64_t kv_capacity,
+                            int64_t head_dim, const uint8_t* lineage, int64_t beams, const int32_t* starts,
+                            const int32_t* counts, int64_t batch, int64_t tokens, int64_t first_slot, uint16_t* k,
+                            uint16_t* v, void* stream);
+
+/* Attention of one new token per sequence: softmax((q . k) * scale) . v over positions 0 .. prefix_lens[b / beams] - 1
+ * of the prompt's slot of `prefix` and positions 0 .. lens[b] - 1 of slot b of `cache`, both of format `type`; either may be
+ * NULL.  q is `[batch, num_heads, head_dim]`, q_stride elements from one sequence to the next; head h reads kv head
+ * h / (num_heads / num_kv_heads); out is contiguous `[batch, num_heads, head_dim]` and may share no memory with the rest.  A
+ * sequence without any position gives zeros.  Lengths above max_prefix_len (max_len), the caller's bounds, count as
+ * those, negative ones as zero; the work is shared out by the bounds.  With `lineage`, `[slots][kv_capacity rounded up to
+ * 32]`, position p of sequence b is in the slot of beam lineage[b][p] of its prompt; a position whose entry is no beam
+ * (>= beams) does not count. */
+int izwi_decode_shared_attention_f32(int type, const float* q, int64_t q_stride, int64_t batch, int64_t beams,
+                                     int64_t num_heads, int64_t num_kv_heads, int64_t head_dim, const void* prefix,
+                                     int64_t prefix_slots, int64_t prefix_capacity, const int32_t* prefix_lens,
+                                     int64_t max_prefix_len, const void* cache, int64_t slots, int64_t kv_capacity,
+                                     const int32_t* lens, int64_t max_len, const uint8_t* lineage, float scale,
+                                     float* out, void* stream);
+int izwi_decode_shared_attention_f16(int type, const uint16_t* q, int64_t q_stride, int64_t batch, int64_t beams,
+                                     int64_t num_heads, int64_t num_kv_heads, int64_t head_dim, const void* prefix,
+                                     int64_t prefix_slots, int64_t prefix_capacity, const int32_t* prefix_lens,
+                                     int64_t max_prefix_len, const void* cache, int64_t slots, int64_t kv_capacity,
+                                     const int32_t* lens, int64_t max_len, const uint8_t* lineage, float scale,
+                                     uint16_t* out, void* stream);
+
+/* One step of beam search.  logits is `[prompts, beams, vocab]`, scores the beams' sums of log-probabilities so far
+ * `[prompts, beams]`; candidate (w, t) of a prompt is worth scores[w] + logits[w][t] - ln sum_i e^logits[w][i], and the best
+ * `beams` of beams * vocab candidates become the new beams, best first, equal ones by rising w * vocab + t.  Sums and order are
+ * in 64 bits; scores_out is rounded once.  A beam that `finished` marks (NULL: none; any nonzero byte) has the one
+ * candidate (eos_token, scores[w]); a new beam is finished if its parent was or its token is eos_token (-1: no such
+ * token; then finished must be NULL).  A NaN among logits or scores counts as -infinity, +infinity as the largest finite float; a first step
+ * starts from scores 0, -infinity, -infinity, ..  beams <= 64, beams * vocab below 2^31.
+ *
+ * tokens, parents, scores_out, finished_out: `[prompts, beams]` (finished_out may be NULL).  lineage_out (NULL: none), `[prompts *
+ * beams][lineage_capacity rounded up to 32]`: row i is the parent's row of `lineage` with i at position lens[parent], where
+ * the new beam's next key and value go (slot i); lens `[prompts * beams]`, a position outside the row is left out.  Outputs may be the
+ * corresponding inputs (lineage_out lineage, scores_out scores, finished_out finished) but overlap them no other way.  Uses the
+ * library's per-stream scratch. */
+int izwi_decode_beam_select_f32(const float* logits, int64_t prompts, int64_t beams, int64_t vocab, const float* scores,
+                                const uint8_t* finished, int64_t eos_token, int32_t* tokens, int32_t* parents,
+                                float* scores_out, uint8_t* finished_out, const uint8_t* lineage,
+                                int64_t lineage_capacity, const int32_t* lens, uint8_t* lineage_out, void* stream);
 
 #ifdef __cplusplus
 }

@@ -18,6 +18,7 @@ from .decode_ops import (  # noqa: F401
     try_fused_rope_pair_bshd,
 )
 from .gguf import GgufLoader, GgufMmapMode, GgufModelInfo, GgufReaderKind, is_gguf_file, resolve_gguf_mmap_mode  # noqa: F401
+from .kv_decode import BeamStep, KvCacheType, QuantizedKvCache, beam_select, shared_prefix_attention  # noqa: F401
 from .qmatmul import (  # noqa: F401
     ActivationRecords,
     DecodeChain,

@@ -106,6 +106,16 @@ PROTOTYPES = {
                                                  _i64, C.c_float, _vp, _vp]),
     "izwi_decode_gqa_attention_f32": (C.c_int, [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, C.c_float, _vp,
                                                 C.c_int, _vp]),
+    "izwi_decode_kv_cache_bytes": (_u64, [C.c_int, _i64, _i64, _i64, _i64]),
+    "izwi_decode_kv_append_f32": (C.c_int, [C.c_int, _vp, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp]),
+    "izwi_decode_kv_append_f16": (C.c_int, [C.c_int, _vp, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp]),
+    "izwi_decode_kv_read_f32": (C.c_int, [C.c_int, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp]),
+    "izwi_decode_kv_read_f16": (C.c_int, [C.c_int, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp]),
+    "izwi_decode_shared_attention_f32": (C.c_int, [C.c_int, _vp] + [_i64] * 6 + [_vp, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp,
+                                                   C.c_float, _vp, _vp]),
+    "izwi_decode_shared_attention_f16": (C.c_int, [C.c_int, _vp] + [_i64] * 6 + [_vp, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp,
+                                                   C.c_float, _vp, _vp]),
+    "izwi_decode_beam_select_f32": (C.c_int, [_vp, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp]),
     "izwi_moe_route": (C.c_int, [_vp, _i64, _i32, _i32, _vp, _vp, C.c_int, _vp]),
     "izwi_moe_sort": (C.c_int, [_vp, _i64, _i32, _i32, _vp, _vp, C.c_int, _vp]),
     "izwi_moe_layer_f32": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i32, _vp, _vp, _vp, C.c_int, _vp]),

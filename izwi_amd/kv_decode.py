@@ -1,0 +1,226 @@
+"""Several continuations of one prompt: the quantized key / value cache, the attention that reads it and the step of
+beam search, over the C ABI of include/izwi_decode_ops.h.
+
+``prompts`` prompts of ``beams`` sequences each decode together, sequence b belongs to prompt b // beams.  What the sequences of a
+prompt share stands once, in a cache with a slot per prompt; what each adds stands in a cache with a slot per sequence, and
+a beam's *lineage* says for each of its positions which beam of the prompt wrote it, so that a beam that takes over another's
+history copies a row of bytes instead of keys and values.  The reference keeps such caches as pages of 8- or 4-bit values
+(models/shared/attention/paged.rs:160-342) and gathers them for its eager attention; here the attention reads them in place.
+
+    prompt = QuantizedKvCache(KvCacheType.Q8_0, prompts, kv_heads, prompt_capacity, head_dim)
+    answers = QuantizedKvCache(KvCacheType.Q8_0, prompts * beams, kv_heads, answer_capacity, head_dim)
+    prompt.append(k, v, starts)                                   # once, k / v [prompts, tokens, kv_heads, head_dim]
+    lineage, lens = answers.new_lineage(), zeros of int32
+    # a step: per layer append and attend, then pick (the lineage is every layer's)
+    answers.append(k, v, lens)                                    # k / v [prompts * beams, 1, kv_heads, head_dim]
+    out = shared_prefix_attention(q, answers, lens + 1, prefix=prompt, prefix_lens=prompt_lens, lineage=lineage)
+    picked = beam_select(logits, scores, lineage=lineage, lens=lens + 1)
+
+Everything runs on the current stream; nothing waits for the device.  Arguments that do not fit raise ``QmmError``."""
+from __future__ import annotations
+
+import enum
+from typing import NamedTuple
+
+import torch
+
+from .capi import QmmError, check, lib
+from .qmatmul import _current_device, _raw_stream
+
+_PAD = 32  # positions of a cache, and bytes of a lineage row, come in multiples of this
+
+
+class KvCacheType(enum.IntEnum):
+    """Formats of a cache, by their ggml ids: blocks of 32 values with an f16 scale, 8 or 4 bits a value."""
+    Q4_0 = 2
+    Q8_0 = 8
+
+
+def _refuse(what: str):
+    raise QmmError(-1, what)
+
+
+def _ints(t, n: int, device, what: str) -> int:
+    if t is None:
+        return 0
+    if t.dtype is not torch.int32 or t.shape != (n,) or not t.is_contiguous() or t.device != device:
+        _refuse(f"{what}: a contiguous int32 tensor of {n} on {device} expected")
+    return t.data_ptr()
+
+
+def _rows(t, shape, device, what: str) -> int:
+    """Elements from one row of heads to the next, rows being all leading dimensions taken together."""
+    if t.shape != shape or t.device != device:
+        _refuse(f"{what}: a tensor {tuple(shape)} on {device} expected")
+    heads, d = shape[-2:]
+    if t.is_contiguous():
+        return heads * d
+    stride = t.stride()
+    if stride[-1] != 1 or (heads > 1 and stride[-2] != d):
+        _refuse(f"{what}: heads of a row must be contiguous")
+    step = None
+    for size, at in zip(reversed(shape[:-2]), reversed(stride[:-2])):
+        if size == 1:
+            continue
+        if step is None:
+            step, count = at, size
+        elif at != step * count:
+            _refuse(f"{what}: rows must be equally far apart")
+        else:
+            count *= size
+    if step is None:  # one row
+        return heads * d
+    if step < heads * d:
+        _refuse(f"{what}: rows overlap")
+    return step
+
+
+def _launch(fn, device, *args):
+    """The call on the current stream of the tensors' device."""
+    if device.index == _current_device():
+        check(fn(*args, _raw_stream(device.index)))
+    else:
+        with torch.cuda.device(device):
+            check(fn(*args, _raw_stream(device.index)))
+
+
+class QuantizedKvCache:
+    """Keys and values of ``slots`` sequences, up to ``capacity`` positions of ``kv_heads`` heads each, quantized as they
+    are written.  head_dim 64, 128 or 256."""
+
+    def __init__(self, dtype: KvCacheType, slots: int, kv_heads: int, capacity: int, head_dim: int, device="cuda"):
+        self.dtype, self.slots, self.kv_heads, self.capacity, self.head_dim = KvCacheType(dtype), slots, kv_heads, capacity, head_dim
+        if torch.device(device).type != "cuda":
+            _refuse(f"QuantizedKvCache: a GPU expected, not {device}")
+        nbytes = lib().izwi_decode_kv_cache_bytes(int(dtype), slots, kv_heads, capacity, head_dim)
+        if nbytes == 0:
+            raise QmmError(-1, lib().izwi_qmm_last_error().decode("utf-8", "replace"))
+        self.buffer = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        self.device = self.buffer.device
+        self._ptr = self.buffer.data_ptr()
+
+    def new_lineage(self) -> torch.Tensor:
+        """Lineage rows of all slots, [slots, capacity rounded up to 32] uint8, zeros: no position has been written."""
+        return torch.zeros(self.slots, -(-self.capacity // _PAD) * _PAD, dtype=torch.uint8, device=self.device)
+
+    def append(self, k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor, counts: torch.Tensor | None = None, first_slot: int = 0) -> None:
+        """k, v [sequences, tokens, kv_heads, head_dim] (f32 or f16; rows may be parts of wider ones): token t of
+        sequence b goes to position starts[b] + t of slot first_slot + b, for t < counts[b].  What lies outside the
+        capacity is left out."""
+        if k.dim() != 4 or k.dtype not in (torch.float32, torch.float16) or v.dtype is not k.dtype:
+            _refuse("append: k and v [sequences, tokens, kv_heads, head_dim] of f32 or f16 expected")
+        batch, tokens = k.shape[:2]
+        shape = (batch, tokens, self.kv_heads, self.head_dim)
+        k_stride, v_stride = _rows(k, shape, self.device, "append: k"), _rows(v, shape, self.device, "append: v")
+        fn = lib().izwi_decode_kv_append_f32 if k.dtype is torch.float32 else lib().izwi_decode_kv_append_f16
+        _launch(fn, self.device, int(self.dtype), k.data_ptr(), v.data_ptr(), k_stride, v_stride, _ints(starts, batch, self.device, "append: starts"),
+                _ints(counts, batch, self.device, "append: counts"), batch, tokens, first_slot, self.slots, self.kv_heads, self.capacity, self.head_dim,
+                self._ptr)
+
+    def read(self, starts: torch.Tensor, tokens: int, counts: torch.Tensor | None = None, first_slot: int = 0, lineage: torch.Tensor | None = None,
+             beams: int = 1, dtype: torch.dtype = torch.float32):
+        """(k, v) [sequences, tokens, kv_heads, head_dim]: the values that positions starts[b] .. starts[b] + tokens - 1 of slots
+        first_slot, .. stand for; zeros from counts[b] on and outside the capacity.  With ``lineage`` a position comes from
+        the slot of the beam that wrote it (``beams`` slots a prompt)."""
+        if dtype not in (torch.float32, torch.float16):
+            _refuse("read: f32 or f16 expected")
+        batch = starts.shape[0]
+        k = torch.empty(batch, tokens, self.kv_heads, self.head_dim, dtype=dtype, device=self.device)
+        v = torch.empty_like(k)
+        fn = lib().izwi_decode_kv_read_f32 if dtype is torch.float32 else lib().izwi_decode_kv_read_f16
+        _launch(fn, self.device, int(self.dtype), self._ptr, self.slots, self.kv_heads, self.capacity, self.head_dim, self._lineage(lineage, "read"),
+                beams, _ints(starts, batch, self.device, "read: starts"), _ints(counts, batch, self.device, "read: counts"), batch, tokens, first_slot,
+                k.data_ptr(), v.data_ptr())
+        return k, v
+
+    def _lineage(self, lineage, what: str) -> int:
+        if lineage is None:
+            return 0
+        if (lineage.dtype is not torch.uint8 or lineage.shape != (self.slots, -(-self.capacity // _PAD) * _PAD) or not lineage.is_contiguous()
+                or lineage.device != self.device):
+            _refuse(f"{what}: lineage as new_lineage() makes it expected")
+        return lineage.data_ptr()
+
+
+def shared_prefix_attention(q: torch.Tensor, cache: QuantizedKvCache | None, lens: torch.Tensor | None, prefix: QuantizedKvCache | None = None,
+                            prefix_lens: torch.Tensor | None = None, lineage: torch.Tensor | None = None, beams: int | None = None,
+                            scale: float | None = None, max_len: int | None = None, max_prefix_len: int | None = None) -> torch.Tensor:
+    """Attention of one new token per sequence: q [sequences, heads, head_dim] (f32 or f16) over positions 0 ..
+    prefix_lens[b // beams] - 1 of its prompt's slot of ``prefix`` and 0 .. lens[b] - 1 of its own slot of ``cache`` (found by ``lineage``
+    if given).  Either cache may be None.  A sequence without any position gives zeros.  ``beams``: sequences per prompt,
+    by default sequences // len(prefix_lens), or all of them without a prefix.  ``max_len`` and ``max_prefix_len`` bound the lengths where
+    the caller knows them better than the capacities: the work is shared out by them.  Returns [sequences, heads, head_dim]."""
+    if q.dim() != 3 or q.dtype not in (torch.float32, torch.float16):
+        _refuse("shared_prefix_attention: q [sequences, heads, head_dim] of f32 or f16 expected")
+    one = cache if cache is not None else prefix
+    if one is None:
+        _refuse("shared_prefix_attention: neither a cache nor a prefix")
+    if prefix is not None and cache is not None and (prefix.dtype, prefix.kv_heads, prefix.head_dim, prefix.device) != (
+            cache.dtype, cache.kv_heads, cache.head_dim, cache.device):
+        _refuse("shared_prefix_attention: the two caches differ in format, heads or device")
+    batch, heads, d = q.shape
+    if (prefix is None) != (prefix_lens is None) or (cache is None) != (lens is None) or (lineage is not None and cache is None):
+        _refuse("shared_prefix_attention: a cache and its lengths come together, lineage with a cache")
+    if beams is None:
+        beams = batch if prefix is None else batch // max(1, prefix_lens.shape[0])
+    beams = max(beams, 1)
+    if batch % beams or d != one.head_dim:
+        _refuse(f"shared_prefix_attention: {batch} sequences of head_dim {d}, {beams} a prompt, on a cache of head_dim {one.head_dim}")
+    q_stride = _rows(q, (batch, heads, d), one.device, "shared_prefix_attention: q")
+    out = torch.empty(batch, heads, d, dtype=q.dtype, device=q.device)
+    fn = lib().izwi_decode_shared_attention_f32 if q.dtype is torch.float32 else lib().izwi_decode_shared_attention_f16
+    p_args = (0, 0, 0, 0, 0) if prefix is None else (
+        prefix._ptr, prefix.slots, prefix.capacity, _ints(prefix_lens, batch // beams, one.device, "shared_prefix_attention: prefix_lens"),
+        prefix.capacity if max_prefix_len is None else max_prefix_len)
+    c_args = (0, 0, 0, 0, 0, 0) if cache is None else (
+        cache._ptr, cache.slots, cache.capacity, _ints(lens, batch, one.device, "shared_prefix_attention: lens"),
+        cache.capacity if max_len is None else max_len, cache._lineage(lineage, "shared_prefix_attention"))
+    _launch(fn, one.device, int(one.dtype), q.data_ptr(), q_stride, batch, beams, heads, one.kv_heads, d, *p_args, *c_args,
+            d ** -0.5 if scale is None else scale, out.data_ptr())
+    return out
+
+
+class BeamStep(NamedTuple):
+    """What a step of beam search leaves, [prompts, beams] each, best first; lineage for the next step (None without)."""
+    tokens: torch.Tensor    # int32
+    parents: torch.Tensor   # int32: the beam that each new one continues
+    scores: torch.Tensor    # f32: sums of log-probabilities
+    finished: torch.Tensor  # uint8
+    lineage: torch.Tensor | None
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: torch.Tensor | None = None, eos_token: int | None = None,
+                lineage: torch.Tensor | None = None, lens: torch.Tensor | None = None, out_lineage: torch.Tensor | None = None) -> BeamStep:
+    """One step of beam search on the device: logits [prompts, beams, vocab] f32, scores [prompts, beams] f32 (a first step starts
+    from 0, -inf, -inf, ..).  The best ``beams`` of beams * vocab candidates scores[w] + log_softmax(logits[w])[t], equal ones by
+    rising w * vocab + t; a beam marked in ``finished`` (uint8) keeps its score and its one candidate ``eos_token``.  ``lineage``
+    [prompts * beams, n] uint8 and ``lens`` int32 [prompts * beams]: the new beams' lineage is their parents', with their own index
+    at position lens[parent], where their next key and value go; into ``out_lineage`` (it may be ``lineage``) or a new tensor."""
+    if logits.dim() != 3 or logits.dtype is not torch.float32 or not logits.is_contiguous() or not logits.is_cuda:
+        _refuse("beam_select: contiguous f32 logits [prompts, beams, vocab] on a GPU expected")
+    prompts, beams, vocab = logits.shape
+    device = logits.device
+    for t, dtype, what in ((scores, torch.float32, "scores"), (finished, torch.uint8, "finished")):
+        if t is not None and (t.dtype is not dtype or t.shape != (prompts, beams) or not t.is_contiguous() or t.device != device):
+            _refuse(f"beam_select: {what} [{prompts}, {beams}] of {dtype} expected")
+    if finished is not None and eos_token is None:
+        _refuse("beam_select: finished beams need an eos_token")
+    if (lineage is None) != (lens is None) or (lineage is None and out_lineage is not None):
+        _refuse("beam_select: lineage and lens come together")
+    capacity = 0
+    if lineage is not None:
+        if out_lineage is None:
+            out_lineage = torch.empty_like(lineage)
+        capacity = lineage.shape[-1]
+        for t in (lineage, out_lineage):
+            if (t.dtype is not torch.uint8 or t.shape != (prompts * beams, capacity) or capacity % _PAD or not t.is_contiguous()
+                    or t.device != device):
+                _refuse("beam_select: lineage rows as QuantizedKvCache.new_lineage() makes them expected")
+    ints = torch.empty(2, prompts, beams, dtype=torch.int32, device=device)
+    scores_out, finished_out = torch.empty_like(scores), torch.empty(prompts, beams, dtype=torch.uint8, device=device)
+    tokens, parents = ints[0], ints[1]
+    _launch(lib().izwi_decode_beam_select_f32, device, logits.data_ptr(), prompts, beams, vocab, scores.data_ptr(),
+            0 if finished is None else finished.data_ptr(), -1 if eos_token is None else eos_token, tokens.data_ptr(), parents.data_ptr(),
+            scores_out.data_ptr(), finished_out.data_ptr(), 0 if lineage is None else lineage.data_ptr(), capacity,
+            _ints(lens, prompts * beams, device, "beam_select: lens"), 0 if lineage is None else out_lineage.data_ptr())
+    return BeamStep(tokens, parents, scores_out, finished_out, out_lineage)

@@ -28,6 +28,10 @@ pub const IZWI_QMM_Q8_0: c_int = 8;
 pub const IZWI_QMM_Q4_K: c_int = 12;
 pub const IZWI_QMM_Q6_K: c_int = 14;
 
+/// formats of the quantized key / value cache, by their ggml ids
+pub const IZWI_KV_Q4_0: c_int = 2;
+pub const IZWI_KV_Q8_0: c_int = 8;
+
 /// `izwi_qmm_large_m`
 pub const IZWI_QMM_LARGE_M_BF16: c_int = 0;
 pub const IZWI_QMM_LARGE_M_INT8: c_int = 1;
@@ -259,6 +263,31 @@ extern "C" {
     pub fn izwi_decode_gqa_attention_f32(q: *const f32, k: *const f32, v: *const f32, num_heads: i64,
         num_kv_heads: i64, head_dim: i64, kv_len: i64, kv_capacity: i64, scale: f32, out: *mut f32,
         mem_space: c_int, stream: *mut c_void) -> c_int;
+    pub fn izwi_decode_kv_cache_bytes(type_: c_int, slots: i64, num_kv_heads: i64, kv_capacity: i64, head_dim: i64) -> u64;
+    pub fn izwi_decode_kv_append_f32(type_: c_int, k: *const f32, v: *const f32, k_stride: i64, v_stride: i64,
+        starts: *const i32, counts: *const i32, batch: i64, tokens: i64, first_slot: i64, slots: i64, num_kv_heads: i64,
+        kv_capacity: i64, head_dim: i64, cache: *mut c_void, stream: *mut c_void) -> c_int;
+    pub fn izwi_decode_kv_append_f16(type_: c_int, k: *const u16, v: *const u16, k_stride: i64, v_stride: i64,
+        starts: *const i32, counts: *const i32, batch: i64, tokens: i64, first_slot: i64, slots: i64, num_kv_heads: i64,
+        kv_capacity: i64, head_dim: i64, cache: *mut c_void, stream: *mut c_void) -> c_int;
+    pub fn izwi_decode_kv_read_f32(type_: c_int, cache: *const c_void, slots: i64, num_kv_heads: i64, kv_capacity: i64,
+        head_dim: i64, lineage: *const u8, beams: i64, starts: *const i32, counts: *const i32, batch: i64, tokens: i64,
+        first_slot: i64, k: *mut f32, v: *mut f32, stream: *mut c_void) -> c_int;
+    pub fn izwi_decode_kv_read_f16(type_: c_int, cache: *const c_void, slots: i64, num_kv_heads: i64, kv_capacity: i64,
+        head_dim: i64, lineage: *const u8, beams: i64, starts: *const i32, counts: *const i32, batch: i64, tokens: i64,
+        first_slot: i64, k: *mut u16, v: *mut u16, stream: *mut c_void) -> c_int;
+    pub fn izwi_decode_shared_attention_f32(type_: c_int, q: *const f32, q_stride: i64, batch: i64, beams: i64,
+        num_heads: i64, num_kv_heads: i64, head_dim: i64, prefix: *const c_void, prefix_slots: i64, prefix_capacity: i64,
+        prefix_lens: *const i32, max_prefix_len: i64, cache: *const c_void, slots: i64, kv_capacity: i64,
+        lens: *const i32, max_len: i64, lineage: *const u8, scale: f32, out: *mut f32, stream: *mut c_void) -> c_int;
+    pub fn izwi_decode_shared_attention_f16(type_: c_int, q: *const u16, q_stride: i64, batch: i64, beams: i64,
+        num_heads: i64, num_kv_heads: i64, head_dim: i64, prefix: *const c_void, prefix_slots: i64, prefix_capacity: i64,
+        prefix_lens: *const i32, max_prefix_len: i64, cache: *const c_void, slots: i64, kv_capacity: i64,
+        lens: *const i32, max_len: i64, lineage: *const u8, scale: f32, out: *mut u16, stream: *mut c_void) -> c_int;
+    pub fn izwi_decode_beam_select_f32(logits: *const f32, prompts: i64, beams: i64, vocab: i64, scores: *const f32,
+        finished: *const u8, eos_token: i64, tokens: *mut i32, parents: *mut i32, scores_out: *mut f32,
+        finished_out: *mut u8, lineage: *const u8, lineage_capacity: i64, lens: *const i32, lineage_out: *mut u8,
+        stream: *mut c_void) -> c_int;
     pub fn izwi_argmax_f32(logits: *const f32, rows: i64, n: i64, out: *mut u32, mem_space: c_int,
         stream: *mut c_void) -> c_int;
 }
