@@ -1,11 +1,38 @@
 // Attention of one new token per sequence over the quantized cache (layout: kv_cache.h): positions that the sequences of a
 // prompt share, then each sequence's own.
+//
+// One pass over the positions with a running maximum and sum per query row.  A workgroup has a tile of query rows (heads of one kv
+// head, of all sequences of a prompt where the positions are shared) and a split of the positions; its waves take 32 positions
+// in turn and meet in LDS, the splits in a second small kernel.  Both products run on the matrix cores, 16 x 16 x 32 in f16 with f32
+// sums, and both with the query row as the column: what a lane holds of the scores (row x, positions 4 g .. 4 g + 3 of 16) is
+// what it feeds to the second product, and a row's statistics stay in its lanes.
+//  * Quants are exact in f16 (one byte permute and one subtraction for two of them).  A block of 32 is the depth of one matrix
+//    instruction, so the keys' scales multiply finished sums in f32.  The values' scales run along the positions, over which the
+//    second product sums: they multiply the weights, once for each block of 32 elements of the head.
+//  * f32 queries and weights go as two f16 numbers each, 22 bits: with the quants exact, two matrix products instead of one.
+//    Queries are scaled by a power of two per row; weights stand under a reference that keeps the largest between 2^5 and 2^15
+//    (it moves when a score rises 2^10 above it: rarely, so most tiles pay for no rescaling), the values' scales under the power
+//    of two that takes the largest so far to below 1.  Weight times scale is a product of f16 pairs whose loss a fused multiply-add
+//    returns exactly: packed, half the instructions of f32 products split afterwards.
+//    f16 queries are themselves, f16 results take their weights rounded to f16 (2^-11).
+//
+// Bound by the vector instructions around the matrix products where many rows share positions (per tile and row tile of an f32
+// call about 240 beside 32 matrix instructions), by memory where few do.
 #include "kv_cache.h"
+
+#include <algorithm>
+#include <type_traits>
+#include <utility>
+
 #include "qmm_lanes.h"
 
 namespace {
 
 typedef _Float16 f16_t;
+
+typedef f16_t h2 __attribute__((ext_vector_type(2)));
+typedef f16_t h8 __attribute__((ext_vector_type(8)));
+typedef float f4 __attribute__((ext_vector_type(4)));
 
 struct AttendParams {
     const void* q;
@@ -18,104 +45,577 @@ struct AttendParams {
     int batch, beams, heads, kv_heads, group;
     int max_prefix, max_len; // 0: no such positions
     float scale;
+    // workgroups: prefix_wgs of prefix_units (prompt, kv head, split) times prefix_z tiles of rows, then the same of (sequence, ..)
+    int prefix_splits, prefix_units, prefix_z, prefix_wgs, own_splits, own_units, own_z;
+    int parts;     // partial results of a row: prefix_splits + own_splits
+    float* sums;   // [batch * heads][parts][D]
+    float2* stats; // [batch * heads][parts]: reference (a power of two's exponent), sum of weights
 };
 
 __device__ __forceinline__ int clamped_len(const int32_t* lens, int i, int most) { return most ? max(0, min(lens[i], most)) : 0; }
 
-// One workgroup per sequence and query head, sixteen lanes a position.
-template <typename T, int QT, int D>
-__global__ __launch_bounds__(256) void attend_kernel(AttendParams P) {
-    using Row = KvRow<QT, D>;
-    constexpr int NB = Row::kBlocks, NU = (NB + 3) / 4;
-    constexpr float kBias = QT == IZWI_KV_Q8_0 ? 128.0f : 8.0f;
-    __shared__ float red[16][D + 2];
-    const int b = blockIdx.x, h = blockIdx.y, kvh = h / P.group, prompt = b / P.beams;
-    const int x = threadIdx.x & 15, slot16 = threadIdx.x >> 4, g = x & 3;
-    const T* q = static_cast<const T*>(P.q) + b * P.q_stride + (int64_t)h * D;
-    float qr[NU][8];
-#pragma unroll
-    for (int u = 0; u < NU; u++)
-#pragma unroll
-        for (int j = 0; j < 8; j++) qr[u][j] = (x >> 2) + 4 * u < NB ? (float)q[32 * ((x >> 2) + 4 * u) + 8 * g + j] : 0.0f;
-    float m = -INFINITY, l = 0.0f, acc[NB][2] = {};
-    const int np = clamped_len(P.prefix_lens, prompt, P.max_prefix), ns = clamped_len(P.lens, b, P.max_len);
-    for (int p = slot16; p < np + ns; p += 16) {
-        const bool shared = p < np;
-        const KvPlanes& C = shared ? P.prefix : P.own;
-        const int at = shared ? p : p - np;
-        int slot = shared ? prompt : b;
-        if (!shared && P.lineage) {
-            const int beam = P.lineage[(int64_t)b * C.padded + at];
-            if (beam >= P.beams) continue;
-            slot = prompt * P.beams + beam;
-        }
-        const int64_t row = ((int64_t)slot * C.kv_heads + kvh) * C.padded + at;
-        float dot = 0.0f;
-#pragma unroll
-        for (int u = 0; u < NU; u++) {
-            const int blk = (x >> 2) + 4 * u;
-            if (blk < NB) {
-                const uint8_t* unit = C.kq + row * Row::kBytes + Row::unit(blk, g);
-                float part = 0.0f;
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const int n = (j >> 1) + 4 * (j & 1);
-                    const float k = QT == IZWI_KV_Q8_0 ? (float)unit[j] : (float)(unit[n >> 1] >> (4 * (n & 1)) & 15);
-                    part += qr[u][j] * (k - kBias);
-                }
-                dot += part * (float)C.ks[row * NB + blk];
-            }
-        }
-        dot = sum8(dot);
-        dot += dpp_f<0x140>(dot);
-        const float s = dot * P.scale, mn = fmaxf(m, s), alpha = merge_weight(m, mn), pe = exp_neg(s - mn);
-        m = mn, l = l * alpha + pe;
-        const uint8_t* vr = C.vq + row * Row::kBytes + x * Row::kLaneBytes;
-#pragma unroll
-        for (int blk = 0; blk < NB; blk++) {
-            const float d = (float)C.vs[row * NB + blk];
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const float v = QT == IZWI_KV_Q8_0 ? (float)vr[2 * blk + i] : (float)(vr[blk] >> (4 * i) & 15);
-                acc[blk][i] = acc[blk][i] * alpha + pe * (d * (v - kBias));
-            }
-        }
+template <int N>
+struct Words {
+    uint32_t w[N];
+    __device__ __forceinline__ void load(const void* p) {
+        __builtin_memcpy(w, __builtin_assume_aligned(p, N % 4 == 0 ? 16 : 4 * N), 4 * N);
     }
-#pragma unroll
-    for (int blk = 0; blk < NB; blk++) red[slot16][32 * blk + 2 * x] = acc[blk][0], red[slot16][32 * blk + 2 * x + 1] = acc[blk][1];
-    if (x == 0) red[slot16][D] = m, red[slot16][D + 1] = l;
-    __syncthreads();
-    if (threadIdx.x < D) {
-        float mn = -INFINITY, a = 0.0f, sum = 0.0f;
-        for (int i = 0; i < 16; i++) mn = fmaxf(mn, red[i][D]);
-        for (int i = 0; i < 16; i++) {
-            const float w = merge_weight(red[i][D], mn);
-            a += red[i][threadIdx.x] * w, sum += red[i][D + 1] * w;
-        }
-        static_cast<T*>(P.out)[((int64_t)b * P.heads + h) * D + threadIdx.x] = (T)(sum != 0.0f ? a / sum : 0.0f);
+};
+
+// Two unsigned quants under the exponent of 1024, less 1024 and the bias: exact
+__device__ __forceinline__ h2 as_h2(uint32_t w) { return __builtin_bit_cast(h2, w); }
+__device__ __forceinline__ h2 bytes_less_128(uint32_t w) { return as_h2(w) + h2{(f16_t)-1152.0f, (f16_t)-1152.0f}; }
+__device__ __forceinline__ h2 low_nibbles(uint32_t w) { // of bits 0-3 and 16-19
+    return as_h2((w & 0x000f000fu) | 0x64006400u) + h2{(f16_t)-1032.0f, (f16_t)-1032.0f};
+}
+__device__ __forceinline__ h2 high_nibbles(uint32_t w) { // of bits 4-7 and 20-23: 1024 + 16 n, so a sixteenth less 64 + 8
+    return __builtin_elementwise_fma(as_h2((w & 0x00f000f0u) | 0x64006400u), h2{(f16_t)0.0625f, (f16_t)0.0625f}, h2{(f16_t)-72.0f, (f16_t)-72.0f});
+}
+typedef unsigned short u2 __attribute__((ext_vector_type(2)));
+template <int QT> // of two scales, as bits; those of Q8_0 have no sign
+__device__ __forceinline__ u2 magnitudes(uint32_t w) { return __builtin_bit_cast(u2, QT == IZWI_KV_Q8_0 ? w : w & 0x7fff7fffu); }
+__device__ __forceinline__ h8 join(h2 a, h2 b, h2 c, h2 d) { return h8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]}; }
+
+// The eight keys' values of a unit
+template <int QT>
+__device__ __forceinline__ h8 key_unit(const uint32_t* w) {
+    if constexpr (QT == IZWI_KV_Q8_0) {
+        const uint32_t e = 0x64646464u;
+        return join(bytes_less_128(__builtin_amdgcn_perm(e, w[0], 0x04010400u)), bytes_less_128(__builtin_amdgcn_perm(e, w[0], 0x04030402u)),
+                    bytes_less_128(__builtin_amdgcn_perm(e, w[1], 0x04010400u)), bytes_less_128(__builtin_amdgcn_perm(e, w[1], 0x04030402u)));
+    } else {
+        const uint32_t u = w[0] >> 8;
+        return join(low_nibbles(w[0]), high_nibbles(w[0]), low_nibbles(u), high_nibbles(u));
     }
 }
 
-template <typename T>
-hipError_t launch_attend(int type, int64_t d, const AttendParams& P, hipStream_t stream) {
-    const dim3 grid(P.batch, P.heads);
-    if (type == IZWI_KV_Q8_0) {
-        if (d == 64) attend_kernel<T, IZWI_KV_Q8_0, 64><<<grid, 256, 0, stream>>>(P);
-        else if (d == 128) attend_kernel<T, IZWI_KV_Q8_0, 128><<<grid, 256, 0, stream>>>(P);
-        else attend_kernel<T, IZWI_KV_Q8_0, 256><<<grid, 256, 0, stream>>>(P);
-    } else {
-        if (d == 64) attend_kernel<T, IZWI_KV_Q4_0, 64><<<grid, 256, 0, stream>>>(P);
-        else if (d == 128) attend_kernel<T, IZWI_KV_Q4_0, 128><<<grid, 256, 0, stream>>>(P);
-        else attend_kernel<T, IZWI_KV_Q4_0, 256><<<grid, 256, 0, stream>>>(P);
+// Of block b the values 2 x (first) and 2 x + 1 at eight positions: v[h] are the lane's quants of four positions, dwords of two
+template <int QT, int N>
+__device__ __forceinline__ void value_pair(const Words<N> (&v)[2], int b, h8& first, h8& second) {
+    h2 lo[4], hi[4];
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        if constexpr (QT == IZWI_KV_Q8_0) {
+            const uint32_t e = 0x64646464u, w = v[r >> 1].w[(r & 1) * (N / 2) + b];
+            lo[r] = bytes_less_128(__builtin_amdgcn_perm(e, w, 0x04020400u));
+            hi[r] = bytes_less_128(__builtin_amdgcn_perm(e, w, 0x04030401u));
+        } else {
+            const uint32_t w = v[r >> 1].w[(r & 1) * (N / 2) + b / 2] >> (8 * (b & 1));
+            lo[r] = low_nibbles(w);
+            hi[r] = high_nibbles(w);
+        }
     }
+    first = join(lo[0], lo[1], lo[2], lo[3]);
+    second = join(hi[0], hi[1], hi[2], hi[3]);
+}
+
+// Lane N of every sixteen, in all of them
+template <int N>
+__device__ __forceinline__ uint32_t of_lane(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x150 + N, 0xf, 0xf, true); // row_newbcast
+}
+
+// f(0), .., f(N - 1), as constants
+template <class F, int... I>
+__device__ __forceinline__ void each_of(F&& f, std::integer_sequence<int, I...>) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, class F>
+__device__ __forceinline__ void each(F&& f) {
+    each_of(f, std::make_integer_sequence<int, N>{});
+}
+
+constexpr float kRise = 10.0f, kHead = 5.0f; // powers of two, see above
+
+template <typename T, int QT, int D, int RT, bool SHARED, bool LIN>
+__device__ __forceinline__ void attend_rows(const AttendParams& P, int id, float* lds) {
+    using Row = KvRow<QT, D>;
+    constexpr int NB = Row::kBlocks, KW = Row::kBytes / 16, VW = Row::kLane, ROWS = 16 * RT;
+    constexpr bool SPLIT = sizeof(T) == 4, QLDS = RT > 1, TWO = RT == 1 && !LIN;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    const int x = lane & 15, g = lane >> 4;
+
+    // what this workgroup works on
+    const int Z = SHARED ? P.prefix_z : P.own_z, splits = SHARED ? P.prefix_splits : P.own_splits;
+    const int unit = id / (8 * Z) * 8 + (id & 7), z = (id >> 3) % Z; // tiles of the same positions on one XCD
+    if (unit >= (SHARED ? P.prefix_units : P.own_units)) return;
+    const int split = unit % splits, kvh = unit / splits % P.kv_heads, seq = unit / splits / P.kv_heads;
+    const KvPlanes& C = SHARED ? P.prefix : P.own;
+    const int len = SHARED ? clamped_len(P.prefix_lens, seq, P.max_prefix) : clamped_len(P.lens, seq, P.max_len);
+    const int n_rows = SHARED ? P.beams * P.group : P.group, b0 = SHARED ? seq * P.beams : seq;
+    const int part = SHARED ? split : P.prefix_splits + split;
+    const int tiles = (len + 31) / 32, share = (tiles + splits - 1) / splits, first = split * share, last = min(tiles, first + share);
+    auto row_index = [&](int r) { // of out, sums and stats
+        const int n = z * ROWS + r, s = n / P.group;
+        return (int64_t)(b0 + s) * P.heads + kvh * P.group + (n - s * P.group);
+    };
+    const int rows_here = min(ROWS, n_rows - z * ROWS);
+    if (first >= last) { // nothing to add
+        if (P.parts == 1) {
+            for (int i = threadIdx.x; i < rows_here * D; i += blockDim.x) static_cast<T*>(P.out)[row_index(i / D) * D + i % D] = (T)0.0f;
+        } else if ((int)threadIdx.x < rows_here) {
+            P.stats[row_index(threadIdx.x) * P.parts + part] = make_float2(-INFINITY, 0.0f);
+        }
+        return;
+    }
+
+    // A tile of 32 positions as this lane holds it: its key row and the values of its four positions, of each half; of the scales,
+    // of keys words of one position, SL lanes a position (lane (h * 4 + i) * SL .. of the sixteen has those of position 16 h + 4 g + i), of
+    // values a word per block for two positions, VL lanes a pair (lane (h * 2 + i) * VL .. has those of positions 16 h + 4 g + 2 i and the next)
+    constexpr int SW = NB > 4 ? NB / 4 : 1, SL = NB / 2 / SW, VL = NB / SW;
+    struct Keys {
+        Words<KW> k[2];
+        Words<SW> s;
+    };
+    struct Values {
+        Words<VW> v[2];
+        Words<LIN ? VW : 1> w[2]; // (LIN) those of the odd positions; v has the even ones'
+    };
+    struct Scales {
+        Words<SW> s;
+        Words<LIN ? SW : 1> w;  // (LIN) that of the odd position; s has the even one's
+        uint32_t beam, beams[2]; // (LIN) of the two positions whose scales are here, of its four positions of each half
+    };
+    const int64_t begin = ((int64_t)(LIN ? seq / P.beams * P.beams : seq) * C.kv_heads + kvh) * C.padded, step = C.kv_heads * C.padded;
+    const int s_index = x / SL & 7, s_pos = 16 * (s_index >> 2) + 4 * g + (s_index & 3);
+    const int v_index = x / VL & 3, v_pos = 16 * (v_index >> 1) + 4 * g + 2 * (v_index & 1);
+    const uint8_t* lineage = LIN ? P.lineage + (int64_t)seq * C.padded : nullptr;
+    uint32_t kb[2] = {}, vb[2] = {}, sb = 0, wb = 0; // (LIN) beams of the lane's key rows, of its positions, of its keys' and values' scales in the tile loaded next
+    auto load_lineage = [&](int tile) {
+        if constexpr (LIN) {
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                kb[t] = lineage[tile * 32 + 16 * t + x];
+                vb[t] = *reinterpret_cast<const uint32_t*>(lineage + tile * 32 + 16 * t + 4 * g);
+            }
+            sb = lineage[tile * 32 + s_pos];
+            wb = *reinterpret_cast<const uint16_t*>(lineage + tile * 32 + v_pos);
+        }
+    };
+    auto beam_at = [&](uint32_t beam) -> int64_t { return LIN ? (int64_t)(beam < (uint32_t)P.beams ? beam : 0) * step : 0; };
+    // (without lineage: uniform bases, 32-bit offsets of the lane)
+    auto load_keys = [&](Keys& t, Scales& sc, int tile) {
+        const int64_t at = begin + (int64_t)tile * 32;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const uint8_t* p = C.kq + (at + 16 * h) * Row::kBytes + (unsigned)(lane * Row::kPiece);
+            if constexpr (LIN) p += beam_at(kb[h]) * Row::kBytes;
+#pragma unroll
+            for (int i = 0; i < Row::kBlocks / Row::kPer; i++)
+                reinterpret_cast<Words<Row::kPiece / 4>*>(t.k[h].w)[i].load(p + 64 * Row::kPiece * i);
+        }
+        t.s.load(C.ks + (at + (LIN ? beam_at(sb) : 0)) * NB + (unsigned)(s_pos * NB + x % SL * (2 * SW)));
+        const f16_t* vs = C.vs + at * NB + (unsigned)(v_pos * NB + x % VL * (2 * SW));
+        if constexpr (LIN) {
+            sc.s.load(vs + beam_at(wb & 255) * NB);
+            sc.w.load(vs + beam_at(wb >> 8) * NB);
+            sc.beam = wb, sc.beams[0] = vb[0], sc.beams[1] = vb[1];
+        } else {
+            sc.s.load(vs);
+        }
+    };
+    auto load_values = [&](Values& t, const Scales& sc, int tile) {
+        constexpr int U = Row::kValuePiece, W = U / 4;
+        const int64_t at = begin + (int64_t)tile * 32;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const uint8_t* p = C.vq + (at + 16 * h) * Row::kBytes + (unsigned)(g * 4 * Row::kBytes + x * U);
+            if constexpr (!LIN) {
+#pragma unroll
+                for (int i = 0; i < VW / W; i++) reinterpret_cast<Words<W>*>(t.v[h].w)[i].load(p + 16 * U * i);
+            } else { // every position from its own beam, a pair of positions at a time
+                constexpr int PW = VW / 2 < W ? VW / 2 : W; // words of a load
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const uint8_t* pi = p + beam_at(sc.beams[h] >> (8 * i) & 255) * Row::kBytes;
+                    uint32_t* w = (i & 1 ? t.w[h].w : t.v[h].w) + (i >> 1) * (VW / 2);
+#pragma unroll
+                    for (int n = 0; n < VW / 2 / PW; n++) {
+                        const int word = (i >> 1) * (VW / 2) + n * PW;
+                        reinterpret_cast<Words<PW>*>(w)[n].load(pi + word / W * (16 * U) + word % W * 4);
+                    }
+                }
+            }
+        }
+    };
+    Keys keys[TWO ? 2 : 1];
+    Values vals[TWO ? 2 : 1];
+    Scales scales[2];
+    int tile = first + wave;
+    const bool any = tile < last;
+    if (any) {
+        load_lineage(tile);
+        load_keys(keys[0], scales[0], tile);
+        load_values(vals[0], scales[0], tile);
+        load_lineage(min(tile + waves, last - 1));
+    }
+
+    // The queries: lane (x, g) holds of row x the values 8 g .. of every block.  f32 ones are scaled by a power of two to
+    // below 2^14 and split.  The sign of the scale goes to them, so that the largest score is the largest product.
+    h8 qh[QLDS ? 1 : RT][NB], ql[SPLIT && !QLDS ? RT : 1][SPLIT ? NB : 1];
+    h8* q_lds = reinterpret_cast<h8*>(lds) + lane; // [RT][NB][SPLIT ? 2 : 1][64]
+    float factor[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        const T* q;
+        {
+            const int n = z * ROWS + min(16 * rt + x, rows_here - 1), s = n / P.group;
+            q = static_cast<const T*>(P.q) + (b0 + s) * P.q_stride + (int64_t)(kvh * P.group + (n - s * P.group)) * D + 8 * g;
+        }
+        float f[NB][8], by = P.scale < 0.0f ? -1.0f : 1.0f;
+        factor[rt] = fmaxf(fabsf(P.scale) * 1.44269504088896340736f, 1e-37f);
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) f[b][j] = (float)q[32 * b + j];
+        if constexpr (SPLIT) {
+            float most = 0.0f;
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) most = fmaxf(most, fabsf(f[b][j]));
+            most = qmm_max_lane_rows(most);
+            // (an infinity or a subnormal gets some power or other)
+            const int up = max(-113, min(113, 140 - (int)(__float_as_uint(most) >> 23)));
+            by *= __uint_as_float((uint32_t)(127 + up) << 23);
+            factor[rt] = fmaxf(factor[rt] * __uint_as_float((uint32_t)(127 - up) << 23), 1e-37f);
+        }
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            h8 hi, lo;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float y = f[b][j] * by;
+                hi[j] = (f16_t)y;
+                lo[j] = (f16_t)(y - (float)hi[j]);
+            }
+            if constexpr (QLDS) {
+                if (rt % waves == wave) {
+                    q_lds[(rt * NB + b) * (SPLIT ? 128 : 64)] = hi;
+                    if constexpr (SPLIT) q_lds[(rt * NB + b) * 128 + 64] = lo;
+                }
+            } else {
+                qh[rt][b] = hi;
+                if constexpr (SPLIT) ql[rt][b] = lo;
+            }
+        }
+    }
+    if constexpr (QLDS) __syncthreads();
+
+    // of the lane's row: the maximum that the reference stands on, the product that makes a new one, the reference, this lane's sum of weights
+    float top[RT], bar[RT], ref[RT], l[RT];
+    f4 o[RT][2 * NB];
+    int e_run = -24;        // 2^(e_run + 1) is above every value scale so far; as f16 bits:
+    uint32_t e_bits = 2;
+    float up = 32768.0f;    // what the value scales are multiplied by: to below 1
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        top[rt] = bar[rt] = ref[rt] = -INFINITY, l[rt] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 2 * NB; i++) o[rt][i] = f4{0, 0, 0, 0};
+    }
+    float s[RT][8];
+    // products of queries and keys, a block of the head at a time under its scale
+    auto scores = [&](const Keys& t) {
+        float d[2 * SW]; // the lane's scales, to be handed round
+#pragma unroll
+        for (int i = 0; i < 2 * SW; i++) d[i] = (float)as_h2(t.s.w[i / 2])[i & 1];
+        each<NB>([&](auto b) {
+            h8 a[2];
+#pragma unroll
+            for (int h = 0; h < 2; h++) a[h] = key_unit<QT>(t.k[h].w + b * (Row::kUnit / 4));
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) {
+                h8 hi, lo;
+                if constexpr (QLDS) {
+                    hi = q_lds[(rt * NB + b) * (SPLIT ? 128 : 64)];
+                    if constexpr (SPLIT) lo = q_lds[(rt * NB + b) * 128 + 64];
+                } else {
+                    hi = qh[rt][b];
+                    if constexpr (SPLIT) lo = ql[rt][b];
+                }
+                f4 acc[2];
+#pragma unroll
+                for (int h = 0; h < 2; h++) acc[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[h], hi, f4{0, 0, 0, 0}, 0, 0, 0);
+                if constexpr (SPLIT)
+#pragma unroll
+                    for (int h = 0; h < 2; h++) acc[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[h], lo, acc[h], 0, 0, 0);
+                each<8>([&](auto j) {
+                    const float by = __uint_as_float(of_lane<j * SL + b / 2 / SW>(__float_as_uint(d[b / 2 % SW * 2 + (b & 1)])));
+                    s[rt][j] = b == 0 ? acc[j >> 2][j & 3] * by : __builtin_fmaf(acc[j >> 2][j & 3], by, s[rt][j]);
+                });
+            }
+        });
+    };
+    auto weights = [&](Scales& t, int at) {
+        // positions behind the end, or of no beam: no weight, and a scale that is a number
+        if (LIN || at * 32 + 32 > len) {
+            asm volatile(""); // (a branch: without it every tile pays for the selections)
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                bool gone = at * 32 + 16 * (j >> 2) + 4 * g + (j & 3) >= len;
+                if constexpr (LIN) gone |= (t.beams[j >> 2] >> (8 * (j & 3)) & 255) >= (uint32_t)P.beams;
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++) s[rt][j] = gone ? -INFINITY : s[rt][j];
+            }
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                bool gone = at * 32 + v_pos + i >= len;
+                if constexpr (LIN) gone |= (t.beam >> (8 * i) & 255) >= (uint32_t)P.beams;
+#pragma unroll
+                for (int n = 0; n < SW; n++) {
+                    if constexpr (LIN) if (i == 0) t.s.w[n] = (t.s.w[n] & 0xffffu) | (t.w.w[n] & 0xffff0000u);
+                    t.s.w[n] &= gone ? 0xffffu << (16 * (1 - i)) : ~0u;
+                }
+            }
+        }
+        // does a row's maximum, or the values' largest scale, rise?
+        u2 most = magnitudes<QT>(t.s.w[0]);
+#pragma unroll
+        for (int i = 1; i < SW; i++) most = __builtin_elementwise_max(most, magnitudes<QT>(t.s.w[i]));
+        bool rise = max((uint32_t)most[0], (uint32_t)most[1]) >= e_bits;
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+            float m = s[rt][0];
+#pragma unroll
+            for (int j = 1; j < 8; j++) m = fmaxf(m, s[rt][j]);
+            rise |= m > bar[rt];
+        }
+        if (__any(rise)) {
+            float d = 0.0f;
+#pragma unroll
+            for (int i = 0; i < SW; i++) { // (fmaxf passes over the NaN of a block that holds one)
+                const h2 two = __builtin_bit_cast(h2, magnitudes<QT>(t.s.w[i]));
+                d = fmaxf(d, fmaxf((float)two[0], (float)two[1]));
+            }
+#pragma unroll
+            for (int i = 1; i < 16; i *= 2) d = fmaxf(d, __shfl_xor(d, i));
+            e_run = max(e_run, (int)(__float_as_uint(qmm_max_lane_rows(d)) >> 23) - 127);
+            e_run = __builtin_amdgcn_readfirstlane(e_run);
+            const float old_up = up;
+            up = __uint_as_float((uint32_t)(127 + min(15, -1 - e_run)) << 23);
+            e_bits = __builtin_bit_cast(uint16_t, (f16_t)__uint_as_float((uint32_t)(e_run + 128) << 23));
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) {
+                float m = s[rt][0];
+#pragma unroll
+                for (int j = 1; j < 8; j++) m = fmaxf(m, s[rt][j]);
+                top[rt] = fmaxf(top[rt], qmm_max_lane_rows(m) * factor[rt]);
+                bar[rt] = (top[rt] + kRise) / factor[rt];
+                const float to = top[rt] - kHead, by = ref[rt] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ref[rt] - to), by_o = by * (up / old_up);
+                ref[rt] = to, l[rt] *= by;
+#pragma unroll
+                for (int i = 0; i < 2 * NB; i++) o[rt][i] *= by_o;
+            }
+        }
+        // weights
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+            const float from = ref[rt] == -INFINITY ? 0.0f : -ref[rt];
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                s[rt][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rt][j], factor[rt], from));
+                l[rt] += s[rt][j];
+            }
+        }
+    };
+    // products of weights (under the values' scales) and values
+    auto products = [&](Values& t, const Scales& sc) {
+        if constexpr (LIN)
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int i = 0; i < VW; i++) t.v[h].w[i] = (t.v[h].w[i] & 0xffffu) | (t.w[h].w[i] & 0xffff0000u);
+        const f16_t by = (f16_t)up;
+        uint32_t scale[SW];
+#pragma unroll
+        for (int i = 0; i < SW; i++) scale[i] = __builtin_bit_cast(uint32_t, as_h2(sc.s.w[i]) * h2{by, by});
+        h2 ph[RT][4], pl[SPLIT ? RT : 1][4];
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const float a = s[rt][2 * r], c = s[rt][2 * r + 1];
+                ph[rt][r] = h2{(f16_t)a, (f16_t)c};
+                if constexpr (SPLIT) pl[rt][r] = h2{(f16_t)(a - (float)ph[rt][r][0]), (f16_t)(c - (float)ph[rt][r][1])};
+            }
+        each<NB>([&](auto b) {
+            h2 d[4];
+            each<4>([&](auto r) { d[r] = as_h2(of_lane<r * VL + b / SW>(scale[b % SW])); });
+            h8 va, vc;
+            value_pair<QT>(t.v, b, va, vc);
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) {
+                h2 w[4], e[4];
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    w[r] = ph[rt][r] * d[r];
+                    // what the product lost, and the weight's second part
+                    if constexpr (SPLIT) e[r] = __builtin_elementwise_fma(pl[rt][r], d[r], __builtin_elementwise_fma(ph[rt][r], d[r], -w[r]));
+                }
+                const h8 wh = join(w[0], w[1], w[2], w[3]);
+                o[rt][2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, wh, o[rt][2 * b], 0, 0, 0);
+                o[rt][2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vc, wh, o[rt][2 * b + 1], 0, 0, 0);
+                if constexpr (SPLIT) {
+                    const h8 wl = join(e[0], e[1], e[2], e[3]);
+                    o[rt][2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, wl, o[rt][2 * b], 0, 0, 0);
+                    o[rt][2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vc, wl, o[rt][2 * b + 1], 0, 0, 0);
+                }
+            }
+        });
+    };
+    if (any) {
+        if constexpr (TWO) { // two sets of registers in turns: a tile is requested before the one in front of it is worked on
+            for (;;) {
+                load_keys(keys[1], scales[1], min(tile + waves, last - 1));
+                load_values(vals[1], scales[1], min(tile + waves, last - 1));
+                load_lineage(min(tile + 2 * waves, last - 1));
+                scores(keys[0]);
+                weights(scales[0], tile);
+                products(vals[0], scales[0]);
+                tile += waves;
+                if (tile >= last) break;
+                load_keys(keys[0], scales[0], min(tile + waves, last - 1));
+                load_values(vals[0], scales[0], min(tile + waves, last - 1));
+                load_lineage(min(tile + 2 * waves, last - 1));
+                scores(keys[1]);
+                weights(scales[1], tile);
+                products(vals[1], scales[1]);
+                tile += waves;
+                if (tile >= last) break;
+            }
+        } else { // one set: keys are requested when the last ones have been used, so are values
+            for (; tile < last; tile += waves) {
+                const int next = min(tile + waves, last - 1);
+                scores(keys[0]);
+                load_keys(keys[0], scales[1], next);
+                load_lineage(min(tile + 2 * waves, last - 1));
+                weights(scales[0], tile);
+                products(vals[0], scales[0]);
+                load_values(vals[0], scales[1], next);
+                scales[0] = scales[1];
+            }
+        }
+    }
+    if constexpr (QLDS) __syncthreads();
+
+    // the waves' results meet in LDS; lane (x, g) has of block b the values 8 g .. 8 g + 7 of row x
+    float2* stat = reinterpret_cast<float2*>(lds + waves * ROWS * (D + 4));
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        float* dst = lds + (wave * ROWS + 16 * rt + x) * (D + 4) + 8 * g;
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            const f4 a = o[rt][2 * b] * (1.0f / up), c = o[rt][2 * b + 1] * (1.0f / up);
+            *reinterpret_cast<f4*>(dst + 32 * b) = f4{a[0], c[0], a[1], c[1]};
+            *reinterpret_cast<f4*>(dst + 32 * b + 4) = f4{a[2], c[2], a[3], c[3]};
+        }
+        const float sum = qmm_add_lane32(qmm_add_lane16(l[rt]));
+        if (g == 0) stat[wave * ROWS + 16 * rt + x] = make_float2(ref[rt], sum);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < rows_here * (D / 4); i += blockDim.x) {
+        const int r = i / (D / 4), d = i % (D / 4) * 4;
+        float to = -INFINITY, sum = 0.0f;
+        for (int w = 0; w < waves; w++) to = fmaxf(to, stat[w * ROWS + r].x);
+        f4 a = f4{0, 0, 0, 0};
+        for (int w = 0; w < waves; w++) {
+            const float2 st = stat[w * ROWS + r];
+            if (st.x == -INFINITY) continue;
+            const float by = __builtin_amdgcn_exp2f(st.x - to);
+            a += *reinterpret_cast<const f4*>(lds + (w * ROWS + r) * (D + 4) + d) * by;
+            sum += st.y * by;
+        }
+        const int64_t row = row_index(r);
+        if (P.parts == 1) {
+            T* out = static_cast<T*>(P.out) + row * D + d;
+            const float by = to == -INFINITY ? 0.0f : 1.0f / sum;
+#pragma unroll
+            for (int j = 0; j < 4; j++) out[j] = (T)(a[j] * by);
+        } else {
+            *reinterpret_cast<f4*>(P.sums + (row * P.parts + part) * D + d) = a;
+            if (d == 0) P.stats[row * P.parts + part] = make_float2(to, sum);
+        }
+    }
+}
+
+// RT: tiles of 16 query rows that a workgroup has of a prompt; the own positions of a sequence go by one.
+template <typename T, int QT, int D, int RT, bool LIN>
+__global__ __launch_bounds__(D <= 128 && RT <= 2 ? 512 : 256) void attend_kernel(AttendParams P) {
+    extern __shared__ __attribute__((aligned(16))) float lds[]; // the queries of several tiles; at the end [waves][16 RT][D + 4], then [waves][16 RT] of (reference, sum)
+    const int id = blockIdx.x;
+    if (id < P.prefix_wgs) attend_rows<T, QT, D, RT, true, false>(P, id, lds);
+    else attend_rows<T, QT, D, 1, false, LIN>(P, id - P.prefix_wgs, lds);
+}
+
+// A row's parts joined: a workgroup per row, its four waves take the parts in turn.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void attend_join_kernel(const float* __restrict__ sums, const float2* __restrict__ stats, T* __restrict__ out, int parts) {
+    constexpr int N = D / 64;
+    __shared__ float red[4][D + 2];
+    const int64_t row = blockIdx.x;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    stats += row * parts, sums += row * parts * D + lane * N;
+    float to = -INFINITY;
+    for (int p = lane; p < parts; p += 64) to = fmaxf(to, stats[p].x);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) to = fmaxf(to, __shfl_xor(to, o));
+    float a[N] = {}, sum = 0.0f;
+    for (int p = wave; p < parts; p += 4) {
+        const float2 st = stats[p];
+        if (st.x == -INFINITY) continue; // its sums were not written
+        const float by = __builtin_amdgcn_exp2f(st.x - to);
+        sum += st.y * by;
+#pragma unroll
+        for (int i = 0; i < N; i++) a[i] += sums[(int64_t)p * D + i] * by;
+    }
+#pragma unroll
+    for (int i = 0; i < N; i++) red[wave][lane * N + i] = a[i];
+    if (lane == 0) red[wave][D] = sum;
+    __syncthreads();
+    if (threadIdx.x < D) {
+        const float total = red[0][D] + red[1][D] + red[2][D] + red[3][D];
+        const float v = red[0][threadIdx.x] + red[1][threadIdx.x] + red[2][threadIdx.x] + red[3][threadIdx.x];
+        out[row * D + threadIdx.x] = (T)(to == -INFINITY ? 0.0f : v / total);
+    }
+}
+
+template <typename T, int QT, int D>
+hipError_t launch_attend_of(const AttendParams& P, int rt, int waves, hipStream_t stream) {
+    const unsigned wgs = (unsigned)(P.prefix_wgs + (P.own_units + 7) / 8 * 8 * P.own_z);
+    const size_t lds = (size_t)waves * 16 * rt * ((D + 4) * sizeof(float) + sizeof(float2)); // (the queries take less)
+    const auto run = [&](auto kernel) {
+        if (lds > 64 * 1024) {
+            const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+            if (e != hipSuccess) return e;
+        }
+        kernel<<<wgs, 64 * waves, lds, stream>>>(P);
+        return hipGetLastError();
+    };
+    hipError_t e;
+    constexpr int R2 = D <= 128 ? 2 : 1;
+    if (P.lineage) e = rt == 1 ? run(attend_kernel<T, QT, D, 1, true>) : run(attend_kernel<T, QT, D, R2, true>);
+    else e = rt == 1 ? run(attend_kernel<T, QT, D, 1, false>) : run(attend_kernel<T, QT, D, R2, false>);
+    if (e != hipSuccess || P.parts == 1) return e;
+    attend_join_kernel<T, D><<<(unsigned)(P.batch * P.heads), 256, 0, stream>>>(P.sums, P.stats, static_cast<T*>(P.out), P.parts);
     return hipGetLastError();
+}
+template <typename T>
+hipError_t launch_attend(int type, int64_t d, const AttendParams& P, int rt, int waves, hipStream_t stream) {
+    if (type == IZWI_KV_Q8_0)
+        return d == 64    ? launch_attend_of<T, IZWI_KV_Q8_0, 64>(P, rt, waves, stream)
+               : d == 128 ? launch_attend_of<T, IZWI_KV_Q8_0, 128>(P, rt, waves, stream)
+                          : launch_attend_of<T, IZWI_KV_Q8_0, 256>(P, rt, waves, stream);
+    return d == 64    ? launch_attend_of<T, IZWI_KV_Q4_0, 64>(P, rt, waves, stream)
+           : d == 128 ? launch_attend_of<T, IZWI_KV_Q4_0, 128>(P, rt, waves, stream)
+                      : launch_attend_of<T, IZWI_KV_Q4_0, 256>(P, rt, waves, stream);
 }
 
 template <typename T>
 int shared_attention_impl(int type, const T* q, int64_t q_stride, int64_t batch, int64_t beams, int64_t heads, int64_t kv_heads, int64_t d,
                           const void* prefix, int64_t prefix_slots, int64_t prefix_capacity, const int32_t* prefix_lens, int64_t max_prefix,
                           const void* cache, int64_t slots, int64_t capacity, const int32_t* lens, int64_t max_len, const uint8_t* lineage, float scale,
-                          T* out, void* stream) {
+                          T* out, void* stream_) {
     constexpr const char* what = "decode_shared_attention";
     if (batch < 0 || beams <= 0 || batch % beams || heads <= 0 || kv_heads <= 0 || heads % kv_heads || heads > 65535 || batch > 0xfffff ||
         q_stride < heads * d)
@@ -130,9 +630,12 @@ int shared_attention_impl(int type, const T* q, int64_t q_stride, int64_t batch,
     if (cache && (slots < batch || max_len < 0 || max_len > capacity))
         return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: %lld sequences of up to %lld positions in %lld slots of %lld", what, (long long)batch,
                         (long long)max_len, (long long)slots, (long long)capacity);
+    if (batch > 0x3ffffff / heads)
+        return qmm_fail(IZWI_QMM_ERR_UNSUPPORTED, "%s: %lld sequences of %lld heads", what, (long long)batch, (long long)heads);
     if (lineage && (beams > 255 || !cache))
         return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: lineage of %lld beams (at most 255, of a cache)", what, (long long)beams);
     if (batch == 0) return IZWI_QMM_OK;
+    if (!prefix && !cache) return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: neither a prefix nor a cache", what);
     if (!q || !out || (prefix && !prefix_lens) || (cache && !lens)) return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: NULL buffer", what);
     if (!kv_aligned(prefix, 16) || !kv_aligned(cache, 16)) return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: caches must be 16-byte aligned", what);
     int device = 0, n_cus = 0;
@@ -145,7 +648,44 @@ int shared_attention_impl(int type, const T* q, int64_t q_stride, int64_t batch,
     P.batch = (int)batch, P.beams = (int)beams, P.heads = (int)heads, P.kv_heads = (int)kv_heads, P.group = (int)(heads / kv_heads);
     P.max_prefix = prefix ? (int)max_prefix : 0, P.max_len = cache ? (int)max_len : 0;
     P.scale = scale;
-    KV_TRY(launch_attend<T>(type, d, P, (hipStream_t)stream));
+    hipStream_t stream = (hipStream_t)stream_;
+    // Workgroups of four waves, about one per compute unit, each with the positions of a split in turns of 32 per wave; two per compute
+    // unit where their waves still have 32 turns.
+    constexpr int waves = 4;
+    const auto turns = [&](int64_t n_seq, int most, int rows, int rt) { // of a wave, with one workgroup per compute unit
+        const int64_t base = n_seq * kv_heads * ((rows + 16 * rt - 1) / (16 * rt)), tiles = (most + 31) / 32;
+        const int64_t splits = std::max<int64_t>(1, std::min((n_cus + base - 1) / base, (tiles + waves - 1) / waves));
+        return tiles / (splits * waves);
+    };
+    const auto units = [&](int64_t n_seq, int most, int rows, int rt, int& splits, int& n_units, int& z) {
+        splits = n_units = 0, z = 1;
+        if (most == 0) return;
+        z = (rows + 16 * rt - 1) / (16 * rt);
+        const int64_t base = n_seq * kv_heads * z, tiles = (most + 31) / 32, want = turns(n_seq, most, rows, rt) >= 64 ? 2 * n_cus : n_cus;
+        const int64_t s = std::max<int64_t>(1, std::min((want + base - 1) / base, (tiles + waves - 1) / waves)), share = (tiles + s - 1) / s;
+        splits = (int)((tiles + share - 1) / share);
+        n_units = (int)(n_seq * kv_heads * splits);
+    };
+    // two tiles of query rows to a workgroup where there are two and the waves have enough to do all the same
+    const int prompt_rows = (int)(beams * P.group);
+    const int rt = d <= 128 && prompt_rows > 16 && turns(batch / beams, P.max_prefix, prompt_rows, 2) >= 8 ? 2 : 1;
+    units(batch / beams, P.max_prefix, prompt_rows, rt, P.prefix_splits, P.prefix_units, P.prefix_z);
+    units(batch, P.max_len, P.group, 1, P.own_splits, P.own_units, P.own_z);
+    P.prefix_wgs = (P.prefix_units + 7) / 8 * 8 * P.prefix_z;
+    P.parts = P.prefix_splits + P.own_splits;
+    if (P.parts == 0) { // bounds of zero: zeros
+        P.parts = P.own_splits = 1, P.own_units = (int)(batch * kv_heads);
+        P.own_z = (P.group + 15) / 16;
+    }
+    QmmCallScope call;
+    if (P.parts > 1) {
+        const size_t rows = (size_t)batch * heads * P.parts;
+        void* scratch = nullptr;
+        KV_TRY(qmm_get_scratch(device, stream, rows * (d * sizeof(float) + sizeof(float2)), &scratch));
+        P.sums = static_cast<float*>(scratch);
+        P.stats = reinterpret_cast<float2*>(P.sums + rows * d);
+    }
+    KV_TRY(launch_attend<T>(type, d, P, rt, waves, stream));
     return IZWI_QMM_OK;
 }
 

@@ -2,14 +2,16 @@
 //
 // A cache holds, for every (slot, kv head), `capacity` positions (rounded up to 32) of a key row and a value row of D
 // values, quantized in blocks of 32 along the row: an f16 scale per block and a quant of 8 (Q8_0) or 4 (Q4_0) bits per
-// value.  Four planes one behind the other, [slot][kv head][position][row bytes] each: key quants, key scales, value
-// quants, value scales; a position's scales are its D / 32 halves in order.
-//
-// The quants of a row stand where the matrix-core operands of the attention want them, so that it loads whole pieces
-// and never moves a value between lanes:
-//  * keys: lane group g (of four) multiplies the values 8 g .. 8 g + 7 of every block: these are one unit of 8 bytes (Q8_0) or
-//    4 (Q4_0), and the units that one lane takes are neighbours, up to 16 bytes of them.
-//  * values: lane x (of sixteen) takes the values 2 x and 2 x + 1 of every block: its D / 16 quants are neighbours.
+// value.  Four planes one behind the other: key quants, key scales, value quants, value scales.  Key scales are
+// [slot][kv head][position][D / 32], value scales [slot][kv head][position / 2][D / 32][2].  The quants of a (slot, kv head) stand where the lanes of a wave want them as matrix-core operands, so that
+// a load brings 16 bytes to every lane from neighbouring addresses and no value moves between lanes.  (With rows of positions
+// instead, the lanes' 16-byte pieces of the keys were 128 bytes apart and each was an access to the L1 of its own: 662 accesses per 32
+// positions bound the whole kernel, 154 us where this layout takes 80: sixteen sequences of 32 heads on 8, 131072 positions.)
+//  * keys: lane (x, g) of the wave (x of sixteen, g of four) multiplies of position 16 t + x the values 8 g .. 8 g + 7 of
+//    every block, a unit of 8 bytes (Q8_0) or 4 (Q4_0).  Units that fill 16 bytes are neighbours (a piece): [16 positions][piece][g][x].
+//  * values: lane (x, g) takes of positions 4 g .. 4 g + 3 of 16 the values 2 x and 2 x + 1 of every block.  A dword holds
+//    16 bits of an even position, then 16 bits of the next: two values (Q8_0: of block j) or four (Q4_0: of blocks 2 j and 2 j + 1).
+//    [4 positions][pieces of 16 bytes][x].
 // Q8_0 quants are stored + 128, Q4_0 ones + 8: an unsigned byte or nibble under the exponent of 1024 is an f16, and one
 // subtraction (exact) leaves the quant.  The eight nibbles of a key unit go in the order 0 2 4 6 1 3 5 7: bits 0-3 and
 // 16-19 of the unit, shifted right by 4 r, are the values 2 r and 2 r + 1, a register of the operand.
@@ -29,7 +31,7 @@ constexpr int kKvBlock = 32, kKvPad = 32;
 struct KvPlanes {
     uint8_t *kq, *vq;
     _Float16 *ks, *vs;
-    int64_t kv_heads, padded; // row (slot, head, position) = (slot * kv_heads + head) * padded + position of every plane
+    int64_t kv_heads, padded; // (slot, head) begins at position (slot * kv_heads + head) * padded of every plane
 };
 inline int64_t kv_padded(int64_t capacity) { return (capacity + kKvPad - 1) / kKvPad * kKvPad; }
 inline int64_t kv_row_bytes(int type, int64_t d) { return type == IZWI_KV_Q8_0 ? d : d / 2; }
@@ -71,12 +73,22 @@ inline bool kv_aligned(const void* p, size_t to) { return (reinterpret_cast<uint
 template <int QT, int D>
 struct KvRow {
     static constexpr int kBlocks = D / kKvBlock;
-    static constexpr int kBytes = QT == IZWI_KV_Q8_0 ? D : D / 2;
+    static constexpr int kBytes = QT == IZWI_KV_Q8_0 ? D : D / 2; // of a position's keys, or values
     static constexpr int kUnit = QT == IZWI_KV_Q8_0 ? 8 : 4;
-    static constexpr int kPer = 16 / kUnit < kBlocks ? 16 / kUnit : kBlocks; // units of a lane that are neighbours
-    static constexpr int kLaneBytes = kBytes / 16;                          // of a value row, per lane x
-    // where the unit of block b, lane group g of a key row begins
-    static __host__ __device__ constexpr int unit(int b, int g) { return ((b / kPer) * 4 + g) * kPer * kUnit + (b % kPer) * kUnit; }
+    static constexpr int kPer = 16 / kUnit < kBlocks ? 16 / kUnit : kBlocks, kPiece = kPer * kUnit; // units, bytes of a key piece
+    static constexpr int kLane = kBytes / 16;                        // bytes of a position's values that lane x takes
+    static constexpr int kValuePiece = 4 * kLane < 16 ? 4 * kLane : 16; // of four positions' values
+    // scales from the first position of the slot and head to that of block b of the values
+    static __host__ __device__ constexpr int64_t value_scale(int64_t pos, int b) { return ((pos >> 1) * kBlocks + b) * 2 + (pos & 1); }
+    // bytes from there to the unit of block b, lane group g of the keys, and to
+    // the 16 bits j of lane x of the values
+    static __host__ __device__ constexpr int64_t key(int64_t pos, int b, int g) {
+        return (pos >> 4) * (16 * kBytes) + (b / kPer) * (64 * kPiece) + (g * 16 + (int)(pos & 15)) * kPiece + (b % kPer) * kUnit;
+    }
+    static __host__ __device__ constexpr int64_t value(int64_t pos, int x, int j) {
+        const int at = (int)(pos >> 1 & 1) * (2 * kLane) + 4 * j + 2 * (int)(pos & 1);
+        return (pos >> 2) * (4 * kBytes) + (at / kValuePiece) * (16 * kValuePiece) + x * kValuePiece + at % kValuePiece;
+    }
 };
 
 } // namespace

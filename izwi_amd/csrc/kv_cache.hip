@@ -97,7 +97,7 @@ __device__ __forceinline__ void load_values(const T* p, float (&v)[N]) {
 // where the row of `item` stands: its sequence, token and head, and whether the cache has (or gets) it
 struct KvItem {
     unsigned row, head;
-    int64_t cache_row;
+    int64_t begin, pos; // the first position of its slot and head in the planes, its own from there
     bool there;
 };
 template <bool READ>
@@ -115,7 +115,7 @@ __device__ __forceinline__ KvItem kv_item(const KvRowsParams& P, unsigned item) 
             if (it.there) slot = slot / P.beams * P.beams + beam;
         }
     }
-    it.cache_row = (slot * P.cache.kv_heads + it.head) * P.cache.padded + (it.there ? pos : 0);
+    it.begin = (slot * P.cache.kv_heads + it.head) * P.cache.padded, it.pos = it.there ? pos : 0;
     return it;
 }
 
@@ -133,7 +133,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvRowsParams P) {
         load_values<T, 4, VEC>(static_cast<const T*>(P.k_in) + it.row * P.k_stride + it.head * D + e, v);
         unsigned q[4];
         const f16_t d = quantize_block<QT, 4, 8>(v, threadIdx.x & 7, q);
-        uint8_t* dst = P.cache.kq + it.cache_row * Row::kBytes + Row::unit(b, g);
+        uint8_t* dst = P.cache.kq + it.begin * Row::kBytes + Row::key(it.pos, b, g);
         const bool mine = asked < P.items && it.there;
         if constexpr (QT == IZWI_KV_Q8_0) {
             if (mine) *reinterpret_cast<uint32_t*>(dst + 4 * second) = q[0] | q[1] << 8 | q[2] << 16 | q[3] << 24;
@@ -143,7 +143,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvRowsParams P) {
             bits |= (unsigned)__builtin_amdgcn_update_dpp((int)bits, (int)bits, 0xB1, 0xf, 0xf, false);
             if (mine && !second) *reinterpret_cast<uint32_t*>(dst) = bits;
         }
-        if (mine && (threadIdx.x & 7) == 0) P.cache.ks[it.cache_row * Row::kBlocks + b] = d;
+        if (mine && (threadIdx.x & 7) == 0) P.cache.ks[(it.begin + it.pos) * Row::kBlocks + b] = d;
         return;
     }
     const unsigned thread = (blockIdx.x - P.k_blocks) * 256 + threadIdx.x, asked = thread / 16, item = min(asked, P.items - 1);
@@ -151,7 +151,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvRowsParams P) {
     const KvItem it = kv_item<false>(P, item);
     const T* src = static_cast<const T*>(P.v_in) + it.row * P.v_stride + it.head * D + 2 * x;
     float v[Row::kBlocks][2];
-    unsigned word[(Row::kLaneBytes + 3) / 4] = {};
+    uint16_t half[Row::kLane / 2] = {};
     f16_t d[Row::kBlocks];
 #pragma unroll
     for (int b = 0; b < Row::kBlocks; b++) load_values<T, 2, VEC>(src + 32 * b, v[b]);
@@ -159,24 +159,15 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvRowsParams P) {
     for (int b = 0; b < Row::kBlocks; b++) {
         unsigned q[2];
         d[b] = quantize_block<QT, 2, 16>(v[b], x, q);
-        if constexpr (QT == IZWI_KV_Q8_0) word[b / 2] |= (q[0] | q[1] << 8) << (16 * (b & 1));
-        else word[b / 4] |= (q[0] | q[1] << 4) << (8 * (b & 3));
+        if constexpr (QT == IZWI_KV_Q8_0) half[b] = (uint16_t)(q[0] | q[1] << 8);
+        else half[b / 2] |= (uint16_t)((q[0] | q[1] << 4) << (8 * (b & 1)));
     }
     if (asked >= P.items || !it.there) return;
-    uint8_t* dst = P.cache.vq + it.cache_row * Row::kBytes + x * Row::kLaneBytes;
-    if constexpr (Row::kLaneBytes == 2) {
-        *reinterpret_cast<uint16_t*>(dst) = (uint16_t)word[0];
-    } else {
-        constexpr int W = Row::kLaneBytes / 4;
-        typedef uint32_t vec __attribute__((ext_vector_type(W)));
-        vec t;
 #pragma unroll
-        for (int i = 0; i < W; i++) t[i] = word[i];
-        *reinterpret_cast<vec*>(dst) = t;
-    }
+    for (int j = 0; j < Row::kLane / 2; j++) *reinterpret_cast<uint16_t*>(P.cache.vq + it.begin * Row::kBytes + Row::value(it.pos, x, j)) = half[j];
 #pragma unroll
     for (int b = 0; b < Row::kBlocks; b++)
-        if (x == b) P.cache.vs[it.cache_row * Row::kBlocks + b] = d[b];
+        if (x == b) P.cache.vs[it.begin * Row::kBlocks + Row::value_scale(it.pos, b)] = d[b];
 }
 
 // The same lanes the other way; what the cache does not have reads as zeros.
@@ -205,8 +196,8 @@ __global__ __launch_bounds__(256) void kv_read_kernel(KvRowsParams P) {
         const KvItem it = kv_item<true>(P, item);
         float v[4] = {};
         if (it.there) {
-            const uint32_t* unit = reinterpret_cast<const uint32_t*>(P.cache.kq + it.cache_row * Row::kBytes + Row::unit(b, g));
-            const float d = (float)P.cache.ks[it.cache_row * Row::kBlocks + b];
+            const uint32_t* unit = reinterpret_cast<const uint32_t*>(P.cache.kq + it.begin * Row::kBytes + Row::key(it.pos, b, g));
+            const float d = (float)P.cache.ks[(it.begin + it.pos) * Row::kBlocks + b];
             const uint32_t w = QT == IZWI_KV_Q8_0 ? unit[second] : unit[0] >> (8 * second);
 #pragma unroll
             for (int i = 0; i < 4; i++) {
@@ -222,14 +213,16 @@ __global__ __launch_bounds__(256) void kv_read_kernel(KvRowsParams P) {
     const int x = threadIdx.x & 15;
     const KvItem it = kv_item<true>(P, item);
     T* dst = static_cast<T*>(P.v_out) + ((int64_t)it.row * P.kv_heads + it.head) * D + 2 * x;
-    const uint8_t* src = P.cache.vq + it.cache_row * Row::kBytes + x * Row::kLaneBytes;
-    uint8_t q[Row::kLaneBytes];
+    uint16_t half[Row::kLane / 2];
     f16_t d[Row::kBlocks];
-    __builtin_memcpy(q, __builtin_assume_aligned(src, Row::kLaneBytes), Row::kLaneBytes);
-    __builtin_memcpy(d, __builtin_assume_aligned(P.cache.vs + it.cache_row * Row::kBlocks, 2 * Row::kBlocks), 2 * Row::kBlocks);
+#pragma unroll
+    for (int j = 0; j < Row::kLane / 2; j++) half[j] = *reinterpret_cast<const uint16_t*>(P.cache.vq + it.begin * Row::kBytes + Row::value(it.pos, x, j));
+#pragma unroll
+    for (int b = 0; b < Row::kBlocks; b++) d[b] = P.cache.vs[it.begin * Row::kBlocks + Row::value_scale(it.pos, b)];
 #pragma unroll
     for (int b = 0; b < Row::kBlocks; b++) {
-        const int q0 = QT == IZWI_KV_Q8_0 ? q[2 * b] : q[b] & 15, q1 = QT == IZWI_KV_Q8_0 ? q[2 * b + 1] : q[b] >> 4;
+        const int q = QT == IZWI_KV_Q8_0 ? half[b] : half[b / 2] >> (8 * (b & 1)) & 255;
+        const int q0 = QT == IZWI_KV_Q8_0 ? q & 255 : q & 15, q1 = QT == IZWI_KV_Q8_0 ? q >> 8 : q >> 4;
         const float v[2] = {it.there ? (float)d[b] * (float)(q0 - kBias) : 0.0f, it.there ? (float)d[b] * (float)(q1 - kBias) : 0.0f};
         store(dst + 32 * b, v, std::integral_constant<int, 2>{});
     }
