@@ -21,8 +21,6 @@
 #include "kv_cache.h"
 
 #include <algorithm>
-#include <type_traits>
-#include <utility>
 
 #include "qmm_lanes.h"
 
@@ -107,22 +105,6 @@ __device__ __forceinline__ void value_pair(const Words<N> (&v)[2], int b, h8& fi
     }
     first = join(lo[0], lo[1], lo[2], lo[3]);
     second = join(hi[0], hi[1], hi[2], hi[3]);
-}
-
-// Lane N of every sixteen, in all of them
-template <int N>
-__device__ __forceinline__ uint32_t of_lane(uint32_t v) {
-    return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x150 + N, 0xf, 0xf, true); // row_newbcast
-}
-
-// f(0), .., f(N - 1), as constants
-template <class F, int... I>
-__device__ __forceinline__ void each_of(F&& f, std::integer_sequence<int, I...>) {
-    (f(std::integral_constant<int, I>{}), ...);
-}
-template <int N, class F>
-__device__ __forceinline__ void each(F&& f) {
-    each_of(f, std::make_integer_sequence<int, N>{});
 }
 
 constexpr float kRise = 10.0f, kHead = 5.0f; // powers of two, see above

@@ -1,9 +1,12 @@
 // Reductions over lanes on the vector ALU and the pieces of a running softmax, shared by the decode-step kernels
-// (decode_ops.hip, kv_attention.hip); unnamed namespace, one copy per including file.
+// (decode_ops.hip, kv_cache.hip, kv_attention.hip, beam_select.hip); unnamed namespace, one copy per including file.
 #ifndef IZWI_QMM_LANES_H
 #define IZWI_QMM_LANES_H
 
 #include <hip/hip_runtime.h>
+
+#include <type_traits>
+#include <utility>
 
 #include "qmm_internal.h"
 
@@ -37,6 +40,22 @@ __device__ __forceinline__ float sum8(float v) {
     v += dpp_f<0x4E>(v);  // quad_perm [2,3,0,1]
     v += dpp_f<0x141>(v); // row_half_mirror
     return v;
+}
+
+// Lane N of every sixteen, in all of them
+template <int N>
+__device__ __forceinline__ uint32_t of_lane(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x150 + N, 0xf, 0xf, true); // row_newbcast
+}
+
+// f(0), .., f(N - 1), as constants
+template <class F, int... I>
+__device__ __forceinline__ void each_of(F&& f, std::integer_sequence<int, I...>) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, class F>
+__device__ __forceinline__ void each(F&& f) {
+    each_of(f, std::make_integer_sequence<int, N>{});
 }
 
 } // namespace
