@@ -10,6 +10,7 @@
 // a whole number.  Within a beam the order is the logits' own, in f32.
 #include "kv_cache.h"
 #include "qmm_lanes.h"
+#include "qmm_records.h"
 
 namespace {
 
@@ -33,11 +34,11 @@ struct BeamParams {
     int64_t padded; // bytes of a lineage row
 };
 
-// NaN as -infinity, +infinity as the largest float, -0 as 0
-__device__ __forceinline__ float clean(float v) { return v != v ? -INFINITY : fminf(v, 3.402823466e38f) + 0.0f; }
+// NaN as -infinity, +infinity as the largest float (fmaxf and fminf pass over a NaN)
+__device__ __forceinline__ float clean(float v) { return fminf(fmaxf(v, -INFINITY), 3.402823466e38f); }
 // floats, doubles (no NaN) in the order of unsigned numbers, and back
 __device__ __forceinline__ uint32_t order_of(float v) {
-    const uint32_t u = __float_as_uint(v);
+    const uint32_t u = __float_as_uint(v + 0.0f); // (-0 as 0)
     return u ^ ((int32_t)u < 0 ? 0xffffffffu : 0x80000000u);
 }
 __device__ __forceinline__ float value_of(uint32_t o) { return __uint_as_float(o ^ ((int32_t)o < 0 ? 0x80000000u : 0xffffffffu)); }
@@ -61,65 +62,105 @@ __device__ __forceinline__ U kth_of_lanes(U v, int k) {
     return t;
 }
 
+template <int CTRL>
+__device__ __forceinline__ double dpp_d(double v) {
+    const uint64_t u = (uint64_t)__double_as_longlong(v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp((int)u, (int)u, CTRL, 0xf, 0xf, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp((int)(u >> 32), (int)(u >> 32), CTRL, 0xf, 0xf, false);
+    return __longlong_as_double((long long)((uint64_t)hi << 32 | lo));
+}
+// in every lane
 __device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    return v;
+    v += dpp_d<0xB1>(v);
+    v += dpp_d<0x4E>(v);
+    v += dpp_d<0x141>(v);
+    v += dpp_d<0x140>(v);
+    v += __shfl_xor(v, 16);
+    return v + __shfl_xor(v, 32);
 }
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-    return v;
+__device__ __forceinline__ float wave_max(float v) { return qmm_max_lane_rows(row16_max(v)); }
+
+// e^d for d <= 0 (or -infinity: 0) in f64 to 2e-10 of itself: 2^n 2^f with n + f = d log2(e), |f| <= 1/2, the series of 2^f to f^8
+// (the next term is (ln 2 / 2)^9 / 9!).  Half of what the library's exp takes: 78 MB of logits 42 -> 24 us.
+__device__ __forceinline__ double exp_of(double d) {
+    const double y = __builtin_fmax(d * 1.4426950408889634, -1100.0), n = __builtin_rint(y), f = y - n;
+    double p = 1.3215486790144307e-06; // ln(2)^k / k!, k = 8 .. 0
+    p = __builtin_fma(p, f, 1.5252733804059838e-05);
+    p = __builtin_fma(p, f, 1.5403530393381606e-04);
+    p = __builtin_fma(p, f, 1.3333558146428441e-03);
+    p = __builtin_fma(p, f, 9.6181291076284769e-03);
+    p = __builtin_fma(p, f, 5.5504108664821576e-02);
+    p = __builtin_fma(p, f, 2.4022650695910072e-01);
+    p = __builtin_fma(p, f, 6.9314718055994529e-01);
+    p = __builtin_fma(p, f, 1.0);
+    return __builtin_ldexp(p, (int)n);
 }
 
-constexpr int kChunkThreads = 256, kPer = 16, kChunk = kChunkThreads * kPer;
+constexpr int kChunkThreads = 256, kChunkRoom = 1024;
 
+// PER: logits of a thread
+template <int PER>
 __global__ __launch_bounds__(kChunkThreads) void beam_chunk_kernel(BeamParams P) {
+    constexpr int kChunk = kChunkThreads * PER;
     __shared__ float top[4];
     __shared__ double sum[4];
     __shared__ uint32_t threshold[4];
-    __shared__ uint64_t found[kChunk];
+    __shared__ uint64_t found[kChunkRoom];
     __shared__ uint64_t best[4];
     __shared__ unsigned n_found;
     const int row = blockIdx.y, chunk = blockIdx.x, begin = chunk * kChunk, n = min(kChunk, P.vocab - begin);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     uint64_t* keys = P.keys + ((int64_t)row * P.chunks + chunk) * P.beams;
+    const float* x = P.logits + (int64_t)row * P.vocab + begin;
+    float v[PER];
+#pragma unroll
+    for (int i = 0; i < PER; i++) v[i] = x[min(i * kChunkThreads + tid, n - 1)];
     if (P.finished && P.finished[row]) return; // the second launch looks at neither
     const float score = clean(P.scores[row]);
     if (score == -INFINITY) { // every candidate of the beam is -infinity: the lowest tokens
         if (tid < P.beams) keys[tid] = tid < n ? (uint64_t)order_of(-INFINITY) << 32 | ~(uint32_t)(begin + tid) : 0;
         return;
     }
-    const float* x = P.logits + (int64_t)row * P.vocab + begin;
-    float v[kPer], m = -INFINITY;
-    uint32_t most = 0;
-#pragma unroll
-    for (int i = 0; i < kPer; i++) v[i] = x[min(i * kChunkThreads + tid, n - 1)];
-#pragma unroll
-    for (int i = 0; i < kPer; i++) {
-        v[i] = clean(v[i]);
-        if (i * kChunkThreads + tid < n) m = fmaxf(m, v[i]), most = max(most, order_of(v[i]));
-    }
-    const float wm = wave_max(m);
-    const uint32_t kth = kth_of_lanes<uint32_t>(most, P.beams);
-    if (lane == 0) top[wave] = wm, threshold[wave] = kth;
     if (tid == 0) n_found = 0;
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        v[i] = i * kChunkThreads + tid < n ? clean(v[i]) : -INFINITY;
+        m = fmaxf(m, v[i]);
+    }
+    // the largest value that as many lanes reach as there are beams: that many of the chunk's logits are no smaller
+    const uint32_t kth = kth_of_lanes<uint32_t>(tid < n ? order_of(m) : 0, P.beams);
+    m = wave_max(m);
+    if (lane == 0) top[wave] = m, threshold[wave] = kth;
     __syncthreads();
     m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
     const uint32_t t = max(max(threshold[0], threshold[1]), max(threshold[2], threshold[3]));
-    double s = 0.0;
+    const float least = t ? value_of(t) : -INFINITY;
+    const auto key_of = [&](int i) { return (uint64_t)order_of(v[i]) << 32 | ~(uint32_t)(begin + i * kChunkThreads + tid); };
+    unsigned passed = 0;
 #pragma unroll
-    for (int i = 0; i < kPer; i++) {
-        if (i * kChunkThreads + tid >= n) break;
-        if (v[i] != -INFINITY) s += exp((double)v[i] - (double)m);
-        if (order_of(v[i]) >= t) found[atomicAdd(&n_found, 1u)] = (uint64_t)order_of(v[i]) << 32 | ~(uint32_t)(begin + i * kChunkThreads + tid);
+    for (int i = 0; i < PER; i++) passed |= v[i] >= least && i * kChunkThreads + tid < n ? 1u << i : 0u;
+    while (passed) { // (few)
+        const int i = __ffs(passed) - 1;
+        passed &= passed - 1;
+        float vi = v[0];
+#pragma unroll
+        for (int k = 1; k < PER; k++) vi = i == k ? v[k] : vi;
+        const unsigned at = atomicAdd(&n_found, 1u);
+        if (at < kChunkRoom) found[at] = (uint64_t)order_of(vi) << 32 | ~(uint32_t)(begin + i * kChunkThreads + tid);
     }
+    double s = 0.0, s2 = 0.0; // (what is behind the end is -infinity: nothing)
+    const double md = m;
+#pragma unroll
+    for (int i = 0; i < PER; i += 2) s += exp_of((double)v[i] - md), s2 += exp_of((double)v[i + 1] - md);
+    s += s2;
+    if (m == -INFINITY) s = 0.0; // (no number)
     s = wave_sum(s);
     if (lane == 0) sum[wave] = s;
     __syncthreads();
     if (tid == 0) P.sums[(int64_t)row * P.chunks + chunk] = make_double2((double)m, sum[0] + sum[1] + sum[2] + sum[3]);
     const int got = (int)n_found; // (in any order; the keys are all different)
-    if (got <= 4 * kChunkThreads) {
+    if (got <= kChunkRoom) {
         for (int i = tid; i < got; i += kChunkThreads) {
             const uint64_t key = found[i];
             int rank = 0;
@@ -133,8 +174,9 @@ __global__ __launch_bounds__(kChunkThreads) void beam_chunk_kernel(BeamParams P)
     uint64_t last = ~0ull;
     for (int k = 0; k < P.beams; k++) {
         uint64_t mine = 0;
-        for (int i = tid; i < got; i += kChunkThreads)
-            if (found[i] < last) mine = max(mine, found[i]);
+#pragma unroll
+        for (int i = 0; i < PER; i++)
+            if (i * kChunkThreads + tid < n && key_of(i) < last) mine = max(mine, key_of(i));
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) mine = max(mine, (uint64_t)__shfl_xor((unsigned long long)mine, o));
         __syncthreads();
@@ -145,7 +187,7 @@ __global__ __launch_bounds__(kChunkThreads) void beam_chunk_kernel(BeamParams P)
     }
 }
 
-constexpr int kPickThreads = 1024, kPickRoom = 4096;
+constexpr int kPickThreads = 1024, kPickRoom = 4096, kPickKept = 4; // candidates that a thread keeps in registers
 
 struct Candidate {
     uint64_t score; // order of the score
@@ -156,7 +198,7 @@ __device__ __forceinline__ bool before(const Candidate& a, const Candidate& b) {
 __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(BeamParams P) {
     __shared__ double offset[kMaxBeams]; // of a beam's logits: score - logsumexp
     __shared__ uint8_t ended[kMaxBeams];
-    __shared__ uint64_t thresholds[kPickThreads / 64];
+    __shared__ uint32_t thresholds[kPickThreads / 64];
     __shared__ __attribute__((aligned(16))) uint32_t room[3 * kPickRoom]; // what passes the threshold, then pieces of the lineage
     __shared__ uint64_t best_score[kPickThreads / 64];
     __shared__ uint32_t best_flat[kPickThreads / 64];
@@ -167,56 +209,69 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(BeamParams P) {
     uint32_t* found_flat = room + 2 * kPickRoom;
     const int prompt = blockIdx.x, W = P.beams, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t row0 = (int64_t)prompt * W;
+    const int per_beam = P.chunks * W, total = W * per_beam;
+    // the first candidates are requested before the sums are joined
+    uint64_t kept[kPickKept];
+    const uint64_t* all_keys = P.keys + row0 * per_beam;
+#pragma unroll
+    for (int c = 0; c < kPickKept; c++) kept[c] = all_keys[min(tid + c * kPickThreads, total - 1)];
     for (int w = wave; w < W; w += kPickThreads / 64) {
         const float score = clean(P.scores[row0 + w]);
         const bool end = P.finished && P.finished[row0 + w];
         double o = score;
         if (!end && score != -INFINITY) {
             const double2* part = P.sums + (row0 + w) * P.chunks;
-            double m = -INFINITY, s = 0.0;
-            for (int c = lane; c < P.chunks; c += 64) m = fmax(m, part[c].x);
-#pragma unroll
-            for (int d = 32; d > 0; d >>= 1) m = fmax(m, __shfl_xor(m, d));
-            if (m != -INFINITY)
-                for (int c = lane; c < P.chunks; c += 64) s += part[c].y == 0.0 ? 0.0 : part[c].y * exp(part[c].x - m);
+            float m = -INFINITY; // (the chunks' maxima are floats)
+            double s = 0.0;
+            const double2 one = part[min(lane, P.chunks - 1)];
+            for (int c = lane; c < P.chunks; c += 64) m = fmaxf(m, (float)(c == lane ? one : part[c]).x);
+            m = wave_max(m);
+            for (int c = lane; c < P.chunks; c += 64) {
+                const double2 p = c == lane ? one : part[c];
+                if (p.y != 0.0) s += p.y * exp_of(p.x - (double)m);
+            }
             s = wave_sum(s);
-            o = m == -INFINITY ? -INFINITY : (double)score - m - log(s);
+            o = m == -INFINITY ? -INFINITY : (double)score - (double)m - log(s);
         }
         if (lane == 0) offset[w] = o, ended[w] = end;
     }
     if (tid == 0) n_found = 0;
     __syncthreads();
-    const int per_beam = P.chunks * W, total = W * per_beam;
-    // candidate i: score order 0 for none
-    auto candidate = [&](int i) {
-        const int w = i / per_beam, j = i - w * per_beam;
+    // candidate i (score order 0: none) from its key
+    auto candidate = [&](int i, uint64_t key) {
         Candidate c{0, 0xffffffffu};
+        if (i >= total) return c;
+        const int w = i / per_beam;
         if (ended[w]) {
-            if (j == 0) c.score = order_of(offset[w]), c.flat = (uint32_t)w * P.vocab + (uint32_t)P.eos;
-            return c;
-        }
-        const uint64_t key = P.keys[(row0 + w) * per_beam + j];
-        if (key) {
+            if (i == w * per_beam) c.score = order_of(offset[w]), c.flat = (uint32_t)w * P.vocab + (uint32_t)P.eos;
+        } else if (key) {
             const float logit = value_of((uint32_t)(key >> 32));
             c.score = order_of(offset[w] == -INFINITY || logit == -INFINITY ? (double)-INFINITY : offset[w] + (double)logit);
             c.flat = (uint32_t)w * P.vocab + ~(uint32_t)key;
         }
         return c;
     };
-    uint64_t most = 0;
-    for (int i = tid; i < total; i += kPickThreads) most = max(most, candidate(i).score);
-    const uint64_t kth = kth_of_lanes<uint64_t>(most, W);
+    // scores rounded to f32 keep their order: the threshold is found among those
+    const auto coarse = [&](const Candidate& c) { return c.score ? order_of((float)double_of(c.score)) : 0u; };
+    Candidate mine[kPickKept];
+    uint32_t most = 0;
+#pragma unroll
+    for (int c = 0; c < kPickKept; c++) mine[c] = candidate(tid + c * kPickThreads, kept[c]), most = max(most, coarse(mine[c]));
+    for (int i = tid + kPickKept * kPickThreads; i < total; i += kPickThreads) most = max(most, coarse(candidate(i, all_keys[i])));
+    const uint32_t kth = kth_of_lanes<uint32_t>(most, W);
     if (lane == 0) thresholds[wave] = kth;
     __syncthreads();
-    uint64_t t = 1;
+    uint32_t t = 1;
+#pragma unroll
     for (int i = 0; i < kPickThreads / 64; i++) t = max(t, thresholds[i]);
-    for (int i = tid; i < total; i += kPickThreads) {
-        const Candidate c = candidate(i);
-        if (c.score >= t) {
-            const unsigned at = atomicAdd(&n_found, 1u);
-            if (at < kPickRoom) found_score[at] = c.score, found_flat[at] = c.flat;
-        }
-    }
+    const auto keep = [&](const Candidate& c) {
+        if (coarse(c) < t) return;
+        const unsigned at = atomicAdd(&n_found, 1u);
+        if (at < kPickRoom) found_score[at] = c.score, found_flat[at] = c.flat;
+    };
+#pragma unroll
+    for (int c = 0; c < kPickKept; c++) keep(mine[c]);
+    for (int i = tid + kPickKept * kPickThreads; i < total; i += kPickThreads) keep(candidate(i, all_keys[i]));
     __syncthreads();
     const int got = (int)n_found;
     if (got <= kPickRoom) {
@@ -231,7 +286,7 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(BeamParams P) {
         for (int k = 0; k < W; k++) {
             Candidate mine{0, 0xffffffffu};
             for (int i = tid; i < total; i += kPickThreads) {
-                const Candidate c = candidate(i);
+                const Candidate c = candidate(i, all_keys[i]);
                 if (before(last, c) && before(c, mine)) mine = c;
             }
 #pragma unroll
@@ -306,13 +361,18 @@ int izwi_decode_beam_select_f32(const float* logits, int64_t prompts, int64_t be
     hipStream_t stream = (hipStream_t)stream_;
     BeamParams P{logits, scores, finished, tokens, parents, scores_out, finished_out, lineage, lineage_out, lens, nullptr, nullptr, (int)beams, (int)vocab,
                  0, eos_token, kv_padded(lineage_capacity)};
-    P.chunks = (int)((vocab + kChunk - 1) / kChunk);
+    // 4096 logits to a workgroup, 2048 where that leaves fewer than two workgroups to a compute unit
+    const bool small = prompts * beams * ((vocab + 4095) / 4096) < 2 * n_cus;
+    const int chunk = small ? 2048 : 4096;
+    P.chunks = (int)((vocab + chunk - 1) / chunk);
     const size_t parts = (size_t)prompts * beams * P.chunks;
     void* scratch = nullptr;
     KV_TRY(qmm_get_scratch(device, stream, parts * (sizeof(double2) + (size_t)beams * sizeof(uint64_t)), &scratch));
     P.sums = static_cast<double2*>(scratch);
     P.keys = reinterpret_cast<uint64_t*>(P.sums + parts);
-    beam_chunk_kernel<<<dim3((unsigned)P.chunks, (unsigned)(prompts * beams)), kChunkThreads, 0, stream>>>(P);
+    const dim3 grid((unsigned)P.chunks, (unsigned)(prompts * beams));
+    if (small) beam_chunk_kernel<8><<<grid, kChunkThreads, 0, stream>>>(P);
+    else beam_chunk_kernel<16><<<grid, kChunkThreads, 0, stream>>>(P);
     KV_TRY(hipGetLastError());
     beam_pick_kernel<<<(unsigned)prompts, kPickThreads, 0, stream>>>(P);
     KV_TRY(hipGetLastError());
