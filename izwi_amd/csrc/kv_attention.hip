@@ -32,6 +32,18 @@ typedef f16_t h2 __attribute__((ext_vector_type(2)));
 typedef f16_t h8 __attribute__((ext_vector_type(8)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 
+// n / d for 0 <= n < 2^31 as a product: with s = ceil(log2 d) and m = floor(2^(31 + s) / d) + 1, the error of m n / 2^(31 + s) is
+// below 1 / d.  (The compiler's divisions by arguments were most of the 1500 cycles before a workgroup's first load.)
+struct Divisor {
+    uint32_t d, m, s;
+    Divisor() = default;
+    explicit Divisor(int64_t by) : d((uint32_t)by), s(0) {
+        while ((int64_t(1) << s) < by) s++;
+        m = (uint32_t)(((uint64_t(1) << (31 + s)) / (uint64_t)by + 1));
+    }
+    __device__ __forceinline__ int of(int n) const { return d == 1 ? n : (int)(__umulhi((uint32_t)n << 1, m) >> s); }
+};
+
 struct AttendParams {
     const void* q;
     void* out;
@@ -45,6 +57,7 @@ struct AttendParams {
     float scale;
     // workgroups: prefix_wgs of prefix_units (prompt, kv head, split) times prefix_z tiles of rows, then the same of (sequence, ..)
     int prefix_splits, prefix_units, prefix_z, prefix_wgs, own_splits, own_units, own_z;
+    Divisor by_group, by_kv_heads, by_beams, by_prefix_splits, by_own_splits, by_prefix_z, by_own_z;
     int parts;     // partial results of a row: prefix_splits + own_splits
     float* sums;   // [batch * heads][parts][D]
     float2* stats; // [batch * heads][parts]: reference (a power of two's exponent), sum of weights
@@ -107,34 +120,37 @@ __device__ __forceinline__ void value_pair(const Words<N> (&v)[2], int b, h8& fi
     second = join(hi[0], hi[1], hi[2], hi[3]);
 }
 
+constexpr int kWaves = 4; // of a workgroup
 constexpr float kRise = 10.0f, kHead = 5.0f; // powers of two, see above
 
 template <typename T, int QT, int D, int RT, bool SHARED, bool LIN>
 __device__ __forceinline__ void attend_rows(const AttendParams& P, int id, float* lds) {
     using Row = KvRow<QT, D>;
     constexpr int NB = Row::kBlocks, KW = Row::kBytes / 16, VW = Row::kLane, ROWS = 16 * RT;
-    constexpr bool SPLIT = sizeof(T) == 4, QLDS = RT > 1, TWO = RT == 1 && !LIN;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    constexpr bool SPLIT = sizeof(T) == 4, TWO = RT == 1 && !LIN;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int x = lane & 15, g = lane >> 4;
 
     // what this workgroup works on
     const int Z = SHARED ? P.prefix_z : P.own_z, splits = SHARED ? P.prefix_splits : P.own_splits;
-    const int unit = id / (8 * Z) * 8 + (id & 7), z = (id >> 3) % Z; // tiles of the same positions on one XCD
+    const int eighth = (SHARED ? P.by_prefix_z : P.by_own_z).of(id >> 3);
+    const int unit = eighth * 8 + (id & 7), z = (id >> 3) - eighth * Z; // tiles of the same positions on one XCD
     if (unit >= (SHARED ? P.prefix_units : P.own_units)) return;
-    const int split = unit % splits, kvh = unit / splits % P.kv_heads, seq = unit / splits / P.kv_heads;
+    const int of_split = (SHARED ? P.by_prefix_splits : P.by_own_splits).of(unit), split = unit - of_split * splits;
+    const int seq = P.by_kv_heads.of(of_split), kvh = of_split - seq * P.kv_heads;
     const KvPlanes& C = SHARED ? P.prefix : P.own;
     const int len = SHARED ? clamped_len(P.prefix_lens, seq, P.max_prefix) : clamped_len(P.lens, seq, P.max_len);
     const int n_rows = SHARED ? P.beams * P.group : P.group, b0 = SHARED ? seq * P.beams : seq;
     const int part = SHARED ? split : P.prefix_splits + split;
-    const int tiles = (len + 31) / 32, share = (tiles + splits - 1) / splits, first = split * share, last = min(tiles, first + share);
+    const int tiles = (len + 31) / 32, share = (SHARED ? P.by_prefix_splits : P.by_own_splits).of(tiles + splits - 1), first = split * share, last = min(tiles, first + share);
     auto row_index = [&](int r) { // of out, sums and stats
-        const int n = z * ROWS + r, s = n / P.group;
+        const int n = z * ROWS + r, s = P.by_group.of(n);
         return (int64_t)(b0 + s) * P.heads + kvh * P.group + (n - s * P.group);
     };
     const int rows_here = min(ROWS, n_rows - z * ROWS);
     if (first >= last) { // nothing to add
         if (P.parts == 1) {
-            for (int i = threadIdx.x; i < rows_here * D; i += blockDim.x) static_cast<T*>(P.out)[row_index(i / D) * D + i % D] = (T)0.0f;
+            for (int i = threadIdx.x; i < rows_here * D; i += (64 * kWaves)) static_cast<T*>(P.out)[row_index(i / D) * D + i % D] = (T)0.0f;
         } else if ((int)threadIdx.x < rows_here) {
             P.stats[row_index(threadIdx.x) * P.parts + part] = make_float2(-INFINITY, 0.0f);
         }
@@ -158,7 +174,7 @@ __device__ __forceinline__ void attend_rows(const AttendParams& P, int id, float
         Words<LIN ? SW : 1> w;  // (LIN) that of the odd position; s has the even one's
         uint32_t beam, beams[2]; // (LIN) of the two positions whose scales are here, of its four positions of each half
     };
-    const int64_t begin = ((int64_t)(LIN ? seq / P.beams * P.beams : seq) * C.kv_heads + kvh) * C.padded, step = C.kv_heads * C.padded;
+    const int64_t begin = ((int64_t)(LIN ? P.by_beams.of(seq) * P.beams : seq) * C.kv_heads + kvh) * C.padded, step = C.kv_heads * C.padded;
     const int s_index = x / SL & 7, s_pos = 16 * (s_index >> 2) + 4 * g + (s_index & 3);
     const int v_index = x / VL & 3, v_pos = 16 * (v_index >> 1) + 4 * g + 2 * (v_index & 1);
     const uint8_t* lineage = LIN ? P.lineage + (int64_t)seq * C.padded : nullptr;
@@ -229,19 +245,18 @@ __device__ __forceinline__ void attend_rows(const AttendParams& P, int id, float
         load_lineage(tile);
         load_keys(keys[0], scales[0], tile);
         load_values(vals[0], scales[0], tile);
-        load_lineage(min(tile + waves, last - 1));
+        load_lineage(min(tile + kWaves, last - 1));
     }
 
     // The queries: lane (x, g) holds of row x the values 8 g .. of every block.  f32 ones are scaled by a power of two to
     // below 2^14 and split.  The sign of the scale goes to them, so that the largest score is the largest product.
-    h8 qh[QLDS ? 1 : RT][NB], ql[SPLIT && !QLDS ? RT : 1][SPLIT ? NB : 1];
-    h8* q_lds = reinterpret_cast<h8*>(lds) + lane; // [RT][NB][SPLIT ? 2 : 1][64]
+    h8 qh[RT][NB], ql[SPLIT ? RT : 1][SPLIT ? NB : 1];
     float factor[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
         const T* q;
         {
-            const int n = z * ROWS + min(16 * rt + x, rows_here - 1), s = n / P.group;
+            const int n = z * ROWS + min(16 * rt + x, rows_here - 1), s = P.by_group.of(n);
             q = static_cast<const T*>(P.q) + (b0 + s) * P.q_stride + (int64_t)(kvh * P.group + (n - s * P.group)) * D + 8 * g;
         }
         float f[NB][8], by = P.scale < 0.0f ? -1.0f : 1.0f;
@@ -271,18 +286,10 @@ __device__ __forceinline__ void attend_rows(const AttendParams& P, int id, float
                 hi[j] = (f16_t)y;
                 lo[j] = (f16_t)(y - (float)hi[j]);
             }
-            if constexpr (QLDS) {
-                if (rt % waves == wave) {
-                    q_lds[(rt * NB + b) * (SPLIT ? 128 : 64)] = hi;
-                    if constexpr (SPLIT) q_lds[(rt * NB + b) * 128 + 64] = lo;
-                }
-            } else {
-                qh[rt][b] = hi;
-                if constexpr (SPLIT) ql[rt][b] = lo;
-            }
+            qh[rt][b] = hi;
+            if constexpr (SPLIT) ql[rt][b] = lo;
         }
     }
-    if constexpr (QLDS) __syncthreads();
 
     // of the lane's row: the maximum that the reference stands on, the product that makes a new one, the reference, this lane's sum of weights
     float top[RT], bar[RT], ref[RT], l[RT];
@@ -308,23 +315,15 @@ __device__ __forceinline__ void attend_rows(const AttendParams& P, int id, float
             for (int h = 0; h < 2; h++) a[h] = key_unit<QT>(t.k[h].w + b * (Row::kUnit / 4));
 #pragma unroll
             for (int rt = 0; rt < RT; rt++) {
-                h8 hi, lo;
-                if constexpr (QLDS) {
-                    hi = q_lds[(rt * NB + b) * (SPLIT ? 128 : 64)];
-                    if constexpr (SPLIT) lo = q_lds[(rt * NB + b) * 128 + 64];
-                } else {
-                    hi = qh[rt][b];
-                    if constexpr (SPLIT) lo = ql[rt][b];
-                }
                 f4 acc[2];
 #pragma unroll
-                for (int h = 0; h < 2; h++) acc[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[h], hi, f4{0, 0, 0, 0}, 0, 0, 0);
+                for (int h = 0; h < 2; h++) acc[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[h], qh[rt][b], f4{0, 0, 0, 0}, 0, 0, 0);
                 if constexpr (SPLIT)
 #pragma unroll
-                    for (int h = 0; h < 2; h++) acc[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[h], lo, acc[h], 0, 0, 0);
+                    for (int h = 0; h < 2; h++) acc[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[h], ql[rt][b], acc[h], 0, 0, 0);
                 each<8>([&](auto j) {
                     const float by = __uint_as_float(of_lane<j * SL + b / 2 / SW>(__float_as_uint(d[b / 2 % SW * 2 + (b & 1)])));
-                    s[rt][j] = b == 0 ? acc[j >> 2][j & 3] * by : __builtin_fmaf(acc[j >> 2][j & 3], by, s[rt][j]);
+                    s[rt][j] = b == 0 ? by * acc[j >> 2][j & 3] : __builtin_fmaf(by, acc[j >> 2][j & 3], s[rt][j]);
                 });
             }
         });
@@ -449,29 +448,29 @@ __device__ __forceinline__ void attend_rows(const AttendParams& P, int id, float
     if (any) {
         if constexpr (TWO) { // two sets of registers in turns: a tile is requested before the one in front of it is worked on
             for (;;) {
-                load_keys(keys[1], scales[1], min(tile + waves, last - 1));
-                load_values(vals[1], scales[1], min(tile + waves, last - 1));
-                load_lineage(min(tile + 2 * waves, last - 1));
+                load_keys(keys[1], scales[1], min(tile + kWaves, last - 1));
+                load_values(vals[1], scales[1], min(tile + kWaves, last - 1));
+                load_lineage(min(tile + 2 * kWaves, last - 1));
                 scores(keys[0]);
                 weights(scales[0], tile);
                 products(vals[0], scales[0]);
-                tile += waves;
+                tile += kWaves;
                 if (tile >= last) break;
-                load_keys(keys[0], scales[0], min(tile + waves, last - 1));
-                load_values(vals[0], scales[0], min(tile + waves, last - 1));
-                load_lineage(min(tile + 2 * waves, last - 1));
+                load_keys(keys[0], scales[0], min(tile + kWaves, last - 1));
+                load_values(vals[0], scales[0], min(tile + kWaves, last - 1));
+                load_lineage(min(tile + 2 * kWaves, last - 1));
                 scores(keys[1]);
                 weights(scales[1], tile);
                 products(vals[1], scales[1]);
-                tile += waves;
+                tile += kWaves;
                 if (tile >= last) break;
             }
         } else { // one set: keys are requested when the last ones have been used, so are values
-            for (; tile < last; tile += waves) {
-                const int next = min(tile + waves, last - 1);
+            for (; tile < last; tile += kWaves) {
+                const int next = min(tile + kWaves, last - 1);
                 scores(keys[0]);
                 load_keys(keys[0], scales[1], next);
-                load_lineage(min(tile + 2 * waves, last - 1));
+                load_lineage(min(tile + 2 * kWaves, last - 1));
                 weights(scales[0], tile);
                 products(vals[0], scales[0]);
                 load_values(vals[0], scales[1], next);
@@ -479,10 +478,8 @@ __device__ __forceinline__ void attend_rows(const AttendParams& P, int id, float
             }
         }
     }
-    if constexpr (QLDS) __syncthreads();
-
     // the waves' results meet in LDS; lane (x, g) has of block b the values 8 g .. 8 g + 7 of row x
-    float2* stat = reinterpret_cast<float2*>(lds + waves * ROWS * (D + 4));
+    float2* stat = reinterpret_cast<float2*>(lds + kWaves * ROWS * (D + 4));
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
         float* dst = lds + (wave * ROWS + 16 * rt + x) * (D + 4) + 8 * g;
@@ -496,82 +493,124 @@ __device__ __forceinline__ void attend_rows(const AttendParams& P, int id, float
         if (g == 0) stat[wave * ROWS + 16 * rt + x] = make_float2(ref[rt], sum);
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < rows_here * (D / 4); i += blockDim.x) {
-        const int r = i / (D / 4), d = i % (D / 4) * 4;
-        float to = -INFINITY, sum = 0.0f;
-        for (int w = 0; w < waves; w++) to = fmaxf(to, stat[w * ROWS + r].x);
-        f4 a = f4{0, 0, 0, 0};
-        for (int w = 0; w < waves; w++) {
-            const float2 st = stat[w * ROWS + r];
-            if (st.x == -INFINITY) continue;
-            const float by = __builtin_amdgcn_exp2f(st.x - to);
-            a += *reinterpret_cast<const f4*>(lds + (w * ROWS + r) * (D + 4) + d) * by;
-            sum += st.y * by;
+    // a thread per row turns the references into the waves' weights and leaves where the row goes
+    f4* weight = reinterpret_cast<f4*>(stat + kWaves * ROWS); // a row's waves
+    float* total = reinterpret_cast<float*>(weight + ROWS);
+    int64_t* where = reinterpret_cast<int64_t*>(total + ROWS);
+    static_assert(kWaves == 4);
+    if ((int)threadIdx.x < rows_here) {
+        const int r = threadIdx.x;
+        float2 st[kWaves];
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) st[w] = stat[w * ROWS + r];
+        const float to = fmaxf(fmaxf(st[0].x, st[1].x), fmaxf(st[2].x, st[3].x));
+        float sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) {
+            const float by = st[w].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(st[w].x - to);
+            sum += by == 0.0f ? 0.0f : st[w].y * by;
+            weight[r][w] = by;
         }
         const int64_t row = row_index(r);
-        if (P.parts == 1) {
-            T* out = static_cast<T*>(P.out) + row * D + d;
-            const float by = to == -INFINITY ? 0.0f : 1.0f / sum;
+        where[r] = row;
+        if (P.parts > 1) P.stats[row * P.parts + part] = make_float2(to, sum);
+        else total[r] = to == -INFINITY ? 0.0f : 1.0f / sum;
+    }
+    __syncthreads();
+    constexpr int kTurns = ROWS * (D / 4) / (64 * kWaves);
 #pragma unroll
-            for (int j = 0; j < 4; j++) out[j] = (T)(a[j] * by);
-        } else {
+    for (int turn = 0; turn < kTurns; turn++) {
+        const int i = threadIdx.x + turn * (64 * kWaves), r = i / (D / 4), d = i % (D / 4) * 4;
+        if (r >= rows_here) break;
+        const int64_t row = where[r];
+        const f4 by = weight[r];
+        f4 v[kWaves], a = f4{0, 0, 0, 0};
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) v[w] = *reinterpret_cast<const f4*>(lds + (w * ROWS + r) * (D + 4) + d);
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) // (a wave without a position left zeros)
+            a += v[w] * by[w];
+        if (P.parts > 1) {
             *reinterpret_cast<f4*>(P.sums + (row * P.parts + part) * D + d) = a;
-            if (d == 0) P.stats[row * P.parts + part] = make_float2(to, sum);
+        } else {
+            T* out = static_cast<T*>(P.out) + row * D + d;
+            const float inv = total[r];
+#pragma unroll
+            for (int j = 0; j < 4; j++) out[j] = (T)(a[j] * inv);
         }
     }
 }
 
 // RT: tiles of 16 query rows that a workgroup has of a prompt; the own positions of a sequence go by one.
 template <typename T, int QT, int D, int RT, bool LIN>
-__global__ __launch_bounds__(D <= 128 && RT <= 2 ? 512 : 256) void attend_kernel(AttendParams P) {
-    extern __shared__ __attribute__((aligned(16))) float lds[]; // the queries of several tiles; at the end [waves][16 RT][D + 4], then [waves][16 RT] of (reference, sum)
+__global__ __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) void attend_kernel(AttendParams P) {
+    extern __shared__ __attribute__((aligned(16))) float lds[]; // see the end of attend_rows
     const int id = blockIdx.x;
     if (id < P.prefix_wgs) attend_rows<T, QT, D, RT, true, false>(P, id, lds);
     else attend_rows<T, QT, D, 1, false, LIN>(P, id - P.prefix_wgs, lds);
 }
 
-// A row's parts joined: a workgroup per row, its four waves take the parts in turn.
+// A row's parts joined: a workgroup per row, its four waves take the parts in turn.  Statistics and sums are requested together, eight
+// parts a wave at a time; what a part did not write (no position of the row) is in its place and not looked at.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void attend_join_kernel(const float* __restrict__ sums, const float2* __restrict__ stats, T* __restrict__ out, int parts) {
-    constexpr int N = D / 64;
+    constexpr int N = D / 64, A = 8;
+    typedef float vec __attribute__((ext_vector_type(N)));
     __shared__ float red[4][D + 2];
     const int64_t row = blockIdx.x;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     stats += row * parts, sums += row * parts * D + lane * N;
-    float to = -INFINITY;
-    for (int p = lane; p < parts; p += 64) to = fmaxf(to, stats[p].x);
+    float to = -INFINITY, sum = 0.0f; // of this wave's parts so far
+    vec a = 0.0f;
+    for (int p0 = wave; p0 < parts; p0 += 4 * A) {
+        vec v[A];
+        const int mine = p0 + 4 * (lane & (A - 1)); // lane i of eight: the statistics of part i
+        const float2 st = stats[min(mine, parts - 1)];
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) to = fmaxf(to, __shfl_xor(to, o));
-    float a[N] = {}, sum = 0.0f;
-    for (int p = wave; p < parts; p += 4) {
-        const float2 st = stats[p];
-        if (st.x == -INFINITY) continue; // its sums were not written
-        const float by = __builtin_amdgcn_exp2f(st.x - to);
-        sum += st.y * by;
+        for (int i = 0; i < A; i++) v[i] = *reinterpret_cast<const vec*>(sums + (int64_t)min(p0 + 4 * i, parts - 1) * D);
+        const float ref = mine < parts ? st.x : -INFINITY;
+        float most = ref;
+        most = fmaxf(most, dpp_f<0xB1>(most));
+        most = fmaxf(most, dpp_f<0x4E>(most));
+        most = fmaxf(most, dpp_f<0x141>(most)); // over the eight
+        const float next = fmaxf(to, most);
+        const float by = ref == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ref - next), old = to == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(to - next);
+        sum = sum * old + sum8(by == 0.0f ? 0.0f : st.y * by);
+        a *= old;
 #pragma unroll
-        for (int i = 0; i < N; i++) a[i] += sums[(int64_t)p * D + i] * by;
+        for (int i = 0; i < A; i++) {
+            const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(by), i));
+            if (w != 0.0f) a += v[i] * w; // uniform
+        }
+        to = next;
     }
 #pragma unroll
     for (int i = 0; i < N; i++) red[wave][lane * N + i] = a[i];
-    if (lane == 0) red[wave][D] = sum;
+    if (lane == 0) red[wave][D] = sum, red[wave][D + 1] = to;
     __syncthreads();
     if (threadIdx.x < D) {
-        const float total = red[0][D] + red[1][D] + red[2][D] + red[3][D];
-        const float v = red[0][threadIdx.x] + red[1][threadIdx.x] + red[2][threadIdx.x] + red[3][threadIdx.x];
-        out[row * D + threadIdx.x] = (T)(to == -INFINITY ? 0.0f : v / total);
+        float most = -INFINITY, total = 0.0f, v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; w++) most = fmaxf(most, red[w][D + 1]);
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            const float by = red[w][D + 1] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(red[w][D + 1] - most);
+            total += red[w][D] * by, v += red[w][threadIdx.x] * by;
+        }
+        out[row * D + threadIdx.x] = (T)(most == -INFINITY ? 0.0f : v / total);
     }
 }
 
 template <typename T, int QT, int D>
-hipError_t launch_attend_of(const AttendParams& P, int rt, int waves, hipStream_t stream) {
+hipError_t launch_attend_of(const AttendParams& P, int rt, hipStream_t stream) {
     const unsigned wgs = (unsigned)(P.prefix_wgs + (P.own_units + 7) / 8 * 8 * P.own_z);
-    const size_t lds = (size_t)waves * 16 * rt * ((D + 4) * sizeof(float) + sizeof(float2)); // (the queries take less)
+    const size_t lds = (size_t)16 * rt * (kWaves * ((D + 4) * sizeof(float) + sizeof(float2)) + sizeof(f4) + sizeof(float) + sizeof(int64_t));
     const auto run = [&](auto kernel) {
         if (lds > 64 * 1024) {
             const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
             if (e != hipSuccess) return e;
         }
-        kernel<<<wgs, 64 * waves, lds, stream>>>(P);
+        kernel<<<wgs, 64 * kWaves, lds, stream>>>(P);
         return hipGetLastError();
     };
     hipError_t e;
@@ -583,14 +622,14 @@ hipError_t launch_attend_of(const AttendParams& P, int rt, int waves, hipStream_
     return hipGetLastError();
 }
 template <typename T>
-hipError_t launch_attend(int type, int64_t d, const AttendParams& P, int rt, int waves, hipStream_t stream) {
+hipError_t launch_attend(int type, int64_t d, const AttendParams& P, int rt, hipStream_t stream) {
     if (type == IZWI_KV_Q8_0)
-        return d == 64    ? launch_attend_of<T, IZWI_KV_Q8_0, 64>(P, rt, waves, stream)
-               : d == 128 ? launch_attend_of<T, IZWI_KV_Q8_0, 128>(P, rt, waves, stream)
-                          : launch_attend_of<T, IZWI_KV_Q8_0, 256>(P, rt, waves, stream);
-    return d == 64    ? launch_attend_of<T, IZWI_KV_Q4_0, 64>(P, rt, waves, stream)
-           : d == 128 ? launch_attend_of<T, IZWI_KV_Q4_0, 128>(P, rt, waves, stream)
-                      : launch_attend_of<T, IZWI_KV_Q4_0, 256>(P, rt, waves, stream);
+        return d == 64    ? launch_attend_of<T, IZWI_KV_Q8_0, 64>(P, rt, stream)
+               : d == 128 ? launch_attend_of<T, IZWI_KV_Q8_0, 128>(P, rt, stream)
+                          : launch_attend_of<T, IZWI_KV_Q8_0, 256>(P, rt, stream);
+    return d == 64    ? launch_attend_of<T, IZWI_KV_Q4_0, 64>(P, rt, stream)
+           : d == 128 ? launch_attend_of<T, IZWI_KV_Q4_0, 128>(P, rt, stream)
+                      : launch_attend_of<T, IZWI_KV_Q4_0, 256>(P, rt, stream);
 }
 
 template <typename T>
@@ -633,17 +672,26 @@ int shared_attention_impl(int type, const T* q, int64_t q_stride, int64_t batch,
     hipStream_t stream = (hipStream_t)stream_;
     // Workgroups of four waves, about one per compute unit, each with the positions of a split in turns of 32 per wave; two per compute
     // unit where their waves still have 32 turns.
-    constexpr int waves = 4;
+    constexpr int waves = kWaves;
     const auto turns = [&](int64_t n_seq, int most, int rows, int rt) { // of a wave, with one workgroup per compute unit
         const int64_t base = n_seq * kv_heads * ((rows + 16 * rt - 1) / (16 * rt)), tiles = (most + 31) / 32;
         const int64_t splits = std::max<int64_t>(1, std::min((n_cus + base - 1) / base, (tiles + waves - 1) / waves));
         return tiles / (splits * waves);
     };
+    // Few positions of one kind stay with one workgroup per sequence and kv head: nothing is left to join (16 heads on 8, 300 positions: 6.9 us
+    // in a graph where three splits take 7.5, and a launch less for the host).
+    constexpr int kOneLaunchTiles = 12;
+    const bool alone = P.max_prefix == 0 || P.max_len == 0;
     const auto units = [&](int64_t n_seq, int most, int rows, int rt, int& splits, int& n_units, int& z) {
         splits = n_units = 0, z = 1;
         if (most == 0) return;
         z = (rows + 16 * rt - 1) / (16 * rt);
-        const int64_t base = n_seq * kv_heads * z, tiles = (most + 31) / 32, want = turns(n_seq, most, rows, rt) >= 64 ? 2 * n_cus : n_cus;
+        const int64_t base = n_seq * kv_heads * z, tiles = (most + 31) / 32;
+        if (alone && tiles <= kOneLaunchTiles) { // no second kernel
+            splits = 1, n_units = (int)base / z;
+            return;
+        }
+        const int64_t want = turns(n_seq, most, rows, rt) >= 64 ? 2 * n_cus : n_cus;
         const int64_t s = std::max<int64_t>(1, std::min((want + base - 1) / base, (tiles + waves - 1) / waves)), share = (tiles + s - 1) / s;
         splits = (int)((tiles + share - 1) / share);
         n_units = (int)(n_seq * kv_heads * splits);
@@ -659,6 +707,9 @@ int shared_attention_impl(int type, const T* q, int64_t q_stride, int64_t batch,
         P.parts = P.own_splits = 1, P.own_units = (int)(batch * kv_heads);
         P.own_z = (P.group + 15) / 16;
     }
+    P.by_group = Divisor(P.group), P.by_kv_heads = Divisor(kv_heads), P.by_beams = Divisor(beams);
+    P.by_prefix_splits = Divisor(std::max(1, P.prefix_splits)), P.by_own_splits = Divisor(std::max(1, P.own_splits));
+    P.by_prefix_z = Divisor(P.prefix_z), P.by_own_z = Divisor(P.own_z);
     QmmCallScope call;
     if (P.parts > 1) {
         const size_t rows = (size_t)batch * heads * P.parts;
@@ -667,7 +718,7 @@ int shared_attention_impl(int type, const T* q, int64_t q_stride, int64_t batch,
         P.sums = static_cast<float*>(scratch);
         P.stats = reinterpret_cast<float2*>(P.sums + rows * d);
     }
-    KV_TRY(launch_attend<T>(type, d, P, rt, waves, stream));
+    KV_TRY(launch_attend<T>(type, d, P, rt, stream));
     return IZWI_QMM_OK;
 }
 

@@ -40,21 +40,31 @@ def _refuse(what: str):
     raise QmmError(-1, what)
 
 
-def _ints(t, n: int, device, what: str) -> int:
+# (What a call checks and looks up is paid for once per layer and token: device numbers are compared instead of devices, and the
+# library's functions are looked up once.)
+_f32, _f16, _i32, _u8 = torch.float32, torch.float16, torch.int32, torch.uint8
+_fns = {}
+
+
+def _fn(name: str):
+    fn = _fns.get(name)
+    if fn is None:
+        fn = _fns[name] = getattr(lib(), f"izwi_decode_{name}")
+    return fn
+
+
+def _ints(t, n: int, index: int, what: str) -> int:
     if t is None:
         return 0
-    if t.dtype is not torch.int32 or t.shape != (n,) or not t.is_contiguous() or t.device != device:
-        _refuse(f"{what}: a contiguous int32 tensor of {n} on {device} expected")
+    if t.dtype is not _i32 or t.get_device() != index or t.shape != (n,) or not t.is_contiguous():
+        _refuse(f"{what}: a contiguous int32 tensor of {n} on GPU {index} expected")
     return t.data_ptr()
 
 
-def _rows(t, shape, device, what: str) -> int:
+def _rows(t, what: str) -> int:
     """Elements from one row of heads to the next, rows being all leading dimensions taken together."""
-    if t.shape != shape or t.device != device:
-        _refuse(f"{what}: a tensor {tuple(shape)} on {device} expected")
+    shape = t.shape
     heads, d = shape[-2:]
-    if t.is_contiguous():
-        return heads * d
     stride = t.stride()
     if stride[-1] != 1 or (heads > 1 and stride[-2] != d):
         _refuse(f"{what}: heads of a row must be contiguous")
@@ -75,15 +85,6 @@ def _rows(t, shape, device, what: str) -> int:
     return step
 
 
-def _launch(fn, device, *args):
-    """The call on the current stream of the tensors' device."""
-    if device.index == _current_device():
-        check(fn(*args, _raw_stream(device.index)))
-    else:
-        with torch.cuda.device(device):
-            check(fn(*args, _raw_stream(device.index)))
-
-
 class QuantizedKvCache:
     """Keys and values of ``slots`` sequences, up to ``capacity`` positions of ``kv_heads`` heads each, quantized as they
     are written.  head_dim 64, 128 or 256."""
@@ -97,47 +98,57 @@ class QuantizedKvCache:
             raise QmmError(-1, lib().izwi_qmm_last_error().decode("utf-8", "replace"))
         self.buffer = torch.empty(nbytes, dtype=torch.uint8, device=device)
         self.device = self.buffer.device
-        self._ptr = self.buffer.data_ptr()
+        self._index, self._ptr, self._type, self._row = self.buffer.get_device(), self.buffer.data_ptr(), int(dtype), kv_heads * head_dim
+        self._lineage_shape = (slots, -(-capacity // _PAD) * _PAD)
 
     def new_lineage(self) -> torch.Tensor:
         """Lineage rows of all slots, [slots, capacity rounded up to 32] uint8, zeros: no position has been written."""
-        return torch.zeros(self.slots, -(-self.capacity // _PAD) * _PAD, dtype=torch.uint8, device=self.device)
+        return torch.zeros(self._lineage_shape, dtype=torch.uint8, device=self.device)
 
     def append(self, k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor, counts: torch.Tensor | None = None, first_slot: int = 0) -> None:
         """k, v [sequences, tokens, kv_heads, head_dim] (f32 or f16; rows may be parts of wider ones): token t of
         sequence b goes to position starts[b] + t of slot first_slot + b, for t < counts[b].  What lies outside the
         capacity is left out."""
-        if k.dim() != 4 or k.dtype not in (torch.float32, torch.float16) or v.dtype is not k.dtype:
-            _refuse("append: k and v [sequences, tokens, kv_heads, head_dim] of f32 or f16 expected")
-        batch, tokens = k.shape[:2]
-        shape = (batch, tokens, self.kv_heads, self.head_dim)
-        k_stride, v_stride = _rows(k, shape, self.device, "append: k"), _rows(v, shape, self.device, "append: v")
-        fn = lib().izwi_decode_kv_append_f32 if k.dtype is torch.float32 else lib().izwi_decode_kv_append_f16
-        _launch(fn, self.device, int(self.dtype), k.data_ptr(), v.data_ptr(), k_stride, v_stride, _ints(starts, batch, self.device, "append: starts"),
-                _ints(counts, batch, self.device, "append: counts"), batch, tokens, first_slot, self.slots, self.kv_heads, self.capacity, self.head_dim,
-                self._ptr)
+        dtype, shape, index = k.dtype, k.shape, self._index
+        if (dtype is not _f32 and dtype is not _f16 or v.dtype is not dtype or len(shape) != 4 or v.shape != shape or shape[2] != self.kv_heads
+                or shape[3] != self.head_dim or k.get_device() != index or v.get_device() != index):
+            _refuse(f"append: k and v [sequences, tokens, {self.kv_heads}, {self.head_dim}] of f32 or f16 on {self.device} expected")
+        if index != _current_device():
+            with torch.cuda.device(index):
+                return self.append(k, v, starts, counts, first_slot)
+        batch = shape[0]
+        rc = _fn("kv_append_f32" if dtype is _f32 else "kv_append_f16")(
+            self._type, k.data_ptr(), v.data_ptr(), self._row if k.is_contiguous() else _rows(k, "append: k"),
+            self._row if v.is_contiguous() else _rows(v, "append: v"), _ints(starts, batch, index, "append: starts"),
+            _ints(counts, batch, index, "append: counts"), batch, shape[1], first_slot, self.slots, self.kv_heads, self.capacity, self.head_dim, self._ptr,
+            _raw_stream(index))
+        if rc:
+            check(rc)
 
     def read(self, starts: torch.Tensor, tokens: int, counts: torch.Tensor | None = None, first_slot: int = 0, lineage: torch.Tensor | None = None,
              beams: int = 1, dtype: torch.dtype = torch.float32):
         """(k, v) [sequences, tokens, kv_heads, head_dim]: the values that positions starts[b] .. starts[b] + tokens - 1 of slots
         first_slot, .. stand for; zeros from counts[b] on and outside the capacity.  With ``lineage`` a position comes from
         the slot of the beam that wrote it (``beams`` slots a prompt)."""
-        if dtype not in (torch.float32, torch.float16):
+        if dtype is not _f32 and dtype is not _f16:
             _refuse("read: f32 or f16 expected")
+        index = self._index
+        if index != _current_device():
+            with torch.cuda.device(index):
+                return self.read(starts, tokens, counts, first_slot, lineage, beams, dtype)
         batch = starts.shape[0]
-        k = torch.empty(batch, tokens, self.kv_heads, self.head_dim, dtype=dtype, device=self.device)
+        at, until = _ints(starts, batch, index, "read: starts"), _ints(counts, batch, index, "read: counts")
+        k = torch.empty((batch, tokens, self.kv_heads, self.head_dim), dtype=dtype, device=self.device)
         v = torch.empty_like(k)
-        fn = lib().izwi_decode_kv_read_f32 if dtype is torch.float32 else lib().izwi_decode_kv_read_f16
-        _launch(fn, self.device, int(self.dtype), self._ptr, self.slots, self.kv_heads, self.capacity, self.head_dim, self._lineage(lineage, "read"),
-                beams, _ints(starts, batch, self.device, "read: starts"), _ints(counts, batch, self.device, "read: counts"), batch, tokens, first_slot,
-                k.data_ptr(), v.data_ptr())
+        rc = _fn("kv_read_f32" if dtype is _f32 else "kv_read_f16")(
+            self._type, self._ptr, self.slots, self.kv_heads, self.capacity, self.head_dim, 0 if lineage is None else self._lineage(lineage, "read"), beams,
+            at, until, batch, tokens, first_slot, k.data_ptr(), v.data_ptr(), _raw_stream(index))
+        if rc:
+            check(rc)
         return k, v
 
     def _lineage(self, lineage, what: str) -> int:
-        if lineage is None:
-            return 0
-        if (lineage.dtype is not torch.uint8 or lineage.shape != (self.slots, -(-self.capacity // _PAD) * _PAD) or not lineage.is_contiguous()
-                or lineage.device != self.device):
+        if (lineage.dtype is not _u8 or lineage.get_device() != self._index or lineage.shape != self._lineage_shape or not lineage.is_contiguous()):
             _refuse(f"{what}: lineage as new_lineage() makes it expected")
         return lineage.data_ptr()
 
@@ -150,33 +161,43 @@ def shared_prefix_attention(q: torch.Tensor, cache: QuantizedKvCache | None, len
     if given).  Either cache may be None.  A sequence without any position gives zeros.  ``beams``: sequences per prompt,
     by default sequences // len(prefix_lens), or all of them without a prefix.  ``max_len`` and ``max_prefix_len`` bound the lengths where
     the caller knows them better than the capacities: the work is shared out by them.  Returns [sequences, heads, head_dim]."""
-    if q.dim() != 3 or q.dtype not in (torch.float32, torch.float16):
+    dtype, shape = q.dtype, q.shape
+    if dtype is not _f32 and dtype is not _f16 or len(shape) != 3:
         _refuse("shared_prefix_attention: q [sequences, heads, head_dim] of f32 or f16 expected")
     one = cache if cache is not None else prefix
     if one is None:
         _refuse("shared_prefix_attention: neither a cache nor a prefix")
-    if prefix is not None and cache is not None and (prefix.dtype, prefix.kv_heads, prefix.head_dim, prefix.device) != (
-            cache.dtype, cache.kv_heads, cache.head_dim, cache.device):
+    index = one._index
+    if prefix is not None and cache is not None and (prefix._type != cache._type or prefix.kv_heads != cache.kv_heads or prefix.head_dim != cache.head_dim
+                                                     or prefix._index != index):
         _refuse("shared_prefix_attention: the two caches differ in format, heads or device")
-    batch, heads, d = q.shape
+    batch, heads, d = shape
     if (prefix is None) != (prefix_lens is None) or (cache is None) != (lens is None) or (lineage is not None and cache is None):
         _refuse("shared_prefix_attention: a cache and its lengths come together, lineage with a cache")
     if beams is None:
         beams = batch if prefix is None else batch // max(1, prefix_lens.shape[0])
-    beams = max(beams, 1)
-    if batch % beams or d != one.head_dim:
-        _refuse(f"shared_prefix_attention: {batch} sequences of head_dim {d}, {beams} a prompt, on a cache of head_dim {one.head_dim}")
-    q_stride = _rows(q, (batch, heads, d), one.device, "shared_prefix_attention: q")
-    out = torch.empty(batch, heads, d, dtype=q.dtype, device=q.device)
-    fn = lib().izwi_decode_shared_attention_f32 if q.dtype is torch.float32 else lib().izwi_decode_shared_attention_f16
-    p_args = (0, 0, 0, 0, 0) if prefix is None else (
-        prefix._ptr, prefix.slots, prefix.capacity, _ints(prefix_lens, batch // beams, one.device, "shared_prefix_attention: prefix_lens"),
-        prefix.capacity if max_prefix_len is None else max_prefix_len)
-    c_args = (0, 0, 0, 0, 0, 0) if cache is None else (
-        cache._ptr, cache.slots, cache.capacity, _ints(lens, batch, one.device, "shared_prefix_attention: lens"),
-        cache.capacity if max_len is None else max_len, cache._lineage(lineage, "shared_prefix_attention"))
-    _launch(fn, one.device, int(one.dtype), q.data_ptr(), q_stride, batch, beams, heads, one.kv_heads, d, *p_args, *c_args,
-            d ** -0.5 if scale is None else scale, out.data_ptr())
+    beams = beams or 1
+    if beams < 0 or batch % beams or d != one.head_dim or q.get_device() != index:
+        _refuse(f"shared_prefix_attention: {batch} sequences of head_dim {d}, {beams} a prompt, on a cache of head_dim {one.head_dim} on {one.device}")
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return shared_prefix_attention(q, cache, lens, prefix, prefix_lens, lineage, beams, scale, max_len, max_prefix_len)
+    p = p_slots = p_capacity = p_lens = c = c_slots = c_capacity = c_lens = c_lineage = 0
+    if prefix is not None:
+        p, p_slots, p_capacity = prefix._ptr, prefix.slots, prefix.capacity
+        p_lens = _ints(prefix_lens, batch // beams, index, "shared_prefix_attention: prefix_lens")
+    if cache is not None:
+        c, c_slots, c_capacity, c_lens = cache._ptr, cache.slots, cache.capacity, _ints(lens, batch, index, "shared_prefix_attention: lens")
+        if lineage is not None:
+            c_lineage = cache._lineage(lineage, "shared_prefix_attention")
+    whole = q.is_contiguous()
+    out = torch.empty_like(q) if whole else torch.empty(shape, dtype=dtype, device=q.device)
+    rc = _fn("shared_attention_f32" if dtype is _f32 else "shared_attention_f16")(
+        one._type, q.data_ptr(), heads * d if whole else _rows(q, "shared_prefix_attention: q"), batch, beams, heads, one.kv_heads, d, p, p_slots, p_capacity,
+        p_lens, p_capacity if max_prefix_len is None else max_prefix_len, c, c_slots, c_capacity, c_lens, c_capacity if max_len is None else max_len,
+        c_lineage, d ** -0.5 if scale is None else scale, out.data_ptr(), _raw_stream(index))
+    if rc:
+        check(rc)
     return out
 
 
@@ -196,31 +217,38 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: torch.Tens
     rising w * vocab + t; a beam marked in ``finished`` (uint8) keeps its score and its one candidate ``eos_token``.  ``lineage``
     [prompts * beams, n] uint8 and ``lens`` int32 [prompts * beams]: the new beams' lineage is their parents', with their own index
     at position lens[parent], where their next key and value go; into ``out_lineage`` (it may be ``lineage``) or a new tensor."""
-    if logits.dim() != 3 or logits.dtype is not torch.float32 or not logits.is_contiguous() or not logits.is_cuda:
+    shape = logits.shape
+    if len(shape) != 3 or logits.dtype is not _f32 or not logits.is_contiguous() or not logits.is_cuda:
         _refuse("beam_select: contiguous f32 logits [prompts, beams, vocab] on a GPU expected")
-    prompts, beams, vocab = logits.shape
-    device = logits.device
-    for t, dtype, what in ((scores, torch.float32, "scores"), (finished, torch.uint8, "finished")):
-        if t is not None and (t.dtype is not dtype or t.shape != (prompts, beams) or not t.is_contiguous() or t.device != device):
-            _refuse(f"beam_select: {what} [{prompts}, {beams}] of {dtype} expected")
-    if finished is not None and eos_token is None:
-        _refuse("beam_select: finished beams need an eos_token")
+    prompts, beams, vocab = shape
+    rows, index = shape[:2], logits.get_device()
+    if scores.dtype is not _f32 or scores.shape != rows or not scores.is_contiguous() or scores.get_device() != index:
+        _refuse(f"beam_select: scores [{prompts}, {beams}] of f32 expected")
+    if finished is not None:
+        if eos_token is None:
+            _refuse("beam_select: finished beams need an eos_token")
+        if finished.dtype is not _u8 or finished.shape != rows or not finished.is_contiguous() or finished.get_device() != index:
+            _refuse(f"beam_select: finished [{prompts}, {beams}] of uint8 expected")
     if (lineage is None) != (lens is None) or (lineage is None and out_lineage is not None):
         _refuse("beam_select: lineage and lens come together")
-    capacity = 0
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return beam_select(logits, scores, finished, eos_token, lineage, lens, out_lineage)
+    capacity = from_lineage = to_lineage = at = 0
     if lineage is not None:
         if out_lineage is None:
             out_lineage = torch.empty_like(lineage)
         capacity = lineage.shape[-1]
         for t in (lineage, out_lineage):
-            if (t.dtype is not torch.uint8 or t.shape != (prompts * beams, capacity) or capacity % _PAD or not t.is_contiguous()
-                    or t.device != device):
+            if t.dtype is not _u8 or t.shape != (prompts * beams, capacity) or capacity % _PAD or not t.is_contiguous() or t.get_device() != index:
                 _refuse("beam_select: lineage rows as QuantizedKvCache.new_lineage() makes them expected")
-    ints = torch.empty(2, prompts, beams, dtype=torch.int32, device=device)
-    scores_out, finished_out = torch.empty_like(scores), torch.empty(prompts, beams, dtype=torch.uint8, device=device)
-    tokens, parents = ints[0], ints[1]
-    _launch(lib().izwi_decode_beam_select_f32, device, logits.data_ptr(), prompts, beams, vocab, scores.data_ptr(),
-            0 if finished is None else finished.data_ptr(), -1 if eos_token is None else eos_token, tokens.data_ptr(), parents.data_ptr(),
-            scores_out.data_ptr(), finished_out.data_ptr(), 0 if lineage is None else lineage.data_ptr(), capacity,
-            _ints(lens, prompts * beams, device, "beam_select: lens"), 0 if lineage is None else out_lineage.data_ptr())
+        from_lineage, to_lineage, at = lineage.data_ptr(), out_lineage.data_ptr(), _ints(lens, prompts * beams, index, "beam_select: lens")
+    tokens = torch.empty(rows, dtype=_i32, device=logits.device)
+    parents, scores_out = torch.empty_like(tokens), torch.empty_like(scores)
+    finished_out = torch.empty(rows, dtype=_u8, device=logits.device) if finished is None else torch.empty_like(finished)
+    rc = _fn("beam_select_f32")(logits.data_ptr(), prompts, beams, vocab, scores.data_ptr(), 0 if finished is None else finished.data_ptr(),
+                                -1 if eos_token is None else eos_token, tokens.data_ptr(), parents.data_ptr(), scores_out.data_ptr(), finished_out.data_ptr(),
+                                from_lineage, capacity, at, to_lineage, _raw_stream(index))
+    if rc:
+        check(rc)
     return BeamStep(tokens, parents, scores_out, finished_out, out_lineage)
