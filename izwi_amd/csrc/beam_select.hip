@@ -50,13 +50,13 @@ __device__ __forceinline__ double double_of(uint64_t o) {
     return __longlong_as_double((long long)(o ^ ((int64_t)o < 0 ? 1ull << 63 : ~0ull)));
 }
 
-// The largest T that `k` lanes' values reach, bit by bit (0 where fewer lanes hold a value)
-template <typename U>
-__device__ __forceinline__ U kth_of_lanes(U v, int k) {
-    U t = 0;
+// Of the numbers whose last LOW bits are zero the largest that `k` lanes' values reach, bit by bit (0 where fewer lanes hold a value).
+template <int LOW>
+__device__ __forceinline__ uint32_t kth_of_lanes(uint32_t v, int k) {
+    uint32_t t = 0;
 #pragma unroll
-    for (int bit = 8 * (int)sizeof(U) - 1; bit >= 0; bit--) {
-        const U trial = t | (U)1 << bit;
+    for (int bit = 31; bit >= LOW; bit--) {
+        const uint32_t trial = t | 1u << bit;
         if (__popcll(__ballot(v >= trial)) >= k) t = trial;
     }
     return t;
@@ -97,97 +97,118 @@ __device__ __forceinline__ double exp_of(double d) {
 }
 
 constexpr int kChunkThreads = 256, kChunkRoom = 1024;
+struct ChunkShared {
+    uint64_t found[kChunkRoom];
+    double sum[4];
+    uint64_t best[4];
+    float top[4];
+    uint32_t threshold[4];
+    unsigned n_found;
+};
 
-// PER: logits of a thread
+// A chunk of a beam's row by 256 threads (tid; PER logits each): its maximum, sum and best candidates.  Every thread of the workgroup
+// calls it (barriers); without `on` it does nothing.
 template <int PER>
-__global__ __launch_bounds__(kChunkThreads) void beam_chunk_kernel(BeamParams P) {
+__device__ __forceinline__ void beam_chunk(const BeamParams& P, int row, int chunk, bool on, ChunkShared& S, int tid) {
     constexpr int kChunk = kChunkThreads * PER;
-    __shared__ float top[4];
-    __shared__ double sum[4];
-    __shared__ uint32_t threshold[4];
-    __shared__ uint64_t found[kChunkRoom];
-    __shared__ uint64_t best[4];
-    __shared__ unsigned n_found;
-    const int row = blockIdx.y, chunk = blockIdx.x, begin = chunk * kChunk, n = min(kChunk, P.vocab - begin);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int begin = chunk * kChunk, n = min(kChunk, P.vocab - begin), lane = tid & 63, wave = tid >> 6;
     uint64_t* keys = P.keys + ((int64_t)row * P.chunks + chunk) * P.beams;
     const float* x = P.logits + (int64_t)row * P.vocab + begin;
-    float v[PER];
+    float v[PER], m = -INFINITY;
+    if (on) {
+        if (n == kChunk) {
 #pragma unroll
-    for (int i = 0; i < PER; i++) v[i] = x[min(i * kChunkThreads + tid, n - 1)];
-    if (P.finished && P.finished[row]) return; // the second launch looks at neither
-    const float score = clean(P.scores[row]);
-    if (score == -INFINITY) { // every candidate of the beam is -infinity: the lowest tokens
-        if (tid < P.beams) keys[tid] = tid < n ? (uint64_t)order_of(-INFINITY) << 32 | ~(uint32_t)(begin + tid) : 0;
-        return;
-    }
-    if (tid == 0) n_found = 0;
-    float m = -INFINITY;
+            for (int i = 0; i < PER; i++) v[i] = x[tid + i * kChunkThreads];
+        } else {
 #pragma unroll
-    for (int i = 0; i < PER; i++) {
-        v[i] = i * kChunkThreads + tid < n ? clean(v[i]) : -INFINITY;
-        m = fmaxf(m, v[i]);
-    }
-    // the largest value that as many lanes reach as there are beams: that many of the chunk's logits are no smaller
-    const uint32_t kth = kth_of_lanes<uint32_t>(tid < n ? order_of(m) : 0, P.beams);
-    m = wave_max(m);
-    if (lane == 0) top[wave] = m, threshold[wave] = kth;
-    __syncthreads();
-    m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-    const uint32_t t = max(max(threshold[0], threshold[1]), max(threshold[2], threshold[3]));
-    const float least = t ? value_of(t) : -INFINITY;
-    const auto key_of = [&](int i) { return (uint64_t)order_of(v[i]) << 32 | ~(uint32_t)(begin + i * kChunkThreads + tid); };
-    unsigned passed = 0;
-#pragma unroll
-    for (int i = 0; i < PER; i++) passed |= v[i] >= least && i * kChunkThreads + tid < n ? 1u << i : 0u;
-    while (passed) { // (few)
-        const int i = __ffs(passed) - 1;
-        passed &= passed - 1;
-        float vi = v[0];
-#pragma unroll
-        for (int k = 1; k < PER; k++) vi = i == k ? v[k] : vi;
-        const unsigned at = atomicAdd(&n_found, 1u);
-        if (at < kChunkRoom) found[at] = (uint64_t)order_of(vi) << 32 | ~(uint32_t)(begin + i * kChunkThreads + tid);
-    }
-    double s = 0.0, s2 = 0.0; // (what is behind the end is -infinity: nothing)
-    const double md = m;
-#pragma unroll
-    for (int i = 0; i < PER; i += 2) s += exp_of((double)v[i] - md), s2 += exp_of((double)v[i + 1] - md);
-    s += s2;
-    if (m == -INFINITY) s = 0.0; // (no number)
-    s = wave_sum(s);
-    if (lane == 0) sum[wave] = s;
-    __syncthreads();
-    if (tid == 0) P.sums[(int64_t)row * P.chunks + chunk] = make_double2((double)m, sum[0] + sum[1] + sum[2] + sum[3]);
-    const int got = (int)n_found; // (in any order; the keys are all different)
-    if (got <= kChunkRoom) {
-        for (int i = tid; i < got; i += kChunkThreads) {
-            const uint64_t key = found[i];
-            int rank = 0;
-            for (int j = 0; j < got; j++) rank += found[j] > key;
-            if (rank < P.beams) keys[rank] = key;
+            for (int i = 0; i < PER; i++) v[i] = x[min(i * kChunkThreads + tid, n - 1)];
         }
-        if (tid >= got && tid < P.beams) keys[tid] = 0;
-        return;
+        if (P.finished && P.finished[row]) on = false; // its candidate comes from neither
     }
+    if (on && clean(P.scores[row]) == -INFINITY) { // every candidate of the beam is -infinity: the lowest tokens
+        if (tid < P.beams) keys[tid] = tid < n ? (uint64_t)order_of(-INFINITY) << 32 | ~(uint32_t)(begin + tid) : 0;
+        on = false;
+    }
+    if (tid == 0) S.n_found = 0;
+    if (on) {
+#pragma unroll
+        for (int i = 0; i < PER; i++) v[i] = clean(v[i]);
+        if (n != kChunk) {
+            asm volatile(""); // (a branch)
+#pragma unroll
+            for (int i = 0; i < PER; i++) v[i] = i * kChunkThreads + tid < n ? v[i] : -INFINITY;
+        }
+#pragma unroll
+        for (int i = 0; i < PER; i++) m = fmaxf(m, v[i]);
+        // the largest value that as many lanes reach as there are beams: that many of the chunk's logits are no smaller
+        // (to 12 bits of the mantissa: a threshold that lets a few more through, in fewer steps)
+        const uint32_t kth = kth_of_lanes<11>(tid < n ? order_of(m) : 0, P.beams);
+        m = wave_max(m);
+        if (lane == 0) S.top[wave] = m, S.threshold[wave] = kth;
+    }
+    __syncthreads();
+    const auto key_of = [&](int i) { return (uint64_t)order_of(v[i]) << 32 | ~(uint32_t)(begin + i * kChunkThreads + tid); };
+    if (on) {
+        m = fmaxf(fmaxf(S.top[0], S.top[1]), fmaxf(S.top[2], S.top[3]));
+        const uint32_t t = max(max(S.threshold[0], S.threshold[1]), max(S.threshold[2], S.threshold[3]));
+        // (the number of that order; an order below -infinity's is no float's)
+        const float least = t <= order_of(-INFINITY) ? -INFINITY : value_of(t);
+#pragma unroll
+        for (int i = 0; i < PER; i++)
+            if (v[i] >= least && i * kChunkThreads + tid < n) { // (few)
+                const unsigned at = atomicAdd(&S.n_found, 1u);
+                if (at < kChunkRoom) S.found[at] = key_of(i);
+            }
+        double s = 0.0, s2 = 0.0; // (what is behind the end is -infinity: nothing)
+        const double md = m;
+#pragma unroll
+        for (int i = 0; i < PER; i += 2) s += exp_of((double)v[i] - md), s2 += exp_of((double)v[i + 1] - md);
+        s = wave_sum(m == -INFINITY ? 0.0 : s + s2); // (no number: nothing)
+        if (lane == 0) S.sum[wave] = s;
+    }
+    __syncthreads();
+    const int got = on ? (int)S.n_found : 0; // (in any order; the keys are all different)
+    if (on) {
+        if (tid == 0) P.sums[(int64_t)row * P.chunks + chunk] = make_double2((double)m, S.sum[0] + S.sum[1] + S.sum[2] + S.sum[3]);
+        if (got <= kChunkRoom) {
+            for (int i = tid; i < got; i += kChunkThreads) {
+                const uint64_t key = S.found[i];
+                int rank = 0;
+                for (int j = 0; j < got; j++) rank += S.found[j] > key;
+                if (rank < P.beams) keys[rank] = key;
+            }
+            if (tid >= got && tid < P.beams) keys[tid] = 0;
+        }
+    }
+    if (!__syncthreads_or(got > kChunkRoom)) return;
     // a chunk of few different values: the largest, again and again
     uint64_t last = ~0ull;
     for (int k = 0; k < P.beams; k++) {
         uint64_t mine = 0;
+        if (on) {
 #pragma unroll
-        for (int i = 0; i < PER; i++)
-            if (i * kChunkThreads + tid < n && key_of(i) < last) mine = max(mine, key_of(i));
+            for (int i = 0; i < PER; i++)
+                if (i * kChunkThreads + tid < n && key_of(i) < last) mine = max(mine, key_of(i));
+        }
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) mine = max(mine, (uint64_t)__shfl_xor((unsigned long long)mine, o));
         __syncthreads();
-        if (lane == 0) best[wave] = mine;
+        if (lane == 0) S.best[wave] = mine;
         __syncthreads();
-        last = max(max(best[0], best[1]), max(best[2], best[3]));
-        if (tid == 0) keys[k] = last;
+        last = max(max(S.best[0], S.best[1]), max(S.best[2], S.best[3]));
+        if (tid == 0 && got > kChunkRoom) keys[k] = last;
     }
+    __syncthreads();
+}
+
+template <int PER>
+__global__ __launch_bounds__(kChunkThreads) void beam_chunk_kernel(BeamParams P) {
+    __shared__ ChunkShared S;
+    beam_chunk<PER>(P, blockIdx.y, blockIdx.x, true, S, threadIdx.x);
 }
 
 constexpr int kPickThreads = 1024, kPickRoom = 4096, kPickKept = 4; // candidates that a thread keeps in registers
+constexpr int kAheadWords = 4096;                                   // of the lineage, read before they are needed
 
 struct Candidate {
     uint64_t score; // order of the score
@@ -195,6 +216,8 @@ struct Candidate {
 };
 __device__ __forceinline__ bool before(const Candidate& a, const Candidate& b) { return a.score > b.score || (a.score == b.score && a.flat < b.flat); }
 
+// PER > 0: the chunks too, four at a time
+template <int PER>
 __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(BeamParams P) {
     __shared__ double offset[kMaxBeams]; // of a beam's logits: score - logsumexp
     __shared__ uint8_t ended[kMaxBeams];
@@ -210,6 +233,27 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(BeamParams P) {
     const int prompt = blockIdx.x, W = P.beams, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t row0 = (int64_t)prompt * W;
     const int per_beam = P.chunks * W, total = W * per_beam;
+    // a lineage that fits is on its way from the start
+    const int words = (int)(P.padded / 4);
+    const bool ahead = P.lineage_out && W * words <= kAheadWords;
+    const uint32_t* in = reinterpret_cast<const uint32_t*>(P.lineage + row0 * P.padded);
+    uint32_t early[kAheadWords / kPickThreads];
+    int len = 0;
+    if (ahead) {
+#pragma unroll
+        for (int i = 0; i < kAheadWords / kPickThreads; i++) early[i] = in[min(tid + i * kPickThreads, W * words - 1)];
+        len = P.lens[row0 + min(tid, W - 1)];
+    }
+    if constexpr (PER > 0) {
+        static_assert(4 * sizeof(ChunkShared) <= sizeof(room));
+        ChunkShared* S = reinterpret_cast<ChunkShared*>(room);
+        const int group = tid / kChunkThreads;
+        for (int c0 = 0; c0 < W * P.chunks; c0 += kPickThreads / kChunkThreads) {
+            const int c = min(c0 + group, W * P.chunks - 1), w = c / P.chunks;
+            beam_chunk<PER>(P, (int)row0 + w, c - w * P.chunks, c0 + group < W * P.chunks, S[group], tid % kChunkThreads);
+        }
+        __syncthreads();
+    }
     // the first candidates are requested before the sums are joined
     uint64_t kept[kPickKept];
     const uint64_t* all_keys = P.keys + row0 * per_beam;
@@ -258,7 +302,7 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(BeamParams P) {
 #pragma unroll
     for (int c = 0; c < kPickKept; c++) mine[c] = candidate(tid + c * kPickThreads, kept[c]), most = max(most, coarse(mine[c]));
     for (int i = tid + kPickKept * kPickThreads; i < total; i += kPickThreads) most = max(most, coarse(candidate(i, all_keys[i])));
-    const uint32_t kth = kth_of_lanes<uint32_t>(most, W);
+    const uint32_t kth = kth_of_lanes<0>(most, W);
     if (lane == 0) thresholds[wave] = kth;
     __syncthreads();
     uint32_t t = 1;
@@ -314,10 +358,29 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(BeamParams P) {
         if (P.finished_out) P.finished_out[row0 + tid] = ended[parent] || (int64_t)token == P.eos;
     }
     if (!P.lineage_out) return;
-    // the rows in pieces that fit the LDS, read whole before they are written (lineage_out may be lineage)
-    const uint32_t* in = reinterpret_cast<const uint32_t*>(P.lineage + row0 * P.padded);
     uint32_t* out = reinterpret_cast<uint32_t*>(P.lineage_out + row0 * P.padded);
-    const int words = (int)(P.padded / 4), piece = min(words, 3 * kPickRoom / W);
+    // word `word` of the new beam's row: its parent's, with the beam itself at the parent's length
+    const auto successor = [&](uint32_t four, int beam, int word, int at) {
+        return at >= 0 && at >> 2 == word ? (four & ~(255u << (8 * (at & 3)))) | (uint32_t)beam << (8 * (at & 3)) : four;
+    };
+    if (ahead) {
+        __syncthreads(); // (room has been read)
+#pragma unroll
+        for (int i = 0; i < kAheadWords / kPickThreads; i++)
+            if (tid + i * kPickThreads < W * words) room[tid + i * kPickThreads] = early[i];
+        if (tid < W) room[kAheadWords + tid] = (uint32_t)len;
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < kAheadWords / kPickThreads; n++) {
+            const int i = tid + n * kPickThreads;
+            if (i >= W * words) break;
+            const int beam = i / words, word = i - beam * words, parent = (int)(picked[beam] / (uint32_t)P.vocab);
+            out[i] = successor(room[parent * words + word], beam, word, (int)room[kAheadWords + parent]);
+        }
+        return;
+    }
+    // longer ones in pieces that fit the LDS, read whole before they are written (lineage_out may be lineage)
+    const int piece = min(words, 3 * kPickRoom / W);
     for (int from = 0; from < words; from += piece) {
         const int width = min(piece, words - from), all = W * width;
         __syncthreads();
@@ -325,10 +388,7 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(BeamParams P) {
         __syncthreads();
         for (int i = tid; i < all; i += kPickThreads) {
             const int beam = i / width, word = from + i % width, parent = (int)(picked[beam] / (uint32_t)P.vocab);
-            uint32_t four = room[parent * width + i % width];
-            const int at = P.lens[row0 + parent];
-            if (at >= 0 && at >> 2 == word) four = (four & ~(255u << (8 * (at & 3)))) | (uint32_t)beam << (8 * (at & 3));
-            out[(int64_t)beam * words + word] = four;
+            out[(int64_t)beam * words + word] = successor(room[parent * width + i % width], beam, word, P.lens[row0 + parent]);
         }
     }
 }
@@ -361,8 +421,10 @@ int izwi_decode_beam_select_f32(const float* logits, int64_t prompts, int64_t be
     hipStream_t stream = (hipStream_t)stream_;
     BeamParams P{logits, scores, finished, tokens, parents, scores_out, finished_out, lineage, lineage_out, lens, nullptr, nullptr, (int)beams, (int)vocab,
                  0, eos_token, kv_padded(lineage_capacity)};
-    // 4096 logits to a workgroup, 2048 where that leaves fewer than two workgroups to a compute unit
-    const bool small = prompts * beams * ((vocab + 4095) / 4096) < 2 * n_cus;
+    // 4096 logits to a workgroup, 2048 where that leaves fewer than two workgroups to a compute unit; up to eight such chunks of a prompt are
+    // taken by the second launch itself, one launch in all
+    const int64_t chunks = beams * ((vocab + 4095) / 4096);
+    const bool one_launch = chunks <= 8, small = !one_launch && prompts * chunks < 2 * n_cus;
     const int chunk = small ? 2048 : 4096;
     P.chunks = (int)((vocab + chunk - 1) / chunk);
     const size_t parts = (size_t)prompts * beams * P.chunks;
@@ -370,11 +432,16 @@ int izwi_decode_beam_select_f32(const float* logits, int64_t prompts, int64_t be
     KV_TRY(qmm_get_scratch(device, stream, parts * (sizeof(double2) + (size_t)beams * sizeof(uint64_t)), &scratch));
     P.sums = static_cast<double2*>(scratch);
     P.keys = reinterpret_cast<uint64_t*>(P.sums + parts);
+    if (one_launch) {
+        beam_pick_kernel<16><<<(unsigned)prompts, kPickThreads, 0, stream>>>(P);
+        KV_TRY(hipGetLastError());
+        return IZWI_QMM_OK;
+    }
     const dim3 grid((unsigned)P.chunks, (unsigned)(prompts * beams));
     if (small) beam_chunk_kernel<8><<<grid, kChunkThreads, 0, stream>>>(P);
     else beam_chunk_kernel<16><<<grid, kChunkThreads, 0, stream>>>(P);
     KV_TRY(hipGetLastError());
-    beam_pick_kernel<<<(unsigned)prompts, kPickThreads, 0, stream>>>(P);
+    beam_pick_kernel<0><<<(unsigned)prompts, kPickThreads, 0, stream>>>(P);
     KV_TRY(hipGetLastError());
     return IZWI_QMM_OK;
     });
