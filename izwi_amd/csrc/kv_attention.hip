@@ -56,7 +56,7 @@ struct AttendParams {
     int max_prefix, max_len; // 0: no such positions
     float scale;
     // workgroups: prefix_wgs of prefix_units (prompt, kv head, split) times prefix_z tiles of rows, then the same of (sequence, ..)
-    int prefix_splits, prefix_units, prefix_z, prefix_wgs, own_splits, own_units, own_z;
+    int prefix_splits, prefix_units, prefix_z, prefix_wgs, own_splits, own_units, own_z, own_solo;
     Divisor by_group, by_kv_heads, by_beams, by_prefix_splits, by_own_splits, by_prefix_z, by_own_z;
     int parts;     // partial results of a row: prefix_splits + own_splits
     float* sums;   // [batch * heads][parts][D]
@@ -123,18 +123,26 @@ __device__ __forceinline__ void value_pair(const Words<N> (&v)[2], int b, h8& fi
 constexpr int kWaves = 4; // of a workgroup
 constexpr float kRise = 10.0f, kHead = 5.0f; // powers of two, see above
 
-template <typename T, int QT, int D, int RT, bool SHARED, bool LIN>
+template <typename T, int QT, int D, int RT, bool SHARED, bool LIN, bool SOLO = false>
 __device__ __forceinline__ void attend_rows(const AttendParams& P, int id, float* lds) {
     using Row = KvRow<QT, D>;
     constexpr int NB = Row::kBlocks, KW = Row::kBytes / 16, VW = Row::kLane, ROWS = 16 * RT;
     constexpr bool SPLIT = sizeof(T) == 4, TWO = RT == 1 && !LIN;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int x = lane & 15, g = lane >> 4;
+    // SOLO: every wave has a unit of its own, and nothing to meet for
+    constexpr int kStep = SOLO ? 1 : kWaves;
 
-    // what this workgroup works on
+    // what this workgroup (wave) works on
     const int Z = SHARED ? P.prefix_z : P.own_z, splits = SHARED ? P.prefix_splits : P.own_splits;
-    const int eighth = (SHARED ? P.by_prefix_z : P.by_own_z).of(id >> 3);
-    const int unit = eighth * 8 + (id & 7), z = (id >> 3) - eighth * Z; // tiles of the same positions on one XCD
+    int unit, z;
+    if constexpr (SOLO) {
+        const int n = id * kWaves + wave;
+        unit = P.by_own_z.of(n), z = n - unit * Z;
+    } else { // tiles of the same positions on one XCD
+        const int eighth = (SHARED ? P.by_prefix_z : P.by_own_z).of(id >> 3);
+        unit = eighth * 8 + (id & 7), z = (id >> 3) - eighth * Z;
+    }
     if (unit >= (SHARED ? P.prefix_units : P.own_units)) return;
     const int of_split = (SHARED ? P.by_prefix_splits : P.by_own_splits).of(unit), split = unit - of_split * splits;
     const int seq = P.by_kv_heads.of(of_split), kvh = of_split - seq * P.kv_heads;
@@ -149,10 +157,11 @@ __device__ __forceinline__ void attend_rows(const AttendParams& P, int id, float
     };
     const int rows_here = min(ROWS, n_rows - z * ROWS);
     if (first >= last) { // nothing to add
+        const int me = SOLO ? lane : threadIdx.x;
         if (P.parts == 1) {
-            for (int i = threadIdx.x; i < rows_here * D; i += (64 * kWaves)) static_cast<T*>(P.out)[row_index(i / D) * D + i % D] = (T)0.0f;
-        } else if ((int)threadIdx.x < rows_here) {
-            P.stats[row_index(threadIdx.x) * P.parts + part] = make_float2(-INFINITY, 0.0f);
+            for (int i = me; i < rows_here * D; i += 64 * kStep) static_cast<T*>(P.out)[row_index(i / D) * D + i % D] = (T)0.0f;
+        } else if (me < rows_here) {
+            P.stats[row_index(me) * P.parts + part] = make_float2(-INFINITY, 0.0f);
         }
         return;
     }
@@ -239,13 +248,13 @@ __device__ __forceinline__ void attend_rows(const AttendParams& P, int id, float
     Keys keys[TWO ? 2 : 1];
     Values vals[TWO ? 2 : 1];
     Scales scales[2];
-    int tile = first + wave;
+    int tile = first + (SOLO ? 0 : wave);
     const bool any = tile < last;
     if (any) {
         load_lineage(tile);
         load_keys(keys[0], scales[0], tile);
         load_values(vals[0], scales[0], tile);
-        load_lineage(min(tile + kWaves, last - 1));
+        load_lineage(min(tile + kStep, last - 1));
     }
 
     // The queries: lane (x, g) holds of row x the values 8 g .. of every block.  f32 ones are scaled by a power of two to
@@ -448,35 +457,57 @@ __device__ __forceinline__ void attend_rows(const AttendParams& P, int id, float
     if (any) {
         if constexpr (TWO) { // two sets of registers in turns: a tile is requested before the one in front of it is worked on
             for (;;) {
-                load_keys(keys[1], scales[1], min(tile + kWaves, last - 1));
-                load_values(vals[1], scales[1], min(tile + kWaves, last - 1));
-                load_lineage(min(tile + 2 * kWaves, last - 1));
+                load_keys(keys[1], scales[1], min(tile + kStep, last - 1));
+                load_values(vals[1], scales[1], min(tile + kStep, last - 1));
+                load_lineage(min(tile + 2 * kStep, last - 1));
                 scores(keys[0]);
                 weights(scales[0], tile);
                 products(vals[0], scales[0]);
-                tile += kWaves;
+                tile += kStep;
                 if (tile >= last) break;
-                load_keys(keys[0], scales[0], min(tile + kWaves, last - 1));
-                load_values(vals[0], scales[0], min(tile + kWaves, last - 1));
-                load_lineage(min(tile + 2 * kWaves, last - 1));
+                load_keys(keys[0], scales[0], min(tile + kStep, last - 1));
+                load_values(vals[0], scales[0], min(tile + kStep, last - 1));
+                load_lineage(min(tile + 2 * kStep, last - 1));
                 scores(keys[1]);
                 weights(scales[1], tile);
                 products(vals[1], scales[1]);
-                tile += kWaves;
+                tile += kStep;
                 if (tile >= last) break;
             }
         } else { // one set: keys are requested when the last ones have been used, so are values
-            for (; tile < last; tile += kWaves) {
-                const int next = min(tile + kWaves, last - 1);
+            for (; tile < last; tile += kStep) {
+                const int next = min(tile + kStep, last - 1);
                 scores(keys[0]);
                 load_keys(keys[0], scales[1], next);
-                load_lineage(min(tile + 2 * kWaves, last - 1));
+                load_lineage(min(tile + 2 * kStep, last - 1));
                 weights(scales[0], tile);
                 products(vals[0], scales[0]);
                 load_values(vals[0], scales[1], next);
                 scales[0] = scales[1];
             }
         }
+    }
+    if constexpr (SOLO) { // lane (x, g) has of row x and block b the values 8 g .. 8 g + 7
+        static_assert(RT == 1);
+        const float sum = qmm_add_lane32(qmm_add_lane16(l[0])), by = 1.0f / up, inv = by / sum;
+        if (x >= rows_here) return;
+        const int64_t row = row_index(x);
+        if (P.parts > 1 && g == 0) P.stats[row * P.parts + part] = make_float2(ref[0], sum);
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            const f4 a = o[0][2 * b], c = o[0][2 * b + 1];
+            const float v[8] = {a[0], c[0], a[1], c[1], a[2], c[2], a[3], c[3]};
+            if (P.parts > 1) {
+                float* dst = P.sums + (row * P.parts + part) * D + 32 * b + 8 * g;
+#pragma unroll
+                for (int i = 0; i < 8; i++) dst[i] = v[i] * by;
+            } else {
+                T* dst = static_cast<T*>(P.out) + row * D + 32 * b + 8 * g;
+#pragma unroll
+                for (int i = 0; i < 8; i++) dst[i] = (T)(ref[0] == -INFINITY ? 0.0f : v[i] * inv);
+            }
+        }
+        return;
     }
     // the waves' results meet in LDS; lane (x, g) has of block b the values 8 g .. 8 g + 7 of row x
     float2* stat = reinterpret_cast<float2*>(lds + kWaves * ROWS * (D + 4));
@@ -547,27 +578,30 @@ __global__ __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) void attend_kernel(A
     extern __shared__ __attribute__((aligned(16))) float lds[]; // see the end of attend_rows
     const int id = blockIdx.x;
     if (id < P.prefix_wgs) attend_rows<T, QT, D, RT, true, false>(P, id, lds);
+    else if (P.own_solo) attend_rows<T, QT, D, 1, false, LIN, true>(P, id - P.prefix_wgs, lds);
     else attend_rows<T, QT, D, 1, false, LIN>(P, id - P.prefix_wgs, lds);
 }
 
-// A row's parts joined: a workgroup per row, its four waves take the parts in turn.  Statistics and sums are requested together, eight
-// parts a wave at a time; what a part did not write (no position of the row) is in its place and not looked at.
-template <typename T, int D>
-__global__ __launch_bounds__(256) void attend_join_kernel(const float* __restrict__ sums, const float2* __restrict__ stats, T* __restrict__ out, int parts) {
-    constexpr int N = D / 64, A = 8;
+// A row's parts joined: by a wave where there are at most eight (FEW), by the four waves of a workgroup in turn where there are more.
+// Statistics and sums are requested together, eight parts a wave at a time; what a part did not write (no position of the row) is in its
+// place and not looked at.
+template <typename T, int D, bool FEW>
+__global__ __launch_bounds__(256) void attend_join_kernel(const float* __restrict__ sums, const float2* __restrict__ stats, T* __restrict__ out, int parts,
+                                                          int64_t rows) {
+    constexpr int N = D / 64, A = 8, STEP = FEW ? 1 : 4;
     typedef float vec __attribute__((ext_vector_type(N)));
-    __shared__ float red[4][D + 2];
-    const int64_t row = blockIdx.x;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t row = FEW ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
+    if (FEW && row >= rows) return;
     stats += row * parts, sums += row * parts * D + lane * N;
     float to = -INFINITY, sum = 0.0f; // of this wave's parts so far
     vec a = 0.0f;
-    for (int p0 = wave; p0 < parts; p0 += 4 * A) {
+    for (int p0 = FEW ? 0 : wave; p0 < parts; p0 += STEP * A) {
         vec v[A];
-        const int mine = p0 + 4 * (lane & (A - 1)); // lane i of eight: the statistics of part i
+        const int mine = p0 + STEP * (lane & (A - 1)); // lane i of eight: the statistics of part i
         const float2 st = stats[min(mine, parts - 1)];
 #pragma unroll
-        for (int i = 0; i < A; i++) v[i] = *reinterpret_cast<const vec*>(sums + (int64_t)min(p0 + 4 * i, parts - 1) * D);
+        for (int i = 0; i < A; i++) v[i] = *reinterpret_cast<const vec*>(sums + (int64_t)min(p0 + STEP * i, parts - 1) * D);
         const float ref = mine < parts ? st.x : -INFINITY;
         float most = ref;
         most = fmaxf(most, dpp_f<0xB1>(most));
@@ -584,6 +618,13 @@ __global__ __launch_bounds__(256) void attend_join_kernel(const float* __restric
         }
         to = next;
     }
+    if constexpr (FEW) {
+        T* dst = out + row * D + lane * N;
+#pragma unroll
+        for (int i = 0; i < N; i++) dst[i] = (T)(to == -INFINITY ? 0.0f : a[i] / sum);
+        return;
+    }
+    __shared__ float red[4][D + 2];
 #pragma unroll
     for (int i = 0; i < N; i++) red[wave][lane * N + i] = a[i];
     if (lane == 0) red[wave][D] = sum, red[wave][D + 1] = to;
@@ -603,7 +644,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(const float* __restric
 
 template <typename T, int QT, int D>
 hipError_t launch_attend_of(const AttendParams& P, int rt, hipStream_t stream) {
-    const unsigned wgs = (unsigned)(P.prefix_wgs + (P.own_units + 7) / 8 * 8 * P.own_z);
+    const unsigned wgs = (unsigned)(P.prefix_wgs + (P.own_solo ? ((int64_t)P.own_units * P.own_z + kWaves - 1) / kWaves : (int64_t)(P.own_units + 7) / 8 * 8 * P.own_z));
     const size_t lds = (size_t)16 * rt * (kWaves * ((D + 4) * sizeof(float) + sizeof(float2)) + sizeof(f4) + sizeof(float) + sizeof(int64_t));
     const auto run = [&](auto kernel) {
         if (lds > 64 * 1024) {
@@ -618,7 +659,9 @@ hipError_t launch_attend_of(const AttendParams& P, int rt, hipStream_t stream) {
     if (P.lineage) e = rt == 1 ? run(attend_kernel<T, QT, D, 1, true>) : run(attend_kernel<T, QT, D, R2, true>);
     else e = rt == 1 ? run(attend_kernel<T, QT, D, 1, false>) : run(attend_kernel<T, QT, D, R2, false>);
     if (e != hipSuccess || P.parts == 1) return e;
-    attend_join_kernel<T, D><<<(unsigned)(P.batch * P.heads), 256, 0, stream>>>(P.sums, P.stats, static_cast<T*>(P.out), P.parts);
+    const int64_t rows = (int64_t)P.batch * P.heads;
+    if (P.parts <= 8) attend_join_kernel<T, D, true><<<(unsigned)((rows + 3) / 4), 256, 0, stream>>>(P.sums, P.stats, static_cast<T*>(P.out), P.parts, rows);
+    else attend_join_kernel<T, D, false><<<(unsigned)rows, 256, 0, stream>>>(P.sums, P.stats, static_cast<T*>(P.out), P.parts, rows);
     return hipGetLastError();
 }
 template <typename T>
@@ -701,6 +744,10 @@ int shared_attention_impl(int type, const T* q, int64_t q_stride, int64_t batch,
     const int rt = d <= 128 && prompt_rows > 16 && turns(batch / beams, P.max_prefix, prompt_rows, 2) >= 8 ? 2 : 1;
     units(batch / beams, P.max_prefix, prompt_rows, rt, P.prefix_splits, P.prefix_units, P.prefix_z);
     units(batch, P.max_len, P.group, 1, P.own_splits, P.own_units, P.own_z);
+    // A wave to each where that still fills the compute units, the better the shorter they are: a workgroup's prologue, its meeting in LDS and
+    // its idle waves cost more than the positions of a short sequence (371 sequences of up to 14 own positions behind 570, 32 heads on 8: 53 ->
+    // 40 us; but 132 of up to 355: 28 -> 30).
+    P.own_solo = P.own_splits == 1 && (int64_t)P.own_units * P.own_z >= kWaves * n_cus * std::max<int64_t>(1, (P.max_len + 31) / 32 / 4);
     P.prefix_wgs = (P.prefix_units + 7) / 8 * 8 * P.prefix_z;
     P.parts = P.prefix_splits + P.own_splits;
     if (P.parts == 0) { // bounds of zero: zeros
