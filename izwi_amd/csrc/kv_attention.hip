@@ -21,6 +21,7 @@
 #include "kv_cache.h"
 
 #include <algorithm>
+#include <cmath>
 
 #include "qmm_lanes.h"
 
@@ -303,9 +304,13 @@ __device__ __forceinline__ void attend_rows(const AttendParams& P, int id, float
     // of the lane's row: the maximum that the reference stands on, the product that makes a new one, the reference, this lane's sum of weights
     float top[RT], bar[RT], ref[RT], l[RT];
     f4 o[RT][2 * NB];
-    int e_run = -24;        // 2^(e_run + 1) is above every value scale so far; as f16 bits:
-    uint32_t e_bits = 2;
-    float up = 32768.0f;    // what the value scales are multiplied by: to below 1
+    // Of each block of the head: what its value scales are multiplied by, the power of two that takes the largest so far to below 1 (2^15 at most).
+    // A lane has it for the blocks of its value scales, and as f16 bits the scale that needs another.
+    float up[SW];
+    uint32_t e_bits[SW];
+    auto up_of = [&](auto b) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(up[b % SW]), b / SW)); };
+#pragma unroll
+    for (int i = 0; i < SW; i++) up[i] = 32768.0f, e_bits[i] = 0x200;
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
         top[rt] = bar[rt] = ref[rt] = -INFINITY, l[rt] = 0.0f;
@@ -360,10 +365,12 @@ __device__ __forceinline__ void attend_rows(const AttendParams& P, int id, float
             }
         }
         // does a row's maximum, or the values' largest scale, rise?
-        u2 most = magnitudes<QT>(t.s.w[0]);
+        bool rise = false;
 #pragma unroll
-        for (int i = 1; i < SW; i++) most = __builtin_elementwise_max(most, magnitudes<QT>(t.s.w[i]));
-        bool rise = max((uint32_t)most[0], (uint32_t)most[1]) >= e_bits;
+        for (int i = 0; i < SW; i++) {
+            const u2 most = magnitudes<QT>(t.s.w[i]);
+            rise |= max((uint32_t)most[0], (uint32_t)most[1]) >= e_bits[i];
+        }
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) {
             float m = s[rt][0];
@@ -372,30 +379,31 @@ __device__ __forceinline__ void attend_rows(const AttendParams& P, int id, float
             rise |= m > bar[rt];
         }
         if (__any(rise)) {
-            float d = 0.0f;
+            float down[SW]; // of what is there
 #pragma unroll
-            for (int i = 0; i < SW; i++) { // (fmaxf passes over the NaN of a block that holds one)
+            for (int i = 0; i < SW; i++) {
                 const h2 two = __builtin_bit_cast(h2, magnitudes<QT>(t.s.w[i]));
-                d = fmaxf(d, fmaxf((float)two[0], (float)two[1]));
-            }
+                float d = fmaxf(0.0f, fmaxf((float)two[0], (float)two[1])); // (passes over the NaN of a block that holds one)
 #pragma unroll
-            for (int i = 1; i < 16; i *= 2) d = fmaxf(d, __shfl_xor(d, i));
-            e_run = max(e_run, (int)(__float_as_uint(qmm_max_lane_rows(d)) >> 23) - 127);
-            e_run = __builtin_amdgcn_readfirstlane(e_run);
-            const float old_up = up;
-            up = __uint_as_float((uint32_t)(127 + min(15, -1 - e_run)) << 23);
-            e_bits = __builtin_bit_cast(uint16_t, (f16_t)__uint_as_float((uint32_t)(e_run + 128) << 23));
+                for (int n = VL; n < 16; n *= 2) d = fmaxf(d, __shfl_xor(d, n));
+                const int e = (int)(__float_as_uint(qmm_max_lane_rows(d)) >> 23) - 127;
+                const float to = fminf(up[i], __uint_as_float((uint32_t)(127 + min(15, -1 - e)) << 23));
+                down[i] = to / up[i], up[i] = to;
+                e_bits[i] = __builtin_bit_cast(uint16_t, (f16_t)(1.0f / to)); // (1 / 2^-16: infinity's)
+            }
 #pragma unroll
             for (int rt = 0; rt < RT; rt++) {
                 float m = s[rt][0];
 #pragma unroll
                 for (int j = 1; j < 8; j++) m = fmaxf(m, s[rt][j]);
                 top[rt] = fmaxf(top[rt], qmm_max_lane_rows(m) * factor[rt]);
-                bar[rt] = (top[rt] + kRise) / factor[rt];
-                const float to = top[rt] - kHead, by = ref[rt] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ref[rt] - to), by_o = by * (up / old_up);
+                bar[rt] = (top[rt] + (kRise - fabsf(top[rt]) * 0x1p-22f)) / factor[rt]; // (less what rounding may add)
+                const float to = top[rt] - kHead, by = ref[rt] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ref[rt] - to);
                 ref[rt] = to, l[rt] *= by;
-#pragma unroll
-                for (int i = 0; i < 2 * NB; i++) o[rt][i] *= by_o;
+                each<NB>([&](auto b) {
+                    const float by_o = by * __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(down[b % SW]), b / SW));
+                    o[rt][2 * b] *= by_o, o[rt][2 * b + 1] *= by_o;
+                });
             }
         }
         // weights
@@ -404,7 +412,8 @@ __device__ __forceinline__ void attend_rows(const AttendParams& P, int id, float
             const float from = ref[rt] == -INFINITY ? 0.0f : -ref[rt];
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                s[rt][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rt][j], factor[rt], from));
+                // (not fused: where scores are so large that the reference is rounded, the largest product has to round like it)
+                s[rt][j] = __builtin_amdgcn_exp2f(s[rt][j] * factor[rt] + from);
                 l[rt] += s[rt][j];
             }
         }
@@ -416,10 +425,9 @@ __device__ __forceinline__ void attend_rows(const AttendParams& P, int id, float
             for (int h = 0; h < 2; h++)
 #pragma unroll
                 for (int i = 0; i < VW; i++) t.v[h].w[i] = (t.v[h].w[i] & 0xffffu) | (t.w[h].w[i] & 0xffff0000u);
-        const f16_t by = (f16_t)up;
         uint32_t scale[SW];
 #pragma unroll
-        for (int i = 0; i < SW; i++) scale[i] = __builtin_bit_cast(uint32_t, as_h2(sc.s.w[i]) * h2{by, by});
+        for (int i = 0; i < SW; i++) scale[i] = __builtin_bit_cast(uint32_t, as_h2(sc.s.w[i]) * h2{(f16_t)up[i], (f16_t)up[i]});
         h2 ph[RT][4], pl[SPLIT ? RT : 1][4];
 #pragma unroll
         for (int rt = 0; rt < RT; rt++)
@@ -489,14 +497,15 @@ __device__ __forceinline__ void attend_rows(const AttendParams& P, int id, float
     }
     if constexpr (SOLO) { // lane (x, g) has of row x and block b the values 8 g .. 8 g + 7
         static_assert(RT == 1);
-        const float sum = qmm_add_lane32(qmm_add_lane16(l[0])), by = 1.0f / up, inv = by / sum;
+        const float sum = qmm_add_lane32(qmm_add_lane16(l[0])), inv = 1.0f / sum;
+        float down[NB];
+        each<NB>([&](auto b) { down[b] = 1.0f / up_of(b); });
         if (x >= rows_here) return;
         const int64_t row = row_index(x);
         if (P.parts > 1 && g == 0) P.stats[row * P.parts + part] = make_float2(ref[0], sum);
-#pragma unroll
-        for (int b = 0; b < NB; b++) {
+        each<NB>([&](auto b) {
             const f4 a = o[0][2 * b], c = o[0][2 * b + 1];
-            const float v[8] = {a[0], c[0], a[1], c[1], a[2], c[2], a[3], c[3]};
+            const float v[8] = {a[0], c[0], a[1], c[1], a[2], c[2], a[3], c[3]}, by = down[b];
             if (P.parts > 1) {
                 float* dst = P.sums + (row * P.parts + part) * D + 32 * b + 8 * g;
 #pragma unroll
@@ -504,9 +513,9 @@ __device__ __forceinline__ void attend_rows(const AttendParams& P, int id, float
             } else {
                 T* dst = static_cast<T*>(P.out) + row * D + 32 * b + 8 * g;
 #pragma unroll
-                for (int i = 0; i < 8; i++) dst[i] = (T)(ref[0] == -INFINITY ? 0.0f : v[i] * inv);
+                for (int i = 0; i < 8; i++) dst[i] = (T)(ref[0] == -INFINITY ? 0.0f : v[i] * (by * inv));
             }
-        }
+        });
         return;
     }
     // the waves' results meet in LDS; lane (x, g) has of block b the values 8 g .. 8 g + 7 of row x
@@ -514,12 +523,12 @@ __device__ __forceinline__ void attend_rows(const AttendParams& P, int id, float
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
         float* dst = lds + (wave * ROWS + 16 * rt + x) * (D + 4) + 8 * g;
-#pragma unroll
-        for (int b = 0; b < NB; b++) {
-            const f4 a = o[rt][2 * b] * (1.0f / up), c = o[rt][2 * b + 1] * (1.0f / up);
+        each<NB>([&](auto b) {
+            const float by = 1.0f / up_of(b);
+            const f4 a = o[rt][2 * b] * by, c = o[rt][2 * b + 1] * by;
             *reinterpret_cast<f4*>(dst + 32 * b) = f4{a[0], c[0], a[1], c[1]};
             *reinterpret_cast<f4*>(dst + 32 * b + 4) = f4{a[2], c[2], a[3], c[3]};
-        }
+        });
         const float sum = qmm_add_lane32(qmm_add_lane16(l[rt]));
         if (g == 0) stat[wave * ROWS + 16 * rt + x] = make_float2(ref[rt], sum);
     }
@@ -698,6 +707,7 @@ int shared_attention_impl(int type, const T* q, int64_t q_stride, int64_t batch,
         return qmm_fail(IZWI_QMM_ERR_UNSUPPORTED, "%s: %lld sequences of %lld heads", what, (long long)batch, (long long)heads);
     if (lineage && (beams > 255 || !cache))
         return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: lineage of %lld beams (at most 255, of a cache)", what, (long long)beams);
+    if (!std::isfinite(scale)) return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: scale %g", what, (double)scale);
     if (batch == 0) return IZWI_QMM_OK;
     if (!prefix && !cache) return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: neither a prefix nor a cache", what);
     if (!q || !out || (prefix && !prefix_lens) || (cache && !lens)) return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: NULL buffer", what);

@@ -274,6 +274,73 @@ def test_attention_of_nan_positions(qa):
     assert not torch.isnan(qa.shared_prefix_attention(q, cache, ints([20, 60]), beams=1)).any()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("heads,kv_heads,d,prompts,beams,prefix,suffix", [
+    (8, 2, 64, 130, 4, 0, 20), (8, 2, 64, 130, 4, 40, 9), (4, 4, 128, 70, 4, 33, 5), (24, 1, 64, 128, 5, 20, 33), (32, 1, 64, 2, 9, 2200, 40),
+    (32, 1, 64, 1, 33, 9000, 1), (16, 4, 256, 40, 7, 30, 8)])
+def test_attention_of_many_sequences(qa, dtype, heads, kv_heads, d, prompts, beams, prefix, suffix):
+    """So many short sequences that a wave has one, alone or behind a prefix, by lineage too; many rows on one long prefix."""
+    rng = np.random.default_rng(heads * suffix)
+    batch = prompts * beams
+    print("many", dtype, heads, kv_heads, d, prompts, beams, prefix, suffix, flush=True)
+    q = draw(rng, batch, heads, d, dtype=dtype)
+    own, own_ref = make(qa, rng, "Q4_0", dtype, batch, kv_heads, suffix, d)
+    lens = [suffix - b % (suffix + 1) for b in range(batch)]
+    pre = pre_ref = plens = None
+    if prefix:
+        pre, pre_ref = make(qa, rng, "Q4_0", dtype, prompts, kv_heads, prefix, d)
+        plens = [prefix - g % (prefix + 1) if prefix < 100 else prefix - 31 * g for g in range(prompts)]
+    rows = rng.integers(0, beams + 1, size=tuple(own.new_lineage().shape)).astype(np.uint8)
+    for lineage in (None, rows):
+        got = qa.shared_prefix_attention(dev(q, dtype), own, ints(lens), prefix=pre, prefix_lens=None if plens is None else ints(plens), beams=beams,
+                                         lineage=None if lineage is None else torch.from_numpy(lineage).cuda())
+        check_attention(got, kv_ref.attention(q, own_ref, lens, pre_ref, plens, lineage, beams, d ** -0.5), dtype, d)
+
+
+@pytest.mark.parametrize("quant", BITS)
+@pytest.mark.parametrize("d", (64, 128, 256))
+def test_attention_of_blocks_of_every_size(qa, quant, d):
+    """Blocks of the head that are 2^24 smaller than their neighbours are no less exact: the bound by the largest value holds with each
+    block's own."""
+    rng = np.random.default_rng(d)
+    gain = np.repeat(2.0 ** rng.permutation(np.linspace(-14, 10, d // 32).astype(int)), 32).astype(np.float32)
+    k, v = draw(rng, 3, 90, 2, d), rng.normal(size=(3, 90, 2, d)).astype(np.float32) * gain
+    v[:, 50:] *= 4  # so that the largest rises late
+    cache, ref = qa.QuantizedKvCache(qa.KvCacheType[quant], 3, 2, 90, d), kv_ref.Cache(BITS[quant], 3, 2, 90, d)
+    cache.append(dev(k), dev(v), ints([0] * 3))
+    ref.append(k, v, [0] * 3)
+    q, lens = draw(rng, 3, 4, d), [90, 51, 1]
+    got = qa.shared_prefix_attention(dev(q), cache, ints(lens), beams=1).cpu().double().numpy()
+    want, size, _, count = kv_ref.attention(q, ref, lens, beams=1, scale=d ** -0.5)
+    for b in range(3):
+        for h in range(4):
+            top = np.abs(ref.v[1, b, :lens[b], h // 2]).max(0).reshape(-1, 32).max(1).repeat(32)
+            tol = (2 * (size[b, h] * (2.0 ** -22 + (d + 2) * U) + 2.0 ** -21) + 2 * (count[b, h] / 16 + 64) * U + 2 * U) * top
+            assert (np.abs(got[b, h] - want[b, h]) <= tol).all()
+
+
+@pytest.mark.parametrize("reach", (1e5, 1e7, 1e9, 1e12, 1e20))
+def test_attention_of_huge_scores(qa, reach):
+    """Scores whose spacing in f32 is far above 1: one position, or equal ones, take all the weight, and nothing overflows."""
+    rng = np.random.default_rng(4)
+    k, v = rng.integers(-127, 128, size=(2, 300, 2, 64)).astype(np.float32), draw(rng, 2, 300, 2, 64)
+    k[..., ::32] = 127  # scale 1: quants as they are
+    best = rng.integers(0, 300, size=(2, 2))
+    for b in range(2):
+        for h in range(2):
+            k[b, best[b, h], h, 1:32] = 127  # the largest product of all with queries that see the first block only
+    k[0, 299, 0] = k[0, best[0, 0], 0]  # (and once more at the end)
+    cache, ref = qa.QuantizedKvCache(qa.KvCacheType.Q8_0, 2, 2, 300, 64), kv_ref.Cache(8, 2, 2, 300, 64)
+    cache.append(dev(k), dev(v), ints([0, 0]))
+    ref.append(k, v, [0, 0])
+    q = np.zeros((2, 2, 64), np.float32)
+    q[..., :32] = reach
+    got = qa.shared_prefix_attention(dev(q), cache, ints([300, 300]), beams=1, scale=1.0).cpu().double().numpy()
+    want, _, top, _ = kv_ref.attention(q, ref, [300, 300], beams=1, scale=1.0)
+    # (a product with quants is a whole number times the query: next to the best the others are 2^16 or more behind)
+    assert (np.abs(got - want) <= (2.0 ** -21 + 200 * U) * top[..., None]).all()
+
+
 def test_attention_query_rows_inside_wider_ones(qa):
     rng = np.random.default_rng(3)
     cache, _ = make(qa, rng, "Q8_0", "f32", 5, 2, 50, 64)
@@ -508,7 +575,8 @@ def test_python_refusals(qa):
            lambda: cache.read(ints([0]), 1, lineage=cache.new_lineage()[:1], beams=2), lambda: cache.read(ints([0]), 1, lineage=cache.new_lineage(), beams=3),
            lambda: qa.shared_prefix_attention(torch.zeros(2, 4, 64, device="cuda"), None, None), lambda: qa.shared_prefix_attention(torch.zeros(2, 4, 128, device="cuda"), cache, ints([1, 1])),
            lambda: qa.shared_prefix_attention(torch.zeros(2, 3, 64, device="cuda"), cache, ints([1, 1])), lambda: qa.shared_prefix_attention(torch.zeros(3, 4, 64, device="cuda"), cache, ints([1, 1, 1])),
-           lambda: qa.shared_prefix_attention(torch.zeros(2, 4, 64, device="cuda"), cache, ints([1, 1]), max_len=33), lambda: qa.shared_prefix_attention(torch.zeros(2, 4, 64, device="cuda"), cache, None),
+           lambda: qa.shared_prefix_attention(torch.zeros(2, 4, 64, device="cuda"), cache, ints([1, 1]), max_len=33),
+           lambda: qa.shared_prefix_attention(torch.zeros(2, 4, 64, device="cuda"), cache, ints([1, 1]), scale=float("nan")), lambda: qa.shared_prefix_attention(torch.zeros(2, 4, 64, device="cuda"), cache, None),
            lambda: qa.beam_select(torch.zeros(1, 2, 9, device="cuda").half(), torch.zeros(1, 2, device="cuda")), lambda: qa.beam_select(torch.zeros(1, 2, 9), torch.zeros(1, 2)),
            lambda: qa.beam_select(torch.zeros(1, 2, 9, device="cuda"), torch.zeros(2, 1, device="cuda")), lambda: qa.beam_select(torch.zeros(1, 65, 9, device="cuda"), torch.zeros(1, 65, device="cuda")),
            lambda: qa.beam_select(torch.zeros(1, 2, 9, device="cuda"), torch.zeros(1, 2, device="cuda"), torch.zeros(1, 2, dtype=torch.uint8, device="cuda")),
