@@ -80,20 +80,20 @@ __device__ __forceinline__ double wave_sum(double v) {
 }
 __device__ __forceinline__ float wave_max(float v) { return qmm_max_lane_rows(row16_max(v)); }
 
-// e^d for d <= 0 (or -infinity: 0) in f64 to 2e-10 of itself: 2^n 2^f with n + f = d log2(e), |f| <= 1/2, the series of 2^f to f^8
-// (the next term is (ln 2 / 2)^9 / 9!).  Half of what the library's exp takes: 78 MB of logits 42 -> 24 us.
+// e^d for d <= 0 (or -infinity: 0) in f64 to 4e-11 of itself: 2^n 2^f with n + f = d log2(e), |f| <= 1/2, and for 2^f the polynomial of
+// degree 7 with the least largest relative error (Remez' exchange, in 64 bits of mantissa).  Less than half of what the library's exp takes.
 __device__ __forceinline__ double exp_of(double d) {
-    const double y = __builtin_fmax(d * 1.4426950408889634, -1100.0), n = __builtin_rint(y), f = y - n;
-    double p = 1.3215486790144307e-06; // ln(2)^k / k!, k = 8 .. 0
-    p = __builtin_fma(p, f, 1.5252733804059838e-05);
-    p = __builtin_fma(p, f, 1.5403530393381606e-04);
-    p = __builtin_fma(p, f, 1.3333558146428441e-03);
-    p = __builtin_fma(p, f, 9.6181291076284769e-03);
-    p = __builtin_fma(p, f, 5.5504108664821576e-02);
-    p = __builtin_fma(p, f, 2.4022650695910072e-01);
-    p = __builtin_fma(p, f, 6.9314718055994529e-01);
-    p = __builtin_fma(p, f, 1.0);
-    return __builtin_ldexp(p, (int)n);
+    // (1.5 * 2^52 leaves no place behind the point: the low word of the sum is n)
+    const double y = __builtin_fmax(d * 1.4426950408889634, -1100.0), t = y + 0x1.8p52, f = y - (t - 0x1.8p52);
+    double p = 0x1.fe17831d538a2p-17;
+    p = __builtin_fma(p, f, 0x1.446a1fdacba4ep-13);
+    p = __builtin_fma(p, f, 0x1.5d8a7088fdb8dp-10);
+    p = __builtin_fma(p, f, 0x1.3b29dc40d6647p-7);
+    p = __builtin_fma(p, f, 0x1.c6b08aaf2e311p-5);
+    p = __builtin_fma(p, f, 0x1.ebfbe0a4be818p-3);
+    p = __builtin_fma(p, f, 0x1.62e42ff116290p-1);
+    p = __builtin_fma(p, f, 0x1.ffffffffabbcdp-1);
+    return __builtin_ldexp(p, (int)__double_as_longlong(t));
 }
 
 constexpr int kChunkThreads = 256, kChunkRoom = 1024;
@@ -216,7 +216,7 @@ struct Candidate {
 };
 __device__ __forceinline__ bool before(const Candidate& a, const Candidate& b) { return a.score > b.score || (a.score == b.score && a.flat < b.flat); }
 
-// PER > 0: the chunks too, four at a time
+// PER > 0: the chunks too, four at most
 template <int PER>
 __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(BeamParams P) {
     __shared__ double offset[kMaxBeams]; // of a beam's logits: score - logsumexp
@@ -235,7 +235,7 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(BeamParams P) {
     const int per_beam = P.chunks * W, total = W * per_beam;
     // a lineage that fits is on its way from the start
     const int words = (int)(P.padded / 4);
-    const bool ahead = P.lineage_out && W * words <= kAheadWords;
+    const bool ahead = P.lineage_out && (int64_t)W * words <= kAheadWords;
     const uint32_t* in = reinterpret_cast<const uint32_t*>(P.lineage + row0 * P.padded);
     uint32_t early[kAheadWords / kPickThreads];
     int len = 0;
@@ -247,11 +247,8 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(BeamParams P) {
     if constexpr (PER > 0) {
         static_assert(4 * sizeof(ChunkShared) <= sizeof(room));
         ChunkShared* S = reinterpret_cast<ChunkShared*>(room);
-        const int group = tid / kChunkThreads;
-        for (int c0 = 0; c0 < W * P.chunks; c0 += kPickThreads / kChunkThreads) {
-            const int c = min(c0 + group, W * P.chunks - 1), w = c / P.chunks;
-            beam_chunk<PER>(P, (int)row0 + w, c - w * P.chunks, c0 + group < W * P.chunks, S[group], tid % kChunkThreads);
-        }
+        const int group = tid / kChunkThreads, c = min(group, W * P.chunks - 1), w = c / P.chunks;
+        beam_chunk<PER>(P, (int)row0 + w, c - w * P.chunks, group < W * P.chunks, S[group], tid % kChunkThreads);
         __syncthreads();
     }
     // the first candidates are requested before the sums are joined
@@ -421,10 +418,12 @@ int izwi_decode_beam_select_f32(const float* logits, int64_t prompts, int64_t be
     hipStream_t stream = (hipStream_t)stream_;
     BeamParams P{logits, scores, finished, tokens, parents, scores_out, finished_out, lineage, lineage_out, lens, nullptr, nullptr, (int)beams, (int)vocab,
                  0, eos_token, kv_padded(lineage_capacity)};
-    // 4096 logits to a workgroup, 2048 where that leaves fewer than two workgroups to a compute unit; up to eight such chunks of a prompt are
-    // taken by the second launch itself, one launch in all
+    // 4096 logits to a workgroup, 2048 where that leaves fewer than two workgroups to a compute unit and the second launch few lists to look
+    // through (4 prompts of 4 beams of 32000: 9.8 us in a graph instead of 10.3, 1 of 8: 12.0 instead of 11.5).  Up to four chunks of 2048 of
+    // a prompt are taken by the second launch itself, side by side: one launch in all, 3 us less for the host (in a graph, where that counts for
+    // nothing, 2 beams of 2051 take 9.3 us instead of 8.7, a second turn of four chunks 5 us more).
     const int64_t chunks = beams * ((vocab + 4095) / 4096);
-    const bool one_launch = chunks <= 8, small = !one_launch && prompts * chunks < 2 * n_cus;
+    const bool one_launch = beams * ((vocab + 2047) / 2048) <= 4, small = one_launch || (chunks <= 32 && prompts * chunks < 2 * n_cus);
     const int chunk = small ? 2048 : 4096;
     P.chunks = (int)((vocab + chunk - 1) / chunk);
     const size_t parts = (size_t)prompts * beams * P.chunks;
@@ -433,7 +432,7 @@ int izwi_decode_beam_select_f32(const float* logits, int64_t prompts, int64_t be
     P.sums = static_cast<double2*>(scratch);
     P.keys = reinterpret_cast<uint64_t*>(P.sums + parts);
     if (one_launch) {
-        beam_pick_kernel<16><<<(unsigned)prompts, kPickThreads, 0, stream>>>(P);
+        beam_pick_kernel<8><<<(unsigned)prompts, kPickThreads, 0, stream>>>(P);
         KV_TRY(hipGetLastError());
         return IZWI_QMM_OK;
     }

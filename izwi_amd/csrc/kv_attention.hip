@@ -723,16 +723,16 @@ int shared_attention_impl(int type, const T* q, int64_t q_stride, int64_t batch,
     P.max_prefix = prefix ? (int)max_prefix : 0, P.max_len = cache ? (int)max_len : 0;
     P.scale = scale;
     hipStream_t stream = (hipStream_t)stream_;
-    // Workgroups of four waves, about one per compute unit, each with the positions of a split in turns of 32 per wave; two per compute
-    // unit where their waves still have 32 turns.
+    // Workgroups of four waves, about one per compute unit, each with the positions of a split in turns of 32 per wave (two per compute unit
+    // take 2 us more nearly everywhere, for more to join: 8 sequences of 800 positions 8.8 us -> 9.8, 32 of 2000 25.4 -> 27.8, 64 rows on 32000 17.5 -> 19.0).
     constexpr int waves = kWaves;
     const auto turns = [&](int64_t n_seq, int most, int rows, int rt) { // of a wave, with one workgroup per compute unit
         const int64_t base = n_seq * kv_heads * ((rows + 16 * rt - 1) / (16 * rt)), tiles = (most + 31) / 32;
         const int64_t splits = std::max<int64_t>(1, std::min((n_cus + base - 1) / base, (tiles + waves - 1) / waves));
         return tiles / (splits * waves);
     };
-    // Few positions of one kind stay with one workgroup per sequence and kv head: nothing is left to join (16 heads on 8, 300 positions: 6.9 us
-    // in a graph where three splits take 7.5, and a launch less for the host).
+    // Few positions of one kind stay with one workgroup per sequence and kv head: nothing is left to join, and the host has a launch less (16
+    // heads on 8, in a graph: 200 positions 6.0 us instead of 7.2, 380 7.1 instead of 7.3; but 600 8.8 instead of 7.4).
     constexpr int kOneLaunchTiles = 12;
     const bool alone = P.max_prefix == 0 || P.max_len == 0;
     const auto units = [&](int64_t n_seq, int most, int rows, int rt, int& splits, int& n_units, int& z) {
@@ -744,12 +744,12 @@ int shared_attention_impl(int type, const T* q, int64_t q_stride, int64_t batch,
             splits = 1, n_units = (int)base / z;
             return;
         }
-        const int64_t want = turns(n_seq, most, rows, rt) >= 64 ? 2 * n_cus : n_cus;
-        const int64_t s = std::max<int64_t>(1, std::min((want + base - 1) / base, (tiles + waves - 1) / waves)), share = (tiles + s - 1) / s;
+        const int64_t s = std::max<int64_t>(1, std::min((n_cus + base - 1) / base, (tiles + waves - 1) / waves)), share = (tiles + s - 1) / s;
         splits = (int)((tiles + share - 1) / share);
         n_units = (int)(n_seq * kv_heads * splits);
     };
-    // two tiles of query rows to a workgroup where there are two and the waves have enough to do all the same
+    // two tiles of query rows to a workgroup where there are two and the waves have enough to do all the same (32 heads on 8, 16 beams: 60000
+    // positions 65 -> 55 us, 4 prompts of 4000 26.0 -> 23.8; but 2000 12.4 -> 14.1, 8 beams on 1000 8.5 -> 10.7)
     const int prompt_rows = (int)(beams * P.group);
     const int rt = d <= 128 && prompt_rows > 16 && turns(batch / beams, P.max_prefix, prompt_rows, 2) >= 8 ? 2 : 1;
     units(batch / beams, P.max_prefix, prompt_rows, rt, P.prefix_splits, P.prefix_units, P.prefix_z);

@@ -425,8 +425,7 @@ __global__ __launch_bounds__(256) void kv_read_kernel(KvRowsParams P) {
     }
 }
 
-// Few tokens a sequence: a lane per four values of keys, sixteen lanes per row of values, a row at a time (the groups above would be
-// mostly empty: one token of 8 heads of 128 2.7 us instead of 4.6 to write, 2.1 instead of 2.9 to read).
+// Few rows: a lane per four values of keys, sixteen lanes per row of values, a row at a time.
 // Where the row of `item` stands: its sequence, token and head, and whether the cache has (or gets) it
 struct KvItem {
     unsigned row, head;
@@ -548,12 +547,22 @@ __global__ __launch_bounds__(256) void kv_read_rows_kernel(KvRowsParams P) {
     }
 }
 
-constexpr unsigned kFewTokens = 4;
+// The row at a time where sixteen positions would be half empty or more, and for calls that are too small to fill the card with
+// waves of sixteen.  Both sides, 8 heads of 128, Q8_0 and f32: one token of one sequence 2.7 us instead of 4.6 to write, 2.2 instead of 3.1
+// to read; 8 tokens of 256 sequences 8.3 instead of 11.7, and 9.0 instead of 12; 16 of 256: 13.5 instead of 12.6, and 14 instead of 13.  256
+// tokens of one sequence 3.5 instead of 3.9 to write, 2048 of one 8.3 instead of 5.7; 16 of 64 sequences 4.5 instead of 5.9 to read, 256
+// of 8: 7.8 instead of 6.9.
+constexpr unsigned kFewTokens = 8;
+template <bool READ>
+bool by_row(const KvRowsParams& P, int64_t d) {
+    const int64_t values = P.rows * d;
+    return values <= (READ ? 1 << 20 : 1 << 18) || (P.tokens <= kFewTokens && values <= 1 << 30);
+}
 
 template <typename T, int QT, int D, bool READ>
 hipError_t launch_rows(const KvRowsParams& P0, bool vec, hipStream_t stream) {
     KvRowsParams P = P0;
-    if (P.tokens <= kFewTokens) {
+    if (by_row<READ>(P, D)) {
         P.k_blocks = (unsigned)(((uint64_t)P.rows * (D / 4) + 255) / 256);
         const unsigned blocks = P.k_blocks + (unsigned)(((uint64_t)P.rows * 16 + 255) / 256);
         if constexpr (READ) {
@@ -592,8 +601,8 @@ int check_rows(const char* what, const int32_t* starts, int64_t batch, int64_t t
     if (batch < 0 || tokens < 0 || first_slot < 0 || batch > slots || first_slot > slots - batch || tokens > 0x7fffffff)
         return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: sequences %lld of %lld tokens at slot %lld of %lld", what, (long long)batch, (long long)tokens,
                         (long long)first_slot, (long long)slots);
-    if (batch && tokens && batch * ((tokens + 30) / 16) > 0x3ffffff / kv_heads) // (workgroups and rows of either form stay below 2^31)
-        return qmm_fail(IZWI_QMM_ERR_UNSUPPORTED, "%s: more than 2^26 groups of sixteen rows in a call", what);
+    if (batch && tokens && batch * ((tokens + 30) / 16) > 0xffffff / kv_heads) // (threads stay below 2^32)
+        return qmm_fail(IZWI_QMM_ERR_UNSUPPORTED, "%s: more than 2^24 groups of sixteen rows in a call", what);
     if (!cache || !kv_aligned(cache, 16)) return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: the cache must be a 16-byte aligned buffer", what);
     if (batch && tokens && (!starts || !k || !v)) return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: NULL buffer", what);
     return IZWI_QMM_OK;
