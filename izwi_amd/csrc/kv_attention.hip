@@ -12,12 +12,17 @@
 //  * f32 queries and weights go as two f16 numbers each, 22 bits: with the quants exact, two matrix products instead of one.
 //    Queries are scaled by a power of two per row; weights stand under a reference that keeps the largest between 2^5 and 2^15
 //    (it moves when a score rises 2^10 above it: rarely, so most tiles pay for no rescaling), the values' scales under the power
-//    of two that takes the largest so far to below 1.  Weight times scale is a product of f16 pairs whose loss a fused multiply-add
-//    returns exactly: packed, half the instructions of f32 products split afterwards.
-//    f16 queries are themselves, f16 results take their weights rounded to f16 (2^-11).
+//    of two that takes the largest of their block of the head so far to below 1.  Weight times scale is a product of f16 pairs whose loss
+//    a fused multiply-add returns exactly: packed, half the instructions of f32 products split afterwards.
+//    f16 queries are themselves; weights of f16 results are rounded to f16, and once more under the scale (2^-11 each at most, relative:
+//    of the size of the result's own rounding, for half the matrix products).
 //
-// Bound by the vector instructions around the matrix products where many rows share positions (per tile and row tile of an f32
-// call about 240 beside 32 matrix instructions), by memory where few do.
+// Bound by memory where few rows share positions: 32 sequences of 4001 positions of 32 heads on 8, D = 128, Q8_0, 40 us in a graph, 5.5 TB/s.
+// By the issue of vector instructions around the matrix products where many do (per tile of 32 positions and 32 f32 rows about 480 beside 64
+// matrix instructions, some 2650 cycles whether a SIMD has one wave or two): 64 rows a kv head on 131072 positions 107 us, 2.7 TB/s and
+// 320 TFLOP/s; 256 f16 rows a kv head on 8192 positions and 250 own of each sequence, Q4_0, 30 us, 290 TFLOP/s.  By two launches and the way to
+// memory and back where there is little to do: 8 beams behind 1501 positions 9.5 us, one sequence of 300 7.0.
+// Two row tiles a workgroup halve the conversions (65 -> 55 us at 64 rows a kv head on 60000 positions); four do not fit the registers.
 #include "kv_cache.h"
 
 #include <algorithm>
@@ -77,44 +82,51 @@ struct Words {
 // Two unsigned quants under the exponent of 1024, less 1024 and the bias: exact
 __device__ __forceinline__ h2 as_h2(uint32_t w) { return __builtin_bit_cast(h2, w); }
 __device__ __forceinline__ h2 bytes_less_128(uint32_t w) { return as_h2(w) + h2{(f16_t)-1152.0f, (f16_t)-1152.0f}; }
-__device__ __forceinline__ h2 low_nibbles(uint32_t w) { // of bits 0-3 and 16-19
-    return as_h2((w & 0x000f000fu) | 0x64006400u) + h2{(f16_t)-1032.0f, (f16_t)-1032.0f};
+__device__ __forceinline__ h2 low_nibbles(uint32_t w, uint32_t e) { // of bits 0-3 and 16-19
+    return as_h2((w & 0x000f000fu) | e) + h2{(f16_t)-1032.0f, (f16_t)-1032.0f};
 }
-__device__ __forceinline__ h2 high_nibbles(uint32_t w) { // of bits 4-7 and 20-23: 1024 + 16 n, so a sixteenth less 64 + 8
-    return __builtin_elementwise_fma(as_h2((w & 0x00f000f0u) | 0x64006400u), h2{(f16_t)0.0625f, (f16_t)0.0625f}, h2{(f16_t)-72.0f, (f16_t)-72.0f});
+__device__ __forceinline__ h2 high_nibbles(uint32_t w, uint32_t e) { // of bits 4-7 and 20-23: 1024 + 16 n, so a sixteenth less 64 + 8
+    return __builtin_elementwise_fma(as_h2((w & 0x00f000f0u) | e), h2{(f16_t)0.0625f, (f16_t)0.0625f}, h2{(f16_t)-72.0f, (f16_t)-72.0f});
 }
 typedef unsigned short u2 __attribute__((ext_vector_type(2)));
 template <int QT> // of two scales, as bits; those of Q8_0 have no sign
 __device__ __forceinline__ u2 magnitudes(uint32_t w) { return __builtin_bit_cast(u2, QT == IZWI_KV_Q8_0 ? w : w & 0x7fff7fffu); }
 __device__ __forceinline__ h8 join(h2 a, h2 b, h2 c, h2 d) { return h8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]}; }
 
+// The exponent of 1024 for bytes, or for the halves of a word, in a vector register: mask and exponent of a nibble are one instruction only if
+// no more than one of them is a scalar
+template <int QT>
+__device__ __forceinline__ uint32_t exponents() {
+    uint32_t e = QT == IZWI_KV_Q8_0 ? 0x64646464u : 0x64006400u;
+    if constexpr (QT != IZWI_KV_Q8_0) asm volatile("" : "+v"(e));
+    return e;
+}
 // The eight keys' values of a unit
 template <int QT>
-__device__ __forceinline__ h8 key_unit(const uint32_t* w) {
+__device__ __forceinline__ h8 key_unit(const uint32_t* w, uint32_t e) {
     if constexpr (QT == IZWI_KV_Q8_0) {
-        const uint32_t e = 0x64646464u;
         return join(bytes_less_128(__builtin_amdgcn_perm(e, w[0], 0x04010400u)), bytes_less_128(__builtin_amdgcn_perm(e, w[0], 0x04030402u)),
                     bytes_less_128(__builtin_amdgcn_perm(e, w[1], 0x04010400u)), bytes_less_128(__builtin_amdgcn_perm(e, w[1], 0x04030402u)));
     } else {
         const uint32_t u = w[0] >> 8;
-        return join(low_nibbles(w[0]), high_nibbles(w[0]), low_nibbles(u), high_nibbles(u));
+        return join(low_nibbles(w[0], e), high_nibbles(w[0], e), low_nibbles(u, e), high_nibbles(u, e));
     }
 }
 
 // Of block b the values 2 x (first) and 2 x + 1 at eight positions: v[h] are the lane's quants of four positions, dwords of two
 template <int QT, int N>
-__device__ __forceinline__ void value_pair(const Words<N> (&v)[2], int b, h8& first, h8& second) {
+__device__ __forceinline__ void value_pair(const Words<N> (&v)[2], int b, uint32_t e, h8& first, h8& second) {
     h2 lo[4], hi[4];
 #pragma unroll
     for (int r = 0; r < 4; r++) {
         if constexpr (QT == IZWI_KV_Q8_0) {
-            const uint32_t e = 0x64646464u, w = v[r >> 1].w[(r & 1) * (N / 2) + b];
+            const uint32_t w = v[r >> 1].w[(r & 1) * (N / 2) + b];
             lo[r] = bytes_less_128(__builtin_amdgcn_perm(e, w, 0x04020400u));
             hi[r] = bytes_less_128(__builtin_amdgcn_perm(e, w, 0x04030401u));
         } else {
             const uint32_t w = v[r >> 1].w[(r & 1) * (N / 2) + b / 2] >> (8 * (b & 1));
-            lo[r] = low_nibbles(w);
-            hi[r] = high_nibbles(w);
+            lo[r] = low_nibbles(w, e);
+            hi[r] = high_nibbles(w, e);
         }
     }
     first = join(lo[0], lo[1], lo[2], lo[3]);
@@ -318,6 +330,7 @@ __device__ __forceinline__ void attend_rows(const AttendParams& P, int id, float
         for (int i = 0; i < 2 * NB; i++) o[rt][i] = f4{0, 0, 0, 0};
     }
     float s[RT][8];
+    const uint32_t e1024 = exponents<QT>();
     // products of queries and keys, a block of the head at a time under its scale
     auto scores = [&](const Keys& t) {
         float d[2 * SW]; // the lane's scales, to be handed round
@@ -326,7 +339,7 @@ __device__ __forceinline__ void attend_rows(const AttendParams& P, int id, float
         each<NB>([&](auto b) {
             h8 a[2];
 #pragma unroll
-            for (int h = 0; h < 2; h++) a[h] = key_unit<QT>(t.k[h].w + b * (Row::kUnit / 4));
+            for (int h = 0; h < 2; h++) a[h] = key_unit<QT>(t.k[h].w + b * (Row::kUnit / 4), e1024);
 #pragma unroll
             for (int rt = 0; rt < RT; rt++) {
                 f4 acc[2];
@@ -429,19 +442,31 @@ __device__ __forceinline__ void attend_rows(const AttendParams& P, int id, float
 #pragma unroll
         for (int i = 0; i < SW; i++) scale[i] = __builtin_bit_cast(uint32_t, as_h2(sc.s.w[i]) * h2{(f16_t)up[i], (f16_t)up[i]});
         h2 ph[RT][4], pl[SPLIT ? RT : 1][4];
+        float less = -1.0f; // (unknown to the compiler: a fused multiply-add takes an f16 as it is, a subtraction does not)
+        asm("" : "+s"(less));
 #pragma unroll
         for (int rt = 0; rt < RT; rt++)
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 const float a = s[rt][2 * r], c = s[rt][2 * r + 1];
                 ph[rt][r] = h2{(f16_t)a, (f16_t)c};
-                if constexpr (SPLIT) pl[rt][r] = h2{(f16_t)(a - (float)ph[rt][r][0]), (f16_t)(c - (float)ph[rt][r][1])};
+                if constexpr (SPLIT) {
+                    // (as it stands in its register, or each half is rounded again for the difference)
+                    uint32_t w = __builtin_bit_cast(uint32_t, ph[rt][r]);
+                    asm("" : "+v"(w));
+                    const h2 p = as_h2(w);
+                    ph[rt][r] = p;
+                    // (and the differences as f32, or each goes through an instruction of half the rate that rounds it at once)
+                    float da = __builtin_fmaf((float)p[0], less, a), dc = __builtin_fmaf((float)p[1], less, c);
+                    asm("" : "+v"(da), "+v"(dc));
+                    pl[rt][r] = h2{(f16_t)da, (f16_t)dc};
+                }
             }
         each<NB>([&](auto b) {
             h2 d[4];
             each<4>([&](auto r) { d[r] = as_h2(of_lane<r * VL + b / SW>(scale[b % SW])); });
             h8 va, vc;
-            value_pair<QT>(t.v, b, va, vc);
+            value_pair<QT>(t.v, b, e1024, va, vc);
 #pragma unroll
             for (int rt = 0; rt < RT; rt++) {
                 h2 w[4], e[4];

@@ -5,8 +5,8 @@
 // value.  Four planes one behind the other: key quants, key scales, value quants, value scales.  Key scales are
 // [slot][kv head][position][D / 32], value scales [slot][kv head][position / 2][D / 32][2].  The quants of a (slot, kv head) stand where the lanes of a wave want them as matrix-core operands, so that
 // a load brings 16 bytes to every lane from neighbouring addresses and no value moves between lanes.  (With rows of positions
-// instead, the lanes' 16-byte pieces of the keys were 128 bytes apart and each was an access to the L1 of its own: 662 accesses per 32
-// positions bound the whole kernel, 154 us where this layout takes 80: sixteen sequences of 32 heads on 8, 131072 positions.)
+// instead, the lanes' 16-byte pieces of the keys are 128 bytes apart and each is an access to the L1 of its own: 662 accesses per 32
+// positions, which bound the attention of sixteen rows a kv head.)
 //  * keys: lane (x, g) of the wave (x of sixteen, g of four) multiplies of position 16 t + x the values 8 g .. 8 g + 7 of
 //    every block, a unit of 8 bytes (Q8_0) or 4 (Q4_0).  Units that fill 16 bytes are neighbours (a piece): [16 positions][piece][g][x].
 //  * values: lane (x, g) takes of positions 4 g .. 4 g + 3 of 16 the values 2 x and 2 x + 1 of every block.  A dword holds

@@ -308,6 +308,49 @@ inline void argmax(const float* logits, int64_t rows, int64_t n, uint32_t* out, 
                    void* stream = nullptr) {
     check(izwi_argmax_f32(logits, rows, n, out, (int)space, stream));
 }
+
+// A quantized key / value cache in device memory (IZWI_KV_Q8_0 or IZWI_KV_Q4_0) and the calls on it, device pointers
+// throughout (izwi_decode_ops.h); `bytes()` of memory, 16-byte aligned, stays the caller's.
+struct KvCache {
+    int type;
+    int64_t slots, num_kv_heads, capacity, head_dim;
+    void* data;
+
+    uint64_t bytes() const {
+        const uint64_t n = izwi_decode_kv_cache_bytes(type, slots, num_kv_heads, capacity, head_dim);
+        if (n == 0) check(IZWI_QMM_ERR_INVALID);
+        return n;
+    }
+    void append(const float* k, const float* v, const int32_t* starts, const int32_t* counts, int64_t batch, int64_t tokens,
+                int64_t first_slot = 0, void* stream = nullptr) const {
+        const int64_t row = num_kv_heads * head_dim;
+        check(izwi_decode_kv_append_f32(type, k, v, row, row, starts, counts, batch, tokens, first_slot, slots, num_kv_heads, capacity, head_dim,
+                                        data, stream));
+    }
+    void read(const int32_t* starts, const int32_t* counts, int64_t batch, int64_t tokens, float* k, float* v,
+              const uint8_t* lineage = nullptr, int64_t beams = 1, int64_t first_slot = 0, void* stream = nullptr) const {
+        check(izwi_decode_kv_read_f32(type, data, slots, num_kv_heads, capacity, head_dim, lineage, beams, starts, counts, batch, tokens,
+                                      first_slot, k, v, stream));
+    }
+};
+// q `[batch, num_heads, head_dim]` over each prompt's slot of `prefix` (or none), then each sequence's own of `cache`.
+inline void shared_attention(const float* q, int64_t batch, int64_t beams, int64_t num_heads, const KvCache* prefix, const int32_t* prefix_lens,
+                             const KvCache& cache, const int32_t* lens, const uint8_t* lineage, float scale, float* out,
+                             void* stream = nullptr) {
+    if (prefix && (prefix->type != cache.type || prefix->num_kv_heads != cache.num_kv_heads || prefix->head_dim != cache.head_dim))
+        throw Error(Error::Kind::InvalidInput, IZWI_QMM_ERR_INVALID, "shared_attention: the two caches differ in format or heads");
+    check(izwi_decode_shared_attention_f32(cache.type, q, num_heads * cache.head_dim, batch, beams, num_heads, cache.num_kv_heads, cache.head_dim,
+                                           prefix ? prefix->data : nullptr, prefix ? prefix->slots : 0, prefix ? prefix->capacity : 0,
+                                           prefix_lens, prefix ? prefix->capacity : 0, cache.data, cache.slots, cache.capacity, lens,
+                                           cache.capacity, lineage, scale, out, stream));
+}
+inline void beam_select(const float* logits, int64_t prompts, int64_t beams, int64_t vocab, const float* scores, const uint8_t* finished,
+                        int64_t eos_token, int32_t* tokens, int32_t* parents, float* scores_out, uint8_t* finished_out,
+                        const uint8_t* lineage = nullptr, int64_t lineage_capacity = 0, const int32_t* lens = nullptr,
+                        uint8_t* lineage_out = nullptr, void* stream = nullptr) {
+    check(izwi_decode_beam_select_f32(logits, prompts, beams, vocab, scores, finished, eos_token, tokens, parents, scores_out, finished_out,
+                                      lineage, lineage_capacity, lens, lineage_out, stream));
+}
 } // namespace kernels
 
 // `Qwen3Projection` (quantized arm): the op always receives f32 activations and

@@ -243,9 +243,9 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: torch.Tens
             if t.dtype is not _u8 or t.shape != (prompts * beams, capacity) or capacity % _PAD or not t.is_contiguous() or t.get_device() != index:
                 _refuse("beam_select: lineage rows as QuantizedKvCache.new_lineage() makes them expected")
         from_lineage, to_lineage, at = lineage.data_ptr(), out_lineage.data_ptr(), _ints(lens, prompts * beams, index, "beam_select: lens")
-    tokens = torch.empty(rows, dtype=_i32, device=logits.device)
+    tokens = torch.empty_like(scores, dtype=_i32)
     parents, scores_out = torch.empty_like(tokens), torch.empty_like(scores)
-    finished_out = torch.empty(rows, dtype=_u8, device=logits.device) if finished is None else torch.empty_like(finished)
+    finished_out = torch.empty_like(scores, dtype=_u8)
     rc = _fn("beam_select_f32")(logits.data_ptr(), prompts, beams, vocab, scores.data_ptr(), 0 if finished is None else finished.data_ptr(),
                                 -1 if eos_token is None else eos_token, tokens.data_ptr(), parents.data_ptr(), scores_out.data_ptr(), finished_out.data_ptr(),
                                 from_lineage, capacity, at, to_lineage, _raw_stream(index))
