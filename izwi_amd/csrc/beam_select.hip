@@ -416,6 +416,10 @@ int izwi_decode_beam_select_f32(const float* logits, int64_t prompts, int64_t be
     if (prompts == 0) return IZWI_QMM_OK;
     if (!logits || !scores || !tokens || !parents || !scores_out) return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: NULL buffer", what);
     if (!kv_aligned(lineage, 4) || !kv_aligned(lineage_out, 4)) return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: lineage must be 4-byte aligned", what);
+    if (lineage && lineage != lineage_out) {
+        const int64_t bytes = prompts * beams * kv_padded(lineage_capacity);
+        if (kv_overlap(lineage, bytes, lineage_out, bytes)) return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: lineage and its successor overlap", what);
+    }
     QmmCallScope call;
     int device = 0, n_cus = 0;
     if (int rc = qmm_current_device(&device, &n_cus)) return rc;

@@ -736,6 +736,8 @@ int shared_attention_impl(int type, const T* q, int64_t q_stride, int64_t batch,
     if (batch == 0) return IZWI_QMM_OK;
     if (!prefix && !cache) return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: neither a prefix nor a cache", what);
     if (!q || !out || (prefix && !prefix_lens) || (cache && !lens)) return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: NULL buffer", what);
+    if (kv_overlap(q, ((batch - 1) * q_stride + heads * d) * (int64_t)sizeof(T), out, batch * heads * d * (int64_t)sizeof(T)))
+        return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: out shares memory with q", what);
     if (!kv_aligned(prefix, 16) || !kv_aligned(cache, 16)) return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: caches must be 16-byte aligned", what);
     int device = 0, n_cus = 0;
     if (int rc = qmm_current_device(&device, &n_cus)) return rc;

@@ -60,6 +60,10 @@ inline int kv_check_shape(const char* what, int type, int64_t slots, int64_t kv_
     return IZWI_QMM_OK;
 }
 inline bool kv_aligned(const void* p, size_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+inline bool kv_overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x < y + (uintptr_t)b_bytes && y < x + (uintptr_t)a_bytes;
+}
 
 #define KV_TRY(expr)                                                                      \
     do {                                                                                  \

@@ -6,7 +6,8 @@ of a row, V the largest |v|, n its positions, u = 2^-24:
   a score is off by at most A (2^-22 for the two-part f16 split of an f32 query + d u for sums of d terms) + A 2u (scale, log2 e),
   a weight relatively by that + 2^-22 (exponential) and, split into two f16 parts, 2^-22 more,
   a weighted mean by twice its weights' relative error times V, its two sums by (n / 16 + 64) u V each, the quotient by 2u V,
-f16 outputs by 2^-11 |out| more, and where f16 inputs let weights be single f16 numbers by 2^-11 V."""
+f16 outputs by 2^-11 |out| more, and where f16 inputs let weights be single f16 numbers by 2^-11 V (they are rounded twice, to f16 and under the
+value's scale, each by at most that relatively; both at their worst with one sign would be twice this: what is asked is the half)."""
 import numpy as np
 import pytest
 import torch
@@ -141,6 +142,66 @@ def test_cache_rows_inside_wider_ones(qa, dtype):
             b.append(k.contiguous(), v.contiguous(), ints([0, 1, 2]))
             for x, y in zip(a.read(ints([0, 1, 2]), 5), b.read(ints([0, 1, 2]), 5)):
                 assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("quant", BITS)
+@pytest.mark.parametrize("batch,tokens,kv_heads,d,capacity,first", [
+    (3, 500, 3, 256, 510, 1), (70, 50, 5, 64, 57, 0), (9, 40, 24, 128, 33, 2), (700, 9, 2, 128, 12, 0), (1, 2200, 4, 128, 2201, 0), (300, 8, 8, 64, 9, 0)])
+def test_cache_round_trip_of_many_rows(qa, quant, dtype, batch, tokens, kv_heads, d, capacity, first):
+    """Calls of more than 2^20 values, of which more than 8 tokens of a sequence go sixteen positions to a wave (8: one by one)."""
+    test_cache_round_trip(qa, quant, dtype, batch, tokens, kv_heads, d, capacity, first)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_cache_of_many_rows_inside_wider_ones_and_by_lineage(qa, dtype):
+    """Sixteen positions to a wave from rows at odd addresses, and read through a lineage."""
+    rng = np.random.default_rng(21)
+    kv, d, prompts, beams, capacity = 6, 64, 4, 8, 110
+    n = prompts * beams
+    wide = dev(draw(rng, n, capacity, 2 * kv * d + 3, dtype=dtype), dtype)
+    a, b = (qa.QuantizedKvCache(qa.KvCacheType.Q4_0, n, kv, capacity, d) for _ in range(2))
+    k, v = (wide[:, :, at:at + kv * d].unflatten(-1, (kv, d)) for at in (1, kv * d + 3))
+    a.append(k, v, ints([0] * n))
+    b.append(k.contiguous(), v.contiguous(), ints([0] * n))
+    every = a.read(ints([0] * n), capacity, dtype=DTYPES[dtype])
+    for x, y in zip(every, b.read(ints([0] * n), capacity, dtype=DTYPES[dtype])):
+        assert torch.equal(x, y)
+    rows = torch.from_numpy(rng.integers(0, beams + 1, size=tuple(a.new_lineage().shape)).astype(np.uint8)).cuda()
+    at = torch.arange(n, device="cuda").view(n, 1) // beams * beams + rows[:, :capacity].long()
+    there = rows[:, :capacity] < beams
+    for got, x in zip(a.read(ints([0] * n), capacity, lineage=rows, beams=beams, dtype=DTYPES[dtype]), every):
+        want = x[at.clamp(max=n - 1), torch.arange(capacity, device="cuda").view(1, -1)] * there[..., None, None].to(x.dtype)
+        assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("quant", BITS)
+def test_cache_and_attention_past_32_bits(qa, quant):
+    """A slot that begins, and a position that stands, more than 2^32 bytes into its plane (2^33 values of keys)."""
+    rng = np.random.default_rng(13)
+    d, far = 256, 1 << 25
+    for slots, capacity, slot, start in ((40, far // 32, 39, 5), (1, far, 0, far - 37)):
+        cache = qa.QuantizedKvCache(qa.KvCacheType[quant], slots, 1, capacity, d)
+        cache.buffer.zero_()  # scales of zero: keys and values of zero
+        x = draw(rng, 2, 1, 30, 1, d)
+        cache.append(dev(x[0]), dev(x[1]), ints([start]), first_slot=slot)
+        ref = [kv_ref.values(*kv_ref.quantize(x[i], BITS[quant])) for i in range(2)]
+        got = cache.read(ints([start - 2]), 35, first_slot=slot)
+        for g, w in zip(got, ref):
+            same_values(g, np.pad(w, ((0, 0), (2, 3), (0, 0), (0, 0))), "f32")
+        # zeros, then scores of about 20 among them: the softmax by hand
+        k, v = (r[0, :, 0] for r in ref)
+        q, lens = draw(rng, slots, 2, d), [0] * slots
+        lens[slot] = n = start + 30
+        q *= np.float32(20) / np.abs(q[slot] @ k.T).max()
+        got = qa.shared_prefix_attention(dev(q), cache, ints(lens), beams=1, scale=1.0).cpu().double().numpy()
+        assert (got[:slot] == 0).all()
+        s = q[slot].astype(np.float64) @ k.T
+        want = (np.exp(s) @ v) / (np.exp(s).sum(1) + start)[:, None]
+        size, top = (np.abs(q[slot].astype(np.float64)) @ np.abs(k).T).max(1), np.abs(v).max()
+        tol = (2 * (size * (2.0 ** -22 + (d + 2) * U) + 2.0 ** -21) + 2 * (n / 16 / 256 + 64 + 30) * U + 2 * U) * top  # (a split of 256, a wave of four, a lane of four sums its share)
+        assert (np.abs(got[slot] - want) <= tol[:, None]).all()
+        del cache
 
 
 def test_cache_read_by_lineage(qa):

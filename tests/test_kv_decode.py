@@ -124,3 +124,16 @@ def test_beam_select_refusals(L):
     for over in (dict(beams=65), dict(vocab=1 << 30), dict(prompts=20000)):
         assert call(**over) == -2, over
     assert call(prompts=0) == 0
+
+
+def test_refusals_of_shared_memory_and_sizes(L):
+    for name in ("f32", "f16"):
+        fn, size = getattr(L, f"izwi_decode_shared_attention_{name}"), 4 if name == "f32" else 2
+        args = dict(type=8, q=P, q_stride=512, batch=2, beams=1, heads=4, kv=2, d=128, prefix=0, pslots=0, pcap=0, plens=0, maxp=0, cache=P, slots=2, cap=32,
+                    lens=P, maxl=32, lineage=0, scale=1.0, out=P + 512 * size, stream=0)
+        assert fn(*args.values()) == -1 and b"shares memory" in L.izwi_qmm_last_error()
+        for scale in (float("nan"), float("inf"), -float("inf")):
+            assert fn(*{**args, "out": 1 << 30, "scale": scale}.values()) == -1 and b"scale" in L.izwi_qmm_last_error()
+        append = getattr(L, f"izwi_decode_kv_append_{name}")
+        assert append(8, P, P, 128, 128, P, 0, 1, 1 << 28, 0, 1, 1, 64, 128, P, 0) == -2 and b"2^24" in L.izwi_qmm_last_error()
+    assert L.izwi_decode_beam_select_f32(P, 2, 4, 100, P, 0, -1, P, P, P, 0, P, 64, P, P + 64, 0) == -1 and b"overlap" in L.izwi_qmm_last_error()
