@@ -728,7 +728,7 @@ int shared_attention_impl(int type, const T* q, int64_t q_stride, int64_t batch,
     if (cache && (slots < batch || max_len < 0 || max_len > capacity))
         return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: %lld sequences of up to %lld positions in %lld slots of %lld", what, (long long)batch,
                         (long long)max_len, (long long)slots, (long long)capacity);
-    if (batch > 0x3ffffff / heads)
+    if (batch > 0x7fffff / heads) // (threads stay below 2^32)
         return qmm_fail(IZWI_QMM_ERR_UNSUPPORTED, "%s: %lld sequences of %lld heads", what, (long long)batch, (long long)heads);
     if (lineage && (beams > 255 || !cache))
         return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: lineage of %lld beams (at most 255, of a cache)", what, (long long)beams);

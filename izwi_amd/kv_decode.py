@@ -130,8 +130,8 @@ class QuantizedKvCache:
         """(k, v) [sequences, tokens, kv_heads, head_dim]: the values that positions starts[b] .. starts[b] + tokens - 1 of slots
         first_slot, .. stand for; zeros from counts[b] on and outside the capacity.  With ``lineage`` a position comes from
         the slot of the beam that wrote it (``beams`` slots a prompt)."""
-        if dtype is not _f32 and dtype is not _f16:
-            _refuse("read: f32 or f16 expected")
+        if dtype is not _f32 and dtype is not _f16 or tokens < 0:
+            _refuse("read: f32 or f16, and a number of tokens, expected")
         index = self._index
         if index != _current_device():
             with torch.cuda.device(index):
@@ -175,9 +175,8 @@ def shared_prefix_attention(q: torch.Tensor, cache: QuantizedKvCache | None, len
     if (prefix is None) != (prefix_lens is None) or (cache is None) != (lens is None) or (lineage is not None and cache is None):
         _refuse("shared_prefix_attention: a cache and its lengths come together, lineage with a cache")
     if beams is None:
-        beams = batch if prefix is None else batch // max(1, prefix_lens.shape[0])
-    beams = beams or 1
-    if beams < 0 or batch % beams or d != one.head_dim or q.get_device() != index:
+        beams = (batch if prefix is None else batch // max(1, prefix_lens.shape[0])) or 1
+    if beams <= 0 or batch % beams or d != one.head_dim or q.get_device() != index:
         _refuse(f"shared_prefix_attention: {batch} sequences of head_dim {d}, {beams} a prompt, on a cache of head_dim {one.head_dim} on {one.device}")
     if index != _current_device():
         with torch.cuda.device(index):

@@ -624,6 +624,53 @@ def test_other_streams_and_scratch(qa):
         assert all(torch.equal(x, y) for x, y in zip(a, b))
 
 
+def test_more_python_refusals(qa):
+    cache, q = qa.QuantizedKvCache(qa.KvCacheType.Q8_0, 2, 2, 32, 64), torch.zeros(2, 4, 64, device="cuda")
+    lineage = torch.zeros(64 * 3, dtype=torch.uint8, device="cuda")
+    for call in (lambda: cache.read(ints([0]), -1), lambda: qa.shared_prefix_attention(q, cache, ints([1, 1]), beams=0),
+                 lambda: qa.shared_prefix_attention(q, cache, ints([1, 1]), scale=float("inf")), lambda: qa.shared_prefix_attention(q, cache, ints([1, 1]), beams=-1),
+                 lambda: qa.shared_prefix_attention(q, cache, ints([1, 1]), prefix=qa.QuantizedKvCache(qa.KvCacheType.Q4_0, 1, 2, 32, 64), prefix_lens=ints([1])),
+                 lambda: qa.beam_select(torch.zeros(1, 2, 9, device="cuda"), torch.zeros(1, 2, device="cuda"), lineage=lineage[:64].view(2, 32), lens=ints([0, 0]),
+                                        out_lineage=lineage[32:96].view(2, 32))):
+        with pytest.raises(qa.QmmError):
+            call()
+
+
+def test_captured_on_two_streams(qa):
+    """Attention and selection captured on two streams, each with its own scratch, replayed at once and in turn."""
+    rng = np.random.default_rng(5)
+    own, _ = make(qa, rng, "Q4_0", "f32", 6, 2, 900, 64)
+    lens, scores = ints([900, 7, 0, 500, 333, 64]), torch.zeros(2, 3, device="cuda")
+    qs, logits = [dev(draw(rng, 6, 4, 64)) for _ in range(2)], [dev(draw(rng, 2, 3, 20000)) for _ in range(2)]
+
+    def work(i):
+        return [qa.shared_prefix_attention(qs[i], own, lens, beams=1), *qa.beam_select(logits[i], scores)[:4]]
+
+    want, streams, graphs, results = [work(0), work(1)], [torch.cuda.Stream() for _ in range(2)], [], []
+    torch.cuda.synchronize()
+    for i, s in enumerate(streams):
+        with torch.cuda.stream(s):
+            work(i)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            results.append(work(i))
+        graphs.append(graph)
+    for turn in range(4):
+        for t in results[0] + results[1]:
+            t.zero_()
+        torch.cuda.synchronize()
+        for s, graph in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+            if turn % 2:
+                torch.cuda.synchronize()
+                work(0)  # the program's own
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert all(torch.equal(x, y) for x, y in zip(want[i], results[i]))
+
+
 def test_python_refusals(qa):
     cache = qa.QuantizedKvCache(qa.KvCacheType.Q8_0, 2, 2, 32, 64)
     good = torch.zeros(1, 1, 2, 64, device="cuda")
