@@ -18,7 +18,7 @@
 //    of the size of the result's own rounding, for half the matrix products).
 //
 // Bound by memory where few rows share positions: 32 sequences of 4001 positions of 32 heads on 8, D = 128, Q8_0, 40 us in a graph, 5.5 TB/s.
-// By the issue of vector instructions around the matrix products where many do (per tile of 32 positions and 32 f32 rows about 480 beside 64
+// By the issue of vector instructions around the matrix products where many do (per tile of 32 positions and 32 f32 rows about 450 beside 64
 // matrix instructions, some 2650 cycles whether a SIMD has one wave or two): 64 rows a kv head on 131072 positions 107 us, 2.7 TB/s and
 // 320 TFLOP/s; 256 f16 rows a kv head on 8192 positions and 250 own of each sequence, Q4_0, 30 us, 290 TFLOP/s.  By two launches and the way to
 // memory and back where there is little to do: 8 beams behind 1501 positions 9.5 us, one sequence of 300 7.0.
@@ -400,8 +400,9 @@ __device__ __forceinline__ void attend_rows(const AttendParams& P, int id, float
             for (int i = 0; i < SW; i++) {
                 const h2 two = __builtin_bit_cast(h2, magnitudes<QT>(t.s.w[i]));
                 float d = fmaxf(0.0f, fmaxf((float)two[0], (float)two[1])); // (passes over the NaN of a block that holds one)
-#pragma unroll
-                for (int n = VL; n < 16; n *= 2) d = fmaxf(d, __shfl_xor(d, n));
+                d = fmaxf(d, dpp_f<0x128>(d)); // over the lanes x that have this block: row_ror 8, 4 (and 2)
+                d = fmaxf(d, dpp_f<0x124>(d));
+                if constexpr (VL == 2) d = fmaxf(d, dpp_f<0x122>(d));
                 const int e = (int)(__float_as_uint(qmm_max_lane_rows(d)) >> 23) - 127;
                 const float to = fminf(up[i], __uint_as_float((uint32_t)(127 + min(15, -1 - e)) << 23));
                 down[i] = to / up[i], up[i] = to;
