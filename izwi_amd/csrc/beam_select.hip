@@ -157,10 +157,16 @@ __device__ __forceinline__ void beam_chunk(const BeamParams& P, int row, int chu
         const uint32_t t = max(max(S.threshold[0], S.threshold[1]), max(S.threshold[2], S.threshold[3]));
         // (the number of that order; an order below -infinity's is no float's)
         const float least = t <= order_of(-INFINITY) ? -INFINITY : value_of(t);
+        // (Few pass, one or two lanes of a wave at a time: the counter's address is hidden from the compiler, which would otherwise work out one
+        // addition for all of them in some 25 instructions.  What is behind the end is -infinity.)
+        unsigned hidden = 0;
+        asm("" : "+v"(hidden));
+        const bool ends = n != kChunk && least == -INFINITY;
 #pragma unroll
         for (int i = 0; i < PER; i++)
-            if (v[i] >= least && i * kChunkThreads + tid < n) { // (few)
-                const unsigned at = atomicAdd(&S.n_found, 1u);
+            if (v[i] >= least) {
+                if (ends && i * kChunkThreads + tid >= n) continue;
+                const unsigned at = atomicAdd(&S.n_found + hidden, 1u);
                 if (at < kChunkRoom) S.found[at] = key_of(i);
             }
         double s = 0.0, s2 = 0.0; // (what is behind the end is -infinity: nothing)
