@@ -10,7 +10,7 @@
 // a whole number.  Within a beam the order is the logits' own, in f32.
 //
 // Many logits are bound by the issue of vector instructions, half of them the exponentials in f64 (16 prompts of 8 beams over 151936
-// tokens, 78 MB: 27 us, 2.9 TB/s, and 8 for the second launch); fewer by the launches and each one's chain of
+// tokens, 78 MB: 26 us, 3.0 TB/s, and 8 for the second launch); fewer by the launches and each one's chain of
 // loads and barriers (4 beams of 151936: 5 and 6 us).
 #include "kv_cache.h"
 #include "qmm_lanes.h"

@@ -19,9 +19,9 @@
 //
 // Bound by memory where few rows share positions: 32 sequences of 4001 positions of 32 heads on 8, D = 128, Q8_0, 40 us in a graph, 5.5 TB/s.
 // By the issue of vector instructions around the matrix products where many do (per tile of 32 positions and 32 f32 rows about 450 beside 64
-// matrix instructions, some 2650 cycles whether a SIMD has one wave or two): 64 rows a kv head on 131072 positions 107 us, 2.7 TB/s and
-// 320 TFLOP/s; 256 f16 rows a kv head on 8192 positions and 250 own of each sequence, Q4_0, 30 us, 290 TFLOP/s.  By two launches and the way to
-// memory and back where there is little to do: 8 beams behind 1501 positions 9.5 us, one sequence of 300 7.0.
+// matrix instructions, some 2650 cycles whether a SIMD has one wave or two): 64 rows a kv head on 131072 positions 99 to 110 us, 2.7 TB/s and
+// 330 TFLOP/s; 256 f16 rows a kv head on 8192 positions and 250 own of each sequence, Q4_0, 28 us, 310 TFLOP/s.  By two launches and the way to
+// memory and back where there is little to do: 8 beams behind 1501 positions 9.3 us, one sequence of 300 6.8.
 // Two row tiles a workgroup halve the conversions (65 -> 55 us at 64 rows a kv head on 60000 positions); four do not fit the registers.
 #include "kv_cache.h"
 
