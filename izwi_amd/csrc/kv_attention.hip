@@ -9,13 +9,13 @@
 //  * Quants are exact in f16 (one byte permute and one subtraction for two of them).  A block of 32 is the depth of one matrix
 //    instruction, so the keys' scales multiply finished sums in f32.  The values' scales run along the positions, over which the
 //    second product sums: they multiply the weights, once for each block of 32 elements of the head.
-//  * f32 queries and weights go as two f16 numbers each, 22 bits: with the quants exact, two matrix products instead of one.
+//  * f32 queries and the weights go as two f16 numbers each, 22 bits: with the quants exact, two matrix products instead of one.
 //    Queries are scaled by a power of two per row; weights stand under a reference that keeps the largest between 2^5 and 2^15
 //    (it moves when a score rises 2^10 above it: rarely, so most tiles pay for no rescaling), the values' scales under the power
 //    of two that takes the largest of their block of the head so far to below 1.  Weight times scale is a product of f16 pairs whose loss
 //    a fused multiply-add returns exactly: packed, half the instructions of f32 products split afterwards.
-//    f16 queries are themselves; weights of f16 results are rounded to f16, and once more under the scale (2^-11 each at most, relative:
-//    of the size of the result's own rounding, for half the matrix products).
+//    f16 queries are themselves.  (Weights of f16 results as single f16 numbers, rounded to f16 and once more under the scale, left 2.8e-4 of a
+//    result where its own rounding leaves 2.1e-4, and far more where values cancel.)
 //
 // Bound by memory where few rows share positions: 32 sequences of 4001 positions of 32 heads on 8, D = 128, Q8_0, 40 us in a graph, 5.5 TB/s.
 // By the issue of vector instructions around the matrix products where many do (per tile of 32 positions and 32 f32 rows about 450 beside 64
@@ -445,7 +445,7 @@ __device__ __forceinline__ void attend_rows(const AttendParams& P, int id, float
         uint32_t scale[SW];
 #pragma unroll
         for (int i = 0; i < SW; i++) scale[i] = __builtin_bit_cast(uint32_t, as_h2(sc.s.w[i]) * h2{(f16_t)up[i], (f16_t)up[i]});
-        h2 ph[RT][4], pl[SPLIT ? RT : 1][4];
+        h2 ph[RT][4], pl[RT][4];
         float less = -1.0f; // (unknown to the compiler: a fused multiply-add takes an f16 as it is, a subtraction does not)
         asm("" : "+s"(less));
 #pragma unroll
@@ -453,18 +453,15 @@ __device__ __forceinline__ void attend_rows(const AttendParams& P, int id, float
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 const float a = s[rt][2 * r], c = s[rt][2 * r + 1];
-                ph[rt][r] = h2{(f16_t)a, (f16_t)c};
-                if constexpr (SPLIT) {
-                    // (as it stands in its register, or each half is rounded again for the difference)
-                    uint32_t w = __builtin_bit_cast(uint32_t, ph[rt][r]);
-                    asm("" : "+v"(w));
-                    const h2 p = as_h2(w);
-                    ph[rt][r] = p;
-                    // (and the differences as f32, or each goes through an instruction of half the rate that rounds it at once)
-                    float da = __builtin_fmaf((float)p[0], less, a), dc = __builtin_fmaf((float)p[1], less, c);
-                    asm("" : "+v"(da), "+v"(dc));
-                    pl[rt][r] = h2{(f16_t)da, (f16_t)dc};
-                }
+                // (as it stands in its register, or each half is rounded again for the difference)
+                uint32_t w = __builtin_bit_cast(uint32_t, h2{(f16_t)a, (f16_t)c});
+                asm("" : "+v"(w));
+                const h2 p = as_h2(w);
+                ph[rt][r] = p;
+                // (and the differences as f32, or each goes through an instruction of half the rate that rounds it at once)
+                float da = __builtin_fmaf((float)p[0], less, a), dc = __builtin_fmaf((float)p[1], less, c);
+                asm("" : "+v"(da), "+v"(dc));
+                pl[rt][r] = h2{(f16_t)da, (f16_t)dc};
             }
         each<NB>([&](auto b) {
             h2 d[4];
@@ -478,16 +475,13 @@ __device__ __forceinline__ void attend_rows(const AttendParams& P, int id, float
                 for (int r = 0; r < 4; r++) {
                     w[r] = ph[rt][r] * d[r];
                     // what the product lost, and the weight's second part
-                    if constexpr (SPLIT) e[r] = __builtin_elementwise_fma(pl[rt][r], d[r], __builtin_elementwise_fma(ph[rt][r], d[r], -w[r]));
+                    e[r] = __builtin_elementwise_fma(pl[rt][r], d[r], __builtin_elementwise_fma(ph[rt][r], d[r], -w[r]));
                 }
-                const h8 wh = join(w[0], w[1], w[2], w[3]);
+                const h8 wh = join(w[0], w[1], w[2], w[3]), wl = join(e[0], e[1], e[2], e[3]);
                 o[rt][2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, wh, o[rt][2 * b], 0, 0, 0);
                 o[rt][2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vc, wh, o[rt][2 * b + 1], 0, 0, 0);
-                if constexpr (SPLIT) {
-                    const h8 wl = join(e[0], e[1], e[2], e[3]);
-                    o[rt][2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, wl, o[rt][2 * b], 0, 0, 0);
-                    o[rt][2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vc, wl, o[rt][2 * b + 1], 0, 0, 0);
-                }
+                o[rt][2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, wl, o[rt][2 * b], 0, 0, 0);
+                o[rt][2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vc, wl, o[rt][2 * b + 1], 0, 0, 0);
             }
         });
     };
