@@ -173,7 +173,8 @@ int izwi_decode_kv_read_f16(int type, const void* cache, int64_t slots, int64_t 
  * of the prompt's slot of `prefix` and positions 0 .. lens[b] - 1 of slot b of `cache`, both of format `type`; either may be
  * NULL.  q is `[batch, num_heads, head_dim]`, q_stride elements from one sequence to the next; head h reads kv head
  * h / (num_heads / num_kv_heads); out is contiguous `[batch, num_heads, head_dim]` and may share no memory with the rest.  A
- * sequence without any position gives zeros.  Lengths above max_prefix_len (max_len), the caller's bounds, count as
+ * sequence without any position gives zeros, one that reads a NaN (in q, a key, a value; an infinity in q) NaN: the whole
+ * head, or a value's block of 32.  Lengths above max_prefix_len (max_len), the caller's bounds, count as
  * those, negative ones as zero; the work is shared out by the bounds.  With `lineage`, `[slots][kv_capacity rounded up to
  * 32]`, position p of sequence b is in the slot of beam lineage[b][p] of its prompt; a position whose entry is no beam
  * (>= beams) does not count.  The products run on the matrix cores with f32 sums; f32 queries and the weights go as

@@ -66,7 +66,7 @@ struct AttendParams {
     Divisor by_group, by_kv_heads, by_beams, by_prefix_splits, by_own_splits, by_prefix_z, by_own_z;
     int parts;     // partial results of a row: prefix_splits + own_splits
     float* sums;   // [batch * heads][parts][D]
-    float2* stats; // [batch * heads][parts]: reference (a power of two's exponent), sum of weights
+    float2* stats; // [batch * heads][parts]: reference (a power of two's exponent), sum of weights; (-infinity, 0) without a position, NaN with a score that is none
 };
 
 __device__ __forceinline__ int clamped_len(const int32_t* lens, int i, int most) { return most ? max(0, min(lens[i], most)) : 0; }
@@ -290,12 +290,14 @@ __device__ __forceinline__ void attend_rows(const AttendParams& P, int id, float
         for (int b = 0; b < NB; b++)
 #pragma unroll
             for (int j = 0; j < 8; j++) f[b][j] = (float)q[32 * b + j];
-        if constexpr (SPLIT) {
-            float most = 0.0f;
+        float most = 0.0f;
 #pragma unroll
-            for (int b = 0; b < NB; b++)
+        for (int b = 0; b < NB; b++)
 #pragma unroll
-                for (int j = 0; j < 8; j++) most = fmaxf(most, fabsf(f[b][j]));
+            for (int j = 0; j < 8; j++) most = fmaxf(most, fabsf(f[b][j]));
+        if constexpr (!SPLIT) { // an infinity among the queries leaves no number (f32: infinity less infinity in the split)
+            if (most == INFINITY) by = NAN;
+        } else {
             most = qmm_max_lane_rows(most);
             // (an infinity or a subnormal gets some power or other)
             const int up = max(-113, min(113, 140 - (int)(__float_as_uint(most) >> 23)));
@@ -518,14 +520,17 @@ __device__ __forceinline__ void attend_rows(const AttendParams& P, int id, float
             }
         }
     }
+    // What is known of a row's scores when all is read: the reference, and the sum of weights.  No position: -infinity and zero.  A score that
+    // is NaN: both NaN, because the maximum passes over it and the reference of scores that are all NaN would stay at "no position".
+    const auto statistics = [](float reference, float sum) { return make_float2(sum != sum ? sum : reference, sum); };
     if constexpr (SOLO) { // lane (x, g) has of row x and block b the values 8 g .. 8 g + 7
         static_assert(RT == 1);
-        const float sum = qmm_add_lane32(qmm_add_lane16(l[0])), inv = 1.0f / sum;
+        const float sum = qmm_add_lane32(qmm_add_lane16(l[0])), inv = sum == 0.0f ? 0.0f : 1.0f / sum;
         float down[NB];
         each<NB>([&](auto b) { down[b] = 1.0f / up_of(b); });
         if (x >= rows_here) return;
         const int64_t row = row_index(x);
-        if (P.parts > 1 && g == 0) P.stats[row * P.parts + part] = make_float2(ref[0], sum);
+        if (P.parts > 1 && g == 0) P.stats[row * P.parts + part] = statistics(ref[0], sum);
         each<NB>([&](auto b) {
             const f4 a = o[0][2 * b], c = o[0][2 * b + 1];
             const float v[8] = {a[0], c[0], a[1], c[1], a[2], c[2], a[3], c[3]}, by = down[b];
@@ -536,7 +541,7 @@ __device__ __forceinline__ void attend_rows(const AttendParams& P, int id, float
             } else {
                 T* dst = static_cast<T*>(P.out) + row * D + 32 * b + 8 * g;
 #pragma unroll
-                for (int i = 0; i < 8; i++) dst[i] = (T)(ref[0] == -INFINITY ? 0.0f : v[i] * (by * inv));
+                for (int i = 0; i < 8; i++) dst[i] = (T)(v[i] * (by * inv));
             }
         });
         return;
@@ -553,7 +558,7 @@ __device__ __forceinline__ void attend_rows(const AttendParams& P, int id, float
             *reinterpret_cast<f4*>(dst + 32 * b + 4) = f4{a[2], c[2], a[3], c[3]};
         });
         const float sum = qmm_add_lane32(qmm_add_lane16(l[rt]));
-        if (g == 0) stat[wave * ROWS + 16 * rt + x] = make_float2(ref[rt], sum);
+        if (g == 0) stat[wave * ROWS + 16 * rt + x] = statistics(ref[rt], sum);
     }
     __syncthreads();
     // a thread per row turns the references into the waves' weights and leaves where the row goes
@@ -576,8 +581,8 @@ __device__ __forceinline__ void attend_rows(const AttendParams& P, int id, float
         }
         const int64_t row = row_index(r);
         where[r] = row;
-        if (P.parts > 1) P.stats[row * P.parts + part] = make_float2(to, sum);
-        else total[r] = to == -INFINITY ? 0.0f : 1.0f / sum;
+        if (P.parts > 1) P.stats[row * P.parts + part] = statistics(to, sum);
+        else total[r] = sum == 0.0f ? 0.0f : 1.0f / sum;
     }
     __syncthreads();
     constexpr int kTurns = ROWS * (D / 4) / (64 * kWaves);
@@ -616,7 +621,7 @@ __global__ __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) void attend_kernel(A
 
 // A row's parts joined: by a wave where there are at most eight (FEW), by the four waves of a workgroup in turn where there are more.
 // Statistics and sums are requested together, eight parts a wave at a time; what a part did not write (no position of the row) is in its
-// place and not looked at.
+// place and not looked at.  (Scores that are NaN: see `statistics` above; a sum of zero is a row without positions.)
 template <typename T, int D, bool FEW>
 __global__ __launch_bounds__(256) void attend_join_kernel(const float* __restrict__ sums, const float2* __restrict__ stats, T* __restrict__ out, int parts,
                                                           int64_t rows) {
@@ -653,7 +658,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(const float* __restric
     if constexpr (FEW) {
         T* dst = out + row * D + lane * N;
 #pragma unroll
-        for (int i = 0; i < N; i++) dst[i] = (T)(to == -INFINITY ? 0.0f : a[i] / sum);
+        for (int i = 0; i < N; i++) dst[i] = (T)(sum == 0.0f ? 0.0f : a[i] / sum);
         return;
     }
     __shared__ float red[4][D + 2];
@@ -670,7 +675,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(const float* __restric
             const float by = red[w][D + 1] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(red[w][D + 1] - most);
             total += red[w][D] * by, v += red[w][threadIdx.x] * by;
         }
-        out[row * D + threadIdx.x] = (T)(most == -INFINITY ? 0.0f : v / total);
+        out[row * D + threadIdx.x] = (T)(total == 0.0f ? 0.0f : v / total);
     }
 }
 
