@@ -276,6 +276,10 @@ __device__ __forceinline__ void attend_rows(const AttendParams& P, int id, float
     // The queries: lane (x, g) holds of row x the values 8 g .. of every block.  f32 ones are scaled by a power of two to
     // below 2^14 and split.  The sign of the scale goes to them, so that the largest score is the largest product.
     h8 qh[RT][NB], ql[SPLIT ? RT : 1][SPLIT ? NB : 1];
+    // What makes scores (in powers of two) of products.  A product of numbers is below 2^47 (queries 2^16, quants 2^7, scales 2^16, a head 2^8) and
+    // two that differ do by 2^-48 or more, so a factor above 2^80 makes a weight of one of the largest and zero of the others whatever it is: with
+    // 2^80 instead no score is beyond f32.
+    constexpr float kMostFactor = 0x1p80f;
     float factor[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
@@ -304,6 +308,7 @@ __device__ __forceinline__ void attend_rows(const AttendParams& P, int id, float
             by *= __uint_as_float((uint32_t)(127 + up) << 23);
             factor[rt] = fmaxf(factor[rt] * __uint_as_float((uint32_t)(127 - up) << 23), 1e-37f);
         }
+        factor[rt] = fminf(factor[rt], kMostFactor);
 #pragma unroll
         for (int b = 0; b < NB; b++) {
             h8 hi, lo;

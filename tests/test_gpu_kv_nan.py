@@ -70,3 +70,19 @@ def test_no_position_by_lineage_stays_zero(qa, dtype, batch):
     q = torch.full((batch, 4, 64), float("nan"), device="cuda", dtype=DTYPES[dtype])
     out = qa.shared_prefix_attention(q, cache, lens, beams=2, lineage=torch.full_like(cache.new_lineage(), 255))
     assert (out == 0).all()
+
+
+@pytest.mark.parametrize("sign", (1.0, -1.0))
+def test_scores_beyond_f32(qa, sign):
+    """Scores that have no f32 take all the weight, or none, as in 64 bits: no infinity stands for them."""
+    d, n = 64, 40
+    k = np.zeros((4, n, 2, d), np.float32)
+    k[..., 0] = 1.0
+    k[:, 7, :, 0] = 3.0 if sign > 0 else 0.5  # the largest score
+    v = np.random.default_rng(1).normal(size=k.shape).astype(np.float32)
+    call = Attend(qa, "one_launch", "Q8_0", "f32", k, v, [n] * 4)
+    q = np.zeros(rows_of("one_launch", d), np.float32)
+    q[..., 0] = sign * 3e38
+    for scale in (1e-3, 1.0, 1e10):
+        want, _, top, _ = call.exact(q, scale)
+        assert (np.abs(call.run(q, scale) - want) <= 200 * 2.0 ** -24 * top[..., None]).all()
