@@ -645,6 +645,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(const float* __restric
 #pragma unroll
         for (int i = 0; i < A; i++) v[i] = *reinterpret_cast<const vec*>(sums + (int64_t)min(p0 + STEP * i, parts - 1) * D);
         const float ref = mine < parts ? st.x : -INFINITY;
+        const unsigned there = (unsigned)__ballot(ref != -INFINITY); // parts that wrote sums: also under a weight of zero, a NaN is not lost
         float most = ref;
         most = fmaxf(most, dpp_f<0xB1>(most));
         most = fmaxf(most, dpp_f<0x4E>(most));
@@ -654,10 +655,8 @@ __global__ __launch_bounds__(256) void attend_join_kernel(const float* __restric
         sum = sum * old + sum8(by == 0.0f ? 0.0f : st.y * by);
         a *= old;
 #pragma unroll
-        for (int i = 0; i < A; i++) {
-            const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(by), i));
-            if (w != 0.0f) a += v[i] * w; // uniform
-        }
+        for (int i = 0; i < A; i++) // uniform
+            if (there >> i & 1) a += v[i] * __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(by), i));
         to = next;
     }
     if constexpr (FEW) {

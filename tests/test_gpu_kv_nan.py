@@ -60,6 +60,23 @@ def test_numbers_that_are_none(qa, quant, d, dtype, plan):
         assert np.isnan(check_nan(call, q, d ** -0.5, dtype)).any()
 
 
+@pytest.mark.parametrize("plan", [p for p in PLANS if "prefix" in PLANS[p]])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_value_that_is_none_under_a_weight_of_zero(qa, dtype, plan):
+    """0 * NaN is NaN in the part that holds it and where parts are joined."""
+    n, d, kv, slots = 3, 64, 2, slots_of(plan)
+    k = np.zeros((slots, n, kv, d), np.float32)
+    k[..., 0] = -1.0
+    v = np.ones_like(k)
+    v[0, 1, 0, 40] = np.nan
+    shape = (slots // PLANS[plan]["beams"], PLANS[plan]["prefix"], kv, d)
+    call = Attend(qa, plan, "Q8_0", dtype, k, v, [n] * slots, (np.zeros(shape, np.float32), np.ones(shape, np.float32)))
+    q = np.zeros(rows_of(plan, d), np.float32)
+    q[..., 0] = 2000.0  # own positions score 2000 below the prefix
+    want = check_nan(call, q, 1.0, dtype)
+    assert np.isnan(want[0, :GROUP, 32:]).all() and not np.isnan(want[0, :GROUP, :32]).any() and not np.isnan(want[1:]).any()
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("batch", (6, 512))
 def test_no_position_by_lineage_stays_zero(qa, dtype, batch):
