@@ -10,8 +10,11 @@
 //    instruction, so the keys' scales multiply finished sums in f32.  The values' scales run along the positions, over which the
 //    second product sums: they multiply the weights, once for each block of 32 elements of the head.
 //  * f32 queries and the weights go as two f16 numbers each, 22 bits: with the quants exact, two matrix products instead of one.
-//    Queries are scaled by a power of two per row; weights stand under a reference that keeps the largest between 2^5 and 2^15
-//    (it moves when a score rises 2^10 above it: rarely, so most tiles pay for no rescaling), the values' scales under the power
+//    Queries are scaled by a power of two per row.  Weights stand under a reference that keeps the largest between 2^12 and 2^15.5 (it moves
+//    when a score rises by a factor of 11: rarely, so most tiles pay for no rescaling): a weight is right to 2^-22 of itself or 2^-37 of the
+//    largest, where the second number ends, whichever is more, so that many positions far below a few that dominate keep their sum.  (With the
+//    largest between 2^5 and 2^15, which moves even less, 2^15 positions that have 2^-13 to 2^-27 of four others' weight each came out up to
+//    28 % of their sum wrong, now 0.3 %, 2^-22 of the whole; moving costs some 2 % where many rows share positions.)  The values' scales stand under the power
 //    of two that takes the largest of their block of the head so far to below 1.  Weight times scale is a product of f16 pairs whose loss
 //    a fused multiply-add returns exactly: packed, half the instructions of f32 products split afterwards.
 //    f16 queries are themselves.  (Weights of f16 results as single f16 numbers, rounded to f16 and once more under the scale, left 2.8e-4 of a
@@ -134,7 +137,7 @@ __device__ __forceinline__ void value_pair(const Words<N> (&v)[2], int b, uint32
 }
 
 constexpr int kWaves = 4; // of a workgroup
-constexpr float kRise = 10.0f, kHead = 5.0f; // powers of two, see above
+constexpr float kRise = 3.5f, kHead = 12.0f; // powers of two, see above
 
 template <typename T, int QT, int D, int RT, bool SHARED, bool LIN, bool SOLO = false>
 __device__ __forceinline__ void attend_rows(const AttendParams& P, int id, float* lds) {
@@ -422,7 +425,8 @@ __device__ __forceinline__ void attend_rows(const AttendParams& P, int id, float
                 for (int j = 1; j < 8; j++) m = fmaxf(m, s[rt][j]);
                 top[rt] = fmaxf(top[rt], qmm_max_lane_rows(m) * factor[rt]);
                 bar[rt] = (top[rt] + (kRise - fabsf(top[rt]) * 0x1p-22f)) / factor[rt]; // (less what rounding may add)
-                const float to = top[rt] - kHead, by = ref[rt] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ref[rt] - to);
+                // (from 2^24 on scores are whole numbers two or more apart, and a reference rounded further up would take a weight beyond f16)
+                const float to = fabsf(top[rt]) < 0x1p24f ? top[rt] - kHead : top[rt], by = ref[rt] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ref[rt] - to);
                 ref[rt] = to, l[rt] *= by;
                 each<NB>([&](auto b) {
                     const float by_o = by * __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(down[b % SW]), b / SW));

@@ -4,10 +4,10 @@ plain 64-bit restatement of kv_ref.py.
 The arithmetic that bounds it.  u = 2^-24; A the largest sum of |q_i k_i| scale of a row, p_i its softmax weights, v_i the values, n its positions.
   A score is off by A (2^-22 for an f32 query as two f16 numbers, d u for the sums of products, 4 u for the two scales and log2 e);
   a weight, relatively, by that + ln2 2^-21 (its exponent is a number below 16, rounded once) + 2^-22 (exponential) + 2^-22 (two f16 numbers);
-  and by 2^-36 of the row's largest weight (the second f16 number ends at 2^-24, and so does what the value's scale leaves of it, half a step each,
-  where the largest weight is 2^12 or more).
+  and by 5 2^-37 of the row's largest weight: where the largest is 2^12 or more, the second f16 number ends at 2^-24, half a step (2^-37) off; what
+  its product with the value's scale d loses is made up for by two fused multiply-adds that end there too, 2^-25 / d each, d >= 1/2 for the largest value.
   A weighted mean is off by twice the weights' relative error times sum p|v|, its two sums by (n / 16 + 64) u sum p|v| each (a lane sums a
-  sixteenth at the most; 64 for the joins of lanes, waves and parts), the quotient by 2 u, and by 2^-36 n of the largest |v|.
+  sixteenth at the most; 64 for the joins of lanes, waves and parts), the quotient by 2 u, and by 5 2^-37 n of the largest |v|.
   An f16 result is rounded once more: 2^-11 of itself."""
 import numpy as np
 import pytest
@@ -105,7 +105,7 @@ def rows_of(plan, d):
 def tolerance(dtype, d, want, size, count, mean, top):
     """The bound at the head of this file; `mean` = sum p|v| per element, `top` = the largest |v| of a row."""
     relative = size * (2.0 ** -22 + (d + 4) * U) + np.log(2) * 2.0 ** -21 + 2.0 ** -21
-    tol = (2 * relative + 2 * (count / 16 + 64) * U + 2 * U)[..., None] * mean + (count * 2.0 ** -36 * top)[..., None]
+    tol = (2 * relative + 2 * (count / 16 + 64) * U + 2 * U)[..., None] * mean + (count * 5 * 2.0 ** -37 * top)[..., None]
     return tol + 2.0 ** -11 * np.abs(want) + 2.0 ** -25 if dtype == "f16" else tol
 
 
