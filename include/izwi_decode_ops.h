@@ -179,7 +179,8 @@ int izwi_decode_kv_read_f16(int type, const void* cache, int64_t slots, int64_t 
  * 32]`, position p of sequence b is in the slot of beam lineage[b][p] of its prompt; a position whose entry is no beam
  * (>= beams) does not count.  The products run on the matrix cores with f32 sums; f32 queries and the weights go as
  * two f16 numbers each, 22 bits down to 2^-16 of the row's largest number in q and 2^-14 of its largest weight, fewer of
- * what is smaller; f16 results are rounded once.  Uses the library's per-stream scratch. */
+ * what is smaller; a value counts to 2^-24 of the largest of its block of 32 among 32 neighbouring positions; f16
+ * results are rounded once.  Uses the library's per-stream scratch. */
 int izwi_decode_shared_attention_f32(int type, const float* q, int64_t q_stride, int64_t batch, int64_t beams,
                                      int64_t num_heads, int64_t num_kv_heads, int64_t head_dim, const void* prefix,
                                      int64_t prefix_slots, int64_t prefix_capacity, const int32_t* prefix_lens,

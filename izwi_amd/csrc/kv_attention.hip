@@ -15,7 +15,9 @@
 //    largest, where the second number ends, whichever is more, so that many positions far below a few that dominate keep their sum.  (With the
 //    largest between 2^5 and 2^15, which moves even less, 2^15 positions that have 2^-13 to 2^-27 of four others' weight each came out up to
 //    28 % of their sum wrong, now 0.3 %, 2^-22 of the whole; moving costs some 2 % where many rows share positions.)  The values' scales stand under the power
-//    of two that takes the largest of their block of the head so far to below 1.  Weight times scale is a product of f16 pairs whose loss
+//    of two that takes the largest of their block of the head and of the 32 positions to below 1, where those between 2^-12 and 1 of the last one
+//    keep it: a scale is exact down to 2^-14 of the largest there, and off by 2^-25 of it below that.  (A power of two that never fell again let a single
+//    large value cost all that follow their bits; looking for one costs 1 % where little is to do: 300 positions 6.8 us, not 6.7.)  Weight times scale is a product of f16 pairs whose loss
 //    a fused multiply-add returns exactly: packed, half the instructions of f32 products split afterwards.
 //    f16 queries are themselves.  (Weights of f16 results as single f16 numbers, rounded to f16 and once more under the scale, left 2.8e-4 of a
 //    result where its own rounding leaves 2.1e-4, and far more where values cancel.)
@@ -329,13 +331,20 @@ __device__ __forceinline__ void attend_rows(const AttendParams& P, int id, float
     // of the lane's row: the maximum that the reference stands on, the product that makes a new one, the reference, this lane's sum of weights
     float top[RT], bar[RT], ref[RT], l[RT];
     f4 o[RT][2 * NB];
-    // Of each block of the head: what its value scales are multiplied by, the power of two that takes the largest so far to below 1 (2^15 at most).
-    // A lane has it for the blocks of its value scales, and as f16 bits the scale that needs another.
+    // Of each block of the head: what its value scales are multiplied by, the power of two that takes the largest of a tile to below 1 (2^15 at
+    // most).  A lane has it for the blocks of its value scales, and as f16 bits which scales need another: at or above 1 / it, or (less one) below
+    // 2^-12 of that.
     float up[SW];
-    uint32_t e_bits[SW];
+    uint32_t over[SW], under[SW];
+    auto two_to = [](int n) { return __uint_as_float((uint32_t)(127 + n) << 23); };
+    auto set_up = [&](int i, int n) { // 2^n
+        up[i] = two_to(n);
+        over[i] = __builtin_bit_cast(uint16_t, (f16_t)two_to(-n)); // (2^16: infinity's)
+        under[i] = max(1u, (uint32_t)__builtin_bit_cast(uint16_t, (f16_t)two_to(-12 - n))) - 1;
+    };
     auto up_of = [&](auto b) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(up[b % SW]), b / SW)); };
 #pragma unroll
-    for (int i = 0; i < SW; i++) up[i] = 32768.0f, e_bits[i] = 0x200;
+    for (int i = 0; i < SW; i++) set_up(i, 15);
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
         top[rt] = bar[rt] = ref[rt] = -INFINITY, l[rt] = 0.0f;
@@ -390,36 +399,24 @@ __device__ __forceinline__ void attend_rows(const AttendParams& P, int id, float
                 }
             }
         }
-        // does a row's maximum, or the values' largest scale, rise?
-        bool rise = false;
-#pragma unroll
-        for (int i = 0; i < SW; i++) {
-            const u2 most = magnitudes<QT>(t.s.w[i]);
-            rise |= max((uint32_t)most[0], (uint32_t)most[1]) >= e_bits[i];
-        }
+        // does a row's maximum rise, or do the values' scales leave the range of their power of two?
+        bool rise[RT], any_rise = false, odd = false;
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) {
             float m = s[rt][0];
 #pragma unroll
             for (int j = 1; j < 8; j++) m = fmaxf(m, s[rt][j]);
-            rise |= m > bar[rt];
+            rise[rt] = m > bar[rt], any_rise |= rise[rt];
         }
-        if (__any(rise)) {
-            float down[SW]; // of what is there
 #pragma unroll
-            for (int i = 0; i < SW; i++) {
-                const h2 two = __builtin_bit_cast(h2, magnitudes<QT>(t.s.w[i]));
-                float d = fmaxf(0.0f, fmaxf((float)two[0], (float)two[1])); // (passes over the NaN of a block that holds one)
-                d = fmaxf(d, dpp_f<0x128>(d)); // over the lanes x that have this block: row_ror 8, 4 (and 2)
-                d = fmaxf(d, dpp_f<0x124>(d));
-                if constexpr (VL == 2) d = fmaxf(d, dpp_f<0x122>(d));
-                const int e = (int)(__float_as_uint(qmm_max_lane_rows(d)) >> 23) - 127;
-                const float to = fminf(up[i], __uint_as_float((uint32_t)(127 + min(15, -1 - e)) << 23));
-                down[i] = to / up[i], up[i] = to;
-                e_bits[i] = __builtin_bit_cast(uint16_t, (f16_t)(1.0f / to)); // (1 / 2^-16: infinity's)
-            }
+        for (int i = 0; i < SW; i++) {
+            const u2 size = magnitudes<QT>(t.s.w[i]), less_one = size - u2{1, 1}; // (a scale of zero is not a small one)
+            odd |= max((uint32_t)size[0], (uint32_t)size[1]) >= over[i] || min((uint32_t)less_one[0], (uint32_t)less_one[1]) < under[i];
+        }
+        if (__any(any_rise || odd)) {
 #pragma unroll
             for (int rt = 0; rt < RT; rt++) {
+                if (!__any(rise[rt])) continue;
                 float m = s[rt][0];
 #pragma unroll
                 for (int j = 1; j < 8; j++) m = fmaxf(m, s[rt][j]);
@@ -428,9 +425,28 @@ __device__ __forceinline__ void attend_rows(const AttendParams& P, int id, float
                 // (from 2^24 on scores are whole numbers two or more apart, and a reference rounded further up would take a weight beyond f16)
                 const float to = fabsf(top[rt]) < 0x1p24f ? top[rt] - kHead : top[rt], by = ref[rt] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ref[rt] - to);
                 ref[rt] = to, l[rt] *= by;
+#pragma unroll
+                for (int i = 0; i < 2 * NB; i++) o[rt][i] *= by;
+            }
+            if (__any(odd)) {
+                float down[SW]; // of what is there
+#pragma unroll
+                for (int i = 0; i < SW; i++) {
+                    const h2 two = __builtin_bit_cast(h2, magnitudes<QT>(t.s.w[i]));
+                    float d = fmaxf(0.0f, fmaxf((float)two[0], (float)two[1])); // (passes over the NaN of a block that holds one)
+                    d = fmaxf(d, dpp_f<0x128>(d)); // over the lanes x that have this block: row_ror 8, 4 (and 2)
+                    d = fmaxf(d, dpp_f<0x124>(d));
+                    if constexpr (VL == 2) d = fmaxf(d, dpp_f<0x122>(d));
+                    d = qmm_max_lane_rows(d);
+                    const int was = (int)(__float_as_uint(up[i]) >> 23) - 127, e = (int)(__float_as_uint(d) >> 23) - 127;
+                    const int n = d == 0.0f ? was : min(15, -1 - e);
+                    down[i] = two_to(n - was);
+                    set_up(i, n);
+                }
                 each<NB>([&](auto b) {
-                    const float by_o = by * __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(down[b % SW]), b / SW));
-                    o[rt][2 * b] *= by_o, o[rt][2 * b + 1] *= by_o;
+                    const float by = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(down[b % SW]), b / SW));
+#pragma unroll
+                    for (int rt = 0; rt < RT; rt++) o[rt][2 * b] *= by, o[rt][2 * b + 1] *= by;
                 });
             }
         }

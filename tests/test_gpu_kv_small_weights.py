@@ -1,9 +1,11 @@
-"""GPU tests (pytest -m gpu) of what small weights add to the attention over the quantized cache.  Bounds: test_gpu_kv_exactness.py."""
+"""GPU tests (pytest -m gpu) of what small weights and small values add to the attention over the quantized cache: many positions far below a few
+that dominate, and values of one size beside values of another.  Bounds: test_gpu_kv_exactness.py."""
 import numpy as np
 import pytest
 import torch
 
 from test_gpu_kv_decode import dev, ints, qa  # noqa: F401
+from test_gpu_kv_exactness import PLANS, Attend, check, rows_of, slots_of
 
 pytestmark = pytest.mark.gpu
 
@@ -35,3 +37,27 @@ def test_many_positions_behind_a_few(qa, beams, quant):
     got = out.cpu().double().numpy()
     print(f"worst error / tolerance {np.max(np.abs(got - want[..., None]) / tol[..., None]):.3f}", flush=True)
     assert (np.abs(got - want[..., None]) <= tol[..., None]).all()
+
+
+@pytest.mark.parametrize("dtype", ("f32", "f16"))
+@pytest.mark.parametrize("plan", PLANS)
+@pytest.mark.parametrize("quant,d", [("Q8_0", 128), ("Q4_0", 64), ("Q4_0", 256)])
+def test_values_beside_far_larger_ones(qa, quant, d, dtype, plan):
+    """Values 2^10 larger than their neighbours in the tile of 32 positions, and a tile of values 2^19 larger in front of it or behind it, all under a
+    weight that leaves nothing of them, cost the others no bits: the bound's largest value is that of the tile."""
+    rng = np.random.default_rng(d)
+    n, slots, kv = 45, slots_of(plan), PLANS[plan]["kv"]
+    k, v = (rng.normal(size=(slots, n, kv, d)).astype(np.float16).astype(np.float32) for _ in range(2))
+    k[..., 0] = 0.0
+    v *= 2.0 ** -6
+    for b in range(slots):
+        far = np.arange(32, n) if b % 2 else np.arange(32)
+        near = [33 + b % 5, 40] if b % 2 == 0 else [b % 16, 20]
+        v[b, far] *= 2.0 ** 19
+        v[b, near] *= 2.0 ** 10
+        k[b, far, :, 0] = k[b, near, :, 0] = -1.0
+    v = np.clip(v.astype(np.float16).astype(np.float32), -6e4, 6e4)
+    call = Attend(qa, plan, quant, dtype, k, v, [n - b % 3 for b in range(slots)], prefix_len=0)
+    q = rng.normal(size=rows_of(plan, d)).astype(np.float16).astype(np.float32)
+    q[..., 0] = 200.0 * d ** 0.5 * 2  # positions with the large values: some 2^-290 and less of the largest weight
+    check(call, q, 0.5 * d ** -0.5, dtype, largest=2.0 ** 10 * 5 * 2.0 ** -6)
