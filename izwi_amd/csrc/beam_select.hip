@@ -47,7 +47,7 @@ __device__ __forceinline__ uint32_t order_of(float v) {
 }
 __device__ __forceinline__ float value_of(uint32_t o) { return __uint_as_float(o ^ ((int32_t)o < 0 ? 0x80000000u : 0xffffffffu)); }
 __device__ __forceinline__ uint64_t order_of(double v) {
-    const uint64_t u = (uint64_t)__double_as_longlong(v);
+    const uint64_t u = (uint64_t)__double_as_longlong(v + 0.0); // (a finished beam's score may be -0)
     return u ^ ((int64_t)u < 0 ? ~0ull : 1ull << 63);
 }
 __device__ __forceinline__ double double_of(uint64_t o) {
