@@ -84,19 +84,24 @@ __device__ __forceinline__ double wave_sum(double v) {
 }
 __device__ __forceinline__ float wave_max(float v) { return qmm_max_lane_rows(row16_max(v)); }
 
-// e^d for d <= 0 (or -infinity: 0) in f64 to 4e-11 of itself: 2^n 2^f with n + f = d log2(e), |f| <= 1/2, and for 2^f the polynomial of
-// degree 7 with the least largest relative error (Remez' exchange, in 64 bits of mantissa).  Less than half of what the library's exp takes.
+// e^d for d <= 0 (or -infinity: 0) in f64 to 7e-16 of itself, e^0 = 1: 2^n 2^f with n + f = d log2(e), |f| <= 1/2, and 2^f as 1 + f times the
+// polynomial of degree 9 that meets (2^f - 1) / f at its Chebyshev nodes (worked out with 60 digits).  Less than half of what the library's exp
+// takes.  (Three degrees less leave 4e-11, e^0 among it: a beam with one token left had a log-probability of 8e-11 instead of 0, and beams that
+// close changed places.  They are 1.8 us of 36.7 for 16 prompts of 8 beams over 151936 tokens.)
 __device__ __forceinline__ double exp_of(double d) {
     // (1.5 * 2^52 leaves no place behind the point: the low word of the sum is n)
     const double y = __builtin_fmax(d * 1.4426950408889634, -1100.0), t = y + 0x1.8p52, f = y - (t - 0x1.8p52);
-    double p = 0x1.fe17831d538a2p-17;
-    p = __builtin_fma(p, f, 0x1.446a1fdacba4ep-13);
-    p = __builtin_fma(p, f, 0x1.5d8a7088fdb8dp-10);
-    p = __builtin_fma(p, f, 0x1.3b29dc40d6647p-7);
-    p = __builtin_fma(p, f, 0x1.c6b08aaf2e311p-5);
-    p = __builtin_fma(p, f, 0x1.ebfbe0a4be818p-3);
-    p = __builtin_fma(p, f, 0x1.62e42ff116290p-1);
-    p = __builtin_fma(p, f, 0x1.ffffffffabbcdp-1);
+    double p = 0x1.e5e9f548e5725p-28;
+    p = __builtin_fma(p, f, 0x1.b6571de2f2351p-24);
+    p = __builtin_fma(p, f, 0x1.62bfe46117445p-20);
+    p = __builtin_fma(p, f, 0x1.ffcb76789860fp-17);
+    p = __builtin_fma(p, f, 0x1.4309130378460p-13);
+    p = __builtin_fma(p, f, 0x1.5d87fe908f88ap-10);
+    p = __builtin_fma(p, f, 0x1.3b2ab6fba385fp-7);
+    p = __builtin_fma(p, f, 0x1.c6b08d7044119p-5);
+    p = __builtin_fma(p, f, 0x1.ebfbdff82c590p-3);
+    p = __builtin_fma(p, f, 0x1.62e42fefa39f7p-1);
+    p = __builtin_fma(p, f, 1.0);
     return __builtin_ldexp(p, (int)__double_as_longlong(t));
 }
 
