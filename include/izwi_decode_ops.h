@@ -177,7 +177,8 @@ int izwi_decode_kv_read_f16(int type, const void* cache, int64_t slots, int64_t 
  * head, or a value's block of 32.  Lengths above max_prefix_len (max_len), the caller's bounds, count as
  * those, negative ones as zero; the work is shared out by the bounds.  With `lineage`, `[slots][kv_capacity rounded up to
  * 32]`, position p of sequence b is in the slot of beam lineage[b][p] of its prompt; a position whose entry is no beam
- * (>= beams) does not count.  The products run on the matrix cores with f32 sums; f32 queries and the weights go as
+ * (>= beams) does not count.  What a sequence writes before the first selection is its own: rows begin as b % beams (zeros would
+ * read the first beam's positions).  The products run on the matrix cores with f32 sums; f32 queries and the weights go as
  * two f16 numbers each, 22 bits down to 2^-16 of the row's largest number in q and 2^-14 of its largest weight, fewer of
  * what is smaller; a value counts to 2^-24 of the largest of its block of 32 among 32 neighbouring positions; f16
  * results are rounded once.  Uses the library's per-stream scratch. */

@@ -10,7 +10,7 @@ history copies a row of bytes instead of keys and values.  The reference keeps s
     prompt = QuantizedKvCache(KvCacheType.Q8_0, prompts, kv_heads, prompt_capacity, head_dim)
     answers = QuantizedKvCache(KvCacheType.Q8_0, prompts * beams, kv_heads, answer_capacity, head_dim)
     prompt.append(k, v, starts)                                   # once, k / v [prompts, tokens, kv_heads, head_dim]
-    lineage, lens = answers.new_lineage(), zeros of int32
+    lineage, lens = answers.new_lineage(beams), zeros of int32    # every beam begins with positions of its own
     # a step: per layer append and attend, then pick (the lineage is every layer's)
     answers.append(k, v, lens)                                    # k / v [prompts * beams, 1, kv_heads, head_dim]
     out = shared_prefix_attention(q, answers, lens + 1, prefix=prompt, prefix_lens=prompt_lens, lineage=lineage)
@@ -101,9 +101,16 @@ class QuantizedKvCache:
         self._index, self._ptr, self._type, self._row = self.buffer.get_device(), self.buffer.data_ptr(), int(dtype), kv_heads * head_dim
         self._lineage_shape = (slots, -(-capacity // _PAD) * _PAD)
 
-    def new_lineage(self) -> torch.Tensor:
-        """Lineage rows of all slots, [slots, capacity rounded up to 32] uint8, zeros: no position has been written."""
-        return torch.zeros(self._lineage_shape, dtype=torch.uint8, device=self.device)
+    def new_lineage(self, beams: int | None = None) -> torch.Tensor:
+        """Lineage rows of all slots, [slots, capacity rounded up to 32] uint8.  With ``beams`` sequences a prompt every position is its
+        own slot's, as it has to be for what is written before the first ``beam_select`` (which names the beams from then on).
+        Without, zeros: every position is the first beam's of the prompt, which is right where that beam's first token is all beams'."""
+        rows = torch.zeros(self._lineage_shape, dtype=torch.uint8, device=self.device)
+        if beams is not None:
+            if not 0 < beams <= 255 or self.slots % beams:
+                _refuse(f"new_lineage: {beams} beams in {self.slots} slots (at most 255, a divisor)")
+            rows += (torch.arange(self.slots, device=self.device) % beams).to(torch.uint8).unsqueeze(1)
+        return rows
 
     def append(self, k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor, counts: torch.Tensor | None = None, first_slot: int = 0) -> None:
         """k, v [sequences, tokens, kv_heads, head_dim] (f32 or f16; rows may be parts of wider ones): token t of
