@@ -140,3 +140,27 @@ def test_weights_keep_more_bits_than_an_f16(qa, quant, d, dtype, plan):
     r = (1 - want[..., 0]) / (1 + want[..., 0])  # the second weight relative to the first
     rounded = r.astype(np.float16).astype(np.float64)
     assert (np.abs((1 - rounded) / (1 + r) - want[..., 0]) > tol[..., 0]).any()
+
+
+@pytest.mark.parametrize("plan", PLANS)
+@pytest.mark.parametrize("quant,d", [("Q8_0", 64), ("Q4_0", 64), ("Q8_0", 128), ("Q4_0", 128), ("Q8_0", 256), ("Q4_0", 256)])
+def test_f32_queries_keep_more_bits_than_an_f16(qa, quant, d, plan):
+    """Queries whose f16 part is orthogonal to the keys: the scores, and the result, are what is left of an f32 query behind its f16."""
+    print("queries", quant, d, plan, flush=True)
+    rng = np.random.default_rng(d + 1)
+    k, v = np.zeros((slots_of(plan), 2, PLANS[plan]["kv"], d), np.float32), np.ones((slots_of(plan), 2, PLANS[plan]["kv"], d), np.float32)
+    v[:, 1] = -1
+    rows = rows_of(plan, d)
+    q = np.zeros(rows, np.float32)
+    for b in range(0, d, 32):  # of a block: its scale from a key that no query sees, then 15 pairs of keys 7/8, -7/8
+        k[:, 0, :, b] = 1
+        k[:, 0, :, b + 1:b + 31:2], k[:, 0, :, b + 2:b + 31:2] = 0.875, -0.875
+        x = rng.integers(1024, 2048, size=rows[:2] + (15,)) / 1024.0
+        t = rng.uniform(0.2, 0.45, size=x.shape) * 2.0 ** -10  # (less than half an f16's step from x)
+        q[..., b + 1:b + 31:2], q[..., b + 2:b + 31:2] = x + t, x - t
+    k[:, 1] = -k[:, 0]
+    call = Attend(qa, plan, quant, "f32", k, v, [2] * len(k), prefix_len=0)
+    scale = 8.0 / (d * 30 / 32 * 1.5)
+    want, tol = check(call, q, scale, "f32")
+    lost = call.exact(q.astype(np.float16).astype(np.float32), scale)[0]  # the result of f16 queries
+    assert (np.abs(lost - want) > 2 * tol).all()  # (the bound resolves it)
