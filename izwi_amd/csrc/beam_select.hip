@@ -10,8 +10,8 @@
 // a whole number.  Within a beam the order is the logits' own, in f32.
 //
 // Many logits are bound by the issue of vector instructions, half of them the exponentials in f64 (16 prompts of 8 beams over 151936
-// tokens, 78 MB: 26 us, 3.0 TB/s, and 8 for the second launch); fewer by the launches and each one's chain of
-// loads and barriers (4 beams of 151936: 5 and 6 us).
+// tokens, 78 MB: 28 us, 2.8 TB/s, and 9 for the second launch); fewer by the launches and each one's chain of
+// loads and barriers (4 beams of 151936: 5.7 and 5.6 us).
 #include "kv_cache.h"
 #include "qmm_lanes.h"
 #include "qmm_records.h"
@@ -85,9 +85,9 @@ __device__ __forceinline__ double wave_sum(double v) {
 __device__ __forceinline__ float wave_max(float v) { return qmm_max_lane_rows(row16_max(v)); }
 
 // e^d for d <= 0 (or -infinity: 0) in f64 to 7e-16 of itself, e^0 = 1: 2^n 2^f with n + f = d log2(e), |f| <= 1/2, and 2^f as 1 + f times the
-// polynomial of degree 9 that meets (2^f - 1) / f at its Chebyshev nodes (worked out with 60 digits).  Less than half of what the library's exp
-// takes.  (Three degrees less leave 4e-11, e^0 among it: a beam with one token left had a log-probability of 8e-11 instead of 0, and beams that
-// close changed places.  They are 1.8 us of 36.7 for 16 prompts of 8 beams over 151936 tokens.)
+// polynomial of degree 9 that meets (2^f - 1) / f at its Chebyshev nodes (worked out with 60 digits).  (Three degrees less leave 4e-11, e^0
+// among it: a beam with one token left had a log-probability of 8e-11 instead of 0, and beams that close changed places.  They are 1.8 us of
+// 36.7 for 16 prompts of 8 beams over 151936 tokens.)
 __device__ __forceinline__ double exp_of(double d) {
     // (1.5 * 2^52 leaves no place behind the point: the low word of the sum is n)
     const double y = __builtin_fmax(d * 1.4426950408889634, -1100.0), t = y + 0x1.8p52, f = y - (t - 0x1.8p52);

@@ -23,11 +23,12 @@
 //    result where its own rounding leaves 2.1e-4, and far more where values cancel.)
 //
 // Bound by memory where few rows share positions: 32 sequences of 4001 positions of 32 heads on 8, D = 128, Q8_0, 40 us in a graph, 5.5 TB/s.
-// By the issue of vector instructions around the matrix products where many do (per tile of 32 positions and 32 f32 rows about 450 beside 64
-// matrix instructions, some 2650 cycles whether a SIMD has one wave or two): 64 rows a kv head on 131072 positions 99 to 110 us, 2.7 TB/s and
-// 330 TFLOP/s; 256 f16 rows a kv head on 8192 positions and 250 own of each sequence, Q4_0, 28 us, 310 TFLOP/s.  By two launches and the way to
-// memory and back where there is little to do: 8 beams behind 1501 positions 9.3 us, one sequence of 300 6.8.
-// Two row tiles a workgroup halve the conversions (65 -> 55 us at 64 rows a kv head on 60000 positions); four do not fit the registers.
+// By the issue of vector instructions around the matrix products where many do (per tile of 32 positions and 32 f32 rows about 500 beside 64
+// matrix instructions, as fast with one wave on a SIMD as with two): 64 rows a kv head on 131072 positions 108 to 115 us, 2.6 TB/s and
+// 310 TFLOP/s; 256 f16 rows a kv head on 8192 positions and 250 own of each sequence, Q4_0, 34 us, 250 TFLOP/s.  By two launches and the way to
+// memory and back where there is little to do: 8 beams behind 1501 positions 9.3 us; by one and a workgroup's chain of loads: 300 positions of one
+// sequence 6.8.
+// Two row tiles a workgroup halve the conversions (65 -> 53 us at 64 rows a kv head on 60000 positions); four do not fit the registers.
 #include "kv_cache.h"
 
 #include <algorithm>
@@ -146,8 +147,8 @@ __device__ __forceinline__ void attend_rows(const AttendParams& P, int id, float
     using Row = KvRow<QT, D>;
     constexpr int NB = Row::kBlocks, KW = Row::kBytes / 16, VW = Row::kLane, ROWS = 16 * RT;
     // TWO: two tiles in registers.  Not where they do not fit beside the rest: with heads of 256 the second one leaves a SIMD one wave instead
-    // of two or moves values to and fro (88 sequences of 64 heads on 8, f16 and Q4_0, 818 positions and 29 own: 46 us with it, 35 without; f32 and
-    // Q8_0 59 and 56).
+    // of two or moves values to and fro (88 sequences of 64 heads on 8, f16 and Q4_0, 818 positions and 29 own: 50 us with it, 41 without; f32 and
+    // Q8_0 59 and 55).
     constexpr bool SPLIT = sizeof(T) == 4, TWO = RT == 1 && !LIN && D <= 128;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int x = lane & 15, g = lane >> 4;
@@ -778,7 +779,7 @@ int shared_attention_impl(int type, const T* q, int64_t q_stride, int64_t batch,
     P.scale = scale;
     hipStream_t stream = (hipStream_t)stream_;
     // Workgroups of four waves, about one per compute unit, each with the positions of a split in turns of 32 per wave (two per compute unit
-    // take 2 us more nearly everywhere, for more to join: 8 sequences of 800 positions 8.8 us -> 9.8, 32 of 2000 25.4 -> 27.8, 64 rows on 32000 17.5 -> 19.0).
+    // take 2 us more nearly everywhere, for more to join: 8 sequences of 800 positions 8.5 us -> 9.5, 32 of 2000 25.4 -> 27.6, 16 beams on 32000 34 -> 38).
     constexpr int waves = kWaves;
     const auto turns = [&](int64_t n_seq, int most, int rows, int rt) { // of a wave, with one workgroup per compute unit
         const int64_t base = n_seq * kv_heads * ((rows + 16 * rt - 1) / (16 * rt)), tiles = (most + 31) / 32;
@@ -786,7 +787,7 @@ int shared_attention_impl(int type, const T* q, int64_t q_stride, int64_t batch,
         return tiles / (splits * waves);
     };
     // Few positions of one kind stay with one workgroup per sequence and kv head: nothing is left to join, and the host has a launch less (16
-    // heads on 8, in a graph: 200 positions 6.0 us instead of 7.2, 380 7.1 instead of 7.3; but 600 8.8 instead of 7.4).
+    // heads on 8, in a graph: 200 positions 5.9 us instead of 7.1, 380 6.8 instead of 7.2; but 600 8.5 instead of 7.4).
     constexpr int kOneLaunchTiles = 12;
     const bool alone = P.max_prefix == 0 || P.max_len == 0;
     const auto units = [&](int64_t n_seq, int most, int rows, int rt, int& splits, int& n_units, int& z) {
@@ -803,14 +804,14 @@ int shared_attention_impl(int type, const T* q, int64_t q_stride, int64_t batch,
         n_units = (int)(n_seq * kv_heads * splits);
     };
     // two tiles of query rows to a workgroup where there are two and the waves have enough to do all the same (32 heads on 8, 16 beams: 60000
-    // positions 65 -> 55 us, 4 prompts of 4000 26.0 -> 23.8; but 2000 12.4 -> 14.1, 8 beams on 1000 8.5 -> 10.7)
+    // positions 65 -> 53 us, 32000 40 -> 34; but 2000 10.1 -> 12.9, 8 beams on 1000 8.4 -> 10.8; 4 prompts of 4000, just below the bound, 24.6 -> 22.9)
     const int prompt_rows = (int)(beams * P.group);
     const int rt = d <= 128 && prompt_rows > 16 && turns(batch / beams, P.max_prefix, prompt_rows, 2) >= 8 ? 2 : 1;
     units(batch / beams, P.max_prefix, prompt_rows, rt, P.prefix_splits, P.prefix_units, P.prefix_z);
     units(batch, P.max_len, P.group, 1, P.own_splits, P.own_units, P.own_z);
     // A wave to each where that still fills the compute units, the better the shorter they are: a workgroup's prologue, its meeting in LDS and
-    // its idle waves cost more than the positions of a short sequence (371 sequences of up to 14 own positions behind 570, 32 heads on 8: 53 ->
-    // 40 us; but 132 of up to 355: 28 -> 30).
+    // its idle waves cost more than the positions of a short sequence (371 sequences of up to 14 own positions behind 570, 32 heads on 8: 50 ->
+    // 35 us; but 132 of up to 355: 24.5 -> 30).
     P.own_solo = P.own_splits == 1 && (int64_t)P.own_units * P.own_z >= kWaves * n_cus * std::max<int64_t>(1, (P.max_len + 31) / 32 / 4);
     P.prefix_wgs = (P.prefix_units + 7) / 8 * 8 * P.prefix_z;
     P.parts = P.prefix_splits + P.own_splits;
