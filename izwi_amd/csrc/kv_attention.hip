@@ -676,8 +676,8 @@ __global__ __launch_bounds__(256) void attend_join_kernel(const float* __restric
         sum = sum * old + sum8(by == 0.0f ? 0.0f : st.y * by);
         a *= old;
 #pragma unroll
-        for (int i = 0; i < A; i++) // uniform
-            if (there >> i & 1) a += v[i] * __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(by), i));
+        for (int i = 0; i < A; i++) // (no branch: it would take the load with it, one after the other)
+            a += (there >> i & 1 ? v[i] : vec(0.0f)) * __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(by), i));
         to = next;
     }
     if constexpr (FEW) {
