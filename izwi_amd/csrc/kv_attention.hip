@@ -415,6 +415,10 @@ __device__ __forceinline__ void attend_rows(const AttendParams& P, int id, float
             odd |= max((uint32_t)size[0], (uint32_t)size[1]) >= over[i] || min((uint32_t)less_one[0], (uint32_t)less_one[1]) < under[i];
         }
         if (__any(any_rise || odd)) {
+            bool begun = false; // (before a row has a reference there is nothing to rescale)
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) begun |= ref[rt] != -INFINITY;
+            begun = __any(begun);
 #pragma unroll
             for (int rt = 0; rt < RT; rt++) {
                 if (!__any(rise[rt])) continue;
@@ -426,8 +430,9 @@ __device__ __forceinline__ void attend_rows(const AttendParams& P, int id, float
                 // (from 2^24 on scores are whole numbers two or more apart, and a reference rounded further up would take a weight beyond f16)
                 const float to = fabsf(top[rt]) < 0x1p24f ? top[rt] - kHead : top[rt], by = ref[rt] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ref[rt] - to);
                 ref[rt] = to, l[rt] *= by;
+                if (begun)
 #pragma unroll
-                for (int i = 0; i < 2 * NB; i++) o[rt][i] *= by;
+                    for (int i = 0; i < 2 * NB; i++) o[rt][i] *= by;
             }
             if (__any(odd)) {
                 float down[SW]; // of what is there
@@ -444,11 +449,12 @@ __device__ __forceinline__ void attend_rows(const AttendParams& P, int id, float
                     down[i] = two_to(n - was);
                     set_up(i, n);
                 }
-                each<NB>([&](auto b) {
-                    const float by = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(down[b % SW]), b / SW));
+                if (begun)
+                    each<NB>([&](auto b) {
+                        const float by = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(down[b % SW]), b / SW));
 #pragma unroll
-                    for (int rt = 0; rt < RT; rt++) o[rt][2 * b] *= by, o[rt][2 * b + 1] *= by;
-                });
+                        for (int rt = 0; rt < RT; rt++) o[rt][2 * b] *= by, o[rt][2 * b + 1] *= by;
+                    });
             }
         }
         // weights
