@@ -147,8 +147,8 @@ __device__ __forceinline__ void attend_rows(const AttendParams& P, int id, float
     using Row = KvRow<QT, D>;
     constexpr int NB = Row::kBlocks, KW = Row::kBytes / 16, VW = Row::kLane, ROWS = 16 * RT;
     // TWO: two tiles in registers.  Not where they do not fit beside the rest: with heads of 256 the second one leaves a SIMD one wave instead
-    // of two or moves values to and fro (88 sequences of 64 heads on 8, f16 and Q4_0, 818 positions and 29 own: 50 us with it, 41 without; f32 and
-    // Q8_0 59 and 55).
+    // of two or moves values to and fro (88 sequences of 64 heads on 8, f16 and Q4_0, 818 positions and 29 own: 49 us with it, 38 without; f32 and
+    // Q8_0 57 and 53).
     constexpr bool SPLIT = sizeof(T) == 4, TWO = RT == 1 && !LIN && D <= 128;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int x = lane & 15, g = lane >> 4;
