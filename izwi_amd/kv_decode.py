@@ -165,7 +165,8 @@ def shared_prefix_attention(q: torch.Tensor, cache: QuantizedKvCache | None, len
                             scale: float | None = None, max_len: int | None = None, max_prefix_len: int | None = None) -> torch.Tensor:
     """Attention of one new token per sequence: q [sequences, heads, head_dim] (f32 or f16) over positions 0 ..
     prefix_lens[b // beams] - 1 of its prompt's slot of ``prefix`` and 0 .. lens[b] - 1 of its own slot of ``cache`` (found by ``lineage``
-    if given).  Either cache may be None.  A sequence without any position gives zeros.  ``beams``: sequences per prompt,
+    if given).  Either cache may be None.  A sequence without any position gives zeros, a NaN that it reads NaN (a value's: in its block of
+    32).  ``beams``: sequences per prompt,
     by default sequences // len(prefix_lens), or all of them without a prefix.  ``max_len`` and ``max_prefix_len`` bound the lengths where
     the caller knows them better than the capacities: the work is shared out by them.  Returns [sequences, heads, head_dim]."""
     dtype, shape = q.dtype, q.shape
