@@ -1,7 +1,8 @@
 /*
  * izwi_decode_ops — the decode-step neighbours of the quantized projections: RMSNorm, the
  * q/k head norm, rotary embedding and single-token grouped-query attention, f32 and f16; for several
- * continuations of one prompt a quantized key / value cache, the attention over it and beam search's selection.
+ * continuations of one prompt a quantized key / value cache, the attention over it and beam search's selection; for whole prompts
+ * rotary positions and attention, f32, f16 and bf16.
  *
  * Each entry point is the device side of one of the reference's fused-kernel hooks
  * (crates/izwi-core/src/kernels/mod.rs:109-225), which today dispatch to Metal only
@@ -212,6 +213,73 @@ int izwi_decode_beam_select_f32(const float* logits, int64_t prompts, int64_t be
                                 const uint8_t* finished, int64_t eos_token, int32_t* tokens, int32_t* parents,
                                 float* scores_out, uint8_t* finished_out, const uint8_t* lineage,
                                 int64_t lineage_capacity, const int32_t* lens, uint8_t* lineage_out, void* stream);
+
+/* ---- whole prompts ---------------------------------------------------------------------------------------------
+ *
+ * What a prompt's layer needs between its projections: prompts of different lengths stand one behind the other as rows of tokens,
+ * each token with its own position, rows strided (parts of a q|k|v row).  f32, f16 and bf16 (raw bits as uint16_t), every tensor
+ * of a call of one type; arithmetic in f32, results rounded once.  Device pointers only throughout. */
+
+/* Angles per position of the rotary_dim / 2 pairs of a head: base^(-2 i / rotary_dim), for a context stretched to `factor` times
+ * original_len positions (factor >= 1) by
+ *   LINEAR  every frequency divided by factor;
+ *   NTK     base times factor^(rotary_dim / (rotary_dim - 2));
+ *   LLAMA3  frequencies that turn `low` times or less in original_len divided by factor, those that turn `high` times or more
+ *           kept, between them the mean weighted by the turns;
+ *   YARN    the same with weights by the pair's number, between floor(pair that turns `high` times) and ceil(pair that turns
+ *           `low` times), cosine and sine times 0.1 ln(factor) + 1.
+ * (The models' usual low and high: 1 and 4, 1 and 32.)  Host memory: frequencies [rotary_dim / 2], attention_factor what cosine and
+ * sine are to be multiplied by.  No device work. */
+enum { IZWI_ROPE_PLAIN = 0, IZWI_ROPE_LINEAR = 1, IZWI_ROPE_NTK = 2, IZWI_ROPE_LLAMA3 = 3, IZWI_ROPE_YARN = 4 };
+int izwi_rope_frequencies(int scaling, int64_t rotary_dim, double base, double factor, double original_len, double low, double high,
+                          double* frequencies, double* attention_factor);
+
+/* Rotary embedding at each token's own position, of the first rotary_dim (even) elements of every head; the rest is copied.  q is
+ * `[tokens, q_heads, head_dim]`, k `[tokens, k_heads, head_dim]`, strides the elements from one token to the next (heads contiguous;
+ * a number of heads may be 0); positions `[tokens]`, any int32; frequencies `[rotary_dim / 2]` (device), radians a position.  Pairs
+ * are (i, rotary_dim / 2 + i), or with `interleaved` = 1 (2 i, 2 i + 1): (a, b) becomes (a c - b s, a s + b c), c and s being
+ * attention_factor times cosine and sine of position * frequency, which is worked out in 64 bits.  qk_weight `[2 * head_dim]` (NULL:
+ * none): first every head is normed as by izwi_qk_rms_norm, x * rsqrt(mean(x^2) + eps) * weight, without a rounding in between.
+ * head_dim even, at most 1024.  An output may be its own input and shares no other memory (rows of equal stride may lie between each
+ * other, as parts of a q|k|v row do). */
+int izwi_rope_positions_f32(const float* q, int64_t q_stride, const float* k, int64_t k_stride, const int32_t* positions,
+                            const double* frequencies, float attention_factor, int64_t tokens, int64_t q_heads, int64_t k_heads,
+                            int64_t head_dim, int64_t rotary_dim, int interleaved, const float* qk_weight, float eps,
+                            float* q_out, int64_t q_out_stride, float* k_out, int64_t k_out_stride, void* stream);
+int izwi_rope_positions_f16(const uint16_t* q, int64_t q_stride, const uint16_t* k, int64_t k_stride, const int32_t* positions,
+                            const double* frequencies, float attention_factor, int64_t tokens, int64_t q_heads, int64_t k_heads,
+                            int64_t head_dim, int64_t rotary_dim, int interleaved, const uint16_t* qk_weight, float eps,
+                            uint16_t* q_out, int64_t q_out_stride, uint16_t* k_out, int64_t k_out_stride, void* stream);
+int izwi_rope_positions_bf16(const uint16_t* q, int64_t q_stride, const uint16_t* k, int64_t k_stride, const int32_t* positions,
+                             const double* frequencies, float attention_factor, int64_t tokens, int64_t q_heads, int64_t k_heads,
+                             int64_t head_dim, int64_t rotary_dim, int interleaved, const uint16_t* qk_weight, float eps,
+                             uint16_t* q_out, int64_t q_out_stride, uint16_t* k_out, int64_t k_out_stride, void* stream);
+
+/* Attention of packed sequences: softmax((q . k) * scale) . v of every query over the positions of its own sequence, with `causal` those
+ * up to its own, the last query seeing the last key: query i of n sees keys 0 .. i + (m - n) of m (a chunk behind a past; with
+ * fewer keys than queries the first ones see none).  q is `[total_q, num_heads, head_dim]`, k and v `[total_k, num_kv_heads,
+ * head_dim]`, strides the elements from one token to the next; head h reads kv head h / (num_heads / num_kv_heads).  Sequence b has
+ * tokens cu_q[b] .. cu_q[b + 1] - 1 and keys cu_k[b] .. cu_k[b + 1] - 1 (`[batch + 1]` device arrays that do not fall, so that a
+ * captured call can be replayed with other lengths; offsets outside the tensors count as their ends); both NULL: one sequence of
+ * everything.  Rows of out that belong to no sequence stay as they are; a query that sees no key gives zeros.  max_k, the length of the
+ * longest sequence of keys as far as the caller knows it (total_k at most), only decides how the work is shared out.
+ * What a query does not see has no influence, whatever it holds.  A NaN that it sees in q or a key makes its row NaN, one in a
+ * value that element; infinities go as in the formula, in f32 they count as NaN.
+ * The products run on the matrix cores with f32 sums: f16 and bf16 values as they are, weights rounded to the type (2^-11, 2^-8 of
+ * each); f32 ones as three bf16 numbers each, all 24 bits.  head_dim 64, 128 or 256; rows begin on 16 bytes; out shares no memory with
+ * the inputs.  Uses the library's per-stream scratch where few rows meet many keys. */
+int izwi_qmm_prompt_attention_f32(const float* q, int64_t q_stride, const float* k, int64_t k_stride, const float* v, int64_t v_stride,
+                                  const int32_t* cu_q, const int32_t* cu_k, int64_t batch, int64_t total_q, int64_t total_k,
+                                  int64_t max_k, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim, int causal, float scale,
+                                  float* out, int64_t out_stride, void* stream);
+int izwi_qmm_prompt_attention_f16(const uint16_t* q, int64_t q_stride, const uint16_t* k, int64_t k_stride, const uint16_t* v,
+                                  int64_t v_stride, const int32_t* cu_q, const int32_t* cu_k, int64_t batch, int64_t total_q,
+                                  int64_t total_k, int64_t max_k, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim, int causal,
+                                  float scale, uint16_t* out, int64_t out_stride, void* stream);
+int izwi_qmm_prompt_attention_bf16(const uint16_t* q, int64_t q_stride, const uint16_t* k, int64_t k_stride, const uint16_t* v,
+                                   int64_t v_stride, const int32_t* cu_q, const int32_t* cu_k, int64_t batch, int64_t total_q,
+                                   int64_t total_k, int64_t max_k, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim, int causal,
+                                   float scale, uint16_t* out, int64_t out_stride, void* stream);
 
 #ifdef __cplusplus
 }

@@ -484,6 +484,25 @@ int izwi_qmm_quantize_activations(int ggml_weight_dtype, const float* x, int64_t
 int izwi_moe_route(const float* logits, int64_t t, int32_t n_experts, int32_t top_k,
                    int32_t* ids, float* weights, int mem_space, void* stream);
 
+/* Router with scores: s = softmax(logits) over all experts or sigmoid(logits); an expert is chosen by c = s + bias (`[n_experts]`
+ * f32, NULL: by the logits, whose order is that of s).  With `groups` > 1 the experts stand in that many groups of equal size; a group
+ * is worth the sum of its group_best (1 or 2) best c (without a bias: of their s), and only the experts of the best top_groups
+ * groups are chosen from.  ids are the best top_k, best first, ties (of experts and of groups) to the lower index; their weights are
+ * s, divided by the sum of the chosen s if `renormalize`, times `scale`.  Scores, sums and order are in 64 bits; weights are rounded
+ * once.  A NaN logit or c counts as -infinity (score 0), +infinity as the largest finite float; a row without any score has
+ * weights 0.  logits `[t, n_experts]`, stride elements from one token to the next; n_experts <= 1024, groups and top_k <= 64.  Device
+ * pointers only; outputs share no memory with the inputs or each other. */
+enum { IZWI_MOE_SOFTMAX = 0, IZWI_MOE_SIGMOID = 1 };
+int izwi_moe_route_scored_f32(const float* logits, int64_t stride, const float* bias, int64_t t, int32_t n_experts, int32_t top_k,
+                              int32_t scoring, int32_t groups, int32_t top_groups, int32_t group_best, int32_t renormalize,
+                              float scale, int32_t* ids, float* weights, void* stream);
+int izwi_moe_route_scored_f16(const uint16_t* logits, int64_t stride, const float* bias, int64_t t, int32_t n_experts, int32_t top_k,
+                              int32_t scoring, int32_t groups, int32_t top_groups, int32_t group_best, int32_t renormalize,
+                              float scale, int32_t* ids, float* weights, void* stream);
+int izwi_moe_route_scored_bf16(const uint16_t* logits, int64_t stride, const float* bias, int64_t t, int32_t n_experts, int32_t top_k,
+                               int32_t scoring, int32_t groups, int32_t top_groups, int32_t group_best, int32_t renormalize,
+                               float scale, int32_t* ids, float* weights, void* stream);
+
 /* Stable counting sort of the t*top_k (token, slot) pairs by expert id:
  * perm `[t*top_k]` lists pair indices grouped by expert (ascending pair index
  * inside a group), offsets `[n_experts+1]` is the exclusive prefix sum of the

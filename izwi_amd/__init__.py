@@ -19,6 +19,7 @@ from .decode_ops import (  # noqa: F401
 )
 from .gguf import GgufLoader, GgufMmapMode, GgufModelInfo, GgufReaderKind, is_gguf_file, resolve_gguf_mmap_mode  # noqa: F401
 from .kv_decode import BeamStep, KvCacheType, QuantizedKvCache, beam_select, shared_prefix_attention  # noqa: F401
+from .prompt_ops import RopeScaling, RotaryEmbedding, prompt_attention, rope_positions  # noqa: F401
 from .qmatmul import (  # noqa: F401
     ActivationRecords,
     DecodeChain,
@@ -35,6 +36,7 @@ from .qmatmul import (  # noqa: F401
     forward_group,
     get_prefill_form,
     moe_route,
+    moe_route_scored,
     moe_sort,
     packed_qmatmul_from_qtensors,
     profile_snapshot,

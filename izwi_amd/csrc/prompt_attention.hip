@@ -1,0 +1,618 @@
+// Attention over whole prompts: o_i = sum_j softmax_j(scale q_i . k_j) v_j over the positions j that query i sees, for packed
+// sequences of different lengths, causal or not, with grouped heads.
+//
+// One pass over the keys with a running reference and sum.  A workgroup has kRows rows of one kv head, a row being a (token, query
+// head) pair, the heads of a group next to each other: the group shares every tile of keys and values, and a tile of rows spans few
+// tokens, so that little of a causal triangle is worked out in vain.  A wave has 32 of the rows as the columns of both products on
+// the matrix cores:
+//   S^T = K Q^T   keys from LDS as the left operand, queries in registers; a lane has one row's scores of 16 of 32 positions,
+//   O^T = V^T P^T what the first product leaves in a lane is what the second one takes, so weights never leave the registers; values come
+//                 from LDS through the transposing reads.
+// Reference and sum of a row are two numbers of a lane, and rescaling O^T is a multiplication by a lane's own number.
+//
+// f32: queries, keys, values and weights go as three bf16 numbers each, which hold all 24 bits at every exponent, and the six
+// products of weight 2^-16 and more are summed in f32; what is left out is below 2^-23 of a product.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+
+#include "../../include/izwi_decode_ops.h"
+#include "qmm_internal.h"
+#include "qmm_lanes.h"
+#include "qmm_tile.h"
+
+namespace {
+
+typedef _Float16 f16_t;
+typedef __bf16 bf16_t;
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
+
+struct PromptParams {
+    const void *q, *k, *v;
+    void* out;
+    int64_t q_stride, k_stride, v_stride, out_stride; // elements from a token to the next
+    const int32_t *cu_q, *cu_k;                       // NULL: one sequence
+    int64_t total_q, total_k;
+    int batch, heads, kv_heads, group, causal;
+    int tiles, splits; // workgroups: tiles of rows x splits of the positions x kv heads
+    float sign;        // of the scale, or 0: what queries are multiplied by
+    float scale, scale_rest; // |scale| log2(e) as two f32 numbers
+    float* sums;       // [row][split][D], rows as in out (splits > 1)
+    float2* stats;     // [row][split]: reference (base 2) and sum
+};
+
+// ---- the element types ---------------------------------------------------------------------------------------------
+// N: bf16 / f16 numbers a value goes as; Frag: 8 values of a matrix-core operand; kLift: weights stand 2^kLift higher than they are
+// (an f16 has its full 11 bits from 2^-14 on: under a lift of 2^7, from 2^-21 of the row's reference on)
+template <typename T>
+struct Elem;
+template <>
+struct Elem<bf16_t> {
+    static constexpr int N = 1, kLift = 0;
+    static __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_bf16(a, b); }
+    static constexpr uint32_t kExponent = 0x7f807f80u;
+};
+template <>
+struct Elem<f16_t> {
+    static constexpr int N = 1, kLift = 7;
+    static __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {
+        typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, f16x2{(_Float16)a, (_Float16)b});
+    }
+    static constexpr uint32_t kExponent = 0x7c007c00u;
+};
+template <>
+struct Elem<float> {
+    static constexpr int N = 3, kLift = 0;
+    static __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) { return Elem<bf16_t>::mma(a, b, c); }
+    static constexpr uint32_t kExponent = 0x7f807f80u;
+};
+
+// Two f32 numbers as three bf16 numbers each, without a rounding: the top 8 bits, the next 8, the rest.  (An infinity leaves NaN.)
+__device__ __forceinline__ void split3(float a, float b, uint32_t (&to)[3]) {
+    constexpr uint32_t kTop = 0x07060302u; // the upper halves of two dwords
+    const uint32_t a0 = __float_as_uint(a), b0 = __float_as_uint(b);
+    const float a1 = a - __uint_as_float(a0 & 0xffff0000u), b1 = b - __uint_as_float(b0 & 0xffff0000u);
+    const uint32_t a1u = __float_as_uint(a1), b1u = __float_as_uint(b1);
+    const float a2 = a1 - __uint_as_float(a1u & 0xffff0000u), b2 = b1 - __uint_as_float(b1u & 0xffff0000u);
+    to[0] = __builtin_amdgcn_perm(b0, a0, kTop);
+    to[1] = __builtin_amdgcn_perm(b1u, a1u, kTop);
+    to[2] = __builtin_amdgcn_perm(__float_as_uint(b2), __float_as_uint(a2), kTop);
+}
+
+// acc += a b with N numbers a value: the products whose weight is 2^-16 or more
+template <typename T>
+__device__ __forceinline__ f32x16 mma_of(const u32x4 (&a)[Elem<T>::N], const u32x4 (&b)[Elem<T>::N], f32x16 acc) {
+#pragma unroll
+    for (int i = Elem<T>::N - 1; i >= 0; i--)
+#pragma unroll
+        for (int j = Elem<T>::N - 1 - i; j >= 0; j--) acc = Elem<T>::mma(a[i], b[j], acc);
+    return acc;
+}
+
+// ---- a tile of keys or values in LDS -------------------------------------------------------------------------------
+// Rows of D 16-bit numbers in pieces of 16 bytes, piece c of row r at place c ^ turn(r): so that 32 rows' pieces c (keys), and 64
+// bytes of eight neighbouring rows (values), lie on different banks.
+template <int D>
+__device__ __forceinline__ int turn(int row) {
+    return D == 64 ? ((row >> 1 & 1) << 2 | (row >> 2 & 3)) : ((row & 3) << 2 | (row >> 2 & 3));
+}
+
+// The sequence that a tile of rows belongs to: tiles are numbered sequence by sequence.
+struct Sequence {
+    int64_t q0, k0; // its first tokens
+    int len_q, len_k, row0; // row0: the tile's first row within it
+};
+__device__ __forceinline__ int bounded(const int32_t* cu, int i, int64_t total) { return (int)min((int64_t)max(cu[i], 0), total); }
+__device__ __forceinline__ bool find_sequence(const PromptParams& P, int rows, int tile, int lane, Sequence& s) {
+    if (!P.cu_q) {
+        s = Sequence{0, 0, (int)P.total_q, (int)P.total_k, tile * rows};
+        return (int64_t)tile * rows < P.total_q * P.group;
+    }
+    int before = 0;
+    for (int b0 = 0; b0 < P.batch; b0 += 64) {
+        const int b = min(b0 + lane, P.batch - 1);
+        const int from = bounded(P.cu_q, b, P.total_q), to = bounded(P.cu_q, b + 1, P.total_q);
+        const int kfrom = bounded(P.cu_k, b, P.total_k), kto = bounded(P.cu_k, b + 1, P.total_k);
+        const int len = b0 + lane < P.batch ? max(to - from, 0) : 0;
+        const int mine = (int)(((int64_t)len * P.group + rows - 1) / rows);
+        int upto = mine;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int other = __shfl_up(upto, o);
+            if (lane >= o) upto += other;
+        }
+        const unsigned long long past = __ballot(before + upto > tile);
+        if (past) {
+            const int l = __ffsll((long long)past) - 1;
+            s.q0 = __builtin_amdgcn_readlane(from, l), s.len_q = __builtin_amdgcn_readlane(len, l);
+            s.k0 = __builtin_amdgcn_readlane(kfrom, l), s.len_k = max(__builtin_amdgcn_readlane(kto, l) - (int)s.k0, 0);
+            s.row0 = (tile - before - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(mine, l))) * rows;
+            return true;
+        }
+        before += __builtin_amdgcn_readlane(upto, 63);
+    }
+    return false;
+}
+
+// v of the lane 32 away, the larger of both
+__device__ __forceinline__ float max_lane32(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+constexpr float kSlack = 8.0f; // a reference stands until a score passes it by this (base 2): weights stay below 2^8
+
+template <typename T, int D, int W, int KT, bool SPLIT>
+__global__ __launch_bounds__(64 * W) void prompt_attention_kernel(PromptParams P) {
+    using E = Elem<T>;
+    constexpr int N = E::N, kRows = 32 * W, KK = D / 16, PT = KT / 32, DT = D / 32;
+    constexpr bool kDirect = N == 1;          // keys and values go straight from memory into LDS
+    constexpr int kPlane = KT * D * 2;        // bytes of a tile of 16-bit numbers
+    constexpr int kTile = 2 * N * kPlane;     // keys, then values
+    extern __shared__ __attribute__((aligned(16))) uint8_t smem[]; // tiles (two where direct), then a word
+    uint32_t* odd_values = reinterpret_cast<uint32_t*>(smem + kTile * (kDirect ? 2 : 1));
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int x = lane & 31, h = lane >> 5;
+    // the kv head runs fastest: workgroups of a kv head stay on one XCD, whose L2 then holds its keys and values; the last tiles of a
+    // sequence, which see the most positions, begin first
+    const int kv = blockIdx.x % P.kv_heads;
+    const int unit = blockIdx.x / P.kv_heads, split = SPLIT ? unit % P.splits : 0;
+    Sequence s;
+    if (!find_sequence(P, kRows, P.tiles - 1 - (SPLIT ? unit / P.splits : unit), lane, s)) return; // the whole workgroup
+
+    const int rows = s.len_q * P.group; // of the sequence and kv head (fits: checked on the host)
+    const int row = min(s.row0 + wave * 32 + x, rows - 1), token = row / P.group, head = kv * P.group + row % P.group;
+    const int past = s.len_k - s.len_q;
+    // positions up to `limit` count; of the workgroup's rows the first sees the fewest, the last the most
+    const int limit = P.causal ? token + past : s.len_k - 1;
+    const int last_token = min(s.row0 + kRows - 1, rows - 1) / P.group;
+    const int fewest = P.causal ? max(s.row0 / P.group + past + 1, 0) : s.len_k;
+    const int most = P.causal ? min(max(last_token + past + 1, 0), s.len_k) : s.len_k;
+    const int n_tiles = (most + KT - 1) / KT;
+    const int share = SPLIT ? (n_tiles + P.splits - 1) / P.splits : n_tiles;
+    const int first = SPLIT ? min(split * share, n_tiles) : 0, end = min(first + share, n_tiles);
+
+    // queries: lane (x, h) has of row x the elements 16 kk + 8 h .. + 7
+    u32x4 q[KK][N];
+    {
+        const T* from = static_cast<const T*>(P.q) + (s.q0 + token) * P.q_stride + (int64_t)head * D + 8 * h;
+#pragma unroll
+        for (int kk = 0; kk < KK; kk++) {
+            if constexpr (N == 1) {
+                typedef T vec __attribute__((ext_vector_type(8)));
+                const vec v = *reinterpret_cast<const vec*>(from + 16 * kk);
+                vec r;
+#pragma unroll
+                for (int i = 0; i < 8; i++) r[i] = (T)((float)v[i] * P.sign); // exact
+                q[kk][0] = __builtin_bit_cast(u32x4, r);
+            } else {
+                float v[8];
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const f32x4 a = *reinterpret_cast<const f32x4*>(from + 16 * kk + 4 * i) * P.sign;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) v[4 * i + j] = a[j];
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    uint32_t to[3];
+                    split3(v[2 * i], v[2 * i + 1], to);
+#pragma unroll
+                    for (int n = 0; n < 3; n++) q[kk][n][i] = to[n];
+                }
+            }
+        }
+    }
+
+    const uint8_t* const k_rows = reinterpret_cast<const uint8_t*>(static_cast<const T*>(P.k) + s.k0 * P.k_stride + (int64_t)kv * D);
+    const uint8_t* const v_rows = reinterpret_cast<const uint8_t*>(static_cast<const T*>(P.v) + s.k0 * P.v_stride + (int64_t)kv * D);
+    const int64_t k_step = P.k_stride * (int)sizeof(T), v_step = P.v_stride * (int)sizeof(T);
+
+    // A tile on its way into LDS.  Positions behind the last repeat it (they are masked).
+    constexpr int kPer = KT * D / 8 / (64 * W); // pieces of 8 values that a thread has of the keys, and of the values
+    static_assert(kPer * 8 * 64 * W == KT * D);
+    [[maybe_unused]] f32x4 ahead[kDirect ? 1 : 2][kDirect ? 1 : kPer][2];
+    const auto request = [&](int tile, int stage) {
+        const int most_row = min(KT, s.len_k - tile * KT) - 1;
+        const uint8_t* const kb = k_rows + (int64_t)tile * KT * k_step;
+        const uint8_t* const vb = v_rows + (int64_t)tile * KT * v_step;
+        if constexpr (kDirect) {
+            const uint32_t base = (uint32_t)(uintptr_t)smem + stage * kTile;
+#pragma unroll
+            for (int i = 0; i < kPer; i++) {
+                const int piece = (i * W + wave) * 64 + lane, r = piece / (D / 8), c = (piece % (D / 8)) ^ turn<D>(r);
+                const uint32_t at = min(r, most_row);
+                load_to_lds(kb, at * (uint32_t)k_step + 16 * c, base + (i * W + wave) * 1024);
+                load_to_lds(vb, at * (uint32_t)v_step + 16 * c, base + kPlane + (i * W + wave) * 1024);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kPer; i++) {
+                const int piece = i * (64 * W) + threadIdx.x, r = min(piece / (D / 8), most_row), c = piece % (D / 8);
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    ahead[0][i][j] = *reinterpret_cast<const f32x4*>(kb + r * k_step + 32 * c + 16 * j);
+                    ahead[1][i][j] = *reinterpret_cast<const f32x4*>(vb + r * v_step + 32 * c + 16 * j);
+                }
+            }
+        }
+    };
+    const auto deliver = [&]() { // what was requested into registers, as three planes
+        if constexpr (!kDirect) {
+#pragma unroll
+            for (int w = 0; w < 2; w++)
+#pragma unroll
+                for (int i = 0; i < kPer; i++) {
+                    const int piece = i * (64 * W) + threadIdx.x, r = piece / (D / 8), c = (piece % (D / 8)) ^ turn<D>(r);
+                    u32x4 o[3];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        uint32_t to[3];
+                        split3(ahead[w][i][j >> 1][2 * j & 3], ahead[w][i][j >> 1][(2 * j & 3) + 1], to);
+#pragma unroll
+                        for (int n = 0; n < 3; n++) o[n][j] = to[n];
+                    }
+#pragma unroll
+                    for (int n = 0; n < 3; n++) *reinterpret_cast<u32x4*>(smem + (w * 3 + n) * kPlane + r * (2 * D) + 16 * c) = o[n];
+                }
+        }
+    };
+
+    // where a lane reads: keys of position x, piece 2 kk + h; values of positions 4 h + 0..3 (+ 8) through the transposing read, for
+    // which the lanes of a sixteen name four rows of four pieces of 8 bytes
+    const int k_at = x * (2 * D) + ((h ^ turn<D>(x)) << 4);
+    const int i16 = lane & 15, v_row = 4 * h + (i16 >> 2), v_piece = (lane >> 4 & 1) * 2 + (i16 >> 1 & 1);
+    const int v_at0 = v_row * (2 * D) + ((v_piece ^ turn<D>(v_row)) << 4) + (i16 & 1) * 8;
+    const int v_at1 = (v_row + 8) * (2 * D) + ((v_piece ^ turn<D>(v_row + 8)) << 4) + (i16 & 1) * 8;
+
+    f32x16 o[DT];
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) o[d][r] = 0.0f;
+    float ref = -INFINITY, sum = 0.0f; // ref: base 2; sum: of this lane's positions
+    if (threadIdx.x == 0) *odd_values = 0;
+
+    if (first < end) request(first, 0);
+    for (int tile = first; tile < end; tile++) {
+        const uint8_t* here = smem;
+        if constexpr (kDirect) {
+            const int stage = (tile - first) & 1;
+            here = smem + stage * kTile;
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            if (tile + 1 < end) request(tile + 1, stage ^ 1);
+        } else {
+            __syncthreads(); // the tile before is read
+            deliver();
+            if (tile + 1 < end) request(tile + 1, 0);
+            __syncthreads();
+        }
+        const int p0 = tile * KT;
+        const bool masked = p0 + KT > fewest || p0 + KT > s.len_k; // for some row of the workgroup
+        bool odd = false;
+        if (masked) { // a value that is no number must not reach the rows that do not see it: a weight of zero would not keep it out
+            bool any = false;
+            constexpr int kReads = N * kPlane / 16 / (64 * W);
+#pragma unroll
+            for (int i = 0; i < kReads; i++) {
+                const u32x4 v = *reinterpret_cast<const u32x4*>(here + N * kPlane + (i * 64 * W + threadIdx.x) * 16);
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    any |= (v[j] & (E::kExponent >> 16)) == (E::kExponent >> 16) || (v[j] & (E::kExponent & 0xffff0000u)) == (E::kExponent & 0xffff0000u);
+            }
+            if (__any(any) && lane == 0) *odd_values = tile + 1;
+            __syncthreads();
+            odd = *odd_values == (uint32_t)(tile + 1);
+        }
+
+        // scores: lane (x, h), register r of sub-tile pt: row x, position p0 + 32 pt + 8 (r / 4) + 4 h + r % 4
+        f32x16 p[PT];
+#pragma unroll
+        for (int pt = 0; pt < PT; pt++) {
+#pragma unroll
+            for (int r = 0; r < 16; r++) p[pt][r] = 0.0f;
+#pragma unroll
+            for (int kk = 0; kk < KK; kk++) {
+                u32x4 a[N];
+#pragma unroll
+                for (int n = 0; n < N; n++) a[n] = *reinterpret_cast<const u32x4*>(here + n * kPlane + pt * 32 * (2 * D) + (k_at ^ (kk << 5)));
+                p[pt] = mma_of<T>(a, q[kk], p[pt]);
+            }
+        }
+        if (masked) {
+#pragma unroll
+            for (int pt = 0; pt < PT; pt++)
+#pragma unroll
+                for (int r = 0; r < 16; r++)
+                    if (p0 + 32 * pt + 8 * (r >> 2) + 4 * h + (r & 3) > limit) p[pt][r] = -INFINITY;
+        }
+        float top = p[0][0];
+#pragma unroll
+        for (int pt = 0; pt < PT; pt++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) top = fmaxf(top, p[pt][r]);
+        top = max_lane32(top) * P.scale;
+        const bool passed = top > ref + kSlack; // (from -infinity: at the first score)
+        if (__any(passed)) {                    // a row's own reference moves only by its own scores: no other row has a say in its result
+            const float next = passed ? top : ref, by = ref == next ? 1.0f : __builtin_amdgcn_exp2f(ref - next);
+            sum *= by;
+#pragma unroll
+            for (int d = 0; d < DT; d++) o[d] *= by;
+            ref = next;
+        }
+        const float from = ref == -INFINITY ? 0.0f : ref - E::kLift;
+#pragma unroll
+        for (int pt = 0; pt < PT; pt++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                float e = __builtin_fmaf(p[pt][r], P.scale, -from);
+                if constexpr (N == 3) e = p[pt][r] == -INFINITY ? e : __builtin_fmaf(p[pt][r], P.scale_rest, e); // (the rest may be negative)
+                p[pt][r] = __builtin_amdgcn_exp2f(e);
+                sum += p[pt][r];
+            }
+
+        // sixteen positions at a time: the lane's eight are 4 h + 0..3 and 8 + 4 h + 0..3 of them
+#pragma unroll
+        for (int t = 0; t < KT / 16; t++) {
+            u32x4 w[N];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float a = p[t >> 1][8 * (t & 1) + 2 * i], b = p[t >> 1][8 * (t & 1) + 2 * i + 1];
+                if constexpr (N == 1) {
+                    w[0][i] = E::pack(a, b);
+                } else {
+                    uint32_t to[3];
+                    split3(a, b, to);
+#pragma unroll
+                    for (int n = 0; n < 3; n++) w[n][i] = to[n];
+                }
+            }
+#pragma unroll
+            for (int d = 0; d < DT; d++) {
+                u32x4 a[N];
+#pragma unroll
+                for (int n = 0; n < N; n++) {
+                    const uint8_t* const plane = here + (N + n) * kPlane + t * 16 * (2 * D);
+                    const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(plane + (v_at0 ^ (d << 6)))));
+                    const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(plane + (v_at1 ^ (d << 6)))));
+                    a[n] = u32x4{lo[0], lo[1], hi[0], hi[1]};
+                }
+                if (odd) { // (uniform) without what is no number; see below
+#pragma unroll
+                    for (int n = 0; n < N; n++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            if ((a[n][j] & (E::kExponent >> 16)) == (E::kExponent >> 16)) a[n][j] &= 0xffff0000u;
+                            if ((a[n][j] & (E::kExponent & 0xffff0000u)) == (E::kExponent & 0xffff0000u)) a[n][j] &= 0xffffu;
+                        }
+                }
+                o[d] = mma_of<T>(a, w, o[d]);
+            }
+        }
+        if (odd) { // infinities and NaN, to the rows that see them
+#pragma unroll 1
+            for (int j = 0; j < min(KT, s.len_k - p0); j++) {
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int c = (4 * d + i) ^ turn<D>(j);
+#pragma unroll
+                        for (int n = 0; n < N; n++) {
+                            const u32x2 v = *reinterpret_cast<const u32x2*>(here + (N + n) * kPlane + j * (2 * D) + 16 * c + 8 * h);
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                const uint16_t bits = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
+                                const bool is = (bits & (uint16_t)E::kExponent) == (uint16_t)E::kExponent && p0 + j <= limit;
+                                const float value = std::is_same_v<T, f16_t> ? qmm_f16_bits_to_f32(bits) : qmm_bf16_bits_to_f32(bits);
+                                o[d][4 * i + e] += is ? value : 0.0f;
+                            }
+                        }
+                    }
+            }
+        }
+    }
+
+    // rows behind the sequence's last stay as they are
+    if (s.row0 + wave * 32 + x >= rows) return;
+    sum = qmm_add_lane32(sum);
+    const int64_t out_row = (s.q0 + token) * P.heads + head;
+    if constexpr (SPLIT) {
+        // (a sum below zero: the split has no position that the row sees)
+        if (h == 0) P.stats[out_row * P.splits + split] = float2{ref, first < end && limit >= first * KT ? sum : -1.0f};
+        float* to = P.sums + (out_row * P.splits + split) * D + 4 * h;
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) *reinterpret_cast<f32x4*>(to + 32 * d + 8 * i) = f32x4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+        return;
+    }
+    const bool none = limit < 0 || s.len_k == 0;
+    const float inv = none ? 0.0f : 1.0f / sum;
+    T* const to = static_cast<T*>(P.out) + (s.q0 + token) * P.out_stride + (int64_t)head * D;
+#pragma unroll
+    for (int d = 0; d < DT; d++) {
+        float v[16];
+#pragma unroll
+        for (int r = 0; r < 16; r++) v[r] = none ? 0.0f : o[d][r] * inv;
+        if constexpr (N == 3) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) *reinterpret_cast<f32x4*>(to + 32 * d + 8 * i + 4 * h) = f32x4{v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
+        } else {
+            // halves trade: the lower lanes get the eight values of piece 0 (2), the upper ones those of piece 1 (3)
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) {
+                u32x4 piece;
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const auto r = __builtin_amdgcn_permlane32_swap(E::pack(v[4 * i + 2 * j], v[4 * i + 2 * j + 1]), E::pack(v[4 * i + 4 + 2 * j], v[4 * i + 5 + 2 * j]), false, false);
+                    piece[j] = r[0], piece[2 + j] = r[1];
+                }
+                *reinterpret_cast<u32x4*>(to + 32 * d + 8 * (i + h)) = piece;
+            }
+        }
+    }
+}
+
+// A row's splits joined by a wave, lane l having elements l D / 64 on.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void prompt_join_kernel(PromptParams P, int64_t rows) {
+    constexpr int N = D / 64;
+    const int lane = threadIdx.x & 63;
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= rows) return;
+    const int64_t token = row / P.heads;
+    if (P.cu_q) { // rows behind the last sequence, or between two, were not written
+        bool inside = false;
+        for (int b0 = 0; b0 < P.batch && !inside; b0 += 64) {
+            const int b = min(b0 + lane, P.batch - 1);
+            inside = __any(token >= bounded(P.cu_q, b, P.total_q) && token < bounded(P.cu_q, b + 1, P.total_q));
+        }
+        if (!inside) return;
+    }
+    float ref = -INFINITY, sum = 0.0f, a[N] = {};
+    bool any = false;
+    for (int i = 0; i < P.splits; i++) {
+        const float2 st = P.stats[row * P.splits + i];
+        if (st.y < 0.0f) continue; // no position that the row sees
+        any = true;
+        // (a reference of -infinity: no score is above it; a NaN among them is in sum and sums, and stays)
+        const float next = fmaxf(ref, st.x), old = ref == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ref - next);
+        const float by = st.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(st.x - next);
+        sum = sum * old + st.y * by;
+#pragma unroll
+        for (int j = 0; j < N; j++) a[j] = a[j] * old + P.sums[(row * P.splits + i) * D + lane * N + j] * by;
+        ref = next;
+    }
+    T* to = static_cast<T*>(P.out) + token * P.out_stride + (row % P.heads) * D + lane * N;
+#pragma unroll
+    for (int j = 0; j < N; j++) to[j] = (T)(any ? a[j] / sum : 0.0f);
+}
+
+#define PROMPT_TRY(expr)                                                               \
+    do {                                                                               \
+        hipError_t e_ = (expr);                                                        \
+        if (e_ != hipSuccess) {                                                        \
+            (void)hipGetLastError();                                                   \
+            return qmm_fail(IZWI_QMM_ERR_HIP, "%s: %s", #expr, hipGetErrorString(e_)); \
+        }                                                                              \
+    } while (0)
+
+template <typename T, int D, int W>
+hipError_t launch(const PromptParams& P, hipStream_t stream) {
+    constexpr int N = Elem<T>::N, KT = N == 3 || D == 256 ? 32 : 64;
+    constexpr size_t lds = (size_t)2 * N * KT * D * 2 * (N == 1 ? 2 : 1) + 16;
+    static_assert(lds <= 160 * 1024);
+    const auto run = [&](auto kernel) {
+        if (lds > 64 * 1024) {
+            const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+            if (e != hipSuccess) return e;
+        }
+        kernel<<<(unsigned)((int64_t)P.tiles * P.splits * P.kv_heads), 64 * W, lds, stream>>>(P);
+        return hipGetLastError();
+    };
+    if (P.splits == 1) return run(prompt_attention_kernel<T, D, W, KT, false>);
+    const hipError_t e = run(prompt_attention_kernel<T, D, W, KT, true>);
+    if (e != hipSuccess) return e;
+    const int64_t rows = P.total_q * P.heads;
+    prompt_join_kernel<T, D><<<(unsigned)((rows + 3) / 4), 256, 0, stream>>>(P, rows);
+    return hipGetLastError();
+}
+
+template <typename T>
+int prompt_attention_impl(const T* q, int64_t q_stride, const T* k, int64_t k_stride, const T* v, int64_t v_stride, const int32_t* cu_q,
+                          const int32_t* cu_k, int64_t batch, int64_t total_q, int64_t total_k, int64_t max_k, int64_t heads, int64_t kv_heads, int64_t d,
+                          int causal, float scale, T* out, int64_t out_stride, void* stream_) {
+    constexpr const char* what = "prompt_attention";
+    if (d != 64 && d != 128 && d != 256)
+        return qmm_fail(IZWI_QMM_ERR_UNSUPPORTED, "%s: head_dim %lld (64, 128 and 256 are built)", what, (long long)d);
+    if (batch < 0 || total_q < 0 || total_k < 0 || max_k < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || heads > 65535 || batch > 0xfffff)
+        return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: bad shape (batch %lld, tokens %lld on %lld, heads %lld on %lld)", what, (long long)batch,
+                        (long long)total_q, (long long)total_k, (long long)heads, (long long)kv_heads);
+    if ((cu_q == nullptr) != (cu_k == nullptr) || (!cu_q && batch != 1))
+        return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: offsets of queries and keys come together, and only one sequence (not %lld) has none", what, (long long)batch);
+    if (q_stride < heads * d || out_stride < heads * d || k_stride < kv_heads * d || v_stride < kv_heads * d)
+        return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: rows overlap (strides %lld, %lld, %lld, %lld)", what, (long long)q_stride, (long long)k_stride,
+                        (long long)v_stride, (long long)out_stride);
+    if (!std::isfinite(scale)) return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: scale %g", what, (double)scale);
+    constexpr int kPiece = 16 / (int)sizeof(T);
+    if (q_stride % kPiece || k_stride % kPiece || v_stride % kPiece || out_stride % kPiece ||
+        ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(out)) & 15))
+        return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: rows must begin on 16 bytes", what);
+    if (total_q * heads > 0x3fffffff || total_k > 0x3fffffff || k_stride > (1 << 23) || v_stride > (1 << 23) || q_stride > 0x3fffffff ||
+        out_stride > 0x3fffffff)
+        return qmm_fail(IZWI_QMM_ERR_UNSUPPORTED, "%s: %lld tokens of %lld heads on %lld, rows %lld and %lld apart", what, (long long)total_q,
+                        (long long)heads, (long long)total_k, (long long)k_stride, (long long)v_stride);
+    if (batch == 0 || total_q == 0) return IZWI_QMM_OK;
+    if (!q || !out || (total_k && (!k || !v))) return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: NULL buffer", what);
+    const auto overlap = [&](const void* a, int64_t rows, int64_t stride, int64_t width) {
+        const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(out);
+        return rows && x < y + ((uintptr_t)(total_q - 1) * out_stride + heads * d) * sizeof(T) && y < x + ((uintptr_t)(rows - 1) * stride + width) * sizeof(T);
+    };
+    if (overlap(q, total_q, q_stride, heads * d) || overlap(k, total_k, k_stride, kv_heads * d) || overlap(v, total_k, v_stride, kv_heads * d))
+        return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: out shares memory with q, k or v", what);
+    constexpr int W = 4;
+    const int64_t tiles = total_q * (heads / kv_heads) / (32 * W) + batch, wgs = tiles * kv_heads;
+    if (wgs > 0x3fffff) return qmm_fail(IZWI_QMM_ERR_UNSUPPORTED, "%s: %lld sequences on %lld kv heads", what, (long long)batch, (long long)kv_heads);
+    int device = 0, n_cus = 0;
+    if (int rc = qmm_current_device(&device, &n_cus)) return rc;
+    PromptParams P{};
+    P.q = q, P.k = k, P.v = v, P.out = out;
+    P.q_stride = q_stride, P.k_stride = k_stride, P.v_stride = v_stride, P.out_stride = out_stride;
+    P.cu_q = cu_q, P.cu_k = cu_k, P.total_q = total_q, P.total_k = total_k;
+    P.batch = (int)batch, P.heads = (int)heads, P.kv_heads = (int)kv_heads, P.group = (int)(heads / kv_heads), P.causal = causal != 0;
+    const double by = std::fabs((double)scale) * 1.4426950408889634074;
+    P.sign = scale == 0.0f ? 0.0f : scale < 0.0f ? -1.0f : 1.0f;
+    P.scale = scale == 0.0f ? 1.0f : (float)by, P.scale_rest = scale == 0.0f ? 0.0f : (float)(by - (double)P.scale);
+    constexpr int kt = sizeof(T) == 4 ? 32 : 64;
+    P.tiles = (int)tiles;
+    const int64_t pos_tiles = (std::min(max_k, total_k) + kt - 1) / kt;
+    P.splits = (int)std::max<int64_t>(1, std::min(n_cus / wgs, pos_tiles / 4));
+    hipStream_t stream = (hipStream_t)stream_;
+    QmmCallScope call;
+    if (P.splits > 1) {
+        const size_t rows = (size_t)total_q * heads * P.splits;
+        void* scratch = nullptr;
+        PROMPT_TRY(qmm_get_scratch(device, stream, rows * (d * sizeof(float) + sizeof(float2)), &scratch));
+        P.sums = static_cast<float*>(scratch);
+        P.stats = reinterpret_cast<float2*>(P.sums + rows * d);
+    }
+    PROMPT_TRY((d == 64 ? launch<T, 64, W>(P, stream) : d == 128 ? launch<T, 128, W>(P, stream) : launch<T, 256, W>(P, stream)));
+    return IZWI_QMM_OK;
+}
+
+} // namespace
+
+extern "C" {
+
+#define PROMPT_ATTENTION(NAME, C, T)                                                                                                                     \
+    int NAME(const C* q, int64_t q_stride, const C* k, int64_t k_stride, const C* v, int64_t v_stride, const int32_t* cu_q, const int32_t* cu_k,         \
+             int64_t batch, int64_t total_q, int64_t total_k, int64_t max_k, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim, int causal,      \
+             float scale, C* out, int64_t out_stride, void* stream) {                                                                                    \
+        return qmm_guarded(#NAME, [&]() -> int {                                                                                                         \
+            return prompt_attention_impl<T>((const T*)q, q_stride, (const T*)k, k_stride, (const T*)v, v_stride, cu_q, cu_k, batch, total_q, total_k,    \
+                                            max_k, num_heads, num_kv_heads, head_dim, causal, scale, (T*)out, out_stride, stream);                       \
+        });                                                                                                                                              \
+    }
+PROMPT_ATTENTION(izwi_qmm_prompt_attention_f32, float, float)
+PROMPT_ATTENTION(izwi_qmm_prompt_attention_f16, uint16_t, f16_t)
+PROMPT_ATTENTION(izwi_qmm_prompt_attention_bf16, uint16_t, bf16_t)
+
+} // extern "C"

@@ -1,0 +1,188 @@
+// Rotary positions of packed tokens: (a, b) -> (a cos - b sin, a sin + b cos) for the pairs of a head's first rotary_dim elements, angle
+// position * frequency, optionally behind the head's RMSNorm; and the frequencies of models whose context is stretched.
+//
+// Angles are taken in 64 bits and reduced to a fraction of a turn there: position 10^6 in 32 bits would be off by 0.03.  Cosine and
+// sine are then 32-bit functions of that fraction.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "../../include/izwi_decode_ops.h"
+#include "qmm_internal.h"
+#include "qmm_lanes.h"
+
+namespace {
+
+typedef _Float16 f16_t;
+typedef __bf16 bf16_t;
+
+struct RopeParams {
+    const void *q, *k;
+    void *q_out, *k_out;
+    int64_t q_stride, k_stride, q_out_stride, k_out_stride; // elements from a token to the next
+    const int32_t* positions;
+    const double* frequencies; // [rotary / 2]
+    const void* weight;        // [2 d]: q's, then k's; NULL: no norm
+    float factor, eps;
+    int64_t tokens;
+    int q_heads, heads, d, rotary; // heads: q's and k's
+};
+
+constexpr int kMostPairs = 512;
+
+__device__ __forceinline__ void turn_of(const RopeParams& P, int position, int pair, float& c, float& s) {
+    double turns = (double)position * (P.frequencies[pair] * 0.15915494309189533577); // 1 / (2 pi)
+    turns -= __builtin_rint(turns);
+    sincospif(2.0f * (float)turns, &s, &c);
+    c *= P.factor, s *= P.factor;
+}
+
+// A workgroup per token, a wave per head in turn, a lane per pair of elements in turn.
+template <typename T, bool INTER>
+__global__ __launch_bounds__(256) void rope_any_kernel(RopeParams P) {
+    __shared__ float cosine[kMostPairs], sine[kMostPairs];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, pairs = P.rotary / 2;
+    const int64_t token = blockIdx.x;
+    const int position = P.positions[token];
+    for (int i = threadIdx.x; i < pairs; i += 256) turn_of(P, position, i, cosine[i], sine[i]);
+    __syncthreads();
+    for (int head = wave; head < P.heads; head += 4) {
+        const bool is_q = head < P.q_heads;
+        const int at = is_q ? head : head - P.q_heads;
+        const T* const from = static_cast<const T*>(is_q ? P.q : P.k) + token * (is_q ? P.q_stride : P.k_stride) + (int64_t)at * P.d;
+        T* const to = static_cast<T*>(is_q ? P.q_out : P.k_out) + token * (is_q ? P.q_out_stride : P.k_out_stride) + (int64_t)at * P.d;
+        const T* const weight = P.weight ? static_cast<const T*>(P.weight) + (is_q ? 0 : P.d) : nullptr;
+        float by = 1.0f;
+        if (weight) {
+            float sum = 0.0f;
+            for (int i = lane; i < P.d; i += 64) {
+                const float v = (float)from[i];
+                sum += v * v;
+            }
+            by = 1.0f / sqrtf(wave_sum(sum) / (float)P.d + P.eps);
+            asm volatile("" ::: "memory"); // (in place, lanes read others' elements above)
+            __builtin_amdgcn_wave_barrier();
+        }
+        for (int i = lane; i < P.d / 2; i += 64) {
+            const bool turns = i < pairs;
+            const int a = turns && !INTER ? i : 2 * i, b = turns && !INTER ? i + pairs : 2 * i + 1;
+            float u = (float)from[a], v = (float)from[b];
+            if (weight) u = u * by * (float)weight[a], v = v * by * (float)weight[b];
+            const float c = turns ? cosine[i] : 1.0f, s = turns ? sine[i] : 0.0f;
+            to[a] = (T)(turns ? u * c - v * s : u);
+            to[b] = (T)(turns ? u * s + v * c : v);
+        }
+    }
+}
+
+#define ROPE_TRY(expr)                                                                 \
+    do {                                                                               \
+        hipError_t e_ = (expr);                                                        \
+        if (e_ != hipSuccess) {                                                        \
+            (void)hipGetLastError();                                                   \
+            return qmm_fail(IZWI_QMM_ERR_HIP, "%s: %s", #expr, hipGetErrorString(e_)); \
+        }                                                                              \
+    } while (0)
+
+template <typename T>
+int rope_positions_impl(const T* q, int64_t q_stride, const T* k, int64_t k_stride, const int32_t* positions, const double* frequencies, float factor,
+                        int64_t tokens, int64_t q_heads, int64_t k_heads, int64_t d, int64_t rotary, int interleaved, const T* weight, float eps, T* q_out,
+                        int64_t q_out_stride, T* k_out, int64_t k_out_stride, void* stream_) {
+    constexpr const char* what = "rope_positions";
+    if (tokens < 0 || q_heads < 0 || k_heads < 0 || q_heads > 65535 || k_heads > 65535 || d <= 0 || d % 2 || d > 2 * kMostPairs || rotary <= 0 || rotary % 2 || rotary > d)
+        return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: bad shape (tokens %lld, heads %lld and %lld of %lld, of which %lld turn: even, at most %d)", what, (long long)tokens,
+                        (long long)q_heads, (long long)k_heads, (long long)d, (long long)rotary, 2 * kMostPairs);
+    if ((q_heads && (q_stride < q_heads * d || q_out_stride < q_heads * d)) || (k_heads && (k_stride < k_heads * d || k_out_stride < k_heads * d)))
+        return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: rows overlap (strides %lld, %lld, %lld, %lld)", what, (long long)q_stride, (long long)k_stride,
+                        (long long)q_out_stride, (long long)k_out_stride);
+    if (interleaved != 0 && interleaved != 1) return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: layout %d (0 halves, 1 interleaved)", what, interleaved);
+    if (!std::isfinite(factor) || !(eps >= 0.0f) || !std::isfinite(eps)) return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: factor %g, eps %g", what, (double)factor, (double)eps);
+    if (tokens > 0x3fffffff || q_stride > 0x3fffffff || k_stride > 0x3fffffff || q_out_stride > 0x3fffffff || k_out_stride > 0x3fffffff)
+        return qmm_fail(IZWI_QMM_ERR_UNSUPPORTED, "%s: %lld tokens", what, (long long)tokens);
+    if (tokens == 0 || q_heads + k_heads == 0) return IZWI_QMM_OK;
+    if (!positions || !frequencies || (q_heads && (!q || !q_out)) || (k_heads && (!k || !k_out))) return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: NULL buffer", what);
+    // an output may be its input; otherwise it shares no memory with an input or the other output, unless the rows of both interleave (parts of
+    // wider rows): those of one stride, each inside what the other leaves free
+    struct Rows {
+        const void* at;
+        int64_t stride, width;
+    };
+    const auto apart = [&](const Rows& a, const Rows& b) {
+        if (!a.width || !b.width) return true;
+        const uintptr_t x = reinterpret_cast<uintptr_t>(a.at), y = reinterpret_cast<uintptr_t>(b.at);
+        const uintptr_t xn = ((uintptr_t)(tokens - 1) * a.stride + a.width) * sizeof(T), yn = ((uintptr_t)(tokens - 1) * b.stride + b.width) * sizeof(T);
+        if (x + xn <= y || y + yn <= x) return true;
+        if (a.stride != b.stride) return false;
+        const int64_t row = a.stride * (int64_t)sizeof(T), off = (int64_t)((intptr_t)(y - x) % row + row) % row;
+        return off >= a.width * (int64_t)sizeof(T) && off + b.width * (int64_t)sizeof(T) <= row;
+    };
+    const Rows qi{q, q_stride, q_heads * d}, ki{k, k_stride, k_heads * d}, qo{q_out, q_out_stride, q_heads * d}, ko{k_out, k_out_stride, k_heads * d};
+    const auto same = [](const Rows& a, const Rows& b) { return a.at == b.at && a.stride == b.stride; };
+    if ((!same(qi, qo) && !apart(qi, qo)) || (!same(ki, ko) && !apart(ki, ko)) || !apart(qi, ko) || !apart(ki, qo) || !apart(qo, ko))
+        return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: an output shares memory with another tensor (it may be its own input)", what);
+    int device = 0, n_cus = 0;
+    if (int rc = qmm_current_device(&device, &n_cus)) return rc;
+    RopeParams P{q, k, q_out, k_out, q_stride, k_stride, q_out_stride, k_out_stride, positions, frequencies, weight, factor, eps, tokens, (int)q_heads,
+                 (int)(q_heads + k_heads), (int)d, (int)rotary};
+    hipStream_t stream = (hipStream_t)stream_;
+    if (interleaved) rope_any_kernel<T, true><<<(unsigned)tokens, 256, 0, stream>>>(P);
+    else rope_any_kernel<T, false><<<(unsigned)tokens, 256, 0, stream>>>(P);
+    ROPE_TRY(hipGetLastError());
+    return IZWI_QMM_OK;
+}
+
+} // namespace
+
+extern "C" {
+
+#define ROPE_POSITIONS(NAME, C, T)                                                                                                                         \
+    int NAME(const C* q, int64_t q_stride, const C* k, int64_t k_stride, const int32_t* positions, const double* frequencies, float attention_factor,     \
+             int64_t tokens, int64_t q_heads, int64_t k_heads, int64_t head_dim, int64_t rotary_dim, int interleaved, const C* qk_weight, float eps,       \
+             C* q_out, int64_t q_out_stride, C* k_out, int64_t k_out_stride, void* stream) {                                                               \
+        return qmm_guarded(#NAME, [&]() -> int {                                                                                                           \
+            return rope_positions_impl<T>((const T*)q, q_stride, (const T*)k, k_stride, positions, frequencies, attention_factor, tokens, q_heads,         \
+                                          k_heads, head_dim, rotary_dim, interleaved, (const T*)qk_weight, eps, (T*)q_out, q_out_stride, (T*)k_out,        \
+                                          k_out_stride, stream);                                                                                           \
+        });                                                                                                                                                \
+    }
+ROPE_POSITIONS(izwi_rope_positions_f32, float, float)
+ROPE_POSITIONS(izwi_rope_positions_f16, uint16_t, f16_t)
+ROPE_POSITIONS(izwi_rope_positions_bf16, uint16_t, bf16_t)
+
+int izwi_rope_frequencies(int scaling, int64_t rotary_dim, double base, double factor, double original_len, double low, double high, double* frequencies,
+                          double* attention_factor) {
+    return qmm_guarded("izwi_rope_frequencies", [&]() -> int {
+    constexpr const char* what = "rope_frequencies";
+    if (rotary_dim <= 0 || rotary_dim % 2 || rotary_dim > 2 * kMostPairs) return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: rotary_dim %lld", what, (long long)rotary_dim);
+    if (scaling < IZWI_ROPE_PLAIN || scaling > IZWI_ROPE_YARN) return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: scaling %d", what, scaling);
+    if (!(base > 1.0) || !std::isfinite(base)) return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: base %g", what, base);
+    if (scaling != IZWI_ROPE_PLAIN && (!(factor >= 1.0) || !std::isfinite(factor))) return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: factor %g", what, factor);
+    const bool by_waves = scaling == IZWI_ROPE_LLAMA3 || scaling == IZWI_ROPE_YARN;
+    if (by_waves && (!(original_len > 0.0) || !std::isfinite(original_len) || !(low > 0.0) || !(high > low) || !std::isfinite(high)))
+        return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: original length %g, turns %g to %g", what, original_len, low, high);
+    if (scaling == IZWI_ROPE_NTK && rotary_dim == 2) return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: a base of one pair cannot be stretched", what);
+    if (!frequencies || !attention_factor) return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: NULL buffer", what);
+    const double n = (double)rotary_dim, two_pi = 6.283185307179586477;
+    if (scaling == IZWI_ROPE_NTK) base *= std::pow(factor, n / (n - 2.0));
+    // YaRN's ramp runs over the pairs, between those that turn `high` and `low` times in the original length
+    const auto pair_of = [&](double turns) { return n * std::log(original_len / (turns * two_pi)) / (2.0 * std::log(base)); };
+    double from = 0.0, to = 0.0;
+    if (scaling == IZWI_ROPE_YARN) {
+        from = std::max(std::floor(pair_of(high)), 0.0), to = std::min(std::ceil(pair_of(low)), n - 1.0);
+        if (to <= from) to = from + 0.001;
+    }
+    for (int64_t i = 0; i < rotary_dim / 2; i++) {
+        const double f = std::pow(base, -2.0 * (double)i / n);
+        double stretched = 0.0; // the share of the stretched frequency
+        if (scaling == IZWI_ROPE_LINEAR) stretched = 1.0;
+        else if (scaling == IZWI_ROPE_LLAMA3) stretched = 1.0 - std::min(std::max((original_len * f / two_pi - low) / (high - low), 0.0), 1.0);
+        else if (scaling == IZWI_ROPE_YARN) stretched = std::min(std::max(((double)i - from) / (to - from), 0.0), 1.0);
+        frequencies[i] = stretched == 0.0 ? f : f * (1.0 - stretched) + f / factor * stretched;
+    }
+    *attention_factor = scaling == IZWI_ROPE_YARN ? 0.1 * std::log(factor) + 1.0 : 1.0;
+    return IZWI_QMM_OK;
+    });
+}
+
+} // extern "C"

@@ -32,6 +32,17 @@ pub const IZWI_QMM_Q6_K: c_int = 14;
 pub const IZWI_KV_Q4_0: c_int = 2;
 pub const IZWI_KV_Q8_0: c_int = 8;
 
+// scaling of rotary frequencies (izwi_rope_frequencies)
+pub const IZWI_ROPE_PLAIN: c_int = 0;
+pub const IZWI_ROPE_LINEAR: c_int = 1;
+pub const IZWI_ROPE_NTK: c_int = 2;
+pub const IZWI_ROPE_LLAMA3: c_int = 3;
+pub const IZWI_ROPE_YARN: c_int = 4;
+
+// scores of izwi_moe_route_scored_*
+pub const IZWI_MOE_SOFTMAX: c_int = 0;
+pub const IZWI_MOE_SIGMOID: c_int = 1;
+
 /// `izwi_qmm_large_m`
 pub const IZWI_QMM_LARGE_M_BF16: c_int = 0;
 pub const IZWI_QMM_LARGE_M_INT8: c_int = 1;
@@ -193,6 +204,15 @@ extern "C" {
         out_blocks: *mut c_void, mem_space: c_int, stream: *mut c_void) -> c_int;
     pub fn izwi_moe_route(logits: *const f32, t: i64, n_experts: i32, top_k: i32, ids: *mut i32, weights: *mut f32,
         mem_space: c_int, stream: *mut c_void) -> c_int;
+    pub fn izwi_moe_route_scored_f32(logits: *const f32, stride: i64, bias: *const f32, t: i64, n_experts: i32,
+        top_k: i32, scoring: i32, groups: i32, top_groups: i32, group_best: i32, renormalize: i32, scale: f32,
+        ids: *mut i32, weights: *mut f32, stream: *mut c_void) -> c_int;
+    pub fn izwi_moe_route_scored_f16(logits: *const u16, stride: i64, bias: *const f32, t: i64, n_experts: i32,
+        top_k: i32, scoring: i32, groups: i32, top_groups: i32, group_best: i32, renormalize: i32, scale: f32,
+        ids: *mut i32, weights: *mut f32, stream: *mut c_void) -> c_int;
+    pub fn izwi_moe_route_scored_bf16(logits: *const u16, stride: i64, bias: *const f32, t: i64, n_experts: i32,
+        top_k: i32, scoring: i32, groups: i32, top_groups: i32, group_best: i32, renormalize: i32, scale: f32,
+        ids: *mut i32, weights: *mut f32, stream: *mut c_void) -> c_int;
     pub fn izwi_moe_sort(ids: *const i32, t: i64, top_k: i32, n_experts: i32, perm: *mut i32, offsets: *mut i32,
         mem_space: c_int, stream: *mut c_void) -> c_int;
     pub fn izwi_moe_forward_f32(gate: *const IzwiQmmWeight, up: *const IzwiQmmWeight, down: *const IzwiQmmWeight,
@@ -287,6 +307,32 @@ extern "C" {
     pub fn izwi_decode_beam_select_f32(logits: *const f32, prompts: i64, beams: i64, vocab: i64, scores: *const f32,
         finished: *const u8, eos_token: i64, tokens: *mut i32, parents: *mut i32, scores_out: *mut f32,
         finished_out: *mut u8, lineage: *const u8, lineage_capacity: i64, lens: *const i32, lineage_out: *mut u8,
+        stream: *mut c_void) -> c_int;
+    pub fn izwi_rope_frequencies(scaling: c_int, rotary_dim: i64, base: f64, factor: f64, original_len: f64,
+        low: f64, high: f64, frequencies: *mut f64, attention_factor: *mut f64) -> c_int;
+    pub fn izwi_rope_positions_f32(q: *const f32, q_stride: i64, k: *const f32, k_stride: i64, positions: *const i32,
+        frequencies: *const f64, attention_factor: f32, tokens: i64, q_heads: i64, k_heads: i64, head_dim: i64,
+        rotary_dim: i64, interleaved: c_int, qk_weight: *const f32, eps: f32, q_out: *mut f32, q_out_stride: i64,
+        k_out: *mut f32, k_out_stride: i64, stream: *mut c_void) -> c_int;
+    pub fn izwi_rope_positions_f16(q: *const u16, q_stride: i64, k: *const u16, k_stride: i64, positions: *const i32,
+        frequencies: *const f64, attention_factor: f32, tokens: i64, q_heads: i64, k_heads: i64, head_dim: i64,
+        rotary_dim: i64, interleaved: c_int, qk_weight: *const u16, eps: f32, q_out: *mut u16, q_out_stride: i64,
+        k_out: *mut u16, k_out_stride: i64, stream: *mut c_void) -> c_int;
+    pub fn izwi_rope_positions_bf16(q: *const u16, q_stride: i64, k: *const u16, k_stride: i64,
+        positions: *const i32, frequencies: *const f64, attention_factor: f32, tokens: i64, q_heads: i64,
+        k_heads: i64, head_dim: i64, rotary_dim: i64, interleaved: c_int, qk_weight: *const u16, eps: f32,
+        q_out: *mut u16, q_out_stride: i64, k_out: *mut u16, k_out_stride: i64, stream: *mut c_void) -> c_int;
+    pub fn izwi_qmm_prompt_attention_f32(q: *const f32, q_stride: i64, k: *const f32, k_stride: i64, v: *const f32,
+        v_stride: i64, cu_q: *const i32, cu_k: *const i32, batch: i64, total_q: i64, total_k: i64, max_k: i64,
+        num_heads: i64, num_kv_heads: i64, head_dim: i64, causal: c_int, scale: f32, out: *mut f32, out_stride: i64,
+        stream: *mut c_void) -> c_int;
+    pub fn izwi_qmm_prompt_attention_f16(q: *const u16, q_stride: i64, k: *const u16, k_stride: i64, v: *const u16,
+        v_stride: i64, cu_q: *const i32, cu_k: *const i32, batch: i64, total_q: i64, total_k: i64, max_k: i64,
+        num_heads: i64, num_kv_heads: i64, head_dim: i64, causal: c_int, scale: f32, out: *mut u16, out_stride: i64,
+        stream: *mut c_void) -> c_int;
+    pub fn izwi_qmm_prompt_attention_bf16(q: *const u16, q_stride: i64, k: *const u16, k_stride: i64, v: *const u16,
+        v_stride: i64, cu_q: *const i32, cu_k: *const i32, batch: i64, total_q: i64, total_k: i64, max_k: i64,
+        num_heads: i64, num_kv_heads: i64, head_dim: i64, causal: c_int, scale: f32, out: *mut u16, out_stride: i64,
         stream: *mut c_void) -> c_int;
     pub fn izwi_argmax_f32(logits: *const f32, rows: i64, n: i64, out: *mut u32, mem_space: c_int,
         stream: *mut c_void) -> c_int;
