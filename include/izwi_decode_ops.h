@@ -264,7 +264,8 @@ int izwi_rope_positions_bf16(const uint16_t* q, int64_t q_stride, const uint16_t
  * everything.  Rows of out that belong to no sequence stay as they are; a query that sees no key gives zeros.  max_k, the length of the
  * longest sequence of keys as far as the caller knows it (total_k at most), only decides how the work is shared out.
  * What a query does not see has no influence, whatever it holds.  A NaN that it sees in q or a key makes its row NaN, one in a
- * value that element; infinities go as in the formula, in f32 they count as NaN.
+ * value that element; an infinity in a value makes the element that infinity, or NaN (where its weight is too small for the type, and
+ * in f32).
  * The products run on the matrix cores with f32 sums: f16 and bf16 values as they are, weights rounded to the type (2^-11, 2^-8 of
  * each); f32 ones as three bf16 numbers each, all 24 bits.  head_dim 64, 128 or 256; rows begin on 16 bytes; out shares no memory with
  * the inputs.  Uses the library's per-stream scratch where few rows meet many keys. */

@@ -156,10 +156,13 @@ __device__ __forceinline__ float max_lane32(float v) {
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
+// 2^d, d <= 0, for what is summed already: not zero, which would make NaN of an infinity
+__device__ __forceinline__ float rescale(float d) { return fmaxf(__builtin_amdgcn_exp2f(d), 0x1p-126f); }
+
 constexpr float kSlack = 8.0f; // a reference stands until a score passes it by this (base 2): weights stay below 2^8
 
 template <typename T, int D, int W, int KT, bool SPLIT>
-__global__ __launch_bounds__(64 * W) void prompt_attention_kernel(PromptParams P) {
+__global__ __launch_bounds__(64 * W, D == 64 || (D == 128 && Elem<T>::N == 1) ? 2 : 1) void prompt_attention_kernel(PromptParams P) {
     using E = Elem<T>;
     constexpr int N = E::N, kRows = 32 * W, KK = D / 16, PT = KT / 32, DT = D / 32;
     constexpr bool kDirect = N == 1;          // keys and values go straight from memory into LDS
@@ -287,42 +290,14 @@ __global__ __launch_bounds__(64 * W) void prompt_attention_kernel(PromptParams P
     for (int d = 0; d < DT; d++)
 #pragma unroll
         for (int r = 0; r < 16; r++) o[d][r] = 0.0f;
-    float ref = -INFINITY, sum = 0.0f; // ref: base 2; sum: of this lane's positions
+    float ref = -INFINITY, sum[2] = {}; // ref: base 2; sum: of this lane's positions, in two parts
     if (threadIdx.x == 0) *odd_values = 0;
 
-    if (first < end) request(first, 0);
-    for (int tile = first; tile < end; tile++) {
-        const uint8_t* here = smem;
-        if constexpr (kDirect) {
-            const int stage = (tile - first) & 1;
-            here = smem + stage * kTile;
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            if (tile + 1 < end) request(tile + 1, stage ^ 1);
-        } else {
-            __syncthreads(); // the tile before is read
-            deliver();
-            if (tile + 1 < end) request(tile + 1, 0);
-            __syncthreads();
-        }
-        const int p0 = tile * KT;
-        const bool masked = p0 + KT > fewest || p0 + KT > s.len_k; // for some row of the workgroup
-        bool odd = false;
-        if (masked) { // a value that is no number must not reach the rows that do not see it: a weight of zero would not keep it out
-            bool any = false;
-            constexpr int kReads = N * kPlane / 16 / (64 * W);
-#pragma unroll
-            for (int i = 0; i < kReads; i++) {
-                const u32x4 v = *reinterpret_cast<const u32x4*>(here + N * kPlane + (i * 64 * W + threadIdx.x) * 16);
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-                    any |= (v[j] & (E::kExponent >> 16)) == (E::kExponent >> 16) || (v[j] & (E::kExponent & 0xffff0000u)) == (E::kExponent & 0xffff0000u);
-            }
-            if (__any(any) && lane == 0) *odd_values = tile + 1;
-            __syncthreads();
-            odd = *odd_values == (uint32_t)(tile + 1);
-        }
-
-        // scores: lane (x, h), register r of sub-tile pt: row x, position p0 + 32 pt + 8 (r / 4) + 4 h + r % 4
+    // Scores, weights and the weighted values of a tile that has landed.  MASKED: some row of the workgroup does not see all of its
+    // positions.
+    const auto weigh = [&](auto masked, const uint8_t* here, int p0) {
+        constexpr bool MASKED = decltype(masked)::value;
+        // lane (x, h), register r of sub-tile pt: row x, position p0 + 32 pt + 8 (r / 4) + 4 h + r % 4
         f32x16 p[PT];
 #pragma unroll
         for (int pt = 0; pt < PT; pt++) {
@@ -336,7 +311,7 @@ __global__ __launch_bounds__(64 * W) void prompt_attention_kernel(PromptParams P
                 p[pt] = mma_of<T>(a, q[kk], p[pt]);
             }
         }
-        if (masked) {
+        if constexpr (MASKED) {
 #pragma unroll
             for (int pt = 0; pt < PT; pt++)
 #pragma unroll
@@ -351,8 +326,8 @@ __global__ __launch_bounds__(64 * W) void prompt_attention_kernel(PromptParams P
         top = max_lane32(top) * P.scale;
         const bool passed = top > ref + kSlack; // (from -infinity: at the first score)
         if (__any(passed)) {                    // a row's own reference moves only by its own scores: no other row has a say in its result
-            const float next = passed ? top : ref, by = ref == next ? 1.0f : __builtin_amdgcn_exp2f(ref - next);
-            sum *= by;
+            const float next = passed ? top : ref, by = ref == -INFINITY ? 1.0f : rescale(ref - next); // (zeros so far, and what is no number)
+            sum[0] *= by, sum[1] *= by;
 #pragma unroll
             for (int d = 0; d < DT; d++) o[d] *= by;
             ref = next;
@@ -365,7 +340,7 @@ __global__ __launch_bounds__(64 * W) void prompt_attention_kernel(PromptParams P
                 float e = __builtin_fmaf(p[pt][r], P.scale, -from);
                 if constexpr (N == 3) e = p[pt][r] == -INFINITY ? e : __builtin_fmaf(p[pt][r], P.scale_rest, e); // (the rest may be negative)
                 p[pt][r] = __builtin_amdgcn_exp2f(e);
-                sum += p[pt][r];
+                sum[r & 1] += p[pt][r];
             }
 
         // sixteen positions at a time: the lane's eight are 4 h + 0..3 and 8 + 4 h + 0..3 of them
@@ -394,49 +369,81 @@ __global__ __launch_bounds__(64 * W) void prompt_attention_kernel(PromptParams P
                     const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(plane + (v_at1 ^ (d << 6)))));
                     a[n] = u32x4{lo[0], lo[1], hi[0], hi[1]};
                 }
-                if (odd) { // (uniform) without what is no number; see below
-#pragma unroll
-                    for (int n = 0; n < N; n++)
-#pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            if ((a[n][j] & (E::kExponent >> 16)) == (E::kExponent >> 16)) a[n][j] &= 0xffff0000u;
-                            if ((a[n][j] & (E::kExponent & 0xffff0000u)) == (E::kExponent & 0xffff0000u)) a[n][j] &= 0xffffu;
-                        }
-                }
                 o[d] = mma_of<T>(a, w, o[d]);
             }
         }
-        if (odd) { // infinities and NaN, to the rows that see them
+    };
+
+    const auto arrive = [&](int tile) { // the tile is in LDS, the one behind it on its way
+        if constexpr (kDirect) {
+            const int stage = (tile - first) & 1;
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            if (tile + 1 < end) request(tile + 1, stage ^ 1);
+            return smem + stage * kTile;
+        } else {
+            __syncthreads(); // the tile before is read
+            deliver();
+            if (tile + 1 < end) request(tile + 1, 0);
+            __syncthreads();
+            return smem;
+        }
+    };
+    if (first < end) request(first, 0);
+    int tile = first;
+    for (const int whole = min(end, fewest / KT); tile < whole; tile++) weigh(std::false_type{}, arrive(tile), tile * KT); // every row sees all of these
+    for (; tile < end; tile++) {
+        uint8_t* const here = arrive(tile);
+        const int p0 = tile * KT;
+        // A value that is no number must not reach the rows that do not see it, and a weight of zero would not keep it out: where there are
+        // any, the rows that see them get them here and the tile goes on with zeros in their place.
+        constexpr int kReads = N * kPlane / 16 / (64 * W);
+        constexpr uint32_t kLow = E::kExponent & 0xffffu, kHigh = E::kExponent & 0xffff0000u;
+        u32x4* const values = reinterpret_cast<u32x4*>(here + N * kPlane) + threadIdx.x;
+        bool any = false;
+#pragma unroll
+        for (int i = 0; i < kReads; i++) {
+            const u32x4 v = values[i * 64 * W];
+#pragma unroll
+            for (int j = 0; j < 4; j++) any |= (v[j] & kLow) == kLow || (v[j] & kHigh) == kHigh;
+        }
+        if (__any(any) && lane == 0) *odd_values = tile + 1;
+        __syncthreads();
+        if (*odd_values == (uint32_t)(tile + 1)) {
 #pragma unroll 1
             for (int j = 0; j < min(KT, s.len_k - p0); j++) {
+                const bool sees = p0 + j <= limit;
 #pragma unroll
                 for (int d = 0; d < DT; d++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int c = (4 * d + i) ^ turn<D>(j);
+                    for (int r = 0; r < 16; r++)
 #pragma unroll
                         for (int n = 0; n < N; n++) {
-                            const u32x2 v = *reinterpret_cast<const u32x2*>(here + (N + n) * kPlane + j * (2 * D) + 16 * c + 8 * h);
-#pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                const uint16_t bits = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
-                                const bool is = (bits & (uint16_t)E::kExponent) == (uint16_t)E::kExponent && p0 + j <= limit;
-                                const float value = std::is_same_v<T, f16_t> ? qmm_f16_bits_to_f32(bits) : qmm_bf16_bits_to_f32(bits);
-                                o[d][4 * i + e] += is ? value : 0.0f;
-                            }
+                            const int c = (4 * d + (r >> 2)) ^ turn<D>(j);
+                            const uint16_t bits = *reinterpret_cast<const uint16_t*>(here + (N + n) * kPlane + j * (2 * D) + 16 * c + 8 * h + 2 * (r & 3));
+                            const float value = std::is_same_v<T, f16_t> ? qmm_f16_bits_to_f32(bits) : qmm_bf16_bits_to_f32(bits);
+                            o[d][r] += sees && (bits & kLow) == kLow ? value : 0.0f;
                         }
-                    }
             }
+            __syncthreads();
+#pragma unroll 1
+            for (int i = 0; i < kReads; i++) {
+                u32x4 v = values[i * 64 * W];
+#pragma unroll
+                for (int j = 0; j < 4; j++) v[j] &= ((v[j] & kLow) == kLow ? 0u : 0xffffu) | ((v[j] & kHigh) == kHigh ? 0u : 0xffff0000u);
+                values[i * 64 * W] = v;
+            }
+            __syncthreads();
         }
+        weigh(std::true_type{}, here, p0);
     }
 
     // rows behind the sequence's last stay as they are
     if (s.row0 + wave * 32 + x >= rows) return;
-    sum = qmm_add_lane32(sum);
+    const float total = qmm_add_lane32(sum[0] + sum[1]);
     const int64_t out_row = (s.q0 + token) * P.heads + head;
     if constexpr (SPLIT) {
         // (a sum below zero: the split has no position that the row sees)
-        if (h == 0) P.stats[out_row * P.splits + split] = float2{ref, first < end && limit >= first * KT ? sum : -1.0f};
+        if (h == 0) P.stats[out_row * P.splits + split] = float2{ref, first < end && limit >= first * KT ? total : -1.0f};
         float* to = P.sums + (out_row * P.splits + split) * D + 4 * h;
 #pragma unroll
         for (int d = 0; d < DT; d++)
@@ -445,7 +452,7 @@ __global__ __launch_bounds__(64 * W) void prompt_attention_kernel(PromptParams P
         return;
     }
     const bool none = limit < 0 || s.len_k == 0;
-    const float inv = none ? 0.0f : 1.0f / sum;
+    const float inv = none ? 0.0f : 1.0f / total;
     T* const to = static_cast<T*>(P.out) + (s.q0 + token) * P.out_stride + (int64_t)head * D;
 #pragma unroll
     for (int d = 0; d < DT; d++) {
@@ -493,9 +500,9 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(PromptParams P, int64_
         const float2 st = P.stats[row * P.splits + i];
         if (st.y < 0.0f) continue; // no position that the row sees
         any = true;
-        // (a reference of -infinity: no score is above it; a NaN among them is in sum and sums, and stays)
-        const float next = fmaxf(ref, st.x), old = ref == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ref - next);
-        const float by = st.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(st.x - next);
+        // (a reference of -infinity: no score is above it, the sums are zero or no number)
+        const float next = fmaxf(ref, st.x), old = ref == -INFINITY ? 1.0f : rescale(ref - next);
+        const float by = st.x == -INFINITY ? 1.0f : rescale(st.x - next);
         sum = sum * old + st.y * by;
 #pragma unroll
         for (int j = 0; j < N; j++) a[j] = a[j] * old + P.sums[(row * P.splits + i) * D + lane * N + j] * by;
@@ -516,24 +523,38 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(PromptParams P, int64_
     } while (0)
 
 template <typename T, int D, int W>
-hipError_t launch(const PromptParams& P, hipStream_t stream) {
+hipError_t launch(PromptParams P, int64_t max_k, int device, int n_cus, hipStream_t stream) {
     constexpr int N = Elem<T>::N, KT = N == 3 || D == 256 ? 32 : 64;
     constexpr size_t lds = (size_t)2 * N * KT * D * 2 * (N == 1 ? 2 : 1) + 16;
     static_assert(lds <= 160 * 1024);
+    P.tiles = (int)(P.total_q * P.group / (32 * W) + P.batch);
+    const int64_t wgs = (int64_t)P.tiles * P.kv_heads, pos_tiles = (max_k + KT - 1) / KT;
+    P.splits = (int)std::max<int64_t>(1, std::min(n_cus / wgs, pos_tiles / 4));
+    const int64_t rows = P.total_q * P.heads;
+    if (P.splits > 1) {
+        void* scratch = nullptr;
+        const hipError_t e = qmm_get_scratch(device, stream, (size_t)rows * P.splits * (D * sizeof(float) + sizeof(float2)), &scratch);
+        if (e != hipSuccess) return e;
+        P.sums = static_cast<float*>(scratch);
+        P.stats = reinterpret_cast<float2*>(P.sums + (size_t)rows * P.splits * D);
+    }
     const auto run = [&](auto kernel) {
         if (lds > 64 * 1024) {
             const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
             if (e != hipSuccess) return e;
         }
-        kernel<<<(unsigned)((int64_t)P.tiles * P.splits * P.kv_heads), 64 * W, lds, stream>>>(P);
+        kernel<<<(unsigned)(wgs * P.splits), 64 * W, lds, stream>>>(P);
         return hipGetLastError();
     };
     if (P.splits == 1) return run(prompt_attention_kernel<T, D, W, KT, false>);
     const hipError_t e = run(prompt_attention_kernel<T, D, W, KT, true>);
     if (e != hipSuccess) return e;
-    const int64_t rows = P.total_q * P.heads;
     prompt_join_kernel<T, D><<<(unsigned)((rows + 3) / 4), 256, 0, stream>>>(P, rows);
     return hipGetLastError();
+}
+template <typename T, int D>
+hipError_t launch_of(const PromptParams& P, int64_t max_k, int device, int n_cus, hipStream_t stream) {
+    return launch<T, D, 4>(P, max_k, device, n_cus, stream);
 }
 
 template <typename T>
@@ -568,9 +589,8 @@ int prompt_attention_impl(const T* q, int64_t q_stride, const T* k, int64_t k_st
     };
     if (overlap(q, total_q, q_stride, heads * d) || overlap(k, total_k, k_stride, kv_heads * d) || overlap(v, total_k, v_stride, kv_heads * d))
         return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: out shares memory with q, k or v", what);
-    constexpr int W = 4;
-    const int64_t tiles = total_q * (heads / kv_heads) / (32 * W) + batch, wgs = tiles * kv_heads;
-    if (wgs > 0x3fffff) return qmm_fail(IZWI_QMM_ERR_UNSUPPORTED, "%s: %lld sequences on %lld kv heads", what, (long long)batch, (long long)kv_heads);
+    if ((total_q * (heads / kv_heads) / 32 + batch) * kv_heads > 0x3fffff)
+        return qmm_fail(IZWI_QMM_ERR_UNSUPPORTED, "%s: %lld sequences on %lld kv heads", what, (long long)batch, (long long)kv_heads);
     int device = 0, n_cus = 0;
     if (int rc = qmm_current_device(&device, &n_cus)) return rc;
     PromptParams P{};
@@ -581,20 +601,12 @@ int prompt_attention_impl(const T* q, int64_t q_stride, const T* k, int64_t k_st
     const double by = std::fabs((double)scale) * 1.4426950408889634074;
     P.sign = scale == 0.0f ? 0.0f : scale < 0.0f ? -1.0f : 1.0f;
     P.scale = scale == 0.0f ? 1.0f : (float)by, P.scale_rest = scale == 0.0f ? 0.0f : (float)(by - (double)P.scale);
-    constexpr int kt = sizeof(T) == 4 ? 32 : 64;
-    P.tiles = (int)tiles;
-    const int64_t pos_tiles = (std::min(max_k, total_k) + kt - 1) / kt;
-    P.splits = (int)std::max<int64_t>(1, std::min(n_cus / wgs, pos_tiles / 4));
+    max_k = std::min(max_k, total_k);
     hipStream_t stream = (hipStream_t)stream_;
     QmmCallScope call;
-    if (P.splits > 1) {
-        const size_t rows = (size_t)total_q * heads * P.splits;
-        void* scratch = nullptr;
-        PROMPT_TRY(qmm_get_scratch(device, stream, rows * (d * sizeof(float) + sizeof(float2)), &scratch));
-        P.sums = static_cast<float*>(scratch);
-        P.stats = reinterpret_cast<float2*>(P.sums + rows * d);
-    }
-    PROMPT_TRY((d == 64 ? launch<T, 64, W>(P, stream) : d == 128 ? launch<T, 128, W>(P, stream) : launch<T, 256, W>(P, stream)));
+    PROMPT_TRY((d == 64    ? launch_of<T, 64>(P, max_k, device, n_cus, stream)
+                : d == 128 ? launch_of<T, 128>(P, max_k, device, n_cus, stream)
+                           : launch_of<T, 256>(P, max_k, device, n_cus, stream)));
     return IZWI_QMM_OK;
 }
 
