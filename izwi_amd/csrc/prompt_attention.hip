@@ -95,6 +95,16 @@ __device__ __forceinline__ void split3(float a, float b, uint32_t (&to)[3]) {
     to[2] = __builtin_amdgcn_perm(__float_as_uint(b2), __float_as_uint(a2), kTop);
 }
 
+__device__ __forceinline__ void split8(const float (&v)[8], u32x4 (&to)[3]) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        uint32_t three[3];
+        split3(v[2 * i], v[2 * i + 1], three);
+#pragma unroll
+        for (int n = 0; n < 3; n++) to[n][i] = three[n];
+    }
+}
+
 // acc += a b with N numbers a value: the products whose weight is 2^-16 or more
 template <typename T>
 __device__ __forceinline__ f32x16 mma_of(const u32x4 (&a)[Elem<T>::N], const u32x4 (&b)[Elem<T>::N], f32x16 acc) {
@@ -161,18 +171,21 @@ __device__ __forceinline__ float rescale(float d) { return fmaxf(__builtin_amdgc
 
 constexpr float kSlack = 8.0f; // a reference stands until a score passes it by this (base 2): weights stay below 2^8
 
-template <typename T, int D, int W, int KT, bool SPLIT>
-__global__ __launch_bounds__(64 * W, D == 64 || (D == 128 && Elem<T>::N == 1) ? 2 : 1) void prompt_attention_kernel(PromptParams P) {
+// WR sets of waves have 32 rows each, WZ sets KT positions each of a tile, DZ sets a part each of the head's elements: of heads of 256 one wave would hold
+// twice the registers; two add up their scores through LDS and weigh their own halves of the values.
+template <typename T, int D, int WR, int WZ, int DZ, int KT, bool SPLIT>
+__global__ __launch_bounds__(64 * WR * WZ * DZ, Elem<T>::N == 1 || D == 64 ? 2 : 1) void prompt_attention_kernel(PromptParams P) {
     using E = Elem<T>;
-    constexpr int N = E::N, kRows = 32 * W, KK = D / 16, PT = KT / 32, DT = D / 32;
+    constexpr int N = E::N, W = WR * WZ * DZ, kRows = 32 * WR, KS = KT * WZ, DW = D / DZ, KK = DW / 16, PT = KT / 32, DT = DW / 32;
     constexpr bool kDirect = N == 1;          // keys and values go straight from memory into LDS
-    constexpr int kPlane = KT * D * 2;        // bytes of a tile of 16-bit numbers
+    constexpr int kPlane = KS * D * 2;        // bytes of a tile of 16-bit numbers
     constexpr int kTile = 2 * N * kPlane;     // keys, then values
-    extern __shared__ __attribute__((aligned(16))) uint8_t smem[]; // tiles (two where direct), then a word
-    uint32_t* odd_values = reinterpret_cast<uint32_t*>(smem + kTile * (kDirect ? 2 : 1));
+    constexpr int kTiles = kTile * (kDirect ? 2 : 1), kScores = DZ > 1 ? 2 * W * PT * 16 * 256 : 0;
+    extern __shared__ __attribute__((aligned(16))) uint8_t smem[]; // tiles (two where direct), partial scores of two tiles, a word
+    uint32_t* odd_values = reinterpret_cast<uint32_t*>(smem + kTiles + kScores);
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int x = lane & 31, h = lane >> 5;
+    const int x = lane & 31, h = lane >> 5, wr = wave % WR, dz = wave / WR % DZ, wz = wave / (WR * DZ);
     // the kv head runs fastest: workgroups of a kv head stay on one XCD, whose L2 then holds its keys and values; the last tiles of a
     // sequence, which see the most positions, begin first
     const int kv = blockIdx.x % P.kv_heads;
@@ -181,61 +194,29 @@ __global__ __launch_bounds__(64 * W, D == 64 || (D == 128 && Elem<T>::N == 1) ? 
     if (!find_sequence(P, kRows, P.tiles - 1 - (SPLIT ? unit / P.splits : unit), lane, s)) return; // the whole workgroup
 
     const int rows = s.len_q * P.group; // of the sequence and kv head (fits: checked on the host)
-    const int row = min(s.row0 + wave * 32 + x, rows - 1), token = row / P.group, head = kv * P.group + row % P.group;
+    const int row = min(s.row0 + wr * 32 + x, rows - 1), token = row / P.group, head = kv * P.group + row % P.group;
     const int past = s.len_k - s.len_q;
     // positions up to `limit` count; of the workgroup's rows the first sees the fewest, the last the most
     const int limit = P.causal ? token + past : s.len_k - 1;
     const int last_token = min(s.row0 + kRows - 1, rows - 1) / P.group;
     const int fewest = P.causal ? max(s.row0 / P.group + past + 1, 0) : s.len_k;
     const int most = P.causal ? min(max(last_token + past + 1, 0), s.len_k) : s.len_k;
-    const int n_tiles = (most + KT - 1) / KT;
+    const int n_tiles = (most + KS - 1) / KS;
     const int share = SPLIT ? (n_tiles + P.splits - 1) / P.splits : n_tiles;
     const int first = SPLIT ? min(split * share, n_tiles) : 0, end = min(first + share, n_tiles);
-
-    // queries: lane (x, h) has of row x the elements 16 kk + 8 h .. + 7
-    u32x4 q[KK][N];
-    {
-        const T* from = static_cast<const T*>(P.q) + (s.q0 + token) * P.q_stride + (int64_t)head * D + 8 * h;
-#pragma unroll
-        for (int kk = 0; kk < KK; kk++) {
-            if constexpr (N == 1) {
-                typedef T vec __attribute__((ext_vector_type(8)));
-                const vec v = *reinterpret_cast<const vec*>(from + 16 * kk);
-                vec r;
-#pragma unroll
-                for (int i = 0; i < 8; i++) r[i] = (T)((float)v[i] * P.sign); // exact
-                q[kk][0] = __builtin_bit_cast(u32x4, r);
-            } else {
-                float v[8];
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const f32x4 a = *reinterpret_cast<const f32x4*>(from + 16 * kk + 4 * i) * P.sign;
-#pragma unroll
-                    for (int j = 0; j < 4; j++) v[4 * i + j] = a[j];
-                }
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    uint32_t to[3];
-                    split3(v[2 * i], v[2 * i + 1], to);
-#pragma unroll
-                    for (int n = 0; n < 3; n++) q[kk][n][i] = to[n];
-                }
-            }
-        }
-    }
 
     const uint8_t* const k_rows = reinterpret_cast<const uint8_t*>(static_cast<const T*>(P.k) + s.k0 * P.k_stride + (int64_t)kv * D);
     const uint8_t* const v_rows = reinterpret_cast<const uint8_t*>(static_cast<const T*>(P.v) + s.k0 * P.v_stride + (int64_t)kv * D);
     const int64_t k_step = P.k_stride * (int)sizeof(T), v_step = P.v_stride * (int)sizeof(T);
 
     // A tile on its way into LDS.  Positions behind the last repeat it (they are masked).
-    constexpr int kPer = KT * D / 8 / (64 * W); // pieces of 8 values that a thread has of the keys, and of the values
-    static_assert(kPer * 8 * 64 * W == KT * D);
+    constexpr int kPer = KS * D / 8 / (64 * W); // pieces of 8 values that a thread has of the keys, and of the values
+    static_assert(kPer * 8 * 64 * W == KS * D);
     [[maybe_unused]] f32x4 ahead[kDirect ? 1 : 2][kDirect ? 1 : kPer][2];
     const auto request = [&](int tile, int stage) {
-        const int most_row = min(KT, s.len_k - tile * KT) - 1;
-        const uint8_t* const kb = k_rows + (int64_t)tile * KT * k_step;
-        const uint8_t* const vb = v_rows + (int64_t)tile * KT * v_step;
+        const int most_row = min(KS, s.len_k - tile * KS) - 1;
+        const uint8_t* const kb = k_rows + (int64_t)tile * KS * k_step;
+        const uint8_t* const vb = v_rows + (int64_t)tile * KS * v_step;
         if constexpr (kDirect) {
             const uint32_t base = (uint32_t)(uintptr_t)smem + stage * kTile;
 #pragma unroll
@@ -264,26 +245,51 @@ __global__ __launch_bounds__(64 * W, D == 64 || (D == 128 && Elem<T>::N == 1) ? 
 #pragma unroll
                 for (int i = 0; i < kPer; i++) {
                     const int piece = i * (64 * W) + threadIdx.x, r = piece / (D / 8), c = (piece % (D / 8)) ^ turn<D>(r);
+                    float v[8];
+#pragma unroll
+                    for (int j = 0; j < 8; j++) v[j] = ahead[w][i][j >> 2][j & 3];
                     u32x4 o[3];
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        uint32_t to[3];
-                        split3(ahead[w][i][j >> 1][2 * j & 3], ahead[w][i][j >> 1][(2 * j & 3) + 1], to);
-#pragma unroll
-                        for (int n = 0; n < 3; n++) o[n][j] = to[n];
-                    }
+                    split8(v, o);
 #pragma unroll
                     for (int n = 0; n < 3; n++) *reinterpret_cast<u32x4*>(smem + (w * 3 + n) * kPlane + r * (2 * D) + 16 * c) = o[n];
                 }
         }
     };
 
+    if (first < end) request(first, 0); // (ahead of the queries: both ways to memory at once)
+
+    // queries: lane (x, h) has of row x the elements 16 kk + 8 h .. + 7 of the wave's part of the head
+    u32x4 q[KK][N];
+    {
+        const T* from = static_cast<const T*>(P.q) + (s.q0 + token) * P.q_stride + (int64_t)head * D + dz * DW + 8 * h;
+#pragma unroll
+        for (int kk = 0; kk < KK; kk++) {
+            if constexpr (N == 1) {
+                typedef T vec __attribute__((ext_vector_type(8)));
+                const vec v = *reinterpret_cast<const vec*>(from + 16 * kk);
+                vec r;
+#pragma unroll
+                for (int i = 0; i < 8; i++) r[i] = (T)((float)v[i] * P.sign); // exact
+                q[kk][0] = __builtin_bit_cast(u32x4, r);
+            } else {
+                float v[8];
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const f32x4 a = *reinterpret_cast<const f32x4*>(from + 16 * kk + 4 * i) * P.sign;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) v[4 * i + j] = a[j];
+                }
+                split8(v, q[kk]);
+            }
+        }
+    }
+
     // where a lane reads: keys of position x, piece 2 kk + h; values of positions 4 h + 0..3 (+ 8) through the transposing read, for
     // which the lanes of a sixteen name four rows of four pieces of 8 bytes
-    const int k_at = x * (2 * D) + ((h ^ turn<D>(x)) << 4);
+    const int k_at = (wz * KT + x) * (2 * D) + dz * (2 * DW) + ((h ^ turn<D>(x)) << 4);
     const int i16 = lane & 15, v_row = 4 * h + (i16 >> 2), v_piece = (lane >> 4 & 1) * 2 + (i16 >> 1 & 1);
-    const int v_at0 = v_row * (2 * D) + ((v_piece ^ turn<D>(v_row)) << 4) + (i16 & 1) * 8;
-    const int v_at1 = (v_row + 8) * (2 * D) + ((v_piece ^ turn<D>(v_row + 8)) << 4) + (i16 & 1) * 8;
+    const int v_at0 = (wz * KT + v_row) * (2 * D) + dz * (2 * DW) + ((v_piece ^ turn<D>(v_row)) << 4) + (i16 & 1) * 8;
+    const int v_at1 = (wz * KT + v_row + 8) * (2 * D) + dz * (2 * DW) + ((v_piece ^ turn<D>(v_row + 8)) << 4) + (i16 & 1) * 8;
 
     f32x16 o[DT];
 #pragma unroll
@@ -295,6 +301,7 @@ __global__ __launch_bounds__(64 * W, D == 64 || (D == 128 && Elem<T>::N == 1) ? 
 
     // Scores, weights and the weighted values of a tile that has landed.  MASKED: some row of the workgroup does not see all of its
     // positions.
+    [[maybe_unused]] int turns = 0;
     const auto weigh = [&](auto masked, const uint8_t* here, int p0) {
         constexpr bool MASKED = decltype(masked)::value;
         // lane (x, h), register r of sub-tile pt: row x, position p0 + 32 pt + 8 (r / 4) + 4 h + r % 4
@@ -310,6 +317,26 @@ __global__ __launch_bounds__(64 * W, D == 64 || (D == 128 && Elem<T>::N == 1) ? 
                 for (int n = 0; n < N; n++) a[n] = *reinterpret_cast<const u32x4*>(here + n * kPlane + pt * 32 * (2 * D) + (k_at ^ (kk << 5)));
                 p[pt] = mma_of<T>(a, q[kk], p[pt]);
             }
+        }
+        if constexpr (DZ > 1) { // (two places in turn: a wave may still read the last tile's)
+            static_assert(DZ == 2);
+            f32x4* const scores = reinterpret_cast<f32x4*>(smem + kTiles) + turns * (W * PT * 4 * 64) + lane;
+            turns ^= 1;
+#pragma unroll
+            for (int pt = 0; pt < PT; pt++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    scores[((wave * PT + pt) * 4 + i) * 64] = f32x4{p[pt][4 * i], p[pt][4 * i + 1], p[pt][4 * i + 2], p[pt][4 * i + 3]};
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            const int other = wave + (dz ? -WR : WR);
+#pragma unroll
+            for (int pt = 0; pt < PT; pt++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const f32x4 v = scores[((other * PT + pt) * 4 + i) * 64];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) p[pt][4 * i + j] += v[j]; // (the same sum in both)
+                }
         }
         if constexpr (MASKED) {
 #pragma unroll
@@ -347,18 +374,11 @@ __global__ __launch_bounds__(64 * W, D == 64 || (D == 128 && Elem<T>::N == 1) ? 
 #pragma unroll
         for (int t = 0; t < KT / 16; t++) {
             u32x4 w[N];
+            float v[8];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float a = p[t >> 1][8 * (t & 1) + 2 * i], b = p[t >> 1][8 * (t & 1) + 2 * i + 1];
-                if constexpr (N == 1) {
-                    w[0][i] = E::pack(a, b);
-                } else {
-                    uint32_t to[3];
-                    split3(a, b, to);
-#pragma unroll
-                    for (int n = 0; n < 3; n++) w[n][i] = to[n];
-                }
-            }
+            for (int i = 0; i < 8; i++) v[i] = p[t >> 1][8 * (t & 1) + i];
+            if constexpr (N == 1) w[0] = u32x4{E::pack(v[0], v[1]), E::pack(v[2], v[3]), E::pack(v[4], v[5]), E::pack(v[6], v[7])};
+            else split8(v, w);
 #pragma unroll
             for (int d = 0; d < DT; d++) {
                 u32x4 a[N];
@@ -388,63 +408,103 @@ __global__ __launch_bounds__(64 * W, D == 64 || (D == 128 && Elem<T>::N == 1) ? 
             return smem;
         }
     };
-    if (first < end) request(first, 0);
-    int tile = first;
-    for (const int whole = min(end, fewest / KT); tile < whole; tile++) weigh(std::false_type{}, arrive(tile), tile * KT); // every row sees all of these
-    for (; tile < end; tile++) {
-        uint8_t* const here = arrive(tile);
-        const int p0 = tile * KT;
-        // A value that is no number must not reach the rows that do not see it, and a weight of zero would not keep it out: where there are
-        // any, the rows that see them get them here and the tile goes on with zeros in their place.
-        constexpr int kReads = N * kPlane / 16 / (64 * W);
-        constexpr uint32_t kLow = E::kExponent & 0xffffu, kHigh = E::kExponent & 0xffff0000u;
-        u32x4* const values = reinterpret_cast<u32x4*>(here + N * kPlane) + threadIdx.x;
-        bool any = false;
+    // A value that is no number must not reach the rows that do not see it, and a weight of zero would not keep it out.  Results that hold one
+    // are worked out once more, with care: the rows that see such a value get it by itself, and the tile goes on with a zero in its
+    // place.  (A look at the values of every tile that some row does not see all of took 1200 of the 11600 cycles of 37 bf16 tokens.)
+    for (bool care = false;;) {
+        int tile = first;
+        for (const int whole = min(end, fewest / KS); tile < whole; tile++) weigh(std::false_type{}, arrive(tile), 0); // every row sees all of these
+        for (; tile < end; tile++) {
+            uint8_t* const here = arrive(tile);
+            const int p0 = tile * KS;
+            if (care) {
+                constexpr uint32_t kLow = E::kExponent & 0xffffu, kHigh = E::kExponent & 0xffff0000u;
+#pragma unroll 1
+                for (int j = wz * KT; j < min((wz + 1) * KT, s.len_k - p0); j++) {
+                    const bool sees = p0 + j <= limit;
 #pragma unroll
-        for (int i = 0; i < kReads; i++) {
-            const u32x4 v = values[i * 64 * W];
+                    for (int d = 0; d < DT; d++)
 #pragma unroll
-            for (int j = 0; j < 4; j++) any |= (v[j] & kLow) == kLow || (v[j] & kHigh) == kHigh;
+                        for (int r = 0; r < 16; r++)
+#pragma unroll
+                            for (int n = 0; n < N; n++) {
+                                const int c = (dz * (DW / 8) + 4 * d + (r >> 2)) ^ turn<D>(j);
+                                const uint16_t bits = *reinterpret_cast<const uint16_t*>(here + (N + n) * kPlane + j * (2 * D) + 16 * c + 8 * h + 2 * (r & 3));
+                                const float value = std::is_same_v<T, f16_t> ? qmm_f16_bits_to_f32(bits) : qmm_bf16_bits_to_f32(bits);
+                                o[d][r] += sees && (bits & kLow) == kLow ? value : 0.0f;
+                            }
+                }
+                __syncthreads();
+                u32x4* const values = reinterpret_cast<u32x4*>(here + N * kPlane) + threadIdx.x;
+#pragma unroll 1
+                for (int i = 0; i < N * kPlane / 16 / (64 * W); i++) {
+                    u32x4 v = values[i * 64 * W];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) v[j] &= ((v[j] & kLow) == kLow ? 0u : 0xffffu) | ((v[j] & kHigh) == kHigh ? 0u : 0xffff0000u);
+                    values[i * 64 * W] = v;
+                }
+                __syncthreads();
+            }
+            weigh(std::true_type{}, here, p0 + wz * KT);
         }
-        if (__any(any) && lane == 0) *odd_values = tile + 1;
+        if (care || end * KS <= fewest) break;
+        float zero = 0.0f; // NaN where a result is no number
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) zero = __builtin_fmaf(o[d][r], 0.0f, zero);
+        if (__any(zero != 0.0f) && lane == 0) *odd_values = 1;
         __syncthreads();
-        if (*odd_values == (uint32_t)(tile + 1)) {
-#pragma unroll 1
-            for (int j = 0; j < min(KT, s.len_k - p0); j++) {
-                const bool sees = p0 + j <= limit;
+        if (*odd_values == 0) break;
+        care = true;
+        if (first < end) request(first, 0);
 #pragma unroll
-                for (int d = 0; d < DT; d++)
+        for (int d = 0; d < DT; d++)
 #pragma unroll
-                    for (int r = 0; r < 16; r++)
-#pragma unroll
-                        for (int n = 0; n < N; n++) {
-                            const int c = (4 * d + (r >> 2)) ^ turn<D>(j);
-                            const uint16_t bits = *reinterpret_cast<const uint16_t*>(here + (N + n) * kPlane + j * (2 * D) + 16 * c + 8 * h + 2 * (r & 3));
-                            const float value = std::is_same_v<T, f16_t> ? qmm_f16_bits_to_f32(bits) : qmm_bf16_bits_to_f32(bits);
-                            o[d][r] += sees && (bits & kLow) == kLow ? value : 0.0f;
-                        }
-            }
-            __syncthreads();
-#pragma unroll 1
-            for (int i = 0; i < kReads; i++) {
-                u32x4 v = values[i * 64 * W];
-#pragma unroll
-                for (int j = 0; j < 4; j++) v[j] &= ((v[j] & kLow) == kLow ? 0u : 0xffffu) | ((v[j] & kHigh) == kHigh ? 0u : 0xffff0000u);
-                values[i * 64 * W] = v;
-            }
-            __syncthreads();
-        }
-        weigh(std::true_type{}, here, p0);
+            for (int r = 0; r < 16; r++) o[d][r] = 0.0f;
+        ref = -INFINITY, sum[0] = sum[1] = 0.0f;
     }
 
+    sum[0] += sum[1];
+    if constexpr (WZ > 1) { // the sets' results meet in LDS
+        constexpr int kNumbers = DT * 16 + 2;
+        static_assert(DZ == 1 && (WZ - 1) * WR * kNumbers * 256 <= kTiles);
+        float* const meet = reinterpret_cast<float*>(smem) + lane;
+        __syncthreads();
+        if (wz > 0) {
+            float* const to = meet + ((wz - 1) * WR + wr) * kNumbers * 64;
+            to[0] = ref, to[64] = sum[0];
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) to[(2 + 16 * d + r) * 64] = o[d][r];
+        }
+        __syncthreads();
+        if (wz > 0) return;
+        float refs[WZ], all = ref;
+        refs[0] = ref;
+#pragma unroll
+        for (int z = 1; z < WZ; z++) refs[z] = meet[((z - 1) * WR + wr) * kNumbers * 64], all = fmaxf(all, refs[z]);
+#pragma unroll
+        for (int z = 0; z < WZ; z++) {
+            const float by = refs[z] == -INFINITY ? 1.0f : rescale(refs[z] - all);
+            const float* const in = meet + ((z - 1) * WR + wr) * kNumbers * 64;
+            sum[0] = z == 0 ? sum[0] * by : sum[0] + in[64] * by;
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) o[d][r] = z == 0 ? o[d][r] * by : o[d][r] + in[(2 + 16 * d + r) * 64] * by;
+        }
+        ref = all;
+    }
     // rows behind the sequence's last stay as they are
-    if (s.row0 + wave * 32 + x >= rows) return;
-    const float total = qmm_add_lane32(sum[0] + sum[1]);
+    if (s.row0 + wr * 32 + x >= rows) return;
+    const float total = qmm_add_lane32(sum[0]);
     const int64_t out_row = (s.q0 + token) * P.heads + head;
     if constexpr (SPLIT) {
         // (a sum below zero: the split has no position that the row sees)
-        if (h == 0) P.stats[out_row * P.splits + split] = float2{ref, first < end && limit >= first * KT ? total : -1.0f};
-        float* to = P.sums + (out_row * P.splits + split) * D + 4 * h;
+        if (h == 0 && dz == 0) P.stats[out_row * P.splits + split] = float2{ref, first < end && limit >= first * KS ? total : -1.0f};
+        float* to = P.sums + (out_row * P.splits + split) * D + dz * DW + 4 * h;
 #pragma unroll
         for (int d = 0; d < DT; d++)
 #pragma unroll
@@ -453,7 +513,7 @@ __global__ __launch_bounds__(64 * W, D == 64 || (D == 128 && Elem<T>::N == 1) ? 
     }
     const bool none = limit < 0 || s.len_k == 0;
     const float inv = none ? 0.0f : 1.0f / total;
-    T* const to = static_cast<T*>(P.out) + (s.q0 + token) * P.out_stride + (int64_t)head * D;
+    T* const to = static_cast<T*>(P.out) + (s.q0 + token) * P.out_stride + (int64_t)head * D + dz * DW;
 #pragma unroll
     for (int d = 0; d < DT; d++) {
         float v[16];
@@ -478,39 +538,82 @@ __global__ __launch_bounds__(64 * W, D == 64 || (D == 128 && Elem<T>::N == 1) ? 
     }
 }
 
-// A row's splits joined by a wave, lane l having elements l D / 64 on.
-template <typename T, int D>
+// A row's splits joined: by a wave where there are at most eight (FEW), else by a workgroup, D / 4 threads to a split.  Every lane works out
+// the weights itself from statistics that are requested together with the sums.  (One split after the other by a wave: 544 rows of 32
+// splits 19.6 us.)
+template <typename T, int D, bool FEW>
 __global__ __launch_bounds__(256) void prompt_join_kernel(PromptParams P, int64_t rows) {
-    constexpr int N = D / 64;
+    constexpr int E = FEW ? D / 64 : 4, kPer = 64 * 4 * (FEW ? 1 : 4) / D, A = FEW ? 8 : 4; // elements a thread, splits at once, requests at once
+    typedef float vec __attribute__((ext_vector_type(E)));
     const int lane = threadIdx.x & 63;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int64_t row = FEW ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
     if (row >= rows) return;
     const int64_t token = row / P.heads;
+    const float2* const stats = P.stats + row * P.splits;
+    const int at = FEW ? lane : threadIdx.x % (D / 4), mine = FEW ? 0 : threadIdx.x / (D / 4), step = FEW ? 1 : kPer;
+    const float* const sums = P.sums + row * P.splits * D + at * E;
     if (P.cu_q) { // rows behind the last sequence, or between two, were not written
         bool inside = false;
         for (int b0 = 0; b0 < P.batch && !inside; b0 += 64) {
             const int b = min(b0 + lane, P.batch - 1);
             inside = __any(token >= bounded(P.cu_q, b, P.total_q) && token < bounded(P.cu_q, b + 1, P.total_q));
         }
-        if (!inside) return;
+        if (!inside) return; // (the same in the whole workgroup)
     }
-    float ref = -INFINITY, sum = 0.0f, a[N] = {};
+    // (a reference of -infinity: no score is above it, the sums are zero or no number; a sum below zero: no position that the row sees)
+    float ref = -INFINITY;
+    for (int i = lane; i < P.splits; i += 64) {
+        const float2 st = stats[i];
+        ref = fmaxf(ref, st.y < 0.0f ? -INFINITY : st.x);
+    }
+    ref = qmm_max_lane_rows(ref);
+    ref = fmaxf(ref, dpp_f<0x128>(ref)); // row_ror:8, then 4, 2, 1
+    ref = fmaxf(ref, dpp_f<0x124>(ref));
+    ref = fmaxf(ref, dpp_f<0x4E>(ref));
+    ref = fmaxf(ref, dpp_f<0xB1>(ref));
+    float sum = 0.0f;
     bool any = false;
-    for (int i = 0; i < P.splits; i++) {
-        const float2 st = P.stats[row * P.splits + i];
-        if (st.y < 0.0f) continue; // no position that the row sees
-        any = true;
-        // (a reference of -infinity: no score is above it, the sums are zero or no number)
-        const float next = fmaxf(ref, st.x), old = ref == -INFINITY ? 1.0f : rescale(ref - next);
-        const float by = st.x == -INFINITY ? 1.0f : rescale(st.x - next);
-        sum = sum * old + st.y * by;
+    vec a = 0.0f;
+    for (int i0 = mine; i0 < P.splits; i0 += A * step) {
+        vec v[A];
+        float2 st[A];
 #pragma unroll
-        for (int j = 0; j < N; j++) a[j] = a[j] * old + P.sums[(row * P.splits + i) * D + lane * N + j] * by;
-        ref = next;
+        for (int j = 0; j < A; j++) {
+            const int i = min(i0 + j * step, P.splits - 1);
+            st[j] = stats[i];
+            v[j] = *reinterpret_cast<const vec*>(sums + (int64_t)i * D);
+        }
+#pragma unroll
+        for (int j = 0; j < A; j++) {
+            const bool there = i0 + j * step < P.splits && !(st[j].y < 0.0f);
+            const float by = st[j].x == -INFINITY ? 1.0f : rescale(st[j].x - ref);
+            any |= there;
+            sum += there ? st[j].y * by : 0.0f;
+            a += (there ? v[j] : vec(0.0f)) * by;
+        }
     }
-    T* to = static_cast<T*>(P.out) + token * P.out_stride + (row % P.heads) * D + lane * N;
+    T* const to = static_cast<T*>(P.out) + token * P.out_stride + (row % P.heads) * D + at * E;
+    if constexpr (FEW) {
 #pragma unroll
-    for (int j = 0; j < N; j++) to[j] = (T)(any ? a[j] / sum : 0.0f);
+        for (int e = 0; e < E; e++) to[e] = (T)(any ? a[e] / sum : 0.0f);
+    } else {
+        __shared__ vec part[kPer][D / 4];
+        __shared__ float part_sum[kPer]; // below zero: nothing
+        part[mine][at] = a;
+        if (at == 0) part_sum[mine] = any ? sum : -1.0f;
+        __syncthreads();
+        if (threadIdx.x >= D / 4) return;
+        any = false, sum = 0.0f, a = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+            const float s = part_sum[i];
+            any |= !(s < 0.0f);
+            sum += s < 0.0f ? 0.0f : s;
+            a += part[i][at];
+        }
+#pragma unroll
+        for (int e = 0; e < E; e++) to[e] = (T)(any ? a[e] / sum : 0.0f);
+    }
 }
 
 #define PROMPT_TRY(expr)                                                               \
@@ -522,13 +625,13 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(PromptParams P, int64_
         }                                                                              \
     } while (0)
 
-template <typename T, int D, int W>
+template <typename T, int D, int WR, int WZ, int DZ, int KT>
 hipError_t launch(PromptParams P, int64_t max_k, int device, int n_cus, hipStream_t stream) {
-    constexpr int N = Elem<T>::N, KT = N == 3 || D == 256 ? 32 : 64;
-    constexpr size_t lds = (size_t)2 * N * KT * D * 2 * (N == 1 ? 2 : 1) + 16;
+    constexpr int N = Elem<T>::N, KS = KT * WZ;
+    constexpr size_t lds = (size_t)2 * N * KS * D * 2 * (N == 1 ? 2 : 1) + (DZ > 1 ? 2 * 64 * WR * WZ * DZ * KT / 32 * 16 * 4 : 0) + 16;
     static_assert(lds <= 160 * 1024);
-    P.tiles = (int)(P.total_q * P.group / (32 * W) + P.batch);
-    const int64_t wgs = (int64_t)P.tiles * P.kv_heads, pos_tiles = (max_k + KT - 1) / KT;
+    P.tiles = (int)(P.total_q * P.group / (32 * WR) + P.batch);
+    const int64_t wgs = (int64_t)P.tiles * P.kv_heads, pos_tiles = (max_k + KS - 1) / KS;
     P.splits = (int)std::max<int64_t>(1, std::min(n_cus / wgs, pos_tiles / 4));
     const int64_t rows = P.total_q * P.heads;
     if (P.splits > 1) {
@@ -543,18 +646,35 @@ hipError_t launch(PromptParams P, int64_t max_k, int device, int n_cus, hipStrea
             const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
             if (e != hipSuccess) return e;
         }
-        kernel<<<(unsigned)(wgs * P.splits), 64 * W, lds, stream>>>(P);
+        kernel<<<(unsigned)(wgs * P.splits), 64 * WR * WZ * DZ, lds, stream>>>(P);
         return hipGetLastError();
     };
-    if (P.splits == 1) return run(prompt_attention_kernel<T, D, W, KT, false>);
-    const hipError_t e = run(prompt_attention_kernel<T, D, W, KT, true>);
+    if (P.splits == 1) return run(prompt_attention_kernel<T, D, WR, WZ, DZ, KT, false>);
+    const hipError_t e = run(prompt_attention_kernel<T, D, WR, WZ, DZ, KT, true>);
     if (e != hipSuccess) return e;
-    prompt_join_kernel<T, D><<<(unsigned)((rows + 3) / 4), 256, 0, stream>>>(P, rows);
+    if (P.splits <= 8) prompt_join_kernel<T, D, true><<<(unsigned)((rows + 3) / 4), 256, 0, stream>>>(P, rows);
+    else prompt_join_kernel<T, D, false><<<(unsigned)rows, 256, 0, stream>>>(P, rows);
     return hipGetLastError();
 }
 template <typename T, int D>
 hipError_t launch_of(const PromptParams& P, int64_t max_k, int device, int n_cus, hipStream_t stream) {
-    return launch<T, D, 4>(P, max_k, device, n_cus, stream);
+#ifndef CFG
+#define CFG 0
+#endif
+    if constexpr (sizeof(T) == 4) {
+        if constexpr (D == 256) return launch<T, D, 2, 1, 2, 32>(P, max_k, device, n_cus, stream);
+        else if constexpr (CFG == 1) return launch<T, D, 2, 2, 1, 32>(P, max_k, device, n_cus, stream);
+        else return launch<T, D, 4, 1, 1, 32>(P, max_k, device, n_cus, stream);
+    } else {
+        if constexpr (D == 256) {
+            if constexpr (CFG == 1) return launch<T, D, 2, 1, 2, 32>(P, max_k, device, n_cus, stream);
+            else if constexpr (CFG == 2) return launch<T, D, 2, 1, 2, 64>(P, max_k, device, n_cus, stream);
+            else return launch<T, D, 4, 1, 2, 32>(P, max_k, device, n_cus, stream);
+        }
+        else if constexpr (CFG == 1) return launch<T, D, 2, 2, 1, 32>(P, max_k, device, n_cus, stream);
+        else if constexpr (CFG == 2) return launch<T, D, 4, 1, 1, 32>(P, max_k, device, n_cus, stream);
+        else return launch<T, D, 4, 1, 1, 64>(P, max_k, device, n_cus, stream);
+    }
 }
 
 template <typename T>
