@@ -105,15 +105,14 @@ __device__ __forceinline__ void split8(const float (&v)[8], u32x4 (&to)[3]) {
     }
 }
 
-// acc += a b with N numbers a value: the products whose weight is 2^-16 or more
-template <typename T>
-__device__ __forceinline__ f32x16 mma_of(const u32x4 (&a)[Elem<T>::N], const u32x4 (&b)[Elem<T>::N], f32x16 acc) {
-#pragma unroll
-    for (int i = Elem<T>::N - 1; i >= 0; i--)
-#pragma unroll
-        for (int j = Elem<T>::N - 1 - i; j >= 0; j--) acc = Elem<T>::mma(a[i], b[j], acc);
-    return acc;
-}
+// Of N numbers a value the products whose weight is 2^-16 or more, the small ones first: product i is that of number left(i) of one and right(i) of
+// the other.  Products go round between results, so that none adds to what the one before it wrote.
+template <int N>
+struct Products {
+    static constexpr int kCount = N == 1 ? 1 : 6;
+    static constexpr int left(int i) { return N == 1 ? 0 : (i < 3 ? 2 - i : i < 5 ? 4 - i : 0); }
+    static constexpr int right(int i) { return N == 1 ? 0 : (i < 3 ? i : i < 5 ? i - 3 : 0); }
+};
 
 // ---- a tile of keys or values in LDS -------------------------------------------------------------------------------
 // Rows of D 16-bit numbers in pieces of 16 bytes, piece c of row r at place c ^ turn(r): so that 32 rows' pieces c (keys), and 64
@@ -180,7 +179,8 @@ __global__ __launch_bounds__(64 * WR * WZ * DZ, Elem<T>::N == 1 || D == 64 ? 2 :
     constexpr bool kDirect = N == 1;          // keys and values go straight from memory into LDS
     constexpr int kPlane = KS * D * 2;        // bytes of a tile of 16-bit numbers
     constexpr int kTile = 2 * N * kPlane;     // keys, then values
-    constexpr int kTiles = kTile * (kDirect ? 2 : 1), kScores = DZ > 1 ? 2 * W * PT * 16 * 256 : 0;
+    constexpr bool kDouble = !kDirect && DZ == 1 && WZ == 1; // a second tile is taken apart beside the first one's products
+    constexpr int kTiles = kTile * (kDirect || kDouble ? 2 : 1), kScores = DZ > 1 ? 2 * W * PT * 16 * 256 : 0;
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[]; // tiles (two where direct), partial scores of two tiles, a word
     uint32_t* odd_values = reinterpret_cast<uint32_t*>(smem + kTiles + kScores);
 
@@ -238,22 +238,21 @@ __global__ __launch_bounds__(64 * WR * WZ * DZ, Elem<T>::N == 1 || D == 64 ? 2 :
             }
         }
     };
-    const auto deliver = [&]() { // what was requested into registers, as three planes
+    const auto deliver = [&](uint8_t* to, int w, int i) { // piece i of the keys (w = 0) or values requested into registers, as three planes
         if constexpr (!kDirect) {
+            const int piece = i * (64 * W) + threadIdx.x, r = piece / (D / 8), c = (piece % (D / 8)) ^ turn<D>(r);
+            float v[8];
 #pragma unroll
-            for (int w = 0; w < 2; w++)
+            for (int j = 0; j < 8; j++) v[j] = ahead[w][i][j >> 2][j & 3];
+            u32x4 o[3];
+            split8(v, o);
 #pragma unroll
-                for (int i = 0; i < kPer; i++) {
-                    const int piece = i * (64 * W) + threadIdx.x, r = piece / (D / 8), c = (piece % (D / 8)) ^ turn<D>(r);
-                    float v[8];
-#pragma unroll
-                    for (int j = 0; j < 8; j++) v[j] = ahead[w][i][j >> 2][j & 3];
-                    u32x4 o[3];
-                    split8(v, o);
-#pragma unroll
-                    for (int n = 0; n < 3; n++) *reinterpret_cast<u32x4*>(smem + (w * 3 + n) * kPlane + r * (2 * D) + 16 * c) = o[n];
-                }
+            for (int n = 0; n < 3; n++) *reinterpret_cast<u32x4*>(to + (w * 3 + n) * kPlane + r * (2 * D) + 16 * c) = o[n];
         }
+    };
+    const auto deliver_all = [&](uint8_t* to) {
+#pragma unroll
+        for (int i = 0; i < 2 * kPer; i++) deliver(to, i / kPer, i % kPer);
     };
 
     if (first < end) request(first, 0); // (ahead of the queries: both ways to memory at once)
@@ -302,21 +301,42 @@ __global__ __launch_bounds__(64 * WR * WZ * DZ, Elem<T>::N == 1 || D == 64 ? 2 :
     // Scores, weights and the weighted values of a tile that has landed.  MASKED: some row of the workgroup does not see all of its
     // positions.
     [[maybe_unused]] int turns = 0;
-    const auto weigh = [&](auto masked, const uint8_t* here, int p0) {
-        constexpr bool MASKED = decltype(masked)::value;
+    // `there`: where the tile behind it, which waits in registers, goes meanwhile; `behind`: the one to be requested then (MORE)
+    const auto weigh = [&](auto masked, auto more, const uint8_t* here, int p0, uint8_t* there = nullptr, int behind = 0) {
+        constexpr bool MASKED = decltype(masked)::value, MORE = decltype(more)::value;
         // lane (x, h), register r of sub-tile pt: row x, position p0 + 32 pt + 8 (r / 4) + 4 h + r % 4
         f32x16 p[PT];
 #pragma unroll
         for (int pt = 0; pt < PT; pt++) {
+            f32x16 part[N > 1 ? 2 : 1];
 #pragma unroll
-            for (int r = 0; r < 16; r++) p[pt][r] = 0.0f;
+            for (int i = 0; i < (N > 1 ? 2 : 1); i++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) part[i][r] = 0.0f;
 #pragma unroll
             for (int kk = 0; kk < KK; kk++) {
                 u32x4 a[N];
 #pragma unroll
                 for (int n = 0; n < N; n++) a[n] = *reinterpret_cast<const u32x4*>(here + n * kPlane + pt * 32 * (2 * D) + (k_at ^ (kk << 5)));
-                p[pt] = mma_of<T>(a, q[kk], p[pt]);
+#pragma unroll
+                for (int i = 0; i < Products<N>::kCount; i++)
+                    part[N > 1 ? i & 1 : 0] = E::mma(a[Products<N>::left(i)], q[kk][Products<N>::right(i)], part[N > 1 ? i & 1 : 0]);
+                if constexpr (MORE) { // (vector instructions beside the products)
+                    static_assert(PT == 1 && KK % (2 * kPer) == 0);
+                    constexpr int kEvery = KK / (2 * kPer);
+                    if (kk % kEvery == kEvery - 1) deliver(there, kk / kEvery / kPer, kk / kEvery % kPer);
+                }
             }
+            p[pt] = part[0];
+            if constexpr (N > 1) p[pt] += part[1];
+        }
+        if constexpr (MORE) {
+#pragma unroll
+            for (int i = 0; i < Products<N>::kCount * KK; i++) { // (four behind each product: 244 us without, 235 with it, 2048 tokens of 32 heads on 8)
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+            }
+            if (behind < end) request(behind, 0);
         }
         if constexpr (DZ > 1) { // (two places in turn: a wave may still read the last tile's)
             static_assert(DZ == 2);
@@ -379,45 +399,53 @@ __global__ __launch_bounds__(64 * WR * WZ * DZ, Elem<T>::N == 1 || D == 64 ? 2 :
             for (int i = 0; i < 8; i++) v[i] = p[t >> 1][8 * (t & 1) + i];
             if constexpr (N == 1) w[0] = u32x4{E::pack(v[0], v[1]), E::pack(v[2], v[3]), E::pack(v[4], v[5]), E::pack(v[6], v[7])};
             else split8(v, w);
+            u32x4 a[DT][N];
 #pragma unroll
-            for (int d = 0; d < DT; d++) {
-                u32x4 a[N];
+            for (int d = 0; d < DT; d++)
 #pragma unroll
                 for (int n = 0; n < N; n++) {
                     const uint8_t* const plane = here + (N + n) * kPlane + t * 16 * (2 * D);
                     const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(plane + (v_at0 ^ (d << 6)))));
                     const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(plane + (v_at1 ^ (d << 6)))));
-                    a[n] = u32x4{lo[0], lo[1], hi[0], hi[1]};
+                    a[d][n] = u32x4{lo[0], lo[1], hi[0], hi[1]};
                 }
-                o[d] = mma_of<T>(a, w, o[d]);
-            }
+#pragma unroll
+            for (int i = 0; i < Products<N>::kCount; i++)
+#pragma unroll
+                for (int d = 0; d < DT; d++) o[d] = E::mma(a[d][Products<N>::left(i)], w[Products<N>::right(i)], o[d]);
         }
     };
 
     const auto arrive = [&](int tile) { // the tile is in LDS, the one behind it on its way
+        uint8_t* const here = smem + (kDirect || kDouble ? (tile - first & 1) * kTile : 0);
         if constexpr (kDirect) {
-            const int stage = (tile - first) & 1;
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            if (tile + 1 < end) request(tile + 1, stage ^ 1);
-            return smem + stage * kTile;
+            if (tile + 1 < end) request(tile + 1, tile + 1 - first & 1);
+        } else if constexpr (kDouble) {
+            if (tile == first) {
+                deliver_all(here);
+                if (tile + 1 < end) request(tile + 1, 0);
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         } else {
             __syncthreads(); // the tile before is read
-            deliver();
+            deliver_all(here);
             if (tile + 1 < end) request(tile + 1, 0);
             __syncthreads();
-            return smem;
         }
+        return here;
     };
     // A value that is no number must not reach the rows that do not see it, and a weight of zero would not keep it out.  Results that hold one
     // are worked out once more, with care: the rows that see such a value get it by itself, and the tile goes on with a zero in its
     // place.  (A look at the values of every tile that some row does not see all of took 1200 of the 11600 cycles of 37 bf16 tokens.)
     for (bool care = false;;) {
         int tile = first;
-        for (const int whole = min(end, fewest / KS); tile < whole; tile++) weigh(std::false_type{}, arrive(tile), 0); // every row sees all of these
+        if constexpr (!kDouble) // every row sees all of these
+            for (const int whole = min(end, fewest / KS); tile < whole; tile++) weigh(std::false_type{}, std::false_type{}, arrive(tile), 0);
         for (; tile < end; tile++) {
             uint8_t* const here = arrive(tile);
             const int p0 = tile * KS;
-            if (care) {
+            if (care && p0 + KS > fewest) {
                 constexpr uint32_t kLow = E::kExponent & 0xffffu, kHigh = E::kExponent & 0xffff0000u;
 #pragma unroll 1
                 for (int j = wz * KT; j < min((wz + 1) * KT, s.len_k - p0); j++) {
@@ -445,7 +473,8 @@ __global__ __launch_bounds__(64 * WR * WZ * DZ, Elem<T>::N == 1 || D == 64 ? 2 :
                 }
                 __syncthreads();
             }
-            weigh(std::true_type{}, here, p0 + wz * KT);
+            if (kDouble && tile + 1 < end) weigh(std::true_type{}, std::integral_constant<bool, kDouble>{}, here, p0, smem + (tile + 1 - first & 1) * kTile, tile + 2);
+            else weigh(std::true_type{}, std::false_type{}, here, p0 + wz * KT);
         }
         if (care || end * KS <= fewest) break;
         float zero = 0.0f; // NaN where a result is no number
@@ -552,7 +581,7 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(PromptParams P, int64_
     const float2* const stats = P.stats + row * P.splits;
     const int at = FEW ? lane : threadIdx.x % (D / 4), mine = FEW ? 0 : threadIdx.x / (D / 4), step = FEW ? 1 : kPer;
     const float* const sums = P.sums + row * P.splits * D + at * E;
-    if (P.cu_q) { // rows behind the last sequence, or between two, were not written
+    if (P.cu_q) { // rows behind the last sequence, or between two, have no sums
         bool inside = false;
         for (int b0 = 0; b0 < P.batch && !inside; b0 += 64) {
             const int b = min(b0 + lane, P.batch - 1);
@@ -561,28 +590,34 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(PromptParams P, int64_
         if (!inside) return; // (the same in the whole workgroup)
     }
     // (a reference of -infinity: no score is above it, the sums are zero or no number; a sum below zero: no position that the row sees)
-    float ref = -INFINITY;
-    for (int i = lane; i < P.splits; i += 64) {
-        const float2 st = stats[i];
-        ref = fmaxf(ref, st.y < 0.0f ? -INFINITY : st.x);
-    }
-    ref = qmm_max_lane_rows(ref);
-    ref = fmaxf(ref, dpp_f<0x128>(ref)); // row_ror:8, then 4, 2, 1
-    ref = fmaxf(ref, dpp_f<0x124>(ref));
-    ref = fmaxf(ref, dpp_f<0x4E>(ref));
-    ref = fmaxf(ref, dpp_f<0xB1>(ref));
-    float sum = 0.0f;
-    bool any = false;
-    vec a = 0.0f;
-    for (int i0 = mine; i0 < P.splits; i0 += A * step) {
-        vec v[A];
-        float2 st[A];
+    vec v[A], a = 0.0f;
+    float2 st[A];
+    const auto take = [&](int i0) {
 #pragma unroll
         for (int j = 0; j < A; j++) {
             const int i = min(i0 + j * step, P.splits - 1);
             st[j] = stats[i];
             v[j] = *reinterpret_cast<const vec*>(sums + (int64_t)i * D);
         }
+    };
+    take(mine);
+    float ref = -INFINITY, sum = 0.0f;
+    bool any = false;
+    if constexpr (FEW) {
+#pragma unroll
+        for (int j = 0; j < A; j++) ref = fmaxf(ref, st[j].y < 0.0f ? -INFINITY : st[j].x);
+    } else {
+        for (int i = lane; i < P.splits; i += 64) {
+            const float2 one = stats[i];
+            ref = fmaxf(ref, one.y < 0.0f ? -INFINITY : one.x);
+        }
+        ref = qmm_max_lane_rows(ref);
+        ref = fmaxf(ref, dpp_f<0x128>(ref)); // row_ror:8, then 4, 2, 1
+        ref = fmaxf(ref, dpp_f<0x124>(ref));
+        ref = fmaxf(ref, dpp_f<0x4E>(ref));
+        ref = fmaxf(ref, dpp_f<0xB1>(ref));
+    }
+    for (int i0 = mine; i0 < P.splits;) {
 #pragma unroll
         for (int j = 0; j < A; j++) {
             const bool there = i0 + j * step < P.splits && !(st[j].y < 0.0f);
@@ -591,6 +626,8 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(PromptParams P, int64_
             sum += there ? st[j].y * by : 0.0f;
             a += (there ? v[j] : vec(0.0f)) * by;
         }
+        i0 += A * step;
+        if (i0 < P.splits) take(i0);
     }
     T* const to = static_cast<T*>(P.out) + token * P.out_stride + (row % P.heads) * D + at * E;
     if constexpr (FEW) {
@@ -625,14 +662,27 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(PromptParams P, int64_
         }                                                                              \
     } while (0)
 
+// Tiles of `rows` rows, as far as the host can tell (of several sequences the last tiles may be partly filled).
+int64_t row_tiles(const PromptParams& P, int rows) { return P.cu_q ? P.total_q * P.group / rows + P.batch : (P.total_q * P.group + rows - 1) / rows; }
+
+// Parts that the keys are split into where workgroups are few: two tiles of `step` positions a part at the least, as a second launch has to join
+// them: f16 and bf16 from eight tiles on (16 tokens of 16 heads on 8 behind 240: in one part 8.6 us, in two 10.1; behind 500: in two
+// parts 12.3, in four 11.0; behind 1000 15, 11.9, in eight 10.5), f32, whose tiles take three times as long, from four (behind 240: in one
+// part 30.6 us, in two 21.0, in four 14.8).
+template <typename T>
+int splits_of(int64_t wgs, int64_t max_k, int step, int n_cus) {
+    const int64_t tiles = (max_k + step - 1) / step;
+    return tiles < (sizeof(T) == 4 ? 4 : 8) ? 1 : (int)std::max<int64_t>(1, std::min(n_cus / wgs, tiles / 2));
+}
+
 template <typename T, int D, int WR, int WZ, int DZ, int KT>
 hipError_t launch(PromptParams P, int64_t max_k, int device, int n_cus, hipStream_t stream) {
     constexpr int N = Elem<T>::N, KS = KT * WZ;
-    constexpr size_t lds = (size_t)2 * N * KS * D * 2 * (N == 1 ? 2 : 1) + (DZ > 1 ? 2 * 64 * WR * WZ * DZ * KT / 32 * 16 * 4 : 0) + 16;
+    constexpr size_t lds = (size_t)2 * N * KS * D * 2 * (N == 1 || (DZ == 1 && WZ == 1) ? 2 : 1) + (DZ > 1 ? 2 * 64 * WR * WZ * DZ * KT / 32 * 16 * 4 : 0) + 16;
     static_assert(lds <= 160 * 1024);
-    P.tiles = (int)(P.total_q * P.group / (32 * WR) + P.batch);
-    const int64_t wgs = (int64_t)P.tiles * P.kv_heads, pos_tiles = (max_k + KS - 1) / KS;
-    P.splits = (int)std::max<int64_t>(1, std::min(n_cus / wgs, pos_tiles / 4));
+    const int64_t wgs = row_tiles(P, 32 * WR) * P.kv_heads;
+    P.tiles = (int)(wgs / P.kv_heads);
+    P.splits = splits_of<T>(wgs, max_k, KS, n_cus);
     const int64_t rows = P.total_q * P.heads;
     if (P.splits > 1) {
         void* scratch = nullptr;
@@ -656,24 +706,30 @@ hipError_t launch(PromptParams P, int64_t max_k, int device, int n_cus, hipStrea
     else prompt_join_kernel<T, D, false><<<(unsigned)rows, 256, 0, stream>>>(P, rows);
     return hipGetLastError();
 }
+// Which workgroups.  f16 and bf16: four waves of 32 rows on 64 keys at a time (two on halves of the head each for D = 256, 32 keys), or where
+// those would not fill the compute units, two waves of rows on 64 keys and two on the 64 behind them (D = 256: half the rows): causal
+// prompts, whose workgroups are of unequal length, change over later.  16 bf16 heads on 8, us of the larger and the smaller workgroups: D = 128
+// causal 700 tokens 26.6, 15.1; 2600 54.9, 43.9; 3500 76.9, 73.1; not causal 2000 45.8, 46.4; 2600 76.7, 85.9; D = 64 causal 2600 39.7, 28.1; not causal
+// 2600 53.1, 46.7; 3500 72.5, 76.8; D = 256 causal 2000 92.5, 78.1; 2600 119, 137; not causal 700 42, 28.5; 1500 71, 104.  A tile of 65 to
+// 128 rows on very many keys reads them twice with the smaller ones (17 tokens of 32 heads behind 30011 31.5, 36.2).  Up to 64 keys the
+// second pair would have none (37 tokens 5.9, 6.6).
+// f32: the larger ones; the smaller where sequences have few rows and many tiles each (4 tokens behind 1087 of 10 sequences 46.7, 36.5) and for
+// heads of 64 (200 tokens of 6 sequences 18.9, 12.6; 9 of 13, one tile, 5.6, 6.6).
 template <typename T, int D>
 hipError_t launch_of(const PromptParams& P, int64_t max_k, int device, int n_cus, hipStream_t stream) {
-#ifndef CFG
-#define CFG 0
-#endif
-    if constexpr (sizeof(T) == 4) {
-        if constexpr (D == 256) return launch<T, D, 2, 1, 2, 32>(P, max_k, device, n_cus, stream);
-        else if constexpr (CFG == 1) return launch<T, D, 2, 2, 1, 32>(P, max_k, device, n_cus, stream);
-        else return launch<T, D, 4, 1, 1, 32>(P, max_k, device, n_cus, stream);
+    const int64_t wgs = row_tiles(P, 128) * P.kv_heads, rows = P.total_q * P.group / P.batch; // of a sequence, on average
+    constexpr int DZ = D == 256 ? 2 : 1;
+    if constexpr (sizeof(T) == 4 && D == 256) {
+        return launch<T, D, 2, 1, DZ, 32>(P, max_k, device, n_cus, stream);
+    } else if constexpr (sizeof(T) == 4) {
+        const int64_t tiles = (max_k + 31) / 32;
+        const bool small = D == 64 ? tiles > 2 : rows <= 64 && tiles >= 4 * splits_of<T>(wgs, max_k, 32, n_cus);
+        return small ? launch<T, D, 2, 2, DZ, 32>(P, max_k, device, n_cus, stream) : launch<T, D, 4, 1, DZ, 32>(P, max_k, device, n_cus, stream);
     } else {
-        if constexpr (D == 256) {
-            if constexpr (CFG == 1) return launch<T, D, 2, 1, 2, 32>(P, max_k, device, n_cus, stream);
-            else if constexpr (CFG == 2) return launch<T, D, 2, 1, 2, 64>(P, max_k, device, n_cus, stream);
-            else return launch<T, D, 4, 1, 2, 32>(P, max_k, device, n_cus, stream);
-        }
-        else if constexpr (CFG == 1) return launch<T, D, 2, 2, 1, 32>(P, max_k, device, n_cus, stream);
-        else if constexpr (CFG == 2) return launch<T, D, 4, 1, 1, 32>(P, max_k, device, n_cus, stream);
-        else return launch<T, D, 4, 1, 1, 64>(P, max_k, device, n_cus, stream);
+        const int quarters = P.causal ? (D == 64 ? 8 : D == 128 ? 7 : 4) : (D == 64 ? 6 : D == 128 ? 4 : 2);
+        const bool small = 4 * wgs < quarters * n_cus && (D == 256 || max_k > 64) && (rows <= 64 || rows > 128 || max_k < 8192);
+        if constexpr (D == 256) return small ? launch<T, D, 2, 1, DZ, 32>(P, max_k, device, n_cus, stream) : launch<T, D, 4, 1, DZ, 32>(P, max_k, device, n_cus, stream);
+        else return small ? launch<T, D, 2, 2, DZ, 32>(P, max_k, device, n_cus, stream) : launch<T, D, 4, 1, DZ, 64>(P, max_k, device, n_cus, stream);
     }
 }
 
