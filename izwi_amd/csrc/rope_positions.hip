@@ -76,6 +76,124 @@ __global__ __launch_bounds__(256) void rope_any_kernel(RopeParams P) {
     }
 }
 
+// The same in pieces of 16 bytes: a lane has two pieces of a head, those whose elements turn against each other (halves) or two neighbours
+// (interleaved, and what does not turn), LP lanes a head, 64 / LP heads at once; a wave has `passes` such sets of one token's heads, requests
+// kAtOnce of them ahead of working out the angles, and every angle once.
+constexpr int kAtOnce = 4, kPiecePairs = 256;
+
+template <typename T, int V>
+struct Piece {
+    typedef T vec __attribute__((ext_vector_type(V)));
+    vec v;
+    __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const vec*>(p); }
+    __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<vec*>(p) = v; }
+};
+
+// sum over LP neighbouring lanes, in all of them
+__device__ __forceinline__ float sum_lanes(float v, int lp) {
+    if (lp > 1) v += dpp_f<0xB1>(v);  // quad_perm [1,0,3,2]
+    if (lp > 2) v += dpp_f<0x4E>(v);  // quad_perm [2,3,0,1]
+    if (lp > 4) v += dpp_f<0x141>(v); // row_half_mirror
+    if (lp > 8) v += dpp_f<0x128>(v); // row_ror:8
+    if (lp > 16) v = qmm_add_lane16(v);
+    if (lp > 32) v = qmm_add_lane32(v);
+    return v;
+}
+
+template <typename T, bool INTER, bool NORM>
+__global__ __launch_bounds__(256) void rope_pieces_kernel(RopeParams P, int lp, int per_head, int passes, int shares) {
+    constexpr int V = 16 / (int)sizeof(T);
+    __shared__ float2 turns_of[4][kPiecePairs];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t unit = (int64_t)blockIdx.x * 4 + wave, token = unit / shares;
+    if (token >= P.tokens) return; // whole waves
+    const int share = (int)(unit - token * shares), first = share * passes;
+    const int sub = lane & (lp - 1), group = lane / lp, at_once = 64 / lp, pairs = P.rotary / 2;
+    // the lane's pieces of a head
+    const int rotating = pairs / V; // lanes whose pieces turn
+    const bool turns = sub < rotating;
+    const int a = turns ? (INTER ? 2 * sub * V : sub * V) : P.rotary + 2 * (sub - rotating) * V;
+    const int b = turns && !INTER ? a + pairs : a + V;
+    const int n = min(passes, (P.heads + at_once - 1) / at_once - first);
+
+    struct Rows {
+        const T* from;
+        T* to;
+        bool is_q, there;
+    };
+    const auto rows = [&](int pass) {
+        const int head = (first + pass) * at_once + group;
+        Rows r;
+        r.there = sub < per_head && head < P.heads && pass < n;
+        r.is_q = head < P.q_heads;
+        const int64_t at = (int64_t)(r.there ? (r.is_q ? head : head - P.q_heads) : 0) * P.d;
+        r.from = static_cast<const T*>(r.is_q ? P.q : P.k) + token * (r.is_q ? P.q_stride : P.k_stride) + at;
+        r.to = static_cast<T*>(r.is_q ? P.q_out : P.k_out) + token * (r.is_q ? P.q_out_stride : P.k_out_stride) + at;
+        return r;
+    };
+    Piece<T, V> x[kAtOnce], y[kAtOnce], wx[kAtOnce], wy[kAtOnce];
+    const auto request = [&](int pass0) {
+#pragma unroll
+        for (int i = 0; i < kAtOnce; i++) {
+            const Rows r = rows(pass0 + i);
+            if (!r.there) continue;
+            x[i].load(r.from + a), y[i].load(r.from + b);
+            if constexpr (NORM) {
+                const T* const w = static_cast<const T*>(P.weight) + (r.is_q ? 0 : P.d);
+                wx[i].load(w + a), wy[i].load(w + b);
+            }
+        }
+    };
+    const int position = P.positions[token];
+    request(0);
+    for (int i = lane; i < pairs; i += 64) {
+        float c, s;
+        turn_of(P, position, i, c, s);
+        turns_of[wave][i] = float2{c, s};
+    }
+    asm volatile("" ::: "memory"); // (a wave's LDS instructions run in their order)
+    __builtin_amdgcn_wave_barrier();
+    float c[V], s[V];
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        const float2 t = turns_of[wave][turns ? sub * V + i : 0];
+        c[i] = t.x, s[i] = t.y;
+    }
+    for (int pass0 = 0; pass0 < n; pass0 += kAtOnce) {
+        if (pass0) request(pass0);
+#pragma unroll
+        for (int i = 0; i < kAtOnce; i++) {
+            const Rows r = rows(pass0 + i);
+            float u[2 * V]; // the pieces, one behind the other
+            float sum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < V; j++) {
+                u[j] = r.there ? (float)x[i].v[j] : 0.0f, u[V + j] = r.there ? (float)y[i].v[j] : 0.0f;
+                if constexpr (NORM) sum += u[j] * u[j] + u[V + j] * u[V + j];
+            }
+            if constexpr (NORM) {
+                const float by = 1.0f / sqrtf(sum_lanes(sum, lp) / (float)P.d + P.eps);
+                if (!r.there) continue;
+#pragma unroll
+                for (int j = 0; j < V; j++) u[j] = u[j] * by * (float)wx[i].v[j], u[V + j] = u[V + j] * by * (float)wy[i].v[j];
+            }
+            if (!r.there) continue;
+            if (turns) {
+#pragma unroll
+                for (int j = 0; j < V; j++) {
+                    const int p = INTER ? 2 * j : j, q = INTER ? 2 * j + 1 : V + j;
+                    const float e = u[p] * c[j] - u[q] * s[j], f = u[p] * s[j] + u[q] * c[j];
+                    u[p] = e, u[q] = f;
+                }
+            }
+            Piece<T, V> xo, yo;
+#pragma unroll
+            for (int j = 0; j < V; j++) xo.v[j] = (T)u[j], yo.v[j] = (T)u[V + j];
+            xo.store(r.to + a), yo.store(r.to + b);
+        }
+    }
+}
+
 #define ROPE_TRY(expr)                                                                 \
     do {                                                                               \
         hipError_t e_ = (expr);                                                        \
@@ -126,8 +244,23 @@ int rope_positions_impl(const T* q, int64_t q_stride, const T* k, int64_t k_stri
     RopeParams P{q, k, q_out, k_out, q_stride, k_stride, q_out_stride, k_out_stride, positions, frequencies, weight, factor, eps, tokens, (int)q_heads,
                  (int)(q_heads + k_heads), (int)d, (int)rotary};
     hipStream_t stream = (hipStream_t)stream_;
-    if (interleaved) rope_any_kernel<T, true><<<(unsigned)tokens, 256, 0, stream>>>(P);
-    else rope_any_kernel<T, false><<<(unsigned)tokens, 256, 0, stream>>>(P);
+    constexpr int V = 16 / (int)sizeof(T);
+    const auto aligned = [](const void* p, int64_t a, int64_t b) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && a % V == 0 && b % V == 0; };
+    const int per_head = (int)(d / (2 * V));
+    if (d % (2 * V) == 0 && rotary % (2 * V) == 0 && per_head <= 64 && rotary <= 2 * kPiecePairs && (!q_heads || (aligned(q, q_stride, 0) && aligned(q_out, q_out_stride, 0))) &&
+        (!k_heads || (aligned(k, k_stride, 0) && aligned(k_out, k_out_stride, 0))) && aligned(weight, 0, 0)) {
+        int lp = 1;
+        while (lp < per_head) lp *= 2;
+        // a token's heads go to as many waves as make 16 for every compute unit
+        const int sets = (P.heads + 64 / lp - 1) / (64 / lp);
+        const int passes = (int)std::max<int64_t>(1, std::min<int64_t>(sets, tokens * sets / (16 * n_cus)));
+        const int shares = (sets + passes - 1) / passes;
+        const auto run = [&](auto kernel) { kernel<<<(unsigned)((tokens * shares + 3) / 4), 256, 0, stream>>>(P, lp, per_head, passes, shares); };
+        if (weight) interleaved ? run(rope_pieces_kernel<T, true, true>) : run(rope_pieces_kernel<T, false, true>);
+        else interleaved ? run(rope_pieces_kernel<T, true, false>) : run(rope_pieces_kernel<T, false, false>);
+    } else {
+        interleaved ? rope_any_kernel<T, true><<<(unsigned)tokens, 256, 0, stream>>>(P) : rope_any_kernel<T, false><<<(unsigned)tokens, 256, 0, stream>>>(P);
+    }
     ROPE_TRY(hipGetLastError());
     return IZWI_QMM_OK;
 }
