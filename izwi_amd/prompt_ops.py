@@ -23,13 +23,16 @@ from .qmatmul import _current_device, _raw_stream
 
 _NAMES = {torch.float32: "f32", torch.float16: "f16", torch.bfloat16: "bf16"}
 _i32 = torch.int32
-_fns = {}
+# (What a call checks and looks up is paid for once per layer: device numbers are compared instead of devices, and the library's functions are
+# looked up once.)
+_ropes, _attentions = {}, {}
 
 
-def _fn(name: str, dtype):
-    fn = _fns.get((name, dtype))
-    if fn is None:
-        fn = _fns[name, dtype] = getattr(lib(), f"{name}_{_NAMES[dtype]}")
+def _fn(fns: dict, name: str, dtype):
+    """The library's function for the type; None where there is none."""
+    fn = fns.get(dtype)
+    if fn is None and dtype in _NAMES:
+        fn = fns[dtype] = getattr(lib(), f"{name}_{_NAMES[dtype]}")
     return fn
 
 
@@ -40,6 +43,8 @@ def _refuse(what: str):
 def _stride(t, what: str) -> int:
     """Elements from one token to the next of [tokens, heads, d]; the heads of a token are contiguous."""
     tokens, heads, d = t.shape
+    if t.is_contiguous():
+        return heads * d
     s0, s1, s2 = t.stride()
     if (s2 != 1 and d > 1) or (s1 != d and heads > 1):
         _refuse(f"{what}: the heads of a token must be contiguous")
@@ -106,33 +111,47 @@ def rope_positions(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Ten
                    eps: float = 1e-6, out: tuple | None = None):
     """q [tokens, heads, head_dim] and k [tokens, kv_heads, head_dim] (None: q alone), rotated to ``positions`` (int32 [tokens]) -> (q, k).  With
     ``qk_weight`` [2 head_dim] (q's, then k's) every head is normed first.  ``out``: two tensors to write, which may be q and k themselves."""
-    dtype, index = q.dtype, q.get_device()
-    if dtype not in _NAMES or q.dim() != 3 or index < 0 or q.shape[2] != rotary.head_dim or index != rotary._index:
-        _refuse(f"rope_positions: q [tokens, heads, {rotary.head_dim}] of f32, f16 or bf16 on GPU {rotary._index} expected")
-    tokens, heads, d = q.shape
-    if k is not None and (k.dtype is not dtype or k.dim() != 3 or k.shape[0] != tokens or k.shape[2] != d or k.get_device() != index):
-        _refuse(f"rope_positions: k [{tokens}, kv_heads, {d}] of q's type and device expected")
-    if positions.dtype is not _i32 or positions.shape != (tokens,) or not positions.is_contiguous() or positions.get_device() != index:
+    dtype, shape, index = q.dtype, q.shape, rotary._index
+    fn = _ropes.get(dtype) or _fn(_ropes, "izwi_rope_positions", dtype)
+    if fn is None or len(shape) != 3 or shape[2] != rotary.head_dim or q.get_device() != index:
+        _refuse(f"rope_positions: q [tokens, heads, {rotary.head_dim}] of f32, f16 or bf16 on GPU {index} expected")
+    tokens, heads, d = shape
+    kv_heads = 0
+    if k is not None:
+        k_shape = k.shape
+        if k.dtype is not dtype or len(k_shape) != 3 or k_shape[0] != tokens or k_shape[2] != d or k.get_device() != index:
+            _refuse(f"rope_positions: k [{tokens}, kv_heads, {d}] of q's type and device expected")
+        kv_heads = k_shape[1]
+    if positions.dtype is not _i32 or positions.shape != (tokens,) or positions.get_device() != index or not positions.is_contiguous():
         _refuse(f"rope_positions: a contiguous int32 tensor of {tokens} positions on GPU {index} expected")
-    if qk_weight is not None and (qk_weight.dtype is not dtype or qk_weight.shape != (2 * d,) or not qk_weight.is_contiguous() or qk_weight.get_device() != index):
-        _refuse(f"rope_positions: a contiguous qk_weight of {2 * d} of q's type and device expected")
+    weight = 0
+    if qk_weight is not None:
+        if qk_weight.dtype is not dtype or qk_weight.shape != (2 * d,) or qk_weight.get_device() != index or not qk_weight.is_contiguous():
+            _refuse(f"rope_positions: a contiguous qk_weight of {2 * d} of q's type and device expected")
+        weight = qk_weight.data_ptr()
     if index != _current_device():
         with torch.cuda.device(index):
             return rope_positions(q, k, positions, rotary, qk_weight, eps, out)
+    q_step = heads * d if q.is_contiguous() else _stride(q, "rope_positions: q")
+    k_ptr = k_step = k_to = k_to_step = 0
+    if k is not None:
+        k_ptr, k_step = k.data_ptr(), kv_heads * d if k.is_contiguous() else _stride(k, "rope_positions: k")
     if out is None:
-        q_out = torch.empty((tokens, heads, d), dtype=dtype, device=q.device)
-        k_out = None if k is None else torch.empty(k.shape, dtype=dtype, device=q.device)
+        q_out, q_to_step, k_out = torch.empty_like(q), heads * d, None  # (contiguous, whether q is a part of wider rows or not)
+        if k is not None:
+            k_out, k_to_step = torch.empty_like(k), kv_heads * d
     else:
         q_out, k_out = out
         for x, y in ((q, q_out), (k, k_out)):
             if (x is None) != (y is None) or (x is not None and (y.dtype is not dtype or y.shape != x.shape or y.get_device() != index)):
                 _refuse("rope_positions: out has to be as q and k are")
-    kv_heads = 0 if k is None else k.shape[1]
-    rc = _fn("izwi_rope_positions", dtype)(
-        q.data_ptr(), _stride(q, "rope_positions: q"), 0 if k is None else k.data_ptr(), 0 if k is None else _stride(k, "rope_positions: k"),
-        positions.data_ptr(), rotary._ptr, rotary.attention_factor, tokens, heads, kv_heads, d, rotary.rotary_dim, rotary.interleaved,
-        0 if qk_weight is None else qk_weight.data_ptr(), eps, q_out.data_ptr(), _stride(q_out, "rope_positions: out"),
-        0 if k is None else k_out.data_ptr(), 0 if k is None else _stride(k_out, "rope_positions: out"), _raw_stream(index))
+        q_to_step = _stride(q_out, "rope_positions: out")
+        if k is not None:
+            k_to_step = _stride(k_out, "rope_positions: out")
+    if k is not None:
+        k_to = k_out.data_ptr()
+    rc = fn(q.data_ptr(), q_step, k_ptr, k_step, positions.data_ptr(), rotary._ptr, rotary.attention_factor, tokens, heads, kv_heads, d, rotary.rotary_dim,
+            rotary.interleaved, weight, eps, q_out.data_ptr(), q_to_step, k_to, k_to_step, _raw_stream(index))
     if rc:
         check(rc)
     return q_out, k_out
@@ -145,40 +164,48 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: 
     ``starts_k`` (None: as its tokens).  ``causal``: the last query sees the last key, the one before it one key less, and so on, so that a
     prompt with more keys than tokens is a chunk behind a past.  A query without any key gives zeros; rows that belong to no prompt are not
     written.  ``max_len_k``: the longest prompt's keys where the caller knows them; only the division of the work goes by it."""
-    dtype, index = q.dtype, q.get_device()
-    if dtype not in _NAMES or q.dim() != 3 or index < 0:
+    dtype, shape, k_shape, index = q.dtype, q.shape, k.shape, q.get_device()
+    fn = _attentions.get(dtype) or _fn(_attentions, "izwi_qmm_prompt_attention", dtype)
+    if fn is None or len(shape) != 3 or index < 0:
         _refuse("prompt_attention: q [tokens, heads, head_dim] of f32, f16 or bf16 on a GPU expected")
-    tokens, heads, d = q.shape
-    if (k.dim() != 3 or k.shape != v.shape or k.shape[2] != d or k.dtype is not dtype or v.dtype is not dtype or k.get_device() != index
-            or v.get_device() != index or not k.shape[1] or heads % k.shape[1]):
+    tokens, heads, d = shape
+    if (len(k_shape) != 3 or v.shape != k_shape or k_shape[2] != d or k.dtype is not dtype or v.dtype is not dtype or k.get_device() != index
+            or v.get_device() != index or not k_shape[1] or heads % k_shape[1]):
         _refuse(f"prompt_attention: k and v [keys, kv_heads, {d}] of q's type and device expected, {heads} heads a multiple of theirs")
-    keys, kv_heads, _ = k.shape
-    if starts_k is None:
-        starts_k = starts
-        if starts is not None and keys != tokens:
-            _refuse(f"prompt_attention: {keys} keys for {tokens} tokens need starts_k")
-    prompts = 1
-    if starts is None:
+    keys, kv_heads, _ = k_shape
+    prompts, cu_q, cu_k = 1, 0, 0
+    if starts is not None:
+        prompts = len(starts) - 1 if starts.dim() == 1 else -1
+        if starts.dtype is not _i32 or prompts < 0 or starts.get_device() != index or not starts.is_contiguous():
+            _refuse(f"prompt_attention: starts as a contiguous int32 tensor of prompts + 1 on GPU {index} expected")
+        cu_q = cu_k = starts.data_ptr()
         if starts_k is not None:
-            _refuse("prompt_attention: starts_k comes with starts")
-    else:
-        prompts = starts.shape[0] - 1 if starts.dim() == 1 else -1
-        for t in (starts, starts_k):
-            if t.dtype is not _i32 or prompts < 0 or t.shape != (prompts + 1,) or not t.is_contiguous() or t.get_device() != index:
-                _refuse(f"prompt_attention: starts as contiguous int32 tensors of prompts + 1 on GPU {index} expected")
-    if max_len_k is not None and max_len_k < 0:
+            if starts_k.dtype is not _i32 or starts_k.shape != (prompts + 1,) or starts_k.get_device() != index or not starts_k.is_contiguous():
+                _refuse(f"prompt_attention: starts_k as a contiguous int32 tensor of {prompts + 1} on GPU {index} expected")
+            cu_k = starts_k.data_ptr()
+        elif keys != tokens:
+            _refuse(f"prompt_attention: {keys} keys for {tokens} tokens need starts_k")
+    elif starts_k is not None:
+        _refuse("prompt_attention: starts_k comes with starts")
+    if max_len_k is None:
+        max_len_k = keys
+    elif max_len_k < 0:
         _refuse(f"prompt_attention: max_len_k {max_len_k}")
     if index != _current_device():
         with torch.cuda.device(index):
             return prompt_attention(q, k, v, starts, starts_k, causal, scale, max_len_k, out)
+    row = kv_heads * d
+    q_step = heads * d if q.is_contiguous() else _stride(q, "prompt_attention: q")
+    k_step = row if k.is_contiguous() else _stride(k, "prompt_attention: k")
+    v_step = row if v.is_contiguous() else _stride(v, "prompt_attention: v")
     if out is None:
-        out = torch.empty((tokens, heads, d), dtype=dtype, device=q.device)
-    elif out.dtype is not dtype or out.shape != q.shape or out.get_device() != index:
-        _refuse("prompt_attention: out has to be as q is")
-    rc = _fn("izwi_qmm_prompt_attention", dtype)(
-        q.data_ptr(), _stride(q, "prompt_attention: q"), k.data_ptr(), _stride(k, "prompt_attention: k"), v.data_ptr(), _stride(v, "prompt_attention: v"),
-        0 if starts is None else starts.data_ptr(), 0 if starts is None else starts_k.data_ptr(), prompts, tokens, keys, keys if max_len_k is None else max_len_k,
-        heads, kv_heads, d, bool(causal), d ** -0.5 if scale is None else scale, out.data_ptr(), _stride(out, "prompt_attention: out"), _raw_stream(index))
+        out, out_step = torch.empty_like(q), heads * d  # (contiguous, whether q is a part of wider rows or not)
+    else:
+        if out.dtype is not dtype or out.shape != shape or out.get_device() != index:
+            _refuse("prompt_attention: out has to be as q is")
+        out_step = _stride(out, "prompt_attention: out")
+    rc = fn(q.data_ptr(), q_step, k.data_ptr(), k_step, v.data_ptr(), v_step, cu_q, cu_k, prompts, tokens, keys, max_len_k, heads, kv_heads, d, bool(causal),
+            d ** -0.5 if scale is None else scale, out.data_ptr(), out_step, _raw_stream(index))
     if rc:
         check(rc)
     return out

@@ -607,7 +607,8 @@ def moe_route(logits: torch.Tensor, top_k: int):
 
 
 _SCORINGS = {"softmax": 0, "sigmoid": 1}  # IZWI_MOE_SOFTMAX, IZWI_MOE_SIGMOID
-_ROUTE_FNS = {torch.float32: "izwi_moe_route_scored_f32", torch.float16: "izwi_moe_route_scored_f16", torch.bfloat16: "izwi_moe_route_scored_bf16"}
+_ROUTE_NAMES = {torch.float32: "izwi_moe_route_scored_f32", torch.float16: "izwi_moe_route_scored_f16", torch.bfloat16: "izwi_moe_route_scored_bf16"}
+_route_fns = {}
 
 
 def moe_route_scored(logits: torch.Tensor, top_k: int, scoring: str = "softmax", bias: torch.Tensor | None = None, groups: int = 1,
@@ -617,25 +618,33 @@ def moe_route_scored(logits: torch.Tensor, top_k: int, scoring: str = "softmax",
     are chosen by score + ``bias`` ([experts] f32), ties to the lower index, from the ``top_groups`` best of ``groups`` equal groups (a
     group is worth the sum of its ``group_best`` best, by default 2 with a bias and 1 without); weights are the chosen scores, divided
     by their sum if ``renormalize``, times ``scale``.  What follows it is ``moe_sort`` and ``MoeExperts.forward``."""
-    name = _ROUTE_FNS.get(logits.dtype)
-    if name is None or logits.dim() != 2 or not logits.is_cuda or scoring not in _SCORINGS:
-        raise capi.QmmError(-1, "moe_route_scored: logits [tokens, experts] of f32, f16 or bf16 on a GPU, scoring softmax or sigmoid expected")
-    t, n = logits.shape
+    dtype, shape, score = logits.dtype, logits.shape, _SCORINGS.get(scoring)
+    fn = _route_fns.get(dtype)
+    if fn is None and dtype in _ROUTE_NAMES:
+        fn = _route_fns[dtype] = getattr(lib(), _ROUTE_NAMES[dtype])
     index = logits.get_device()
-    if logits.stride(1) != 1 and n > 1:
-        raise capi.QmmError(-1, "moe_route_scored: the logits of a token must be contiguous")
-    if bias is not None and (bias.dtype is not torch.float32 or bias.shape != (n,) or not bias.is_contiguous() or bias.get_device() != index):
-        raise capi.QmmError(-1, f"moe_route_scored: a contiguous f32 bias of {n} on GPU {index} expected")
+    if fn is None or len(shape) != 2 or index < 0 or score is None:
+        raise capi.QmmError(-1, "moe_route_scored: logits [tokens, experts] of f32, f16 or bf16 on a GPU, scoring softmax or sigmoid expected")
+    t, n = shape
+    step, b, best = n, 0, 1
+    if not logits.is_contiguous():
+        step, inner = logits.stride()
+        if inner != 1 and n > 1:
+            raise capi.QmmError(-1, "moe_route_scored: the logits of a token must be contiguous")
+        step = step if t > 1 else n
+    if bias is not None:
+        if bias.dtype is not torch.float32 or bias.shape != (n,) or not bias.is_contiguous() or bias.get_device() != index:
+            raise capi.QmmError(-1, f"moe_route_scored: a contiguous f32 bias of {n} on GPU {index} expected")
+        b, best = bias.data_ptr(), 2
     if not 1 <= top_k <= 64:
         raise capi.QmmError(-1, f"moe_route_scored: top_k {top_k} (1 to 64)")
     if index != _current_device():
         with torch.cuda.device(index):
             return moe_route_scored(logits, top_k, scoring, bias, groups, top_groups, group_best, renormalize, scale)
-    ids = torch.empty((t, top_k), dtype=torch.int32, device=logits.device)
-    weights = torch.empty((t, top_k), dtype=torch.float32, device=logits.device)
-    rc = getattr(lib(), name)(logits.data_ptr(), logits.stride(0) if t > 1 else n, 0 if bias is None else bias.data_ptr(), t, n, top_k, _SCORINGS[scoring], groups,
-                              groups if top_groups is None else top_groups, (1 if bias is None else 2) if group_best is None else group_best, bool(renormalize),
-                              scale, ids.data_ptr(), weights.data_ptr(), _raw_stream(index))
+    weights = logits.new_empty((t, top_k), dtype=torch.float32)
+    ids = torch.empty_like(weights, dtype=torch.int32)
+    rc = fn(logits.data_ptr(), step, b, t, n, top_k, score, groups, groups if top_groups is None else top_groups, best if group_best is None else group_best,
+            bool(renormalize), scale, ids.data_ptr(), weights.data_ptr(), _raw_stream(index))
     if rc:
         check(rc)
     return ids, weights
