@@ -338,6 +338,15 @@ __global__ __launch_bounds__(64 * WR * WZ * DZ, Elem<T>::N == 1 || D == 64 ? 2 :
             }
             if (behind < end) request(behind, 0);
         }
+        if constexpr (N == 1) { // eight operands on their way ahead of the first product (two: 8192 tokens 528 us instead of 522; D = 256 374, 356)
+            constexpr int kReads = PT * KK, kAhead = kReads < 8 ? kReads : 8;
+            __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+#pragma unroll
+            for (int i = 0; i < kReads; i++) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                if (i + kAhead < kReads) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            }
+        }
         if constexpr (DZ > 1) { // (two places in turn: a wave may still read the last tile's)
             static_assert(DZ == 2);
             f32x4* const scores = reinterpret_cast<f32x4*>(smem + kTiles) + turns * (W * PT * 4 * 64) + lane;
@@ -413,6 +422,16 @@ __global__ __launch_bounds__(64 * WR * WZ * DZ, Elem<T>::N == 1 || D == 64 ? 2 :
             for (int i = 0; i < Products<N>::kCount; i++)
 #pragma unroll
                 for (int d = 0; d < DT; d++) o[d] = E::mma(a[d][Products<N>::left(i)], w[Products<N>::right(i)], o[d]);
+        }
+        if constexpr (N == 1) { // the next sixteen positions' operands beside these
+            __builtin_amdgcn_sched_group_barrier(0x100, 2 * DT, 0);
+#pragma unroll
+            for (int t = 0; t < KT / 16; t++)
+#pragma unroll
+                for (int d = 0; d < DT; d++) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    if (t + 1 < KT / 16) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+                }
         }
     };
 
@@ -727,7 +746,7 @@ hipError_t launch_of(const PromptParams& P, int64_t max_k, int device, int n_cus
         return small ? launch<T, D, 2, 2, DZ, 32>(P, max_k, device, n_cus, stream) : launch<T, D, 4, 1, DZ, 32>(P, max_k, device, n_cus, stream);
     } else {
         const int quarters = P.causal ? (D == 64 ? 8 : D == 128 ? 7 : 4) : (D == 64 ? 6 : D == 128 ? 4 : 2);
-        const bool small = 4 * wgs < quarters * n_cus && (D == 256 || max_k > 64) && (rows <= 64 || rows > 128 || max_k < 8192);
+        const bool small = 4 * wgs <= quarters * n_cus && (D == 256 || max_k > 64) && (rows <= 64 || rows > 128 || max_k < 8192);
         if constexpr (D == 256) return small ? launch<T, D, 2, 1, DZ, 32>(P, max_k, device, n_cus, stream) : launch<T, D, 4, 1, DZ, 32>(P, max_k, device, n_cus, stream);
         else return small ? launch<T, D, 2, 2, DZ, 32>(P, max_k, device, n_cus, stream) : launch<T, D, 4, 1, DZ, 64>(P, max_k, device, n_cus, stream);
     }
