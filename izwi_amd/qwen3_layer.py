@@ -1,4 +1,4 @@
-"""One decoder layer of izwi-core's Qwen3 model at one token, composed from the library's calls.
+"""One decoder layer of izwi-core's Qwen3 model at one token, and for whole prompts, composed from the library's calls.
 
 Mirror of `Qwen3Layer::forward` (qwen3/core.rs:1863-1881) with `Qwen3Attention::forward`'s
 single-token path (core.rs:1446-1575: q/k/v projections, per-head q/k norm, rotary embedding, cache
@@ -8,6 +8,10 @@ value rows to the caches in the unfused form and owns the tensors.  Per layer: 5
 the attention is split over the cache (the two RMSNorms ride in the projection launches behind them; q/k norm, rotary and the cache
 append ride in the attention launch) behind one library call, or 11 to 12 with the reference's separate hooks and two copies,
 where the reference's eager path issues one per operator.
+
+`Qwen3PromptLayer` is the same layer for prompts of any lengths, packed one behind the other (the multi-token path of
+core.rs:1446-1575 for a batch without padding): projections, rotary positions with the q/k norm, attention within each
+prompt, output projection, MLP or experts (`SparseMlp`).
 """
 from __future__ import annotations
 
@@ -16,7 +20,8 @@ import torch
 from .capi import ERR_INVALID, check, lib
 from .decode_ops import (decode_attention_step, qk_norm_rope_append, try_fused_decode_gqa_attention_with_kv_len, try_fused_qk_rms_norm,
                          try_fused_rms_norm, try_fused_rope_pair_bshd)
-from .qmatmul import QMatMul, Qwen3GateUpProjection, _stream_ptr, forward_group
+from .prompt_ops import RotaryEmbedding, prompt_attention, rope_positions
+from .qmatmul import MoeExperts, QMatMul, Qwen3GateUpProjection, _stream_ptr, forward_group, moe_route_scored, moe_sort
 
 
 class Qwen3DecodeLayer:
@@ -98,3 +103,46 @@ class Qwen3DecodeLayer:
             return None
         check(rc)
         return y
+
+
+class SparseMlp:
+    """Experts behind a scored router: the router's product, `moe_route_scored` (whose arguments ``routing`` are), the sort by expert and the
+    experts' products."""
+
+    def __init__(self, router: QMatMul, experts: MoeExperts, top_k: int, **routing):
+        self.router, self.experts, self.top_k, self.routing = router, experts, top_k, routing
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        logits = self.router.forward(x)
+        ids, weights = moe_route_scored(logits, self.top_k, **self.routing)
+        perm, offsets = moe_sort(ids, logits.shape[1])
+        return self.experts.forward(x, ids, weights, perm, offsets)
+
+
+class Qwen3PromptLayer:
+    """A decoder layer for whole prompts, f32 activations.  ``mlp``: (gate_proj, up_proj, down_proj), or a `SparseMlp`."""
+
+    def __init__(self, input_layernorm: torch.Tensor, post_attention_layernorm: torch.Tensor, q_proj: QMatMul, k_proj: QMatMul, v_proj: QMatMul,
+                 qk_norm_weight: torch.Tensor, o_proj: QMatMul, mlp, num_heads: int, num_kv_heads: int, head_dim: int, rotary: RotaryEmbedding,
+                 rms_norm_eps: float = 1e-6):
+        self.w_in, self.w_post, self.qk_w = input_layernorm, post_attention_layernorm, qk_norm_weight
+        self.qkv, self.o_proj, self.rotary = (q_proj, k_proj, v_proj), o_proj, rotary
+        self.sparse = mlp if isinstance(mlp, SparseMlp) else None
+        if self.sparse is None:
+            gate, up, self.down_proj = mlp
+            self.gate_up = Qwen3GateUpProjection.new_separate(gate, up)
+        self.heads, self.kv_heads, self.d, self.eps = num_heads, num_kv_heads, head_dim, rms_norm_eps
+
+    def forward(self, x: torch.Tensor, positions: torch.Tensor, starts: torch.Tensor | None = None):
+        """x [tokens, hidden] f32, positions int32 [tokens], starts int32 [prompts + 1] (None: one prompt) -> (the layer's output [tokens,
+        hidden], keys, values [tokens, kv_heads, head_dim], which belong into the caches of the decode step)."""
+        tokens, d = x.shape[0], self.d
+        q, k, v = forward_group(self.qkv, x, norm_weight=self.w_in, eps=self.eps)
+        q, k, v = q.view(tokens, self.heads, d), k.view(tokens, self.kv_heads, d), v.view(tokens, self.kv_heads, d)
+        rope_positions(q, k, positions, self.rotary, qk_weight=self.qk_w, eps=self.eps, out=(q, k))
+        attn = prompt_attention(q, k, v, starts)
+        x = self.o_proj.forward_fused(attn.view(tokens, self.heads * d), residual=x)
+        if self.sparse is not None:
+            return x + self.sparse.forward(try_fused_rms_norm(x, self.w_post, self.eps)), k, v
+        hidden = self.gate_up.forward_silu_mul(x, norm_weight=self.w_post, eps=self.eps)
+        return self.down_proj.forward_fused(hidden, residual=x), k, v
