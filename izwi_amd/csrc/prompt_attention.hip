@@ -15,6 +15,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <type_traits>
 
@@ -122,7 +123,8 @@ __device__ __forceinline__ int turn(int row) {
     return D == 64 ? ((row >> 1 & 1) << 2 | (row >> 2 & 3)) : ((row & 3) << 2 | (row >> 2 & 3));
 }
 
-// The sequence that a tile of rows belongs to: tiles are numbered sequence by sequence.
+// The sequence that a tile of rows belongs to.  Sequence b has the tiles from (its first row among all) / rows + b on, as many as it needs or
+// one more, so that its place is found by its offset alone: 64 at a time, by the lanes.
 struct Sequence {
     int64_t q0, k0; // its first tokens
     int len_q, len_k, row0; // row0: the tile's first row within it
@@ -133,30 +135,26 @@ __device__ __forceinline__ bool find_sequence(const PromptParams& P, int rows, i
         s = Sequence{0, 0, (int)P.total_q, (int)P.total_k, tile * rows};
         return (int64_t)tile * rows < P.total_q * P.group;
     }
-    int before = 0;
-    for (int b0 = 0; b0 < P.batch; b0 += 64) {
-        const int b = min(b0 + lane, P.batch - 1);
-        const int from = bounded(P.cu_q, b, P.total_q), to = bounded(P.cu_q, b + 1, P.total_q);
-        const int kfrom = bounded(P.cu_k, b, P.total_k), kto = bounded(P.cu_k, b + 1, P.total_k);
-        const int len = b0 + lane < P.batch ? max(to - from, 0) : 0;
-        const int mine = (int)(((int64_t)len * P.group + rows - 1) / rows);
-        int upto = mine;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int other = __shfl_up(upto, o);
-            if (lane >= o) upto += other;
+    int from = 0, n = P.batch; // it is among from .. from + n - 1
+    for (;;) {
+        const int step = (n + 63) / 64, b = min(from + lane * step, P.batch - 1);
+        const int q0 = bounded(P.cu_q, b, P.total_q), slot = q0 * P.group / rows + b; // (below 2^31: checked on the host)
+        if (step > 1) {
+            const int found = __popcll(__ballot(lane * step < n && slot <= tile));
+            if (found == 0) return false;
+            from += (found - 1) * step, n = min(step, n - (found - 1) * step);
+            continue;
         }
-        const unsigned long long past = __ballot(before + upto > tile);
-        if (past) {
-            const int l = __ffsll((long long)past) - 1;
-            s.q0 = __builtin_amdgcn_readlane(from, l), s.len_q = __builtin_amdgcn_readlane(len, l);
-            s.k0 = __builtin_amdgcn_readlane(kfrom, l), s.len_k = max(__builtin_amdgcn_readlane(kto, l) - (int)s.k0, 0);
-            s.row0 = (tile - before - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(mine, l))) * rows;
-            return true;
-        }
-        before += __builtin_amdgcn_readlane(upto, 63);
+        const int q1 = bounded(P.cu_q, b + 1, P.total_q), k0 = bounded(P.cu_k, b, P.total_k), k1 = bounded(P.cu_k, b + 1, P.total_k);
+        const int found = __popcll(__ballot(lane < n && slot <= tile));
+        if (found == 0) return false;
+        const int l = found - 1;
+        s.q0 = __builtin_amdgcn_readlane(q0, l), s.k0 = __builtin_amdgcn_readlane(k0, l);
+        s.len_q = max(__builtin_amdgcn_readlane(q1, l) - (int)s.q0, 0), s.len_k = max(__builtin_amdgcn_readlane(k1, l) - (int)s.k0, 0);
+        const int64_t row0 = (int64_t)(tile - __builtin_amdgcn_readlane(slot, l)) * rows;
+        s.row0 = (int)min(row0, (int64_t)0x7fffffff);
+        return row0 < (int64_t)s.len_q * P.group;
     }
-    return false;
 }
 
 // v of the lane 32 away, the larger of both
@@ -710,16 +708,22 @@ hipError_t launch(PromptParams P, int64_t max_k, int device, int n_cus, hipStrea
         P.sums = static_cast<float*>(scratch);
         P.stats = reinterpret_cast<float2*>(P.sums + (size_t)rows * P.splits * D);
     }
-    const auto run = [&](auto kernel) {
-        if (lds > 64 * 1024) {
-            const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
-            if (e != hipSuccess) return e;
+    const auto run = [&](auto split) {
+        constexpr auto kernel = prompt_attention_kernel<T, D, WR, WZ, DZ, KT, decltype(split)::value>;
+        if (lds > 64 * 1024) { // (once per kernel and device: the call takes as long as the checks in front of it)
+            static std::atomic<uint64_t> allowed{0};
+            const uint64_t bit = device < 64 ? 1ull << device : 0;
+            if (!(allowed.load(std::memory_order_relaxed) & bit)) {
+                const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+                if (e != hipSuccess) return e;
+                allowed.fetch_or(bit, std::memory_order_relaxed);
+            }
         }
         kernel<<<(unsigned)(wgs * P.splits), 64 * WR * WZ * DZ, lds, stream>>>(P);
         return hipGetLastError();
     };
-    if (P.splits == 1) return run(prompt_attention_kernel<T, D, WR, WZ, DZ, KT, false>);
-    const hipError_t e = run(prompt_attention_kernel<T, D, WR, WZ, DZ, KT, true>);
+    if (P.splits == 1) return run(std::false_type{});
+    const hipError_t e = run(std::true_type{});
     if (e != hipSuccess) return e;
     if (P.splits <= 8) prompt_join_kernel<T, D, true><<<(unsigned)((rows + 3) / 4), 256, 0, stream>>>(P, rows);
     else prompt_join_kernel<T, D, false><<<(unsigned)rows, 256, 0, stream>>>(P, rows);
@@ -736,7 +740,7 @@ hipError_t launch(PromptParams P, int64_t max_k, int device, int n_cus, hipStrea
 // heads of 64 (200 tokens of 6 sequences 18.9, 12.6; 9 of 13, one tile, 5.6, 6.6).
 template <typename T, int D>
 hipError_t launch_of(const PromptParams& P, int64_t max_k, int device, int n_cus, hipStream_t stream) {
-    const int64_t wgs = row_tiles(P, 128) * P.kv_heads, rows = P.total_q * P.group / P.batch; // of a sequence, on average
+    const int64_t all = P.total_q * P.group, wgs = std::max<int64_t>((all + 127) / 128, P.batch) * P.kv_heads, rows = all / P.batch; // rows: of a sequence, on average
     constexpr int DZ = D == 256 ? 2 : 1;
     if constexpr (sizeof(T) == 4 && D == 256) {
         return launch<T, D, 2, 1, DZ, 32>(P, max_k, device, n_cus, stream);
@@ -767,7 +771,7 @@ int prompt_attention_impl(const T* q, int64_t q_stride, const T* k, int64_t k_st
     if (q_stride < heads * d || out_stride < heads * d || k_stride < kv_heads * d || v_stride < kv_heads * d)
         return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: rows overlap (strides %lld, %lld, %lld, %lld)", what, (long long)q_stride, (long long)k_stride,
                         (long long)v_stride, (long long)out_stride);
-    if (!std::isfinite(scale)) return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: scale %g", what, (double)scale);
+    if (!std::isfinite(scale) || std::fabs(scale) > 0x1p126f) return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: scale %g", what, (double)scale); // (log2(e) as much is a float, too)
     constexpr int kPiece = 16 / (int)sizeof(T);
     if (q_stride % kPiece || k_stride % kPiece || v_stride % kPiece || out_stride % kPiece ||
         ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(out)) & 15))
@@ -778,11 +782,9 @@ int prompt_attention_impl(const T* q, int64_t q_stride, const T* k, int64_t k_st
                         (long long)heads, (long long)total_k, (long long)k_stride, (long long)v_stride);
     if (batch == 0 || total_q == 0) return IZWI_QMM_OK;
     if (!q || !out || (total_k && (!k || !v))) return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: NULL buffer", what);
-    const auto overlap = [&](const void* a, int64_t rows, int64_t stride, int64_t width) {
-        const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(out);
-        return rows && x < y + ((uintptr_t)(total_q - 1) * out_stride + heads * d) * sizeof(T) && y < x + ((uintptr_t)(rows - 1) * stride + width) * sizeof(T);
-    };
-    if (overlap(q, total_q, q_stride, heads * d) || overlap(k, total_k, k_stride, kv_heads * d) || overlap(v, total_k, v_stride, kv_heads * d))
+    const auto rows = [&](const void* at, int64_t n, int64_t stride, int64_t of_heads) { return QmmRows{at, n, stride * (int64_t)sizeof(T), of_heads * d * (int64_t)sizeof(T)}; };
+    const QmmRows to = rows(out, total_q, out_stride, heads);
+    if (!qmm_rows_apart(to, rows(q, total_q, q_stride, heads)) || !qmm_rows_apart(to, rows(k, total_k, k_stride, kv_heads)) || !qmm_rows_apart(to, rows(v, total_k, v_stride, kv_heads)))
         return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: out shares memory with q, k or v", what);
     if ((total_q * (heads / kv_heads) / 32 + batch) * kv_heads > 0x3fffff)
         return qmm_fail(IZWI_QMM_ERR_UNSUPPORTED, "%s: %lld sequences on %lld kv heads", what, (long long)batch, (long long)kv_heads);

@@ -162,6 +162,22 @@ int qmm_guarded(const char* what, F&& f) {
     }
 }
 
+// Rows of `width` bytes, `stride` bytes from one to the next.
+struct QmmRows {
+    const void* at;
+    int64_t rows, stride, width;
+};
+// Whether two sets of rows share no byte, as far as ranges tell, and rows of one stride that lie between each other (parts of wider rows).
+inline bool qmm_rows_apart(const QmmRows& a, const QmmRows& b) {
+    if (a.rows <= 0 || b.rows <= 0 || a.width <= 0 || b.width <= 0) return true;
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a.at), y = reinterpret_cast<uintptr_t>(b.at);
+    const uintptr_t xn = (uintptr_t)(a.rows - 1) * a.stride + a.width, yn = (uintptr_t)(b.rows - 1) * b.stride + b.width;
+    if (x + xn <= y || y + yn <= x) return true;
+    if (a.stride != b.stride) return false;
+    const int64_t off = ((int64_t)(intptr_t)(y - x) % a.stride + a.stride) % a.stride;
+    return off >= a.width && off + b.width <= a.stride;
+}
+
 // The current HIP device, validated (IZWI_QMM_ERR_NO_DEVICE without one), and its CU count.
 int qmm_current_device(int* device, int* n_cus);
 // The library's scratch buffer of (device, stream): at least `bytes`, reused by the next call on

@@ -38,41 +38,43 @@ __device__ __forceinline__ void turn_of(const RopeParams& P, int position, int p
     c *= P.factor, s *= P.factor;
 }
 
-// A workgroup per token, a wave per head in turn, a lane per pair of elements in turn.
+// A workgroup per token (in turn), a wave per head in turn, a lane per pair of elements in turn.
 template <typename T, bool INTER>
 __global__ __launch_bounds__(256) void rope_any_kernel(RopeParams P) {
     __shared__ float cosine[kMostPairs], sine[kMostPairs];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, pairs = P.rotary / 2;
-    const int64_t token = blockIdx.x;
-    const int position = P.positions[token];
-    for (int i = threadIdx.x; i < pairs; i += 256) turn_of(P, position, i, cosine[i], sine[i]);
-    __syncthreads();
-    for (int head = wave; head < P.heads; head += 4) {
-        const bool is_q = head < P.q_heads;
-        const int at = is_q ? head : head - P.q_heads;
-        const T* const from = static_cast<const T*>(is_q ? P.q : P.k) + token * (is_q ? P.q_stride : P.k_stride) + (int64_t)at * P.d;
-        T* const to = static_cast<T*>(is_q ? P.q_out : P.k_out) + token * (is_q ? P.q_out_stride : P.k_out_stride) + (int64_t)at * P.d;
-        const T* const weight = P.weight ? static_cast<const T*>(P.weight) + (is_q ? 0 : P.d) : nullptr;
-        float by = 1.0f;
-        if (weight) {
-            float sum = 0.0f;
-            for (int i = lane; i < P.d; i += 64) {
-                const float v = (float)from[i];
-                sum += v * v;
+    for (int64_t token = blockIdx.x; token < P.tokens; token += gridDim.x) {
+        const int position = P.positions[token];
+        for (int i = threadIdx.x; i < pairs; i += 256) turn_of(P, position, i, cosine[i], sine[i]);
+        __syncthreads();
+        for (int head = wave; head < P.heads; head += 4) {
+            const bool is_q = head < P.q_heads;
+            const int at = is_q ? head : head - P.q_heads;
+            const T* const from = static_cast<const T*>(is_q ? P.q : P.k) + token * (is_q ? P.q_stride : P.k_stride) + (int64_t)at * P.d;
+            T* const to = static_cast<T*>(is_q ? P.q_out : P.k_out) + token * (is_q ? P.q_out_stride : P.k_out_stride) + (int64_t)at * P.d;
+            const T* const weight = P.weight ? static_cast<const T*>(P.weight) + (is_q ? 0 : P.d) : nullptr;
+            float by = 1.0f;
+            if (weight) {
+                float sum = 0.0f;
+                for (int i = lane; i < P.d; i += 64) {
+                    const float v = (float)from[i];
+                    sum += v * v;
+                }
+                by = 1.0f / sqrtf(wave_sum(sum) / (float)P.d + P.eps);
+                asm volatile("" ::: "memory"); // (in place, lanes read others' elements above)
+                __builtin_amdgcn_wave_barrier();
             }
-            by = 1.0f / sqrtf(wave_sum(sum) / (float)P.d + P.eps);
-            asm volatile("" ::: "memory"); // (in place, lanes read others' elements above)
-            __builtin_amdgcn_wave_barrier();
+            for (int i = lane; i < P.d / 2; i += 64) {
+                const bool turns = i < pairs;
+                const int a = turns && !INTER ? i : 2 * i, b = turns && !INTER ? i + pairs : 2 * i + 1;
+                float u = (float)from[a], v = (float)from[b];
+                if (weight) u = u * by * (float)weight[a], v = v * by * (float)weight[b];
+                const float c = turns ? cosine[i] : 1.0f, s = turns ? sine[i] : 0.0f;
+                to[a] = (T)(turns ? u * c - v * s : u);
+                to[b] = (T)(turns ? u * s + v * c : v);
+            }
         }
-        for (int i = lane; i < P.d / 2; i += 64) {
-            const bool turns = i < pairs;
-            const int a = turns && !INTER ? i : 2 * i, b = turns && !INTER ? i + pairs : 2 * i + 1;
-            float u = (float)from[a], v = (float)from[b];
-            if (weight) u = u * by * (float)weight[a], v = v * by * (float)weight[b];
-            const float c = turns ? cosine[i] : 1.0f, s = turns ? sine[i] : 0.0f;
-            to[a] = (T)(turns ? u * c - v * s : u);
-            to[b] = (T)(turns ? u * s + v * c : v);
-        }
+        __syncthreads(); // (cosines and sines are read)
     }
 }
 
@@ -216,28 +218,14 @@ int rope_positions_impl(const T* q, int64_t q_stride, const T* k, int64_t k_stri
                         (long long)q_out_stride, (long long)k_out_stride);
     if (interleaved != 0 && interleaved != 1) return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: layout %d (0 halves, 1 interleaved)", what, interleaved);
     if (!std::isfinite(factor) || !(eps >= 0.0f) || !std::isfinite(eps)) return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: factor %g, eps %g", what, (double)factor, (double)eps);
-    if (tokens > 0x3fffffff || q_stride > 0x3fffffff || k_stride > 0x3fffffff || q_out_stride > 0x3fffffff || k_out_stride > 0x3fffffff)
+    if (tokens > 0x3ffffff || q_stride > 0x3fffffff || k_stride > 0x3fffffff || q_out_stride > 0x3fffffff || k_out_stride > 0x3fffffff)
         return qmm_fail(IZWI_QMM_ERR_UNSUPPORTED, "%s: %lld tokens", what, (long long)tokens);
     if (tokens == 0 || q_heads + k_heads == 0) return IZWI_QMM_OK;
     if (!positions || !frequencies || (q_heads && (!q || !q_out)) || (k_heads && (!k || !k_out))) return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: NULL buffer", what);
-    // an output may be its input; otherwise it shares no memory with an input or the other output, unless the rows of both interleave (parts of
-    // wider rows): those of one stride, each inside what the other leaves free
-    struct Rows {
-        const void* at;
-        int64_t stride, width;
-    };
-    const auto apart = [&](const Rows& a, const Rows& b) {
-        if (!a.width || !b.width) return true;
-        const uintptr_t x = reinterpret_cast<uintptr_t>(a.at), y = reinterpret_cast<uintptr_t>(b.at);
-        const uintptr_t xn = ((uintptr_t)(tokens - 1) * a.stride + a.width) * sizeof(T), yn = ((uintptr_t)(tokens - 1) * b.stride + b.width) * sizeof(T);
-        if (x + xn <= y || y + yn <= x) return true;
-        if (a.stride != b.stride) return false;
-        const int64_t row = a.stride * (int64_t)sizeof(T), off = (int64_t)((intptr_t)(y - x) % row + row) % row;
-        return off >= a.width * (int64_t)sizeof(T) && off + b.width * (int64_t)sizeof(T) <= row;
-    };
-    const Rows qi{q, q_stride, q_heads * d}, ki{k, k_stride, k_heads * d}, qo{q_out, q_out_stride, q_heads * d}, ko{k_out, k_out_stride, k_heads * d};
-    const auto same = [](const Rows& a, const Rows& b) { return a.at == b.at && a.stride == b.stride; };
-    if ((!same(qi, qo) && !apart(qi, qo)) || (!same(ki, ko) && !apart(ki, ko)) || !apart(qi, ko) || !apart(ki, qo) || !apart(qo, ko))
+    const auto rows = [&](const void* at, int64_t stride, int64_t heads) { return QmmRows{at, tokens, stride * (int64_t)sizeof(T), heads * d * (int64_t)sizeof(T)}; };
+    const QmmRows qi = rows(q, q_stride, q_heads), ki = rows(k, k_stride, k_heads), qo = rows(q_out, q_out_stride, q_heads), ko = rows(k_out, k_out_stride, k_heads);
+    const auto same = [](const QmmRows& a, const QmmRows& b) { return a.at == b.at && a.stride == b.stride; };
+    if ((!same(qi, qo) && !qmm_rows_apart(qi, qo)) || (!same(ki, ko) && !qmm_rows_apart(ki, ko)) || !qmm_rows_apart(qi, ko) || !qmm_rows_apart(ki, qo) || !qmm_rows_apart(qo, ko))
         return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: an output shares memory with another tensor (it may be its own input)", what);
     int device = 0, n_cus = 0;
     if (int rc = qmm_current_device(&device, &n_cus)) return rc;
@@ -259,7 +247,8 @@ int rope_positions_impl(const T* q, int64_t q_stride, const T* k, int64_t k_stri
         if (weight) interleaved ? run(rope_pieces_kernel<T, true, true>) : run(rope_pieces_kernel<T, false, true>);
         else interleaved ? run(rope_pieces_kernel<T, true, false>) : run(rope_pieces_kernel<T, false, false>);
     } else {
-        interleaved ? rope_any_kernel<T, true><<<(unsigned)tokens, 256, 0, stream>>>(P) : rope_any_kernel<T, false><<<(unsigned)tokens, 256, 0, stream>>>(P);
+        const unsigned grid = (unsigned)std::min<int64_t>(tokens, 1 << 20);
+        interleaved ? rope_any_kernel<T, true><<<grid, 256, 0, stream>>>(P) : rope_any_kernel<T, false><<<grid, 256, 0, stream>>>(P);
     }
     ROPE_TRY(hipGetLastError());
     return IZWI_QMM_OK;

@@ -117,6 +117,22 @@ def test_rope_positions_of_odd_addresses(qa):
         assert torch.equal(kept, room)  # nothing else was written
 
 
+def test_rope_positions_of_far_offsets(qa):
+    """Rows whose offsets pass 32 bits."""
+    step = 1 << 21
+    rotary = qa.RotaryEmbedding(128)
+    room = torch.empty(2100 * step + 4096, dtype=torch.bfloat16, device="cuda")
+    q = torch.randn(2100, 3, 128, device="cuda").bfloat16()
+    view = room.as_strided(q.shape, (step, 128, 1))
+    view.copy_(q)
+    got, _ = qa.rope_positions(view, None, ints(range(2100)), rotary, out=(view, None))
+    want, _ = qa.rope_positions(q, None, ints(range(2100)), rotary)
+    assert torch.equal(got, want)
+    odd = room[1:].as_strided(q.shape, (step, 128, 1))  # no row begins on 16 bytes
+    odd.copy_(q)
+    assert torch.equal(qa.rope_positions(odd, None, ints(range(2100)), rotary)[0], want)
+
+
 def test_rope_positions_of_no_numbers(qa):
     """A NaN or infinity reaches its pair (with a norm its head) and nothing else; what does not turn is copied."""
     rotary = qa.RotaryEmbedding(128, rotary_dim=64)
@@ -260,6 +276,69 @@ def test_prompt_attention_of_offsets_that_do_not_fit(qa, dtype):
     check_attention(got, q64, k64, v64, [0, 12, 30], [0, 12, 30], True, 0.125, dtype)
     got = qa.prompt_attention(q, k, v, ints([0, 12, 3, 30]), ints([0, 12, 12, 12]), out=torch.zeros_like(q))
     check_attention(got[:3], q64[:3], k64[:12], v64[:12], [0, 3], [0, 3], True, 0.125, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("prompts,heads,kv", [(64, 3, 1), (65, 2, 2), (4097, 2, 1), (130, 40, 2)])
+def test_prompt_attention_of_many_sequences(qa, dtype, prompts, heads, kv):
+    """Short sequences, some empty, as many as need one, two and three looks at the offsets."""
+    rng = np.random.default_rng(prompts)
+    lens = rng.integers(0, 4, size=prompts)
+    lens[prompts // 2] = 150
+    lens_k = lens + rng.integers(0, 3, size=prompts) * (rng.random(prompts) < 0.3)
+    starts, starts_k = np.cumsum([0, *lens]), np.cumsum([0, *lens_k])
+    (q, q64), (k, k64), (v, v64) = (made(rng, n, g, 64, dtype=dtype) for n, g in ((starts[-1], heads), (starts_k[-1], kv), (starts_k[-1], kv)))
+    got = qa.prompt_attention(q, k, v, ints(starts), ints(starts_k), max_len_k=int(lens_k.max()))
+    check_attention(got, q64, k64, v64, starts, starts_k, True, 0.125, dtype)
+
+
+def test_prompt_attention_without_keys(qa):
+    for dtype in DTYPES.values():
+        q, none = torch.randn(5, 4, 128, device="cuda").to(dtype), torch.empty(0, 2, 128, device="cuda", dtype=dtype)
+        assert (qa.prompt_attention(q, none, none) == 0).all()
+        assert (qa.prompt_attention(q, none, none, ints([0, 3, 5]), ints([0, 0, 0]), causal=False) == 0).all()
+        assert qa.prompt_attention(q[:0], none, none).shape == (0, 4, 128)
+
+
+def test_prompt_attention_on_another_stream(qa):
+    """Calls on two streams at once, split ones among them, each with the scratch of its own stream."""
+    rng = np.random.default_rng(14)
+    sets = []
+    for i in range(2):
+        (q, q64), (k, k64), (v, v64) = (made(rng, n, g, 128, dtype="bf16") for n, g in ((9, 8), (2000 + 300 * i, 2), (2000 + 300 * i, 2)))
+        sets.append((q, k, v, q64, k64, v64, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(10):
+        for s, out in zip(sets, outs):
+            with torch.cuda.stream(s[6]):
+                out.append(qa.prompt_attention(*s[:3]))
+    torch.cuda.synchronize()
+    for s, out in zip(sets, outs):
+        check_attention(out[0], *s[3:6], [0, 9], [0, s[1].shape[0]], True, 128 ** -0.5, "bf16")
+        assert all(torch.equal(out[0], o) for o in out)
+
+
+def test_prompt_attention_of_far_offsets(qa):
+    """Rows whose offsets in elements and bytes pass 32 bits: the last rows of keys of a wide stride, the last tokens of q and out."""
+    rng = np.random.default_rng(15)
+    for dtype in ("bf16", "f32"):
+        step = 1 << 20
+        tokens, keys = 2100, 2200
+        room = torch.empty(keys * step + 4096, dtype=DTYPES[dtype], device="cuda")
+        (q, q64), (k, k64), (v, v64) = (made(rng, n, g, 64, dtype=dtype) for n, g in ((tokens, 2), (keys, 1), (keys, 1)))
+        views = []
+        for i, x in enumerate((q, k, v)):
+            view = room[i * 512:].as_strided(x.shape, (step, 64, 1))
+            view.copy_(x)
+            views.append(view)
+        out = room[3 * 512:].as_strided(q.shape, (step, 64, 1))
+        qa.prompt_attention(*views, ints([0, tokens - 5, tokens]), ints([0, 100, keys]), out=out)
+        at, ak = tokens - 5, 100
+        check_attention(out[at:], q64[at:], k64[ak:], v64[ak:], [0, 5], [0, keys - ak], True, 0.125, dtype)
+        assert torch.equal(out, qa.prompt_attention(q, k, v, ints([0, tokens - 5, tokens]), ints([0, 100, keys])))
+        del room, views, view, out
+        torch.cuda.empty_cache()
 
 
 def test_prompt_attention_in_a_graph(qa):

@@ -130,7 +130,7 @@ def test_prompt_attention_refusals(L, name):
         return fn(*{**good, **over}.values())
 
     for over in (dict(batch=-1), dict(tq=-1), dict(tk=-1), dict(mk=-1), dict(heads=0), dict(kv=0), dict(heads=7), dict(cu_q=0), dict(cu_k=0), dict(cu_q=0, cu_k=0),
-                 dict(qs=1023), dict(qs=1016), dict(ks=255), dict(vs=128), dict(os=512), dict(scale=math.nan), dict(scale=-math.inf), dict(q=P + 8), dict(k=far + 2), dict(v=P + 4),
+                 dict(qs=1023), dict(qs=1016), dict(ks=255), dict(vs=128), dict(os=512), dict(scale=math.nan), dict(scale=-math.inf), dict(scale=3e38), dict(q=P + 8), dict(k=far + 2), dict(v=P + 4),
                  dict(out=far + 8), dict(qs=1025), dict(ks=257), dict(q=0), dict(k=0), dict(v=0), dict(out=0), dict(out=P), dict(out=P + 1024 * size * 9),
                  dict(out=far), dict(out=2 * far + 256 * size), dict(heads=65536 * 2, qs=1 << 28, os=1 << 28)):
         assert call(**over) == -1, over
