@@ -730,12 +730,12 @@ hipError_t launch(PromptParams P, int64_t max_k, int device, int n_cus, hipStrea
     return hipGetLastError();
 }
 // Which workgroups.  f16 and bf16: four waves of 32 rows on 64 keys at a time (two on halves of the head each for D = 256, 32 keys), or where
-// those would not fill the compute units, two waves of rows on 64 keys and two on the 64 behind them (D = 256: half the rows): causal
+// those would not fill the compute units, two waves of rows on 32 keys and two on the 32 behind them (D = 256: half the rows): causal
 // prompts, whose workgroups are of unequal length, change over later.  16 bf16 heads on 8, us of the larger and the smaller workgroups: D = 128
-// causal 700 tokens 26.6, 15.1; 2600 54.9, 43.9; 3500 76.9, 73.1; not causal 2000 45.8, 46.4; 2600 76.7, 85.9; D = 64 causal 2600 39.7, 28.1; not causal
-// 2600 53.1, 46.7; 3500 72.5, 76.8; D = 256 causal 2000 92.5, 78.1; 2600 119, 137; not causal 700 42, 28.5; 1500 71, 104.  A tile of 65 to
-// 128 rows on very many keys reads them twice with the smaller ones (17 tokens of 32 heads behind 30011 31.5, 36.2).  Up to 64 keys the
-// second pair would have none (37 tokens 5.9, 6.6).
+// causal 700 tokens 26, 15; 2600 51, 44.6; 3500 73, 70; not causal 700 26, 15; 1500 32, 34; 2000 42.6, 47; D = 64 causal 2600 37.7, 29.5; 3500
+// 49.5, 42; not causal 2600 51, 47; 3500 71, 77; D = 256 causal 2048 90, 77; 2600 112, 137; not causal 700 42, 27; 1500 67, 104.  More than
+// 64 rows on very many keys read them too often with the smaller ones (17 tokens of 32 heads behind 30011 31.5, 36.2; 250 of 16 behind 8000 34,
+// 40, behind 2000 24.7, 21).  Up to 64 keys the second pair would have few (37 tokens 5.9, 6.6).
 // f32: the larger ones; the smaller where sequences have few rows and many tiles each (4 tokens behind 1087 of 10 sequences 46.7, 36.5) and for
 // heads of 64 (200 tokens of 6 sequences 18.9, 12.6; 9 of 13, one tile, 5.6, 6.6).
 template <typename T, int D>
@@ -749,8 +749,8 @@ hipError_t launch_of(const PromptParams& P, int64_t max_k, int device, int n_cus
         const bool small = D == 64 ? tiles > 2 : rows <= 64 && tiles >= 4 * splits_of<T>(wgs, max_k, 32, n_cus);
         return small ? launch<T, D, 2, 2, DZ, 32>(P, max_k, device, n_cus, stream) : launch<T, D, 4, 1, DZ, 32>(P, max_k, device, n_cus, stream);
     } else {
-        const int quarters = P.causal ? (D == 64 ? 8 : D == 128 ? 7 : 4) : (D == 64 ? 6 : D == 128 ? 4 : 2);
-        const bool small = 4 * wgs <= quarters * n_cus && (D == 256 || max_k > 64) && (rows <= 64 || rows > 128 || max_k < 8192);
+        const int quarters = P.causal ? (D == 64 ? 8 : D == 128 ? 7 : 4) : (D == 64 ? 6 : 2); // of a workgroup per compute unit
+        const bool small = 4 * wgs <= quarters * n_cus && (D == 256 || max_k > 64) && (rows <= 64 || max_k < 8192);
         if constexpr (D == 256) return small ? launch<T, D, 2, 1, DZ, 32>(P, max_k, device, n_cus, stream) : launch<T, D, 4, 1, DZ, 32>(P, max_k, device, n_cus, stream);
         else return small ? launch<T, D, 2, 2, DZ, 32>(P, max_k, device, n_cus, stream) : launch<T, D, 4, 1, DZ, 64>(P, max_k, device, n_cus, stream);
     }
