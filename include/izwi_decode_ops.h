@@ -260,15 +260,15 @@ int izwi_rope_positions_bf16(const uint16_t* q, int64_t q_stride, const uint16_t
  * fewer keys than queries the first ones see none).  q is `[total_q, num_heads, head_dim]`, k and v `[total_k, num_kv_heads,
  * head_dim]`, strides the elements from one token to the next; head h reads kv head h / (num_heads / num_kv_heads).  Sequence b has
  * tokens cu_q[b] .. cu_q[b + 1] - 1 and keys cu_k[b] .. cu_k[b + 1] - 1 (`[batch + 1]` device arrays that do not fall, so that a
- * captured call can be replayed with other lengths; offsets outside the tensors count as their ends); both NULL: one sequence of
- * everything.  Rows of out that belong to no sequence stay as they are; a query that sees no key gives zeros.  max_k, the length of the
+ * captured call can be replayed with other lengths; offsets outside the tensors count as their ends; where they fall all the same,
+ * the rows that they touch hold anything); both NULL: one sequence of everything.  Rows of out that belong to no sequence stay as they are; a query that sees no key gives zeros.  max_k, the length of the
  * longest sequence of keys as far as the caller knows it (total_k at most), only decides how the work is shared out.
  * What a query does not see has no influence, whatever it holds.  A NaN that it sees in q or a key makes its row NaN, one in a
  * value that element; an infinity in a value makes the element that infinity, or NaN (where its weight is too small for the type, and
  * in f32).
  * The products run on the matrix cores with f32 sums: f16 and bf16 values as they are, weights rounded to the type (2^-11, 2^-8 of
- * each); f32 ones as three bf16 numbers each, all 24 bits.  head_dim 64, 128 or 256; rows begin on 16 bytes; out shares no memory with
- * the inputs.  Uses the library's per-stream scratch where few rows meet many keys. */
+ * each); f32 ones as three bf16 numbers each, all 24 bits down to 2^-100.  head_dim 64, 128 or 256; rows begin on 16 bytes; out
+ * shares no memory with the inputs.  Uses the library's per-stream scratch where few rows meet many keys. */
 int izwi_qmm_prompt_attention_f32(const float* q, int64_t q_stride, const float* k, int64_t k_stride, const float* v, int64_t v_stride,
                                   const int32_t* cu_q, const int32_t* cu_k, int64_t batch, int64_t total_q, int64_t total_k,
                                   int64_t max_k, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim, int causal, float scale,

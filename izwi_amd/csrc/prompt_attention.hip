@@ -10,8 +10,8 @@
 //                 from LDS through the transposing reads.
 // Reference and sum of a row are two numbers of a lane, and rescaling O^T is a multiplication by a lane's own number.
 //
-// f32: queries, keys, values and weights go as three bf16 numbers each, which hold all 24 bits at every exponent, and the six
-// products of weight 2^-16 and more are summed in f32; what is left out is below 2^-23 of a product.
+// f32: queries, keys, values and weights go as three bf16 numbers each, which hold all 24 bits (down to 2^-100: the third has no bits
+// below 2^-133), and the six products of weight 2^-16 and more are summed in f32; what is left out is below 2^-23 of a product.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -153,7 +153,7 @@ __device__ __forceinline__ bool find_sequence(const PromptParams& P, int rows, i
         s.len_q = max(__builtin_amdgcn_readlane(q1, l) - (int)s.q0, 0), s.len_k = max(__builtin_amdgcn_readlane(k1, l) - (int)s.k0, 0);
         const int64_t row0 = (int64_t)(tile - __builtin_amdgcn_readlane(slot, l)) * rows;
         s.row0 = (int)min(row0, (int64_t)0x7fffffff);
-        return row0 < (int64_t)s.len_q * P.group;
+        return row0 >= 0 && row0 < (int64_t)s.len_q * P.group; // (below 0 where offsets fall)
     }
 }
 

@@ -279,6 +279,18 @@ def test_prompt_attention_of_offsets_that_do_not_fit(qa, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+def test_prompt_attention_of_offsets_that_fall_far(qa, dtype):
+    """Sequences that overlap leave their rows in any state, and what is around the tensor as it was."""
+    rng = np.random.default_rng(16)
+    n = 3000
+    (q, _), (k, _), (v, _) = (made(rng, n, g, 64, dtype=dtype) for g in (2, 1, 1))
+    for starts in ([0, n, 100, n], [0, 2900, 64, 2800, 10, n], [n, 0, n, 0]):
+        room = torch.full((n + 600, 2, 64), 3.0, dtype=DTYPES[dtype], device="cuda")
+        qa.prompt_attention(q, k, v, ints(starts), out=room[300:300 + n])
+        assert (room[:300] == 3.0).all() and (room[300 + n:] == 3.0).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("prompts,heads,kv", [(64, 3, 1), (65, 2, 2), (4097, 2, 1), (130, 40, 2)])
 def test_prompt_attention_of_many_sequences(qa, dtype, prompts, heads, kv):
     """Short sequences, some empty, as many as need one, two and three looks at the offsets."""
@@ -364,6 +376,64 @@ def test_prompt_attention_in_a_graph(qa):
             graph.replay()
             torch.cuda.synchronize()
             check_attention(out, x64, y64, z64, a, b, True, 128 ** -0.5, dtype, untouched=3.0)
+
+
+def test_prompt_operators_in_one_graph(qa):
+    """Rotation, attention of few rows on many keys and routing as one captured sequence, on new values, positions and lengths at every replay, with
+    eager calls of other sizes on the same stream's scratch in between."""
+    rng = np.random.default_rng(17)
+    rotary = qa.RotaryEmbedding(128, base=1e6)
+    for dtype in DTYPES:
+        (q, k), (keys, values) = (torch.zeros(6, g, 128, dtype=DTYPES[dtype], device="cuda") for g in (4, 2)), (torch.zeros(1500, 2, 128, dtype=DTYPES[dtype], device="cuda") for _ in range(2))
+        positions, starts, starts_k = ints([0] * 6), ints([0, 6, 6]), ints([0, 1500, 1500])
+        mix = torch.from_numpy(rng.normal(size=(512, 32)).astype(np.float32)).cuda()
+        logits = torch.zeros(6, 32, dtype=DTYPES[dtype], device="cuda")
+
+        def run():
+            a, _ = qa.rope_positions(q, k, positions, rotary)
+            o = qa.prompt_attention(a, keys, values, starts, starts_k)
+            return o, *qa.moe_route_scored(logits, 4, "sigmoid", groups=4, top_groups=2)
+
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            run()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                kept = run()
+            for step in range(4):
+                for t in (q, k, keys, values, logits):
+                    t.copy_(made(rng, *t.shape, dtype=dtype)[0])
+                positions.copy_(ints(rng.integers(0, 100000, size=6)))
+                cut, cut_k = int(rng.integers(0, 7)), int(rng.integers(0, 1501))
+                starts.copy_(ints([0, cut, 6])), starts_k.copy_(ints([0, cut_k, 1500]))
+                graph.replay()
+                got = [t.clone() for t in kept]
+                qa.prompt_attention(values[:9], values, keys)  # (split, too)
+                want = run()
+                stream.synchronize()
+                assert all(torch.equal(a, b) for a, b in zip(got, want)), step
+
+
+def test_prompt_attention_by_two_threads(qa):
+    """Calls of two host threads on one stream and on two, split ones, each as alone."""
+    import threading
+    rng = np.random.default_rng(18)
+    sets = [[made(rng, n, g, 64, dtype="f16")[0] for n, g in ((5 + i, 4), (900 + 200 * i, 2), (900 + 200 * i, 2))] for i in range(2)]
+    alone = [qa.prompt_attention(*s) for s in sets]
+    torch.cuda.synchronize()
+    for streams in ([torch.cuda.Stream()] * 2, [torch.cuda.Stream(), torch.cuda.Stream()]):
+        outs = [[], []]
+
+        def work(i):
+            with torch.cuda.stream(streams[i]):
+                for _ in range(50):
+                    outs[i].append(qa.prompt_attention(*sets[i]))
+
+        threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+        [t.start() for t in threads], [t.join() for t in threads]
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert len(outs[i]) == 50 and all(torch.equal(o, alone[i]) for o in outs[i])
 
 
 def test_prompt_attention_python_refusals(qa):
