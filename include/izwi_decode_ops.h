@@ -261,8 +261,9 @@ int izwi_rope_positions_bf16(const uint16_t* q, int64_t q_stride, const uint16_t
  * head_dim]`, strides the elements from one token to the next; head h reads kv head h / (num_heads / num_kv_heads).  Sequence b has
  * tokens cu_q[b] .. cu_q[b + 1] - 1 and keys cu_k[b] .. cu_k[b + 1] - 1 (`[batch + 1]` device arrays that do not fall, so that a
  * captured call can be replayed with other lengths; offsets outside the tensors count as their ends; where they fall all the same,
- * the rows that they touch hold anything); both NULL: one sequence of everything.  Rows of out that belong to no sequence stay as they are; a query that sees no key gives zeros.  max_k, the length of the
- * longest sequence of keys as far as the caller knows it (total_k at most), only decides how the work is shared out.
+ * the rows that they touch hold anything); both NULL: one sequence of everything.  Rows of out that belong to no sequence stay as
+ * they are; a query that sees no key gives zeros.  max_k, the length of the longest sequence of keys as far as the caller knows it
+ * (total_k at most), only decides how the work is shared out.
  * What a query does not see has no influence, whatever it holds.  A NaN that it sees in q or a key makes its row NaN, one in a
  * value that element; an infinity in a value makes the element that infinity, or NaN (where its weight is too small for the type, and
  * in f32).
