@@ -45,6 +45,7 @@ struct PromptParams {
     int64_t total_q, total_k;
     int batch, heads, kv_heads, group, causal;
     int tiles, splits; // workgroups: tiles of rows x splits of the positions x kv heads
+    int by_length;     // workgroups begin in the order of the positions that they see
     float sign;        // of the scale, or 0: what queries are multiplied by
     float scale, scale_rest; // |scale| log2(e) as two f32 numbers
     float* sums;       // [row][split][D], rows as in out (splits > 1)
@@ -157,6 +158,43 @@ __device__ __forceinline__ bool find_sequence(const PromptParams& P, int rows, i
     }
 }
 
+// The same for at most 64 sequences, in the order of the positions that a tile sees, the most first: in that of the offsets the last ones begun
+// may be long ones of a long sequence.  A tile's level is that number in whole tiles (causal; else the sequence's); `above` counts the
+// tiles of higher levels, and unit u lies in the level where the count passes it.
+__device__ __forceinline__ bool find_by_length(const PromptParams& P, int rows, int u, int lane, Sequence& s) {
+    const int b = min(lane, P.batch - 1);
+    const int q0 = bounded(P.cu_q, b, P.total_q), q1 = bounded(P.cu_q, b + 1, P.total_q), k0 = bounded(P.cu_k, b, P.total_k), k1 = bounded(P.cu_k, b + 1, P.total_k);
+    const int len_q = max(q1 - q0, 0), len_k = max(k1 - k0, 0), n = lane < P.batch ? (len_q * P.group + rows - 1) / rows : 0;
+    const int top = len_k / max(rows / P.group, 1); // the last tile's level; the one `e` before it is `e` lower (causal)
+    const auto sum = [](int v) { return __builtin_amdgcn_readfirstlane((int)wave_sum((float)v)); }; // (exact: below 2^24)
+    const auto above = [&](int level) { return sum(P.causal ? min(max(top - level, 0), n) : top > level ? n : 0); };
+    if (u >= sum(n)) return false;
+    int least = P.causal ? top - n : top - 1, most = top; // above(least) is all of a sequence's, above(most) none
+    for (int i = 1; i < 64; i <<= 1) least = min(least, __shfl_xor(least, i)), most = max(most, __shfl_xor(most, i));
+    least = __builtin_amdgcn_readfirstlane(least), most = __builtin_amdgcn_readfirstlane(most);
+    while (most - least > 1) {
+        const int middle = least + (most - least) / 2;
+        if (above(middle) > u) least = middle;
+        else most = middle;
+    }
+    // above(most) <= u < above(least)
+    int at = u - above(most);
+    const int here = P.causal ? (top - most >= 0 && top - most < n ? 1 : 0) : top == most ? n : 0;
+    uint64_t left = __ballot(here > 0);
+    int l = 0;
+    for (;; left &= left - 1) { // (at is below the sum of `here`)
+        l = __ffsll((unsigned long long)left) - 1;
+        const int of = __builtin_amdgcn_readlane(here, l);
+        if (at < of) break;
+        at -= of;
+    }
+    const int tile = P.causal ? __builtin_amdgcn_readlane(n, l) - 1 - (__builtin_amdgcn_readlane(top, l) - most) : __builtin_amdgcn_readlane(n, l) - 1 - at;
+    s.q0 = __builtin_amdgcn_readlane(q0, l), s.k0 = __builtin_amdgcn_readlane(k0, l);
+    s.len_q = __builtin_amdgcn_readlane(len_q, l), s.len_k = __builtin_amdgcn_readlane(len_k, l);
+    s.row0 = tile * rows;
+    return true;
+}
+
 // v of the lane 32 away, the larger of both
 __device__ __forceinline__ float max_lane32(float v) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -189,7 +227,8 @@ __global__ __launch_bounds__(64 * WR * WZ * DZ, Elem<T>::N == 1 || D == 64 ? 2 :
     const int kv = blockIdx.x % P.kv_heads;
     const int unit = blockIdx.x / P.kv_heads, split = SPLIT ? unit % P.splits : 0;
     Sequence s;
-    if (!find_sequence(P, kRows, P.tiles - 1 - (SPLIT ? unit / P.splits : unit), lane, s)) return; // the whole workgroup
+    if (!SPLIT && P.by_length ? !find_by_length(P, kRows, unit, lane, s) : !find_sequence(P, kRows, P.tiles - 1 - (SPLIT ? unit / P.splits : unit), lane, s))
+        return; // the whole workgroup
 
     const int rows = s.len_q * P.group; // of the sequence and kv head (fits: checked on the host)
     const int row = min(s.row0 + wr * 32 + x, rows - 1), token = row / P.group, head = kv * P.group + row % P.group;
@@ -700,6 +739,11 @@ hipError_t launch(PromptParams P, int64_t max_k, int device, int n_cus, hipStrea
     const int64_t wgs = row_tiles(P, 32 * WR) * P.kv_heads;
     P.tiles = (int)(wgs / P.kv_heads);
     P.splits = splits_of<T>(wgs, max_k, KS, n_cus);
+    // Sequences of several tiles on a few workgroups a compute unit: by length (unsplit).  Us by the offsets and so: f32 six causal prompts up to 700 124,
+    // 82; bf16 D = 256 twelve up to 1000 139, 127; D = 64 five up to 2500 81, 76, four not causal up to 1500 42, 40; but where workgroups are many,
+    // the last ones matter less than that those of one sequence find its keys in the L2 (30 up to 1501 of 32 heads 460, 500), and many short
+    // sequences are over too soon (64 up to 100 20, 23.5).
+    P.by_length = P.batch > 1 && P.batch <= 64 && wgs > n_cus && wgs <= 8 * (int64_t)n_cus && P.total_q * P.group >= 4 * 128 * (int64_t)P.batch;
     const int64_t rows = P.total_q * P.heads;
     if (P.splits > 1) {
         void* scratch = nullptr;

@@ -304,6 +304,21 @@ def test_prompt_attention_of_many_sequences(qa, dtype, prompts, heads, kv):
     check_attention(got, q64, k64, v64, starts, starts_k, True, 0.125, dtype)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d,causal", [(64, True), (128, True), (256, True), (64, False), (128, False)])
+def test_prompt_attention_of_long_and_short_sequences(qa, dtype, d, causal):
+    """Long sequences among short and empty ones, some with more keys than tokens and some with fewer: workgroups begin by length."""
+    rng = np.random.default_rng(d)
+    lens, lens_k = [0, 700, 1, 5, 900, 0, 330, 64], [3, 700, 250, 2, 1000, 0, 0, 1]
+    starts, starts_k = np.cumsum([0, *lens]), np.cumsum([0, *lens_k])
+    (q, q64), (k, k64), (v, v64) = (made(rng, n, g, d, dtype=dtype) for n, g in ((starts[-1], 24), (starts_k[-1], 8), (starts_k[-1], 8)))
+    got = qa.prompt_attention(q, k, v, ints(starts), ints(starts_k), causal=causal)
+    check_attention(got, q64, k64, v64, starts, starts_k, causal, d ** -0.5, dtype)
+    room = torch.full((starts[-1] + 600, 24, d), 3.0, dtype=DTYPES[dtype], device="cuda")
+    qa.prompt_attention(q, k, v, ints([2000, 0, 1700, 20, 1500, 1, 2000, 0, 1999]), ints(starts_k), causal=causal, out=room[300:300 + starts[-1]])
+    assert (room[:300] == 3.0).all() and (room[300 + starts[-1]:] == 3.0).all()
+
+
 def test_prompt_attention_without_keys(qa):
     for dtype in DTYPES.values():
         q, none = torch.randn(5, 4, 128, device="cuda").to(dtype), torch.empty(0, 2, 128, device="cuda", dtype=dtype)
