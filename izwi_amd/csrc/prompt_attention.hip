@@ -725,10 +725,14 @@ int64_t row_tiles(const PromptParams& P, int rows) { return P.cu_q ? P.total_q *
 // them: f16 and bf16 from eight tiles on (16 tokens of 16 heads on 8 behind 240: in one part 8.6 us, in two 10.1; behind 500: in two
 // parts 12.3, in four 11.0; behind 1000 15, 11.9, in eight 10.5), f32, whose tiles take three times as long, from four (behind 240: in one
 // part 30.6 us, in two 21.0, in four 14.8).
+// A causal f32 prompt in the larger workgroups: their lengths differ, so that one or two parts each are better rounded up to half as many again as
+// there are compute units (16 heads on 8: D = 128 800 tokens in two parts 60, in four 48; 1000 72, in three 57; D = 256 400 47, in four 45; 600 in
+// one part 86, in three 57; 900 128, in two 93; 1200 165, 146; 2048 299, 330; not causal 600 88, in two 109; six causal ones of 128 26, 42).
 template <typename T>
-int splits_of(int64_t wgs, int64_t max_k, int step, int n_cus) {
+int splits_of(int64_t wgs, int64_t max_k, int step, int n_cus, bool unequal = false) {
     const int64_t tiles = (max_k + step - 1) / step;
-    return tiles < (sizeof(T) == 4 ? 4 : 8) ? 1 : (int)std::max<int64_t>(1, std::min(n_cus / wgs, tiles / 2));
+    const int64_t parts = sizeof(T) == 4 && unequal && n_cus / wgs <= 2 ? (6 * n_cus / wgs + 3) / 4 : n_cus / wgs;
+    return tiles < (sizeof(T) == 4 ? 4 : 8) ? 1 : (int)std::max<int64_t>(1, std::min(parts, tiles / 2));
 }
 
 template <typename T, int D, int WR, int WZ, int DZ, int KT>
@@ -738,7 +742,7 @@ hipError_t launch(PromptParams P, int64_t max_k, int device, int n_cus, hipStrea
     static_assert(lds <= 160 * 1024);
     const int64_t wgs = row_tiles(P, 32 * WR) * P.kv_heads;
     P.tiles = (int)(wgs / P.kv_heads);
-    P.splits = splits_of<T>(wgs, max_k, KS, n_cus);
+    P.splits = splits_of<T>(wgs, max_k, KS, n_cus, P.causal && WZ == 1 && P.batch == 1);
     // Sequences of several tiles on a few workgroups a compute unit: by length (unsplit).  Us by the offsets and so: f32 six causal prompts up to 700 124,
     // 82; bf16 D = 256 twelve up to 1000 139, 127; D = 64 five up to 2500 81, 76, four not causal up to 1500 42, 40; but where workgroups are many,
     // the last ones matter less than that those of one sequence find its keys in the L2 (30 up to 1501 of 32 heads 460, 500), and many short

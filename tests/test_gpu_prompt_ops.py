@@ -319,6 +319,14 @@ def test_prompt_attention_of_long_and_short_sequences(qa, dtype, d, causal):
     assert (room[:300] == 3.0).all() and (room[300 + starts[-1]:] == 3.0).all()
 
 
+@pytest.mark.parametrize("n,d", [(520, 256), (700, 128)])
+def test_prompt_attention_of_one_prompt_in_parts(qa, n, d):
+    """A causal f32 prompt whose tiles of rows are nearly as many as the compute units: tiles of unequal length in several parts."""
+    rng = np.random.default_rng(n)
+    (q, q64), (k, k64), (v, v64) = (made(rng, n, 16, d) for _ in range(3))
+    check_attention(qa.prompt_attention(q, k, v), q64, k64, v64, [0, n], [0, n], True, d ** -0.5, "f32")
+
+
 def test_prompt_attention_without_keys(qa):
     for dtype in DTYPES.values():
         q, none = torch.randn(5, 4, 128, device="cuda").to(dtype), torch.empty(0, 2, 128, device="cuda", dtype=dtype)
