@@ -3,6 +3,10 @@
 //
 // Angles are taken in 64 bits and reduced to a fraction of a turn there: position 10^6 in 32 bits would be off by 0.03.  Cosine and
 // sine are then 32-bit functions of that fraction.
+//
+// Bound by memory where there is much to do: 16384 tokens of 32 and 8 heads of 128, f32, 126 us, 5.3 TB/s (a copy of 1 GiB reaches 4.9; part of
+// this fits the last-level cache); 2051 tokens bf16 with the norm, parts of q|k|v rows, 12.5 us, 3.4 TB/s.  By the launch and one chain
+// of loads, angles (f64) and stores where there is little: one token 3.1 us, 777 of 24 heads of 64 3.4.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -80,7 +84,8 @@ __global__ __launch_bounds__(256) void rope_any_kernel(RopeParams P) {
 
 // The same in pieces of 16 bytes: a lane has two pieces of a head, those whose elements turn against each other (halves) or two neighbours
 // (interleaved, and what does not turn), LP lanes a head, 64 / LP heads at once; a wave has `passes` such sets of one token's heads, requests
-// kAtOnce of them ahead of working out the angles, and every angle once.
+// kAtOnce of them ahead of working out the angles, and every angle once.  (Pairs of single elements, a workgroup a token: 2051 tokens 32 us
+// instead of 12.5.)
 constexpr int kAtOnce = 4, kPiecePairs = 256;
 
 template <typename T, int V>

@@ -351,6 +351,38 @@ inline void beam_select(const float* logits, int64_t prompts, int64_t beams, int
     check(izwi_decode_beam_select_f32(logits, prompts, beams, vocab, scores, finished, eos_token, tokens, parents, scores_out, finished_out,
                                       lineage, lineage_capacity, lens, lineage_out, stream));
 }
+
+// Whole prompts, packed one behind the other (izwi_decode_ops.h), device pointers.  Frequencies (rotary_dim / 2 of them, on the host) of a model's
+// rotary positions; `scaling` is one of IZWI_ROPE_*.  Returns the factor on cosine and sine.
+inline double rope_frequencies(int scaling, int64_t rotary_dim, double base, double factor, double original_len, double low, double high,
+                               std::vector<double>& frequencies) {
+    double attention_factor = 1.0;
+    frequencies.assign(rotary_dim > 0 ? (size_t)rotary_dim / 2 : 0, 0.0);
+    check(izwi_rope_frequencies(scaling, rotary_dim, base, factor, original_len, low, high, frequencies.data(), &attention_factor));
+    return attention_factor;
+}
+// q `[tokens, q_heads, head_dim]` and k, rotated to their tokens' positions (in place where the outputs are the inputs); qk_weight: normed first.
+inline void rope_positions(const float* q, int64_t q_stride, const float* k, int64_t k_stride, const int32_t* positions, const double* frequencies,
+                           float attention_factor, int64_t tokens, int64_t q_heads, int64_t k_heads, int64_t head_dim, int64_t rotary_dim,
+                           bool interleaved, const float* qk_weight, float eps, float* q_out, int64_t q_out_stride, float* k_out, int64_t k_out_stride,
+                           void* stream = nullptr) {
+    check(izwi_rope_positions_f32(q, q_stride, k, k_stride, positions, frequencies, attention_factor, tokens, q_heads, k_heads, head_dim, rotary_dim,
+                                  interleaved, qk_weight, eps, q_out, q_out_stride, k_out, k_out_stride, stream));
+}
+// Attention of the `batch` sequences that the offsets bound (both NULL: one of everything).
+inline void prompt_attention(const float* q, int64_t q_stride, const float* k, int64_t k_stride, const float* v, int64_t v_stride, const int32_t* cu_q,
+                             const int32_t* cu_k, int64_t batch, int64_t total_q, int64_t total_k, int64_t max_k, int64_t num_heads, int64_t num_kv_heads,
+                             int64_t head_dim, bool causal, float scale, float* out, int64_t out_stride, void* stream = nullptr) {
+    check(izwi_qmm_prompt_attention_f32(q, q_stride, k, k_stride, v, v_stride, cu_q, cu_k, batch, total_q, total_k, max_k, num_heads, num_kv_heads,
+                                        head_dim, causal, scale, out, out_stride, stream));
+}
+// The experts of each token by scored routing (izwi_qmm.h), what izwi_moe_sort and the experts' products take.
+inline void moe_route_scored(const float* logits, int64_t stride, const float* bias, int64_t tokens, int32_t n_experts, int32_t top_k, int32_t scoring,
+                             int32_t groups, int32_t top_groups, int32_t group_best, bool renormalize, float scale, int32_t* ids, float* weights,
+                             void* stream = nullptr) {
+    check(izwi_moe_route_scored_f32(logits, stride, bias, tokens, n_experts, top_k, scoring, groups, top_groups, group_best, renormalize, scale, ids,
+                                    weights, stream));
+}
 } // namespace kernels
 
 // `Qwen3Projection` (quantized arm): the op always receives f32 activations and
