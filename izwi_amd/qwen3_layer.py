@@ -17,7 +17,7 @@ from __future__ import annotations
 
 import torch
 
-from .capi import ERR_INVALID, check, lib
+from .capi import ERR_INVALID, QmmError, check, lib
 from .decode_ops import (decode_attention_step, qk_norm_rope_append, try_fused_decode_gqa_attention_with_kv_len, try_fused_qk_rms_norm,
                          try_fused_rms_norm, try_fused_rope_pair_bshd)
 from .prompt_ops import RotaryEmbedding, prompt_attention, rope_positions
@@ -110,9 +110,16 @@ class SparseMlp:
     experts' products."""
 
     def __init__(self, router: QMatMul, experts: MoeExperts, top_k: int, **routing):
+        n, hidden = router.qtensor.dims2()
+        if (n, hidden) != (experts.gate.shape()[0], experts.gate.shape()[-1]) or len(experts.gate.shape()) != 3:
+            raise QmmError(ERR_INVALID, f"SparseMlp: a router of {n} experts on {hidden} for experts of {experts.gate.shape()}")
         self.router, self.experts, self.top_k, self.routing = router, experts, top_k, routing
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if x.dim() != 2 or x.dtype is not torch.float32 or x.shape[1] != self.router.qtensor.dims2()[1]:
+            raise QmmError(ERR_INVALID, f"SparseMlp: x [tokens, {self.router.qtensor.dims2()[1]}] of f32 expected")
+        if x.shape[0] == 0:
+            return torch.empty_like(x)
         logits = self.router.forward(x)
         ids, weights = moe_route_scored(logits, self.top_k, **self.routing)
         perm, offsets = moe_sort(ids, logits.shape[1])
@@ -136,7 +143,12 @@ class Qwen3PromptLayer:
     def forward(self, x: torch.Tensor, positions: torch.Tensor, starts: torch.Tensor | None = None):
         """x [tokens, hidden] f32, positions int32 [tokens], starts int32 [prompts + 1] (None: one prompt) -> (the layer's output [tokens,
         hidden], keys, values [tokens, kv_heads, head_dim], which belong into the caches of the decode step)."""
+        if x.dim() != 2 or x.dtype is not torch.float32 or x.shape[1] != self.w_in.numel():
+            raise QmmError(ERR_INVALID, f"Qwen3PromptLayer: x [tokens, {self.w_in.numel()}] of f32 expected")
         tokens, d = x.shape[0], self.d
+        if tokens == 0:
+            none = x.new_empty(0, self.kv_heads, d)
+            return torch.empty_like(x), none, none.clone()
         q, k, v = forward_group(self.qkv, x, norm_weight=self.w_in, eps=self.eps)
         q, k, v = q.view(tokens, self.heads, d), k.view(tokens, self.kv_heads, d), v.view(tokens, self.kv_heads, d)
         rope_positions(q, k, positions, self.rotary, qk_weight=self.qk_w, eps=self.eps, out=(q, k))

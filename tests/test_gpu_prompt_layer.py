@@ -125,3 +125,37 @@ def test_sparse_mlp_is_its_experts(qa, oracle, routing):
             g, u = one["gate"][e].forward(row), one["up"][e].forward(row)
             want[t] += w * one["down"][e].forward((torch.nn.functional.silu(g) * u).contiguous()).double().cpu().numpy()[0]
     assert np.abs(got - want).max() <= 2e-3 * np.abs(want).max()
+
+
+def test_prompt_layer_of_experts_and_its_refusals(qa, oracle):
+    """A layer with experts: no token, one token, several prompts as alone; a router of another size and activations of another width are refused.
+    (Up to two rows have their norm folded into the products, so the prompts are compared among themselves: 5 and 3 tokens in one call and in two.
+    What a row meets is the same then, up to the order of f32 sums where kernels go by the number of rows: 2e-5.)"""
+    from izwi_amd.qwen3_layer import Qwen3PromptLayer, SparseMlp
+    n, hidden, inter, heads, kv_heads, d = 8, 512, 256, 8, 2, 64
+    mm, w_in, w_post, qk_w = parts(qa, oracle, hidden, heads, kv_heads, d, inter)
+
+    def stack(seed, rows, cols, quant=12):
+        return qa.QTensor.from_blocks(qa.GgmlDType(quant), oracle.quantize(quant, oracle.randn(seed, (n * rows, cols), std=0.05)), (n, rows, cols))
+
+    experts = qa.MoeExperts(stack(60, inter, hidden), stack(61, inter, hidden), stack(62, hidden, inter))
+    router = lambda rows: qa.QMatMul.from_qtensor(qa.QTensor.from_blocks(qa.GgmlDType.Q8_0, oracle.quantize(8, oracle.randn(63, (rows, hidden), std=0.06)), (rows, hidden)))  # noqa: E731
+    for rows in (4, 16):
+        with pytest.raises(qa.QmmError):
+            SparseMlp(router(rows), experts, 2)
+    layer = Qwen3PromptLayer(w_in, w_post, mm["q"], mm["k"], mm["v"], qk_w, mm["o"], SparseMlp(router(n), experts, 2), heads, kv_heads, d, qa.RotaryEmbedding(d), 1e-6)
+    x = torch.from_numpy(oracle.randn(64, (8, hidden))).cuda()
+    for bad in (x[:, :256].contiguous(), x.half(), x[0]):
+        with pytest.raises(qa.QmmError):
+            layer.forward(bad, ints(range(8)))
+    with pytest.raises(qa.QmmError):
+        layer.sparse.forward(x[:, :256].contiguous())
+    y, k, v = layer.forward(x[:0], ints([]))
+    assert y.shape == (0, hidden) and k.shape == v.shape == (0, kv_heads, d)
+    y, k, v = layer.forward(x[:1], ints([0]))
+    assert y.shape == (1, hidden) and torch.isfinite(y).all()
+    y, k, v = layer.forward(x, ints([0, 1, 2, 3, 4, 0, 1, 2]), ints([0, 5, 8]))
+    for a, b in ((0, 5), (5, 8)):
+        one = layer.forward(x[a:b].contiguous(), ints(range(b - a)))
+        for got, want in zip((y, k, v), one):
+            assert (got[a:b] - want).abs().max() <= 2e-5 * want.abs().max()
