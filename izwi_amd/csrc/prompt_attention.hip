@@ -742,6 +742,22 @@ int splits_of(int64_t wgs, int64_t max_k, int step, int n_cus, bool unequal = fa
     return tiles < (sizeof(T) == 4 ? 4 : 8) ? 1 : (int)std::max<int64_t>(1, std::min(parts, tiles / 2));
 }
 
+// f32 in the larger workgroups, one to a compute unit, of about equal lengths, that come in one part: in two to eight where a last turn that is nearly
+// empty costs more than the join, by an estimate in us from what a tile (heads of 128 3.3, of 256 4.2) and a part's sums take.  16 heads on 8,
+// not causal, us in one part and so: D = 128 1100 tokens 121, 101; 1400 151, 141; 2500 519, 383; 3500 720, 706; ten sequences of up to 128 behind 500
+// 73, 48; D = 256 1200 329, 256; 17 of up to 28 behind 13484 1850, 1045; 2048, whose turns are full, 547 (in three parts 621).
+int parts_by_turns(int64_t likely, int64_t most, int64_t tiles, int64_t rows, int d, int n_cus) { // (workgroups that have rows: the device knows)
+    const double tile = d == 256 ? 4.2 : 3.3, join = (double)rows * d * 8 / 4e6; // of a part
+    const auto turns = [&](int64_t wgs) { return (double)((wgs + n_cus - 1) / n_cus); };
+    int best = 1;
+    double least = 0.0;
+    for (int parts = 1; parts <= std::max<int64_t>(1, std::min<int64_t>(8, tiles / 2)) && parts * rows * d * 4 <= 1 << 28; parts++) { // (256 MiB of scratch)
+        const double t = (2 * turns(likely * parts) + turns(most * parts)) / 3 * (double)((tiles + parts - 1) / parts) * tile + (parts > 1 ? 4.0 + join * parts : 0.0);
+        if (parts == 1 || t < least) least = t, best = parts;
+    }
+    return best;
+}
+
 template <typename T, int D, int WR, int WZ, int DZ, int KT>
 hipError_t launch(PromptParams P, int64_t max_k, int device, int n_cus, hipStream_t stream) {
     constexpr int N = Elem<T>::N, KS = KT * WZ;
@@ -750,11 +766,16 @@ hipError_t launch(PromptParams P, int64_t max_k, int device, int n_cus, hipStrea
     const int64_t wgs = row_tiles(P, 32 * WR) * P.kv_heads;
     P.tiles = (int)(wgs / P.kv_heads);
     P.splits = splits_of<T>(wgs, max_k, KS, n_cus, P.causal && WZ == 1 && P.batch == 1);
+    if constexpr (sizeof(T) == 4 && D >= 128 && WZ == 1)
+        if (P.splits == 1 && P.batch <= 256 && (!P.causal || P.total_k >= 4 * P.total_q)) { // (the join looks through the offsets, 64 at a time)
+            const int64_t likely = ((P.total_q * P.group + 32 * WR - 1) / (32 * WR) + (P.batch - 1) / 2) * P.kv_heads; // (the bound has a tile more a sequence)
+            P.splits = parts_by_turns(likely, P.batch > 1 ? wgs : likely, (max_k + KS - 1) / KS, P.total_q * P.heads, D, n_cus);
+        }
     // Sequences of several tiles on a few workgroups a compute unit: by length (unsplit).  Us by the offsets and so: f32 six causal prompts up to 700 124,
     // 82; bf16 D = 256 twelve up to 1000 139, 127; D = 64 five up to 2500 81, 76, four not causal up to 1500 42, 40; but where workgroups are many,
     // the last ones matter less than that those of one sequence find its keys in the L2 (30 up to 1501 of 32 heads 460, 500), and many short
     // sequences are over too soon (64 up to 100 20, 23.5).
-    P.by_length = P.batch > 1 && P.batch <= 64 && wgs > n_cus && wgs <= 8 * (int64_t)n_cus && P.total_q * P.group >= 4 * 128 * (int64_t)P.batch;
+    P.by_length = P.splits == 1 && P.batch > 1 && P.batch <= 64 && wgs > n_cus && wgs <= 8 * (int64_t)n_cus && P.total_q * P.group >= 4 * 128 * (int64_t)P.batch;
     const int64_t rows = P.total_q * P.heads;
     if (P.splits > 1) {
         void* scratch = nullptr;

@@ -327,6 +327,17 @@ def test_prompt_attention_of_one_prompt_in_parts(qa, n, d):
     check_attention(qa.prompt_attention(q, k, v), q64, k64, v64, [0, n], [0, n], True, d ** -0.5, "f32")
 
 
+@pytest.mark.parametrize("d,lens,past,heads,kv", [(256, [28 - b % 9 for b in range(17)], 1000, 16, 4), (128, [128 - 7 * b for b in range(10)], 500, 8, 8)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_prompt_attention_of_chunks_in_parts(qa, d, lens, past, heads, kv, causal):
+    """f32 sequences of few rows on many keys each, as many workgroups as would leave a last turn nearly empty: in parts."""
+    rng = np.random.default_rng(d)
+    starts, starts_k = np.cumsum([0, *lens]), np.cumsum([0, *(n + past - 11 * b for b, n in enumerate(lens))])
+    (q, q64), (k, k64), (v, v64) = (made(rng, n, g, d) for n, g in ((starts[-1], heads), (starts_k[-1], kv), (starts_k[-1], kv)))
+    got = qa.prompt_attention(q, k, v, ints(starts), ints(starts_k), causal=causal, max_len_k=max(lens) + past)
+    check_attention(got, q64, k64, v64, starts, starts_k, causal, d ** -0.5, "f32")
+
+
 def test_prompt_attention_without_keys(qa):
     for dtype in DTYPES.values():
         q, none = torch.randn(5, 4, 128, device="cuda").to(dtype), torch.empty(0, 2, 128, device="cuda", dtype=dtype)
