@@ -60,34 +60,42 @@ struct PromptParams {
 };
 
 // ---- the element types ---------------------------------------------------------------------------------------------
-// N: bf16 / f16 numbers a value goes as; Frag: 8 values of a matrix-core operand; kLift: weights stand 2^kLift higher than they are
-// (an f16 has its full 11 bits from 2^-14 on: under a lift of 2^7, from 2^-21 of the row's reference on)
+// N: bf16 / f16 numbers that a query, key or value goes as; NW: those that a weight goes as; kLift: weights stand 2^kLift higher than they are
+// (an f16 has its full 11 bits from 2^-14 on: under a lift of 2^7, from 2^-21 of the row's reference on).  f16 and bf16 weights go as two
+// numbers, rounded and what that left: one alone is off by 2^-12, 2^-9 of the weight, which the sum of the weights does not share, so that
+// results were as far off by it as by their own rounding (against 64 bits bf16 2.1e-3 of the result where the rounding alone leaves 1.6e-3,
+// f16 2.7e-4, 2.1e-4), and the mean of equal values was another value.
 template <typename T>
 struct Elem;
 template <>
 struct Elem<bf16_t> {
-    static constexpr int N = 1, kLift = 0;
+    static constexpr int N = 1, NW = 2, kLift = 0;
     static __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     }
     static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_bf16(a, b); }
+    static __device__ __forceinline__ uint32_t rest(float a, float b, uint32_t of) { // what pack left of them (to 2^-18)
+        return pack_bf16(a - __uint_as_float(of << 16), b - __uint_as_float(of & 0xffff0000u));
+    }
     static constexpr uint32_t kExponent = 0x7f807f80u;
 };
 template <>
 struct Elem<f16_t> {
-    static constexpr int N = 1, kLift = 7;
+    static constexpr int N = 1, NW = 2, kLift = 7;
     static __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
     }
-    static __device__ __forceinline__ uint32_t pack(float a, float b) {
-        typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-        return __builtin_bit_cast(uint32_t, f16x2{(_Float16)a, (_Float16)b});
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    static __device__ __forceinline__ uint32_t pack(float a, float b) { return __builtin_bit_cast(uint32_t, f16x2{(_Float16)a, (_Float16)b}); }
+    static __device__ __forceinline__ uint32_t rest(float a, float b, uint32_t of) { // (an fma by 1 takes the f16 as it is, without a conversion)
+        const f16x2 h = __builtin_bit_cast(f16x2, of);
+        return pack(__builtin_fmaf((float)h[0], -1.0f, a), __builtin_fmaf((float)h[1], -1.0f, b));
     }
     static constexpr uint32_t kExponent = 0x7c007c00u;
 };
 template <>
 struct Elem<float> {
-    static constexpr int N = 3, kLift = 0;
+    static constexpr int N = 3, NW = 3, kLift = 0;
     static __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) { return Elem<bf16_t>::mma(a, b, c); }
     static constexpr uint32_t kExponent = 0x7f807f80u;
 };
@@ -114,13 +122,13 @@ __device__ __forceinline__ void split8(const float (&v)[8], u32x4 (&to)[3]) {
     }
 }
 
-// Of N numbers a value the products whose weight is 2^-16 or more, the small ones first: product i is that of number left(i) of one and right(i) of
+// Of NL numbers by NR the products whose weight is 2^-16 or more, the small ones first: product i is that of number left(i) of one and right(i) of
 // the other.  Products go round between results, so that none adds to what the one before it wrote.
-template <int N>
+template <int NL, int NR = NL>
 struct Products {
-    static constexpr int kCount = N == 1 ? 1 : 6;
-    static constexpr int left(int i) { return N == 1 ? 0 : (i < 3 ? 2 - i : i < 5 ? 4 - i : 0); }
-    static constexpr int right(int i) { return N == 1 ? 0 : (i < 3 ? i : i < 5 ? i - 3 : 0); }
+    static constexpr int kCount = NL == 1 ? NR : 6;
+    static constexpr int left(int i) { return NL == 1 ? 0 : (i < 3 ? 2 - i : i < 5 ? 4 - i : 0); }
+    static constexpr int right(int i) { return NL == 1 ? NR - 1 - i : (i < 3 ? i : i < 5 ? i - 3 : 0); }
 };
 
 // ---- a tile of keys or values in LDS -------------------------------------------------------------------------------
@@ -218,7 +226,7 @@ constexpr float kSlack = 8.0f; // a reference stands until a score passes it by 
 template <typename T, int D, int WR, int WZ, int DZ, int KT, bool SPLIT>
 __global__ __launch_bounds__(64 * WR * WZ * DZ, Elem<T>::N == 1 || D == 64 ? 2 : 1) void prompt_attention_kernel(PromptParams P) {
     using E = Elem<T>;
-    constexpr int N = E::N, W = WR * WZ * DZ, kRows = 32 * WR, KS = KT * WZ, DW = D / DZ, KK = DW / 16, PT = KT / 32, DT = DW / 32;
+    constexpr int N = E::N, NW = E::NW, W = WR * WZ * DZ, kRows = 32 * WR, KS = KT * WZ, DW = D / DZ, KK = DW / 16, PT = KT / 32, DT = DW / 32;
     constexpr bool kDirect = N == 1;          // keys and values go straight from memory into LDS
     constexpr int kPlane = KS * D * 2;        // bytes of a tile of 16-bit numbers
     constexpr int kTile = 2 * N * kPlane;     // keys, then values
@@ -446,12 +454,16 @@ __global__ __launch_bounds__(64 * WR * WZ * DZ, Elem<T>::N == 1 || D == 64 ? 2 :
         // sixteen positions at a time: the lane's eight are 4 h + 0..3 and 8 + 4 h + 0..3 of them
 #pragma unroll
         for (int t = 0; t < KT / 16; t++) {
-            u32x4 w[N];
+            u32x4 w[NW];
             float v[8];
 #pragma unroll
             for (int i = 0; i < 8; i++) v[i] = p[t >> 1][8 * (t & 1) + i];
-            if constexpr (N == 1) w[0] = u32x4{E::pack(v[0], v[1]), E::pack(v[2], v[3]), E::pack(v[4], v[5]), E::pack(v[6], v[7])};
-            else split8(v, w);
+            if constexpr (N == 1) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) w[0][i] = E::pack(v[2 * i], v[2 * i + 1]), w[1][i] = E::rest(v[2 * i], v[2 * i + 1], w[0][i]);
+            } else {
+                split8(v, w);
+            }
             u32x4 a[DT][N];
 #pragma unroll
             for (int d = 0; d < DT; d++)
@@ -463,18 +475,18 @@ __global__ __launch_bounds__(64 * WR * WZ * DZ, Elem<T>::N == 1 || D == 64 ? 2 :
                     a[d][n] = u32x4{lo[0], lo[1], hi[0], hi[1]};
                 }
 #pragma unroll
-            for (int i = 0; i < Products<N>::kCount; i++)
+            for (int i = 0; i < Products<N, NW>::kCount; i++)
 #pragma unroll
-                for (int d = 0; d < DT; d++) o[d] = E::mma(a[d][Products<N>::left(i)], w[Products<N>::right(i)], o[d]);
+                for (int d = 0; d < DT; d++) o[d] = E::mma(a[d][Products<N, NW>::left(i)], w[Products<N, NW>::right(i)], o[d]);
         }
         if constexpr (N == 1) { // the next sixteen positions' operands beside these
             __builtin_amdgcn_sched_group_barrier(0x100, 2 * DT, 0);
 #pragma unroll
             for (int t = 0; t < KT / 16; t++)
 #pragma unroll
-                for (int d = 0; d < DT; d++) {
+                for (int d = 0; d < NW * DT; d++) {
                     __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                    if (t + 1 < KT / 16) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+                    if (t + 1 < KT / 16) __builtin_amdgcn_sched_group_barrier(0x100, 2 / NW, 0);
                 }
         }
     };
@@ -498,18 +510,32 @@ __global__ __launch_bounds__(64 * WR * WZ * DZ, Elem<T>::N == 1 || D == 64 ? 2 :
         }
         return here;
     };
-    // A value that is no number must not reach the rows that do not see it, and a weight of zero would not keep it out.  Results that hold one
-    // are worked out once more, with care: the rows that see such a value get it by itself, and the tile goes on with a zero in its
-    // place.  (A look at the values of every tile that some row does not see all of took 1200 of the 11600 cycles of 37 bf16 tokens.)
+    // A value that is no number must not reach the rows that do not see it, and a weight of zero would not keep it out; nor would what is left of a
+    // weight, zero or below it, leave an infinity that a row does see what it is.  Results that hold one are worked out once more, with
+    // care: the rows that see such a value get it by itself, and the tile goes on with a zero in its place.  (A look at the values of every tile
+    // that some row does not see all of took 1200 of the 11600 cycles of 37 bf16 tokens.)
     for (bool care = false;;) {
         int tile = first;
         if constexpr (!kDouble) // every row sees all of these
-            for (const int whole = min(end, fewest / KS); tile < whole; tile++) weigh(std::false_type{}, std::false_type{}, arrive(tile), 0);
+            for (const int whole = care ? first : min(end, fewest / KS); tile < whole; tile++) weigh(std::false_type{}, std::false_type{}, arrive(tile), 0);
         for (; tile < end; tile++) {
             uint8_t* const here = arrive(tile);
             const int p0 = tile * KS;
-            if (care && p0 + KS > fewest) {
-                constexpr uint32_t kLow = E::kExponent & 0xffffu, kHigh = E::kExponent & 0xffff0000u;
+            constexpr uint32_t kLow = E::kExponent & 0xffffu, kHigh = E::kExponent & 0xffff0000u;
+            constexpr int kPieces = N * kPlane / 16 / (64 * W);
+            u32x4* const values = reinterpret_cast<u32x4*>(here + N * kPlane) + threadIdx.x;
+            if (care) { // is there one in this tile?  (What the word held before differs from `tile + 2`; the barrier of the next tile is behind its reads.)
+                bool odd = false;
+#pragma unroll 1
+                for (int i = 0; i < kPieces; i++) {
+                    const u32x4 v = values[i * 64 * W];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) odd |= (v[j] & kLow) == kLow || (v[j] & kHigh) == kHigh;
+                }
+                if (__any(odd) && lane == 0) *odd_values = tile + 2;
+                __syncthreads();
+            }
+            if (care && *odd_values == (uint32_t)tile + 2) {
 #pragma unroll 1
                 for (int j = wz * KT; j < min((wz + 1) * KT, s.len_k - p0); j++) {
                     const bool sees = p0 + j <= limit;
@@ -526,9 +552,8 @@ __global__ __launch_bounds__(64 * WR * WZ * DZ, Elem<T>::N == 1 || D == 64 ? 2 :
                             }
                 }
                 __syncthreads();
-                u32x4* const values = reinterpret_cast<u32x4*>(here + N * kPlane) + threadIdx.x;
 #pragma unroll 1
-                for (int i = 0; i < N * kPlane / 16 / (64 * W); i++) {
+                for (int i = 0; i < kPieces; i++) {
                     u32x4 v = values[i * 64 * W];
 #pragma unroll
                     for (int j = 0; j < 4; j++) v[j] &= ((v[j] & kLow) == kLow ? 0u : 0xffffu) | ((v[j] & kHigh) == kHigh ? 0u : 0xffff0000u);
@@ -539,7 +564,7 @@ __global__ __launch_bounds__(64 * WR * WZ * DZ, Elem<T>::N == 1 || D == 64 ? 2 :
             if (kDouble && tile + 1 < end) weigh(std::true_type{}, std::integral_constant<bool, kDouble>{}, here, p0, smem + (tile + 1 - first & 1) * kTile, tile + 2);
             else weigh(std::true_type{}, std::false_type{}, here, p0 + wz * KT);
         }
-        if (care || end * KS <= fewest) break;
+        if (care) break;
         float zero = 0.0f; // NaN where a result is no number
 #pragma unroll
         for (int d = 0; d < DT; d++)
