@@ -238,20 +238,20 @@ int izwi_rope_frequencies(int scaling, int64_t rotary_dim, double base, double f
  * `[tokens, q_heads, head_dim]`, k `[tokens, k_heads, head_dim]`, strides the elements from one token to the next (heads contiguous;
  * a number of heads may be 0); positions `[tokens]`, any int32; frequencies `[rotary_dim / 2]` (device), radians a position.  Pairs
  * are (i, rotary_dim / 2 + i), or with `interleaved` = 1 (2 i, 2 i + 1): (a, b) becomes (a c - b s, a s + b c), c and s being
- * attention_factor times cosine and sine of position * frequency, which is worked out in 64 bits.  qk_weight `[2 * head_dim]` (NULL:
+ * attention_factor times cosine and sine of position * frequency, worked out in 64 bits and rounded once.  qk_weight `[2 * head_dim]` (NULL:
  * none): first every head is normed as by izwi_qk_rms_norm, x * rsqrt(mean(x^2) + eps) * weight, without a rounding in between.
  * head_dim even, at most 1024.  An output may be its own input and shares no other memory (rows of equal stride may lie between each
  * other, as parts of a q|k|v row do). */
 int izwi_rope_positions_f32(const float* q, int64_t q_stride, const float* k, int64_t k_stride, const int32_t* positions,
-                            const double* frequencies, float attention_factor, int64_t tokens, int64_t q_heads, int64_t k_heads,
+                            const double* frequencies, double attention_factor, int64_t tokens, int64_t q_heads, int64_t k_heads,
                             int64_t head_dim, int64_t rotary_dim, int interleaved, const float* qk_weight, float eps,
                             float* q_out, int64_t q_out_stride, float* k_out, int64_t k_out_stride, void* stream);
 int izwi_rope_positions_f16(const uint16_t* q, int64_t q_stride, const uint16_t* k, int64_t k_stride, const int32_t* positions,
-                            const double* frequencies, float attention_factor, int64_t tokens, int64_t q_heads, int64_t k_heads,
+                            const double* frequencies, double attention_factor, int64_t tokens, int64_t q_heads, int64_t k_heads,
                             int64_t head_dim, int64_t rotary_dim, int interleaved, const uint16_t* qk_weight, float eps,
                             uint16_t* q_out, int64_t q_out_stride, uint16_t* k_out, int64_t k_out_stride, void* stream);
 int izwi_rope_positions_bf16(const uint16_t* q, int64_t q_stride, const uint16_t* k, int64_t k_stride, const int32_t* positions,
-                             const double* frequencies, float attention_factor, int64_t tokens, int64_t q_heads, int64_t k_heads,
+                             const double* frequencies, double attention_factor, int64_t tokens, int64_t q_heads, int64_t k_heads,
                              int64_t head_dim, int64_t rotary_dim, int interleaved, const uint16_t* qk_weight, float eps,
                              uint16_t* q_out, int64_t q_out_stride, uint16_t* k_out, int64_t k_out_stride, void* stream);
 

@@ -117,7 +117,7 @@ PROTOTYPES = {
                                                    C.c_float, _vp, _vp]),
     "izwi_decode_beam_select_f32": (C.c_int, [_vp, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp]),
     "izwi_rope_frequencies": (C.c_int, [C.c_int, _i64] + [C.c_double] * 5 + [_vp, _vp]),
-    **{f"izwi_rope_positions_{t}": (C.c_int, [_vp, _i64, _vp, _i64, _vp, _vp, C.c_float] + [_i64] * 5 + [C.c_int, _vp, C.c_float, _vp, _i64, _vp, _i64, _vp])
+    **{f"izwi_rope_positions_{t}": (C.c_int, [_vp, _i64, _vp, _i64, _vp, _vp, C.c_double] + [_i64] * 5 + [C.c_int, _vp, C.c_float, _vp, _i64, _vp, _i64, _vp])
        for t in ("f32", "f16", "bf16")},
     **{f"izwi_qmm_prompt_attention_{t}": (C.c_int, [_vp, _i64] * 3 + [_vp, _vp] + [_i64] * 7 + [C.c_int, C.c_float, _vp, _i64, _vp])
        for t in ("f32", "f16", "bf16")},

@@ -1,8 +1,9 @@
 // Rotary positions of packed tokens: (a, b) -> (a cos - b sin, a sin + b cos) for the pairs of a head's first rotary_dim elements, angle
 // position * frequency, optionally behind the head's RMSNorm; and the frequencies of models whose context is stretched.
 //
-// Angles are taken in 64 bits and reduced to a fraction of a turn there: position 10^6 in 32 bits would be off by 0.03.  Cosine and
-// sine are then 32-bit functions of that fraction.
+// Angles are taken in 64 bits (position 10^6 in 32 bits would be off by 0.03), reduced by multiples of a quarter turn there, and cosine and sine
+// worked out in 64 bits, too: times the factor they are rounded to 32 bits once.  (As 32-bit functions of a fraction of a turn in 32 bits
+// they left f32 results 1.4 times as far off.  The f64 instructions are a few more and take no longer.)
 //
 // Bound by memory where there is much to do: 16384 tokens of 32 and 8 heads of 128, f32, 126 us, 5.3 TB/s (a copy of 1 GiB reaches 4.9; part of
 // this fits the last-level cache); 2051 tokens bf16 with the norm, parts of q|k|v rows, 12.5 us, 3.4 TB/s.  By the launch and one chain
@@ -28,18 +29,33 @@ struct RopeParams {
     const int32_t* positions;
     const double* frequencies; // [rotary / 2]
     const void* weight;        // [2 d]: q's, then k's; NULL: no norm
-    float factor, eps;
+    double factor;
+    float eps;
     int64_t tokens;
     int q_heads, heads, d, rotary; // heads: q's and k's
 };
 
 constexpr int kMostPairs = 512;
 
+// Cosine and sine of position * frequency, times the factor.  What is left of the angle, n quarter turns less (pi / 2 as two numbers; the first fma
+// is exact), is at most pi / 4, where the series' next terms are below 2^-36 of the sum.
 __device__ __forceinline__ void turn_of(const RopeParams& P, int position, int pair, float& c, float& s) {
-    double turns = (double)position * (P.frequencies[pair] * 0.15915494309189533577); // 1 / (2 pi)
-    turns -= __builtin_rint(turns);
-    sincospif(2.0f * (float)turns, &s, &c);
-    c *= P.factor, s *= P.factor;
+    const double angle = (double)position * P.frequencies[pair], n = __builtin_rint(angle * 0.63661977236758134308);
+    const double r = __builtin_fma(n, -0x1.1a62633145c07p-54, __builtin_fma(n, -0x1.921fb54442d18p+0, angle)), r2 = r * r;
+    double sine = __builtin_fma(r2, -1.0 / 39916800, 1.0 / 362880);
+    sine = __builtin_fma(sine, r2, -1.0 / 5040);
+    sine = __builtin_fma(sine, r2, 1.0 / 120);
+    sine = __builtin_fma(sine, r2, -1.0 / 6);
+    sine = __builtin_fma(sine * r2, r, r);
+    double cosine = __builtin_fma(r2, 1.0 / 479001600, -1.0 / 3628800);
+    cosine = __builtin_fma(cosine, r2, 1.0 / 40320);
+    cosine = __builtin_fma(cosine, r2, -1.0 / 720);
+    cosine = __builtin_fma(cosine, r2, 1.0 / 24);
+    cosine = __builtin_fma(cosine, r2, -0.5);
+    cosine = __builtin_fma(cosine, r2, 1.0);
+    const int quarter = (int)(n - 4.0 * __builtin_floor(n * 0.25)); // 0 to 3
+    const double x = quarter & 1 ? sine : cosine, y = quarter & 1 ? cosine : sine;
+    c = (float)(((quarter + 1) & 2 ? -x : x) * P.factor), s = (float)((quarter & 2 ? -y : y) * P.factor);
 }
 
 // A workgroup per token (in turn), a wave per head in turn, a lane per pair of elements in turn.
@@ -211,7 +227,7 @@ __global__ __launch_bounds__(256) void rope_pieces_kernel(RopeParams P, int lp, 
     } while (0)
 
 template <typename T>
-int rope_positions_impl(const T* q, int64_t q_stride, const T* k, int64_t k_stride, const int32_t* positions, const double* frequencies, float factor,
+int rope_positions_impl(const T* q, int64_t q_stride, const T* k, int64_t k_stride, const int32_t* positions, const double* frequencies, double factor,
                         int64_t tokens, int64_t q_heads, int64_t k_heads, int64_t d, int64_t rotary, int interleaved, const T* weight, float eps, T* q_out,
                         int64_t q_out_stride, T* k_out, int64_t k_out_stride, void* stream_) {
     constexpr const char* what = "rope_positions";
@@ -222,7 +238,7 @@ int rope_positions_impl(const T* q, int64_t q_stride, const T* k, int64_t k_stri
         return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: rows overlap (strides %lld, %lld, %lld, %lld)", what, (long long)q_stride, (long long)k_stride,
                         (long long)q_out_stride, (long long)k_out_stride);
     if (interleaved != 0 && interleaved != 1) return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: layout %d (0 halves, 1 interleaved)", what, interleaved);
-    if (!std::isfinite(factor) || !(eps >= 0.0f) || !std::isfinite(eps)) return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: factor %g, eps %g", what, (double)factor, (double)eps);
+    if (!std::isfinite((float)factor) || !(eps >= 0.0f) || !std::isfinite(eps)) return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: factor %g, eps %g", what, factor, (double)eps);
     if (tokens > 0x3ffffff || q_stride > 0x3fffffff || k_stride > 0x3fffffff || q_out_stride > 0x3fffffff || k_out_stride > 0x3fffffff)
         return qmm_fail(IZWI_QMM_ERR_UNSUPPORTED, "%s: %lld tokens", what, (long long)tokens);
     if (tokens == 0 || q_heads + k_heads == 0) return IZWI_QMM_OK;
@@ -264,7 +280,7 @@ int rope_positions_impl(const T* q, int64_t q_stride, const T* k, int64_t k_stri
 extern "C" {
 
 #define ROPE_POSITIONS(NAME, C, T)                                                                                                                         \
-    int NAME(const C* q, int64_t q_stride, const C* k, int64_t k_stride, const int32_t* positions, const double* frequencies, float attention_factor,     \
+    int NAME(const C* q, int64_t q_stride, const C* k, int64_t k_stride, const int32_t* positions, const double* frequencies, double attention_factor,    \
              int64_t tokens, int64_t q_heads, int64_t k_heads, int64_t head_dim, int64_t rotary_dim, int interleaved, const C* qk_weight, float eps,       \
              C* q_out, int64_t q_out_stride, C* k_out, int64_t k_out_stride, void* stream) {                                                               \
         return qmm_guarded(#NAME, [&]() -> int {                                                                                                           \

@@ -363,7 +363,7 @@ inline double rope_frequencies(int scaling, int64_t rotary_dim, double base, dou
 }
 // q `[tokens, q_heads, head_dim]` and k, rotated to their tokens' positions (in place where the outputs are the inputs); qk_weight: normed first.
 inline void rope_positions(const float* q, int64_t q_stride, const float* k, int64_t k_stride, const int32_t* positions, const double* frequencies,
-                           float attention_factor, int64_t tokens, int64_t q_heads, int64_t k_heads, int64_t head_dim, int64_t rotary_dim,
+                           double attention_factor, int64_t tokens, int64_t q_heads, int64_t k_heads, int64_t head_dim, int64_t rotary_dim,
                            bool interleaved, const float* qk_weight, float eps, float* q_out, int64_t q_out_stride, float* k_out, int64_t k_out_stride,
                            void* stream = nullptr) {
     check(izwi_rope_positions_f32(q, q_stride, k, k_stride, positions, frequencies, attention_factor, tokens, q_heads, k_heads, head_dim, rotary_dim,

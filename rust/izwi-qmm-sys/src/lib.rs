@@ -311,15 +311,15 @@ extern "C" {
     pub fn izwi_rope_frequencies(scaling: c_int, rotary_dim: i64, base: f64, factor: f64, original_len: f64,
         low: f64, high: f64, frequencies: *mut f64, attention_factor: *mut f64) -> c_int;
     pub fn izwi_rope_positions_f32(q: *const f32, q_stride: i64, k: *const f32, k_stride: i64, positions: *const i32,
-        frequencies: *const f64, attention_factor: f32, tokens: i64, q_heads: i64, k_heads: i64, head_dim: i64,
+        frequencies: *const f64, attention_factor: f64, tokens: i64, q_heads: i64, k_heads: i64, head_dim: i64,
         rotary_dim: i64, interleaved: c_int, qk_weight: *const f32, eps: f32, q_out: *mut f32, q_out_stride: i64,
         k_out: *mut f32, k_out_stride: i64, stream: *mut c_void) -> c_int;
     pub fn izwi_rope_positions_f16(q: *const u16, q_stride: i64, k: *const u16, k_stride: i64, positions: *const i32,
-        frequencies: *const f64, attention_factor: f32, tokens: i64, q_heads: i64, k_heads: i64, head_dim: i64,
+        frequencies: *const f64, attention_factor: f64, tokens: i64, q_heads: i64, k_heads: i64, head_dim: i64,
         rotary_dim: i64, interleaved: c_int, qk_weight: *const u16, eps: f32, q_out: *mut u16, q_out_stride: i64,
         k_out: *mut u16, k_out_stride: i64, stream: *mut c_void) -> c_int;
     pub fn izwi_rope_positions_bf16(q: *const u16, q_stride: i64, k: *const u16, k_stride: i64,
-        positions: *const i32, frequencies: *const f64, attention_factor: f32, tokens: i64, q_heads: i64,
+        positions: *const i32, frequencies: *const f64, attention_factor: f64, tokens: i64, q_heads: i64,
         k_heads: i64, head_dim: i64, rotary_dim: i64, interleaved: c_int, qk_weight: *const u16, eps: f32,
         q_out: *mut u16, q_out_stride: i64, k_out: *mut u16, k_out_stride: i64, stream: *mut c_void) -> c_int;
     pub fn izwi_qmm_prompt_attention_f32(q: *const f32, q_stride: i64, k: *const f32, k_stride: i64, v: *const f32,
