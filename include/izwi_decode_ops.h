@@ -268,8 +268,8 @@ int izwi_rope_positions_bf16(const uint16_t* q, int64_t q_stride, const uint16_t
  * value that element; an infinity in a value makes the element that infinity, or in f32 NaN.
  * The products run on the matrix cores with f32 sums: f16 and bf16 values as they are, weights as two numbers of the type (f16 2^-22,
  * bf16 2^-16 of each); f32 ones as three bf16 numbers each, all 24 bits down to 2^-100.  head_dim 64, 128 or 256; rows begin on 16 bytes; out
- * shares no memory with the inputs.  Uses the library's per-stream scratch (up to 256 MiB) where workgroups have parts of a
- * row's keys. */
+ * shares no memory with the inputs.  Uses the library's per-stream scratch where workgroups have parts of a row's
+ * keys: the call lets it grow to 256 MiB at most (what a stream's scratch was before stays allocated, as everywhere). */
 int izwi_qmm_prompt_attention_f32(const float* q, int64_t q_stride, const float* k, int64_t k_stride, const float* v, int64_t v_stride,
                                   const int32_t* cu_q, const int32_t* cu_k, int64_t batch, int64_t total_q, int64_t total_k,
                                   int64_t max_k, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim, int causal, float scale,

@@ -772,12 +772,14 @@ int splits_of(int64_t wgs, int64_t max_k, int step, int n_cus, bool unequal = fa
 // empty costs more than the join, by an estimate in us from what a tile (heads of 128 3.3, of 256 4.2) and a part's sums take.  16 heads on 8,
 // not causal, us in one part and so: D = 128 1100 tokens 121, 101; 1400 151, 141; 2500 519, 383; 3500 720, 706; ten sequences of up to 128 behind 500
 // 73, 48; D = 256 1200 329, 256; 17 of up to 28 behind 13484 1850, 1045; 2048, whose turns are full, 547 (in three parts 621).
+// As many as leave the stream's buffer within 256 MiB, sums and statistics (it grows to one and a half times what is asked for).
+constexpr int64_t kMostScratch = (1 << 28) / 3 * 2;
 int parts_by_turns(int64_t likely, int64_t most, int64_t tiles, int64_t rows, int d, int n_cus) { // (workgroups that have rows: the device knows)
     const double tile = d == 256 ? 4.2 : 3.3, join = (double)rows * d * 8 / 4e6; // of a part
     const auto turns = [&](int64_t wgs) { return (double)((wgs + n_cus - 1) / n_cus); };
     int best = 1;
     double least = 0.0;
-    for (int parts = 1; parts <= std::max<int64_t>(1, std::min<int64_t>(8, tiles / 2)) && parts * rows * d * 4 <= 1 << 28; parts++) { // (256 MiB of scratch)
+    for (int parts = 1; parts <= std::max<int64_t>(1, std::min<int64_t>(8, tiles / 2)) && parts * rows * (d * 4 + 8) <= kMostScratch; parts++) {
         const double t = (2 * turns(likely * parts) + turns(most * parts)) / 3 * (double)((tiles + parts - 1) / parts) * tile + (parts > 1 ? 4.0 + join * parts : 0.0);
         if (parts == 1 || t < least) least = t, best = parts;
     }
