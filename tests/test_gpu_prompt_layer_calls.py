@@ -1,0 +1,54 @@
+"""GPU tests (pytest -m gpu) of the prompt layer's arguments: what it hands on, leaves alone and refuses."""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def qa():
+    if not torch.cuda.is_available():
+        pytest.fail("no GPU visible: the HIP path cannot run (there is no fallback)")
+    import izwi_amd
+    izwi_amd.lib()
+    torch.cuda.set_device(0)
+    return izwi_amd
+
+
+def ints(values):
+    return torch.tensor([int(v) for v in values], dtype=torch.int32, device="cuda")
+
+
+HIDDEN, HEADS, KV, D, INTER = 512, 8, 2, 64, 1024
+
+
+def arguments(qa, oracle, **shapes):
+    """What a layer of the sizes above is made of, its products of other shapes where they are named."""
+    shapes = {**dict(q=(HEADS * D, HIDDEN), k=(KV * D, HIDDEN), v=(KV * D, HIDDEN), o=(HIDDEN, HEADS * D), gate=(INTER, HIDDEN), up=(INTER, HIDDEN), down=(HIDDEN, INTER)), **shapes}
+    mm = {n: qa.QMatMul.from_qtensor(qa.QTensor.from_blocks(qa.GgmlDType.Q8_0, oracle.quantize(8, oracle.randn(10 + i, s, std=0.03)), s)) for i, (n, s) in enumerate(shapes.items())}
+    dev = lambda seed, n: torch.from_numpy(oracle.randn(seed, (n,), mean=1.0, std=0.1)).cuda()  # noqa: E731
+    return dict(input_layernorm=dev(30, HIDDEN), post_attention_layernorm=dev(31, HIDDEN), q_proj=mm["q"], k_proj=mm["k"], v_proj=mm["v"], qk_norm_weight=dev(32, 2 * D), o_proj=mm["o"],
+                mlp=(mm["gate"], mm["up"], mm["down"]), num_heads=HEADS, num_kv_heads=KV, head_dim=D, rotary=qa.RotaryEmbedding(D))
+
+
+def test_the_longest_prompt_is_handed_on(qa, oracle, monkeypatch):
+    """Four prompts of 100 tokens: the attention hears of 100 keys (or of nothing), and the result is the same up to the order of f32 sums in front of
+    products that quantize (the tolerance of test_gpu_prompt_layer.py)."""
+    from izwi_amd import qwen3_layer
+    heard = []
+
+    def listen(*args, **how):
+        heard.append(how.get("max_len_k"))
+        return attention(*args, **how)
+
+    attention = qwen3_layer.prompt_attention
+    monkeypatch.setattr(qwen3_layer, "prompt_attention", listen)
+    layer = qwen3_layer.Qwen3PromptLayer(**arguments(qa, oracle))
+    x = torch.from_numpy(oracle.randn(40, (400, HIDDEN))).cuda()
+    positions, starts = ints(np.tile(np.arange(100), 4)), ints(range(0, 401, 100))
+    want = layer.forward(x, positions, starts)
+    got = layer.forward(x, positions, starts, max_len=100)
+    assert heard == [None, 100]
+    for a, b in zip(got, want):
+        assert (a - b).abs().max() <= 2e-2 * b.abs().max()
