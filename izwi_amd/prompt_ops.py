@@ -163,7 +163,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: 
     [tokens, heads, head_dim].  Prompt b has tokens starts[b] .. starts[b + 1] - 1 (int32 [prompts + 1] on the GPU; None: one prompt) and keys by
     ``starts_k`` (None: as its tokens).  ``causal``: the last query sees the last key, the one before it one key less, and so on, so that a
     prompt with more keys than tokens is a chunk behind a past.  A query without any key gives zeros; rows that belong to no prompt are not
-    written.  ``max_len_k``: the longest prompt's keys where the caller knows them; only the division of the work goes by it."""
+    written (without ``out`` they hold anything).  ``max_len_k``: the longest prompt's keys where the caller knows them; only the division of the work goes by it."""
     dtype, shape, k_shape, index = q.dtype, q.shape, k.shape, q.get_device()
     fn = _attentions.get(dtype) or _fn(_attentions, "izwi_qmm_prompt_attention", dtype)
     if fn is None or len(shape) != 3 or index < 0:

@@ -143,7 +143,8 @@ class Qwen3PromptLayer:
     def forward(self, x: torch.Tensor, positions: torch.Tensor, starts: torch.Tensor | None = None, max_len: int | None = None):
         """x [tokens, hidden] f32, positions int32 [tokens], starts int32 [prompts + 1] (None: one prompt) -> (the layer's output [tokens,
         hidden], keys, values [tokens, kv_heads, head_dim], which belong into the caches of the decode step).  ``max_len``: the longest
-        prompt's tokens, where the caller knows them (else all tokens count); the attention's division of the work goes by it."""
+        prompt's tokens, where the caller knows them (else all tokens count); the attention's division of the work goes by it.  A token of no
+        prompt, in front of, between or behind them, is one whose attention is zero."""
         if x.dim() != 2 or x.dtype is not torch.float32 or x.shape[1] != self.w_in.numel():
             raise QmmError(ERR_INVALID, f"Qwen3PromptLayer: x [tokens, {self.w_in.numel()}] of f32 expected")
         tokens, d = x.shape[0], self.d
@@ -153,7 +154,8 @@ class Qwen3PromptLayer:
         q, k, v = forward_group(self.qkv, x, norm_weight=self.w_in, eps=self.eps)
         q, k, v = q.view(tokens, self.heads, d), k.view(tokens, self.kv_heads, d), v.view(tokens, self.kv_heads, d)
         rope_positions(q, k, positions, self.rotary, qk_weight=self.qk_w, eps=self.eps, out=(q, k))
-        attn = prompt_attention(q, k, v, starts, max_len_k=max_len)
+        out = None if starts is None else torch.zeros_like(q)  # (rows of no prompt are not written: their attention is zero)
+        attn = prompt_attention(q, k, v, starts, max_len_k=max_len, out=out)
         x = self.o_proj.forward_fused(attn.view(tokens, self.heads * d), residual=x)
         if self.sparse is not None:
             return x + self.sparse.forward(try_fused_rms_norm(x, self.w_post, self.eps)), k, v

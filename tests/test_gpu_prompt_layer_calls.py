@@ -52,3 +52,27 @@ def test_the_longest_prompt_is_handed_on(qa, oracle, monkeypatch):
     assert heard == [None, 100]
     for a, b in zip(got, want):
         assert (a - b).abs().max() <= 2e-2 * b.abs().max()
+
+
+def test_tokens_of_no_prompt_have_no_attention(qa, oracle):
+    """A padded batch: tokens in front of, between and behind the prompts come out as the rest of the layer makes them of their own activations,
+    whatever the memory held that the attention's result stands in; the prompts' own tokens do not notice."""
+    from izwi_amd.qwen3_layer import Qwen3PromptLayer
+    layer = Qwen3PromptLayer(**arguments(qa, oracle))
+    tokens, starts = 90, [5, 45, 70]
+    x = torch.from_numpy(oracle.randn(41, (tokens, HIDDEN))).cuda()
+    positions = ints(range(tokens))
+    outside = torch.ones(tokens, dtype=torch.bool)
+    outside[5:70] = False
+    results = []
+    for poison in (float("nan"), 3e38, 0.0):
+        for n in (tokens * HEADS * D, tokens * HIDDEN, tokens * INTER, tokens * KV * D):  # what the allocator hands out next
+            kept = [torch.full((n,), poison, device="cuda") for _ in range(8)]
+            del kept
+        results.append(layer.forward(x, positions, ints(starts))[0])
+    for got in results:
+        assert torch.isfinite(got).all() and torch.equal(got, results[0])
+    alone = x + 0
+    hidden = layer.gate_up.forward_silu_mul(alone, norm_weight=layer.w_post, eps=layer.eps)
+    want = layer.down_proj.forward_fused(hidden, residual=alone)
+    assert torch.equal(results[0][outside], want[outside])
