@@ -132,6 +132,22 @@ class Qwen3PromptLayer:
     def __init__(self, input_layernorm: torch.Tensor, post_attention_layernorm: torch.Tensor, q_proj: QMatMul, k_proj: QMatMul, v_proj: QMatMul,
                  qk_norm_weight: torch.Tensor, o_proj: QMatMul, mlp, num_heads: int, num_kv_heads: int, head_dim: int, rotary: RotaryEmbedding,
                  rms_norm_eps: float = 1e-6):
+        hidden = input_layernorm.numel()
+        if num_heads <= 0 or num_kv_heads <= 0 or num_heads % num_kv_heads or rotary.head_dim != head_dim:
+            raise QmmError(ERR_INVALID, f"Qwen3PromptLayer: {num_heads} heads of {head_dim} on {num_kv_heads}, rotary positions for heads of {rotary.head_dim}")
+        if post_attention_layernorm.numel() != hidden or qk_norm_weight.numel() != 2 * head_dim:
+            raise QmmError(ERR_INVALID, f"Qwen3PromptLayer: norms of {hidden}, {post_attention_layernorm.numel()} and {qk_norm_weight.numel()} (2 x {head_dim} expected)")
+        q, kv = num_heads * head_dim, num_kv_heads * head_dim
+        parts = [("q_proj", q_proj, (q, hidden)), ("k_proj", k_proj, (kv, hidden)), ("v_proj", v_proj, (kv, hidden)), ("o_proj", o_proj, (hidden, q))]
+        if isinstance(mlp, SparseMlp):
+            if mlp.router.qtensor.dims2()[1] != hidden:
+                raise QmmError(ERR_INVALID, f"Qwen3PromptLayer: experts on {mlp.router.qtensor.dims2()[1]} in a layer of {hidden}")
+        else:
+            inner = mlp[0].qtensor.dims2()[0]
+            parts += [("gate_proj", mlp[0], (inner, hidden)), ("up_proj", mlp[1], (inner, hidden)), ("down_proj", mlp[2], (hidden, inner))]
+        for name, part, shape in parts:
+            if tuple(part.qtensor.dims2()) != shape:
+                raise QmmError(ERR_INVALID, f"Qwen3PromptLayer: {name} is {tuple(part.qtensor.dims2())}, {shape} expected")
         self.w_in, self.w_post, self.qk_w = input_layernorm, post_attention_layernorm, qk_norm_weight
         self.qkv, self.o_proj, self.rotary = (q_proj, k_proj, v_proj), o_proj, rotary
         self.sparse = mlp if isinstance(mlp, SparseMlp) else None

@@ -76,3 +76,17 @@ def test_tokens_of_no_prompt_have_no_attention(qa, oracle):
     hidden = layer.gate_up.forward_silu_mul(alone, norm_weight=layer.w_post, eps=layer.eps)
     want = layer.down_proj.forward_fused(hidden, residual=alone)
     assert torch.equal(results[0][outside], want[outside])
+
+
+def test_parts_that_do_not_fit_are_refused(qa, oracle):
+    """Head numbers that the projections do not have (in any product that comes to the same number of elements, too), norms and products of other sizes."""
+    from izwi_amd.qwen3_layer import Qwen3PromptLayer
+    good = arguments(qa, oracle)
+    Qwen3PromptLayer(**good)
+    ones = lambda n: torch.ones(n, device="cuda")  # noqa: E731
+    for over in (dict(num_heads=4), dict(num_kv_heads=4), dict(num_kv_heads=0), dict(num_heads=9, num_kv_heads=2), dict(num_heads=4, num_kv_heads=1, head_dim=128),
+                 dict(num_heads=4, num_kv_heads=1, head_dim=128, rotary=qa.RotaryEmbedding(128)), dict(rotary=qa.RotaryEmbedding(128)), dict(qk_norm_weight=ones(D)),
+                 dict(post_attention_layernorm=ones(HIDDEN // 2)), dict(input_layernorm=ones(2 * HIDDEN)), dict(k_proj=good["q_proj"]), dict(v_proj=good["q_proj"]),
+                 dict(o_proj=good["k_proj"]), dict(mlp=(good["mlp"][0], good["q_proj"], good["mlp"][2])), dict(mlp=(good["mlp"][0], good["mlp"][1], good["o_proj"]))):
+        with pytest.raises(qa.QmmError):
+            Qwen3PromptLayer(**{**good, **over})
