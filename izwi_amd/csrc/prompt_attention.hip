@@ -896,6 +896,9 @@ int prompt_attention_impl(const T* q, int64_t q_stride, const T* k, int64_t k_st
     const QmmRows to = rows(out, total_q, out_stride, heads);
     if (!qmm_rows_apart(to, rows(q, total_q, q_stride, heads)) || !qmm_rows_apart(to, rows(k, total_k, k_stride, kv_heads)) || !qmm_rows_apart(to, rows(v, total_k, v_stride, kv_heads)))
         return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: out shares memory with q, k or v", what);
+    const int64_t offsets = cu_q ? 1 : 0; // (as one row of out's stride: between two of its rows there may be room)
+    if (!qmm_rows_apart(to, {cu_q, offsets, to.stride, (batch + 1) * 4}) || !qmm_rows_apart(to, {cu_k, offsets, to.stride, (batch + 1) * 4}))
+        return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: out shares memory with the offsets", what);
     if ((total_q * (heads / kv_heads) / 32 + batch) * kv_heads > 0x3fffff)
         return qmm_fail(IZWI_QMM_ERR_UNSUPPORTED, "%s: %lld sequences on %lld kv heads", what, (long long)batch, (long long)kv_heads);
     int device = 0, n_cus = 0;

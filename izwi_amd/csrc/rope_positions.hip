@@ -248,6 +248,10 @@ int rope_positions_impl(const T* q, int64_t q_stride, const T* k, int64_t k_stri
     const auto same = [](const QmmRows& a, const QmmRows& b) { return a.at == b.at && a.stride == b.stride; };
     if ((!same(qi, qo) && !qmm_rows_apart(qi, qo)) || (!same(ki, ko) && !qmm_rows_apart(ki, ko)) || !qmm_rows_apart(qi, ko) || !qmm_rows_apart(ki, qo) || !qmm_rows_apart(qo, ko))
         return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: an output shares memory with another tensor (it may be its own input)", what);
+    for (const QmmRows& to : {qo, ko}) // (one row of the output's stride: between two of its rows there may be room)
+        if (!qmm_rows_apart(to, {positions, 1, to.stride, tokens * 4}) || !qmm_rows_apart(to, {frequencies, 1, to.stride, rotary / 2 * 8}) ||
+            !qmm_rows_apart(to, {weight, weight ? 1 : 0, to.stride, 2 * d * (int64_t)sizeof(T)}))
+            return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: an output shares memory with positions, frequencies or weights", what);
     int device = 0, n_cus = 0;
     if (int rc = qmm_current_device(&device, &n_cus)) return rc;
     RopeParams P{q, k, q_out, k_out, q_stride, k_stride, q_out_stride, k_out_stride, positions, frequencies, weight, factor, eps, tokens, (int)q_heads,
