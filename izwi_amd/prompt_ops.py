@@ -83,7 +83,8 @@ class RopeScaling(NamedTuple):
 
 class RotaryEmbedding:
     """Frequencies of a model's rotary positions, made once: the first ``rotary_dim`` elements of a head (by default all) turn, in pairs
-    (i, rotary_dim / 2 + i) or, ``interleaved``, (2 i, 2 i + 1)."""
+    (i, rotary_dim / 2 + i) or, ``interleaved``, (2 i, 2 i + 1).  ``frequencies`` (f64 [rotary_dim / 2] on the GPU) may be written to, but no other
+    tensor put in its place; ``attention_factor`` may be set."""
 
     def __init__(self, head_dim: int, base: float = 10000.0, rotary_dim: int | None = None, interleaved: bool = False,
                  scaling: RopeScaling | None = None, device="cuda"):
@@ -93,8 +94,12 @@ class RotaryEmbedding:
         if not 0 < self.rotary_dim <= head_dim:
             _refuse(f"RotaryEmbedding: {self.rotary_dim} of {head_dim} elements")
         values, self.attention_factor = rope_frequencies(self.rotary_dim, base, scaling)
-        self.frequencies = torch.tensor(values, dtype=torch.float64, device=device)
-        self._index, self._ptr = self.frequencies.get_device(), self.frequencies.data_ptr()
+        self._frequencies = torch.tensor(values, dtype=torch.float64, device=device)
+        self._index = self._frequencies.get_device()
+
+    @property
+    def frequencies(self) -> torch.Tensor:
+        return self._frequencies
 
 
 def rope_frequencies(rotary_dim: int, base: float = 10000.0, scaling: RopeScaling | None = None):
@@ -150,7 +155,7 @@ def rope_positions(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Ten
             k_to_step = _stride(k_out, "rope_positions: out")
     if k is not None:
         k_to = k_out.data_ptr()
-    rc = fn(q.data_ptr(), q_step, k_ptr, k_step, positions.data_ptr(), rotary._ptr, rotary.attention_factor, tokens, heads, kv_heads, d, rotary.rotary_dim,
+    rc = fn(q.data_ptr(), q_step, k_ptr, k_step, positions.data_ptr(), rotary._frequencies.data_ptr(), rotary.attention_factor, tokens, heads, kv_heads, d, rotary.rotary_dim,
             rotary.interleaved, weight, eps, q_out.data_ptr(), q_to_step, k_to, k_to_step, _raw_stream(index))
     if rc:
         check(rc)

@@ -66,3 +66,17 @@ def test_quarter_turns(qa):
     got = qa.rope_positions(x, None, ints(range(-4, 5)), rotary)[0][:, 0, :2].cpu()
     want = torch.tensor([[1, 0], [0, 1], [-1, 0], [0, -1], [1, 0], [0, 1], [-1, 0], [0, -1], [1, 0.0]])
     assert (got - want).abs().max() <= 2.0 ** -50
+
+
+def test_other_frequencies(qa):
+    """A call reads what the embedding holds then: values written to it count, and another tensor in its place, which a call would not look at, is
+    refused."""
+    x = torch.randn(9, 2, 64, device="cuda")
+    one, other = qa.RotaryEmbedding(64, base=1e4), qa.RotaryEmbedding(64, base=1e6)
+    want = qa.rope_positions(x, None, ints(range(9)), other)[0]
+    kept = one.frequencies
+    with pytest.raises(AttributeError):
+        one.frequencies = other.frequencies
+    assert one.frequencies is kept
+    one.frequencies.copy_(other.frequencies)
+    assert torch.equal(qa.rope_positions(x, None, ints(range(9)), one)[0], want)
