@@ -326,7 +326,8 @@ int route_scored_impl(const T* logits, int64_t stride, const float* bias, int64_
         return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: top_k %d of %d experts in %d of %d groups (at most 64)", what, top_k, n, top_groups, groups);
     if (scoring != IZWI_MOE_SOFTMAX && scoring != IZWI_MOE_SIGMOID) return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: scoring %d", what, scoring);
     if (!std::isfinite(scale)) return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: scale %g", what, (double)scale);
-    if (t > 0x3ffffff || stride > 0x3fffffff) return qmm_fail(IZWI_QMM_ERR_UNSUPPORTED, "%s: %lld tokens, rows %lld apart", what, (long long)t, (long long)stride);
+    // (four tokens to a workgroup of 256 threads, of which a launch has fewer than 2^32)
+    if (t > 0x3fffffc || stride > 0x3fffffff) return qmm_fail(IZWI_QMM_ERR_UNSUPPORTED, "%s: %lld tokens, rows %lld apart", what, (long long)t, (long long)stride);
     if (t == 0) return IZWI_QMM_OK;
     if (!logits || !ids || !weights) return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: NULL buffer", what);
     const auto overlap = [](const void* a, uintptr_t an, const void* b, uintptr_t bn) {

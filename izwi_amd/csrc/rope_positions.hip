@@ -239,7 +239,8 @@ int rope_positions_impl(const T* q, int64_t q_stride, const T* k, int64_t k_stri
                         (long long)q_out_stride, (long long)k_out_stride);
     if (interleaved != 0 && interleaved != 1) return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: layout %d (0 halves, 1 interleaved)", what, interleaved);
     if (!std::isfinite((float)factor) || !(eps >= 0.0f) || !std::isfinite(eps)) return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: factor %g, eps %g", what, factor, (double)eps);
-    if (tokens > 0x3ffffff || q_stride > 0x3fffffff || k_stride > 0x3fffffff || q_out_stride > 0x3fffffff || k_out_stride > 0x3fffffff)
+    // (four tokens to a workgroup of 256 threads, of which a launch has fewer than 2^32)
+    if (tokens > 0x3fffffc || q_stride > 0x3fffffff || k_stride > 0x3fffffff || q_out_stride > 0x3fffffff || k_out_stride > 0x3fffffff)
         return qmm_fail(IZWI_QMM_ERR_UNSUPPORTED, "%s: %lld tokens", what, (long long)tokens);
     if (tokens == 0 || q_heads + k_heads == 0) return IZWI_QMM_OK;
     if (!positions || !frequencies || (q_heads && (!q || !q_out)) || (k_heads && (!k || !k_out))) return qmm_fail(IZWI_QMM_ERR_INVALID, "%s: NULL buffer", what);

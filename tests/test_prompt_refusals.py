@@ -33,3 +33,12 @@ def test_prompt_attention_out_lies_apart_from_the_offsets(L, name):
     for over in (dict(cu_q=6 * FAR), dict(cu_k=end - 4), dict(cu_q=6 * FAR - 8), dict(cu_k=6 * FAR + 512)):
         assert fn(*{**good, **over}.values()) == -1, over
         assert b"shares memory with the offsets" in L.izwi_qmm_last_error()
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_as_many_tokens_as_a_launch_takes(L, name):
+    """Four tokens to a workgroup of 256 threads, below 2^32 threads: 2^26 - 4 tokens.  (That many pass this check and are refused for outputs that overlap.)"""
+    rope, route = getattr(L, f"izwi_rope_positions_{name}"), getattr(L, f"izwi_moe_route_scored_{name}")
+    for tokens, rc in ((2 ** 26 - 4, -1), (2 ** 26 - 3, -2), (2 ** 26 - 1, -2), (2 ** 26, -2)):
+        assert rope(FAR, 64, 0, 0, FAR, FAR, 1.0, tokens, 1, 0, 64, 64, 0, 0, 1e-6, FAR + 64, 64, 0, 0, 0) == rc
+        assert route(FAR, 512, 0, tokens, 512, 8, 0, 1, 1, 1, 1, 1.0, FAR, FAR, 0) == rc
