@@ -793,7 +793,10 @@ hipError_t launch(PromptParams P, int64_t max_k, int device, int n_cus, hipStrea
     static_assert(lds <= 160 * 1024);
     const int64_t wgs = row_tiles(P, 32 * WR) * P.kv_heads;
     P.tiles = (int)(wgs / P.kv_heads);
-    P.splits = splits_of<T>(wgs, max_k, KS, n_cus, P.causal && WZ == 1 && P.batch == 1);
+    // (f32 heads of 64 go to the larger workgroups for one tile, or where these are as many as the compute units, of causal calls twice as many: too
+    // few or too many to be split)
+    constexpr bool kSplits = sizeof(T) != 4 || D != 64 || WZ != 1;
+    P.splits = kSplits ? splits_of<T>(wgs, max_k, KS, n_cus, P.causal && WZ == 1 && P.batch == 1) : 1;
     if constexpr (sizeof(T) == 4 && D >= 128 && WZ == 1)
         if (P.splits == 1 && P.batch <= 256 && (!P.causal || P.total_k >= 4 * P.total_q)) { // (the join looks through the offsets, 64 at a time)
             const int64_t likely = ((P.total_q * P.group + 32 * WR - 1) / (32 * WR) + (P.batch - 1) / 2) * P.kv_heads; // (the bound has a tile more a sequence)
@@ -826,12 +829,15 @@ hipError_t launch(PromptParams P, int64_t max_k, int device, int n_cus, hipStrea
         kernel<<<(unsigned)(wgs * P.splits), 64 * WR * WZ * DZ, lds, stream>>>(P);
         return hipGetLastError();
     };
-    if (P.splits == 1) return run(std::false_type{});
-    const hipError_t e = run(std::true_type{});
-    if (e != hipSuccess) return e;
-    if (P.splits <= 8) prompt_join_kernel<T, D, true><<<(unsigned)((rows + 3) / 4), 256, 0, stream>>>(P, rows);
-    else prompt_join_kernel<T, D, false><<<(unsigned)rows, 256, 0, stream>>>(P, rows);
-    return hipGetLastError();
+    if constexpr (kSplits)
+        if (P.splits > 1) {
+            const hipError_t e = run(std::true_type{});
+            if (e != hipSuccess) return e;
+            if (P.splits <= 8) prompt_join_kernel<T, D, true><<<(unsigned)((rows + 3) / 4), 256, 0, stream>>>(P, rows);
+            else prompt_join_kernel<T, D, false><<<(unsigned)rows, 256, 0, stream>>>(P, rows);
+            return hipGetLastError();
+        }
+    return run(std::false_type{});
 }
 // Which workgroups.  f16 and bf16: four waves of 32 rows on 64 keys at a time (two on halves of the head each for D = 256, 32 keys), or where
 // those would not fill the compute units, two waves of rows on 32 keys and two on the 32 behind them (D = 256: half the rows): causal
