@@ -144,9 +144,9 @@ def test_prompt_attention_of_long_prompts(qa, dtype, d, causal, lens, heads, kv)
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("d", [64, 128, 256])
 @pytest.mark.parametrize("causal", [True, False])
-@pytest.mark.parametrize("lens,past,heads,kv", [([17], [8300], 32, 8), ([33, 20, 70], [8200, 0, 9100], 16, 4)])
+@pytest.mark.parametrize("lens,past,heads,kv", [([17], [8300], 32, 8), ([33, 20, 70], [8200, 0, 9100], 16, 4), ([9], [8300], 16, 8)])
 def test_prompt_attention_of_a_chunk_behind_a_long_past(qa, dtype, d, causal, lens, past, heads, kv):
-    """More than 64 rows on more than 8192 keys: workgroups of 128 rows in parts, also on a stream of its own and captured, replayed on new values."""
+    """More than 64 rows on more than 8192 keys, workgroups of 128 rows in parts, and fewer, in the smaller ones, also on a stream of its own and captured, replayed on new values."""
     print("chunk", dtype, d, causal, lens, past, flush=True)
     rng = np.random.default_rng(d + sum(past))
     starts, starts_k = np.cumsum([0] + lens), np.cumsum([0] + [a + b for a, b in zip(lens, past)])
