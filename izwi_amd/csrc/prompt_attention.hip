@@ -217,8 +217,17 @@ __device__ __forceinline__ float max_lane32(float v) {
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
-// 2^d, d <= 0, for what is summed already: not zero, which would make NaN of an infinity
-__device__ __forceinline__ float rescale(float d) { return fmaxf(__builtin_amdgcn_exp2f(d), 0x1p-126f); }
+// 2^d, d <= 0, for what is summed already: 0 below 2^-126, as a weight is (bounded by that, it left 10^37 under a weight of zero a share of 0.1)
+__device__ __forceinline__ float rescale(float d) { return __builtin_amdgcn_exp2f(d); }
+// v times such a factor; of an infinity, which no factor changes, itself
+template <typename V>
+__device__ __forceinline__ V rescaled(V v, float by) {
+    V r = v * by;
+    if (by == 0.0f)
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(V) / 4); i++) r[i] = __builtin_isinf(v[i]) ? v[i] : r[i];
+    return r;
+}
 
 constexpr float kSlack = 8.0f; // a reference stands until a score passes it by this (base 2): weights stay below 2^8
 
@@ -513,8 +522,11 @@ __global__ __launch_bounds__(64 * WR * WZ * DZ, Elem<T>::N == 1 || D == 64 ? 2 :
     };
     // A value that is no number must not reach the rows that do not see it, and a weight of zero would not keep it out; nor would what is left of a
     // weight, zero or below it, leave an infinity that a row does see what it is.  Results that hold one are worked out once more, with
-    // care: the rows that see such a value get it by itself, and the tile goes on with a zero in its place.  (A look at the values of every tile
-    // that some row does not see all of took 1200 of the 11600 cycles of 37 bf16 tokens.)
+    // care: the tile goes on with a zero in its place, and the rows that see such a value remember it, a bit for each of the lane's elements: up
+    // is an infinity, down a negative one, both NaN (f32: any).  (A look at the values of every tile that some row does not see all of took
+    // 1200 of the 11600 cycles of 37 bf16 tokens.)
+    uint64_t up = 0, down = 0;
+    static_assert(DT * 16 <= 64);
     for (bool care = false;;) {
         int tile = first;
         if constexpr (!kDouble) // every row sees all of these
@@ -540,17 +552,20 @@ __global__ __launch_bounds__(64 * WR * WZ * DZ, Elem<T>::N == 1 || D == 64 ? 2 :
 #pragma unroll 1
                 for (int j = wz * KT; j < min((wz + 1) * KT, s.len_k - p0); j++) {
                     const bool sees = p0 + j <= limit;
+#pragma unroll 1
+                    for (int e = 0; e < DT * 4; e++) // four of the lane's elements, 16 (e / 4) + 4 (e % 4) of o and on
 #pragma unroll
-                    for (int d = 0; d < DT; d++)
+                        for (int n = 0; n < N; n++) {
+                            const int c = (dz * (DW / 8) + e) ^ turn<D>(j);
+                            const u32x2 four = *reinterpret_cast<const u32x2*>(here + (N + n) * kPlane + j * (2 * D) + 16 * c + 8 * h);
 #pragma unroll
-                        for (int r = 0; r < 16; r++)
-#pragma unroll
-                            for (int n = 0; n < N; n++) {
-                                const int c = (dz * (DW / 8) + 4 * d + (r >> 2)) ^ turn<D>(j);
-                                const uint16_t bits = *reinterpret_cast<const uint16_t*>(here + (N + n) * kPlane + j * (2 * D) + 16 * c + 8 * h + 2 * (r & 3));
-                                const float value = std::is_same_v<T, f16_t> ? qmm_f16_bits_to_f32(bits) : qmm_bf16_bits_to_f32(bits);
-                                o[d][r] += sees && (bits & kLow) == kLow ? value : 0.0f;
+                            for (int r = 0; r < 4; r++) {
+                                const uint32_t bits = four[r >> 1] >> (16 * (r & 1)) & 0xffffu;
+                                const bool odd = sees && (bits & kLow) == kLow, nan = N > 1 || (bits & 0x7fffu) != kLow;
+                                up |= (uint64_t)(odd && (nan || !(bits >> 15))) << (4 * e + r);
+                                down |= (uint64_t)(odd && (nan || bits >> 15)) << (4 * e + r);
                             }
+                        }
                 }
                 __syncthreads();
 #pragma unroll 1
@@ -585,7 +600,7 @@ __global__ __launch_bounds__(64 * WR * WZ * DZ, Elem<T>::N == 1 || D == 64 ? 2 :
 
     sum[0] += sum[1];
     if constexpr (WZ > 1) { // the sets' results meet in LDS
-        constexpr int kNumbers = DT * 16 + 2;
+        constexpr int kNumbers = DT * 16 + 6;
         static_assert(DZ == 1 && (WZ - 1) * WR * kNumbers * 256 <= kTiles);
         float* const meet = reinterpret_cast<float*>(smem) + lane;
         __syncthreads();
@@ -593,9 +608,11 @@ __global__ __launch_bounds__(64 * WR * WZ * DZ, Elem<T>::N == 1 || D == 64 ? 2 :
             float* const to = meet + ((wz - 1) * WR + wr) * kNumbers * 64;
             to[0] = ref, to[64] = sum[0];
 #pragma unroll
+            for (int i = 0; i < 4; i++) to[(2 + i) * 64] = __uint_as_float((uint32_t)((i < 2 ? up : down) >> (32 * (i & 1))));
+#pragma unroll
             for (int d = 0; d < DT; d++)
 #pragma unroll
-                for (int r = 0; r < 16; r++) to[(2 + 16 * d + r) * 64] = o[d][r];
+                for (int r = 0; r < 16; r++) to[(6 + 16 * d + r) * 64] = o[d][r];
         }
         __syncthreads();
         if (wz > 0) return;
@@ -608,13 +625,24 @@ __global__ __launch_bounds__(64 * WR * WZ * DZ, Elem<T>::N == 1 || D == 64 ? 2 :
             const float by = refs[z] == -INFINITY ? 1.0f : rescale(refs[z] - all);
             const float* const in = meet + ((z - 1) * WR + wr) * kNumbers * 64;
             sum[0] = z == 0 ? sum[0] * by : sum[0] + in[64] * by;
+            if (z > 0)
+#pragma unroll
+                for (int i = 0; i < 4; i++) (i < 2 ? up : down) |= (uint64_t)__float_as_uint(in[(2 + i) * 64]) << (32 * (i & 1));
 #pragma unroll
             for (int d = 0; d < DT; d++)
 #pragma unroll
-                for (int r = 0; r < 16; r++) o[d][r] = z == 0 ? o[d][r] * by : o[d][r] + in[(2 + 16 * d + r) * 64] * by;
+                for (int r = 0; r < 16; r++) o[d][r] = z == 0 ? o[d][r] * by : o[d][r] + in[(6 + 16 * d + r) * 64] * by;
         }
         ref = all;
     }
+    if (__any((up | down) != 0))
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                o[d][r] += up >> (16 * d + r) & 1 ? INFINITY : 0.0f;
+                o[d][r] += down >> (16 * d + r) & 1 ? -INFINITY : 0.0f;
+            }
     // rows behind the sequence's last stay as they are
     if (s.row0 + wr * 32 + x >= rows) return;
     const float total = qmm_add_lane32(sum[0]);
@@ -713,7 +741,7 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(PromptParams P, int64_
             const float by = st[j].x == -INFINITY ? 1.0f : rescale(st[j].x - ref);
             any |= there;
             sum += there ? st[j].y * by : 0.0f;
-            a += (there ? v[j] : vec(0.0f)) * by;
+            a += there ? rescaled(v[j], by) : vec(0.0f);
         }
         i0 += A * step;
         if (i0 < P.splits) take(i0);
