@@ -876,9 +876,12 @@ hipError_t launch(PromptParams P, int64_t max_k, int device, int n_cus, hipStrea
 // 40, behind 2000 24.7, 21).  Up to 64 keys the second pair would have few (37 tokens 5.9, 6.6).
 // f32: the larger ones, whose next tile is taken apart beside the products, and the smaller where those leave compute units without work.  16
 // heads on 8, us of the larger and the smaller: D = 128 few rows and many tiles each (4 tokens behind 1087 of 10 sequences 46.7, 36.5), two to
-// four tiles (37 tokens 12.4, 11.6; 100 of 6 sequences 23, 16; one tile 8.8, 11.2; seven 28, 31), causal prompts too many to be split (1100 tokens
-// 116, 76; 2048 213, 150; 2500 257, 242; but 1000 in two parts 71, 71; 3500 358, 415; not causal 1100 121, 153); D = 64 causal 1200 tokens 63, 44; 3500
-// 194, 175; 6000 425, 455; 100 of 30 15.7, 17.9; not causal 1200 64, 60; 2048 107, 110; one tile (9 of 13) 5.6, 6.6.
+// four tiles (37 tokens 12.4, 11.6; 100 of 6 sequences 23, 16; one tile 8.8, 11.2; seven 28, 31), several causal prompts that are about as many
+// larger workgroups as compute units, of unequal length and not in parts (700 and 700 tokens 73, 52; four of 400 45, 41; 1000 and 900 101, 82; six of
+// 300 38.5, 40.6; of 8 heads on 8 and 16 on 2 alike, of 32 on 8 450, 150 and 250 50, 44; 500 and 450 55, 52), but neither one prompt nor those behind a
+// past, which come in parts (1100 tokens 64, 75; 2048 137, 144; 3500 332, 408; behind 3000 250, 393; four of 300 behind 1000 110, 152; not causal 1100 98,
+// 149; 8 heads on 8 2200 96, 137; 32 on 8 1024 86, 79); D = 64 causal 1200 tokens 64, 43; 3500 197, 174; 6000 433, 461; 100 of 30 15.7, 17.9; not causal
+// 1200 64, 62; 2048 113, 113; one tile (9 of 13) 5.6, 6.6.
 template <typename T, int D>
 hipError_t launch_of(const PromptParams& P, int64_t max_k, int device, int n_cus, hipStream_t stream) {
     const int64_t all = P.total_q * P.group, wgs = std::max<int64_t>((all + 127) / 128, P.batch) * P.kv_heads, rows = all / P.batch; // rows: of a sequence, on average
@@ -890,7 +893,7 @@ hipError_t launch_of(const PromptParams& P, int64_t max_k, int device, int n_cus
         const int64_t large = row_tiles(P, 128) * P.kv_heads; // workgroups
         const bool small = D == 64 ? tiles > 1 && large < (P.causal ? 2 : 1) * (int64_t)n_cus
                                    : (rows <= 64 && tiles >= 4 * splits_of<T>(wgs, max_k, 32, n_cus)) || (tiles > 1 && tiles <= 4 && 2 * large <= n_cus) ||
-                                         (P.causal && tiles >= 12 && 2 * large > n_cus && 4 * large <= 5 * n_cus);
+                                         (P.causal && P.batch > 1 && P.total_k <= 2 * P.total_q && tiles >= 12 && 2 * large > n_cus && 4 * large <= 5 * n_cus);
         return small ? launch<T, D, 2, 2, DZ, 32>(P, max_k, device, n_cus, stream) : launch<T, D, 4, 1, DZ, 32>(P, max_k, device, n_cus, stream);
     } else {
         const int quarters = P.causal ? (D == 64 ? 8 : D == 128 ? 7 : 4) : (D == 64 ? 6 : 2); // of a workgroup per compute unit
