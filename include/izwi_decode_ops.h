@@ -218,7 +218,7 @@ int izwi_decode_beam_select_f32(const float* logits, int64_t prompts, int64_t be
  *
  * What a prompt's layer needs between its projections: prompts of different lengths stand one behind the other as rows of tokens,
  * each token with its own position, rows strided (parts of a q|k|v row).  f32, f16 and bf16 (raw bits as uint16_t), every tensor
- * of a call of one type; arithmetic in f32, results rounded once.  Device pointers only throughout. */
+ * of a call of one type; sums in f32, results rounded once.  Device pointers only throughout. */
 
 /* Angles per position of the rotary_dim / 2 pairs of a head: base^(-2 i / rotary_dim), for a context stretched to `factor` times
  * original_len positions (factor >= 1) by

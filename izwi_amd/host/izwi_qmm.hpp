@@ -357,7 +357,7 @@ inline void beam_select(const float* logits, int64_t prompts, int64_t beams, int
 inline double rope_frequencies(int scaling, int64_t rotary_dim, double base, double factor, double original_len, double low, double high,
                                std::vector<double>& frequencies) {
     double attention_factor = 1.0;
-    frequencies.assign(rotary_dim > 0 ? (size_t)rotary_dim / 2 : 0, 0.0);
+    frequencies.assign(rotary_dim > 0 && rotary_dim <= 1024 ? (size_t)rotary_dim / 2 : 0, 0.0); // (of others the call says what is wrong)
     check(izwi_rope_frequencies(scaling, rotary_dim, base, factor, original_len, low, high, frequencies.data(), &attention_factor));
     return attention_factor;
 }
