@@ -636,14 +636,15 @@ def moe_route_scored(logits: torch.Tensor, top_k: int, scoring: str = "softmax",
         if bias.dtype is not torch.float32 or bias.shape != (n,) or not bias.is_contiguous() or bias.get_device() != index:
             raise capi.QmmError(-1, f"moe_route_scored: a contiguous f32 bias of {n} on GPU {index} expected")
         b, best = bias.data_ptr(), 2
-    if not 1 <= top_k <= 64:
-        raise capi.QmmError(-1, f"moe_route_scored: top_k {top_k} (1 to 64)")
+    top_groups, best = groups if top_groups is None else top_groups, best if group_best is None else group_best
+    if not (1 <= top_k <= 64 and 1 <= top_groups <= groups <= 64 and 1 <= best <= 2):  # (numbers that 32 bits would cut among them)
+        raise capi.QmmError(-1, f"moe_route_scored: top_k {top_k} (1 to 64), {top_groups} of {groups} groups (1 to 64) by their best {best} (1 or 2)")
     if index != _current_device():
         with torch.cuda.device(index):
             return moe_route_scored(logits, top_k, scoring, bias, groups, top_groups, group_best, renormalize, scale)
     weights = logits.new_empty((t, top_k), dtype=torch.float32)
     ids = torch.empty_like(weights, dtype=torch.int32)
-    rc = fn(logits.data_ptr(), step, b, t, n, top_k, score, groups, groups if top_groups is None else top_groups, best if group_best is None else group_best,
+    rc = fn(logits.data_ptr(), step, b, t, n, top_k, score, groups, top_groups, best,
             bool(renormalize), scale, ids.data_ptr(), weights.data_ptr(), _raw_stream(index))
     if rc:
         check(rc)

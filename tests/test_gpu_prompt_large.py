@@ -193,3 +193,11 @@ def test_prompt_attention_of_values_that_are_no_numbers_in_every_kernel(qa, dtyp
         assert torch.equal(got[..., other], clean[..., other])
         hit = got[..., d - 3][sees]
         assert torch.isnan(hit).all() if bad != bad else (~torch.isfinite(hit)).all() if dtype == "f32" else (hit == bad).all()
+
+
+def test_route_scored_numbers_beyond_32_bits(qa):
+    """Numbers that 32 bits would cut to ones that fit."""
+    x = torch.zeros(4, 16, device="cuda")
+    for over in (dict(top_k=2 ** 32 + 2), dict(groups=2 ** 32 + 1), dict(groups=4, top_groups=2 ** 32 + 2), dict(groups=4, top_groups=2, group_best=2 ** 32 + 1), dict(groups=-4), dict(group_best=0)):
+        with pytest.raises(qa.QmmError):
+            qa.moe_route_scored(**{**dict(logits=x, top_k=2), **over})
