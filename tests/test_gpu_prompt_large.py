@@ -8,6 +8,7 @@ import pytest
 import torch
 
 import prompt_ref
+from gpu_streams import fresh_stream
 from prompt_rows import attention_rows, route_rows
 from test_gpu_prompt_ops import check_rope, ints, made, wide
 from test_gpu_prompt_weights import check_rows
@@ -25,6 +26,11 @@ def qa():
     izwi_amd.lib()
     torch.cuda.set_device(0)
     return izwi_amd
+
+
+@pytest.fixture(scope="module")
+def stream(qa):
+    return fresh_stream()
 
 
 # ---- routing ------------------------------------------------------------------------------------------------------------------
@@ -145,7 +151,7 @@ def test_prompt_attention_of_long_prompts(qa, dtype, d, causal, lens, heads, kv)
 @pytest.mark.parametrize("d", [64, 128, 256])
 @pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("lens,past,heads,kv", [([17], [8300], 32, 8), ([33, 20, 70], [8200, 0, 9100], 16, 4), ([9], [8300], 16, 8)])
-def test_prompt_attention_of_a_chunk_behind_a_long_past(qa, dtype, d, causal, lens, past, heads, kv):
+def test_prompt_attention_of_a_chunk_behind_a_long_past(qa, stream, dtype, d, causal, lens, past, heads, kv):
     """More than 64 rows on more than 8192 keys, workgroups of 128 rows in parts, and fewer, in the smaller ones, also on a stream of its own and captured, replayed on new values."""
     print("chunk", dtype, d, causal, lens, past, flush=True)
     rng = np.random.default_rng(d + sum(past))
@@ -156,7 +162,7 @@ def test_prompt_attention_of_a_chunk_behind_a_long_past(qa, dtype, d, causal, le
     check = lambda got, *x: check_f32(got, *x, starts, starts_k, causal, scale, tokens) if dtype == "f32" else check_rows(got, *x, starts, starts_k, causal, scale, dtype, tokens)  # noqa: E731
     tokens = sampled(starts, 4)
     check(run(), q64, k64, v64)
-    out, stream = torch.zeros_like(q), torch.cuda.Stream()
+    out = torch.zeros_like(q)
     stream.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(stream):
         run(out=out)

@@ -2,6 +2,8 @@
 import pytest
 import torch
 
+from gpu_streams import fresh_stream
+
 pytestmark = pytest.mark.gpu
 
 
@@ -13,7 +15,7 @@ def test_scratch_stays_within_its_bound(tokens, heads, kv, d):
     keys = max(tokens, 1000)
     q, k, v = (torch.randn(n, g, d, device="cuda") for n, g in ((tokens, heads), (keys, kv), (keys, kv)))
     out = izwi_amd.prompt_attention(q, k, v, causal=False)  # (code and the default stream's scratch)
-    stream = torch.cuda.Stream()
+    stream = fresh_stream()
     torch.cuda.synchronize()
     before = torch.cuda.mem_get_info()[0]
     with torch.cuda.stream(stream):
