@@ -8,8 +8,9 @@
 // LANES lanes have a token's experts, e = i LANES + lane: 64 where tokens are few, 16 where they are many, so that a round of the selection
 // (a maximum over the lanes on the vector ALU, the lowest expert that has it, its removal) serves four tokens.
 //
-// Bound by vector instructions where tokens are many, most of them the f64 exponentials and top_k rounds: 16384 tokens of 128 experts with a bias
-// 11 us, 0.86 TB/s; by launch and the chain of rounds where they are few: one token 3.2 us, 509 of 256 experts in eight groups 6.4.
+// Bound by vector instructions where tokens are many, most of them the rounds of the selection: 16384 tokens of 128 experts with a bias 10.2 us, 0.86 TB/s, 1350
+// instructions a wave, of which the exponentials, nineteen for each of a lane's eight experts, are an eighth; by launch and the chain of rounds where
+// they are few: one token 3.3 us, 509 of 256 experts in eight groups 7.1.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

@@ -13,12 +13,15 @@
 // f32: queries, keys, values and weights go as three bf16 numbers each, which hold all 24 bits (down to 2^-100: the third has no bits
 // below 2^-133), and the six products of weight 2^-16 and more are summed in f32; what is left out is at most 2^-22 of a product, of either sign.
 //
-// Bound by the matrix cores and the power that they may draw in long prompts: 8192 tokens of 32 bf16 heads of 128 on 8, causal, 522 us, 1050 TFLOP/s
-// (a library product of 8192^3 1115): they are at work 59 % of the cycles, at a clock of 1.8 GHz; exponentials and rounding of one wave
-// overlap the products of the other on its SIMD only in part.  By the same, and the beginnings and ends of workgroups, in shorter ones: nine of 775 to 1501
-// tokens 144 us, 715 TFLOP/s; four clips of 867 to 1500 f16, heads of 64, not causal, 40 us, 590 TFLOP/s (an exponential takes as long there
-// as a quarter of the products of its score).  By memory where few rows meet many keys: 17 tokens behind 30011 30 us, 4.1 TB/s.  By launch and
-// latency below that: 37 f32 tokens 11.7 us, bf16 5.8.  f32: six products where bf16 has one, 3500 tokens of 16 heads on 8 358 us, 140 TFLOP/s.
+// f16 and bf16: weights go as two numbers of the type (Elem), so that values take two products where queries and keys take one.
+//
+// Bound by the matrix cores and the power that they may draw in long prompts: 8192 tokens of 32 bf16 heads of 128 on 8, causal, 719 us, 765 TFLOP/s (1150 with
+// the weights' second product; a library product of 8192^3 1372, both operands along k 1622): they are at work 65 % of the cycles, at a clock of 1.8 GHz; exponentials
+// and rounding of one wave overlap the products of the other on its SIMD only in part.  By the same, and the beginnings and ends of workgroups, in shorter
+// ones: nine of 775 to 1501 tokens 186 us, 551 TFLOP/s; four clips of 867 to 1500 f16, heads of 64, not causal, 53 us, 450 TFLOP/s (an exponential
+// takes as long there as a quarter of the products of its score).  By memory where few rows meet many keys: 17 tokens behind 30011 33 us, 3.7
+// TB/s, and 5 to join them.  By launch and latency below that: 37 f32 tokens 11.5 us, bf16 6.0.  f32: six products for queries and keys, and for weights and values,
+// 3500 tokens of 16 heads on 8 332 us, 151 TFLOP/s; 2048 138, 125; 1100 67, 74; 300 25, 15, in parts and with a launch to join them.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -400,7 +403,7 @@ __global__ __launch_bounds__(64 * WR * WZ * DZ, Elem<T>::N == 1 || D == 64 ? 2 :
             }
             if (behind < end) request(behind, 0);
         }
-        if constexpr (N == 1) { // eight operands on their way ahead of the first product (two: 8192 tokens 528 us instead of 522; D = 256 374, 356)
+        if constexpr (N == 1) { // eight operands on their way ahead of the first product (two: D = 256 2600 tokens 138 us instead of 134, 37 of D = 128 6.3, 6.0)
             constexpr int kReads = PT * KK, kAhead = kReads < 8 ? kReads : 8;
             __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
 #pragma unroll
@@ -783,12 +786,12 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(PromptParams P, int64_
 int64_t row_tiles(const PromptParams& P, int rows) { return P.cu_q ? P.total_q * P.group / rows + P.batch : (P.total_q * P.group + rows - 1) / rows; }
 
 // Parts that the keys are split into where workgroups are few: two tiles of `step` positions a part at the least, as a second launch has to join
-// them: f16 and bf16 from eight tiles on (16 tokens of 16 heads on 8 behind 240: in one part 8.6 us, in two 10.1; behind 500: in two
-// parts 12.3, in four 11.0; behind 1000 15, 11.9, in eight 10.5), f32, whose tiles take three times as long, from four (behind 240: in one
+// them: f16 and bf16 from eight tiles on (16 tokens of 16 heads on 8 behind 240: in one part 8.8 us, in two 10.8; behind 500: 13.0,
+// 13.3, in four 11.7; behind 1000 18.8, 15.8, 12.6, in eight 11.1; of 32 on 8 and 16 on 2 alike), f32, whose tiles take three times as long, from four (behind 240: in one
 // part 30.6 us, in two 21.0, in four 14.8).
 // A causal f32 prompt in the larger workgroups: their lengths differ, so that one or two parts each are better rounded up to half as many again as
-// there are compute units (16 heads on 8: D = 128 800 tokens in two parts 60, in four 48; 1000 72, in three 57; D = 256 400 47, in four 45; 600 in
-// one part 86, in three 57; 900 128, in two 93; 1200 165, 146; 2048 299, 330; not causal 600 88, in two 109; six causal ones of 128 26, 42).
+// there are compute units (16 heads on 8: D = 128 800 tokens in two parts 57, in four 45; 1000 69, in three 55; D = 256 400 47, in four 45; 600 in
+// one part 87, in three 55; 900 128, in two 93; 1200 169, 142; 2048 299, 330; not causal 600 88, in two 109; six causal ones of 128 26, 42).
 template <typename T>
 int splits_of(int64_t wgs, int64_t max_k, int step, int n_cus, bool unequal = false) {
     const int64_t tiles = (max_k + step - 1) / step;
@@ -798,8 +801,8 @@ int splits_of(int64_t wgs, int64_t max_k, int step, int n_cus, bool unequal = fa
 
 // f32 in the larger workgroups, one to a compute unit, of about equal lengths, that come in one part: in two to eight where a last turn that is nearly
 // empty costs more than the join, by an estimate in us from what a tile (heads of 128 3.3, of 256 4.2) and a part's sums take.  16 heads on 8,
-// not causal, us in one part and so: D = 128 1100 tokens 121, 101; 1400 151, 141; 2500 519, 383; 3500 720, 706; ten sequences of up to 128 behind 500
-// 73, 48; D = 256 1200 329, 256; 17 of up to 28 behind 13484 1850, 1045; 2048, whose turns are full, 547 (in three parts 621).
+// not causal, us in one part and so: D = 128 1100 tokens 109, 97; 1400 151, 141; 2500 476, 358; 3500 661, 664; 8 heads on 8 2200 208, 159; 5000 933, 658; 32 on
+// 8 550 60, 63; 1250 248, 208; ten sequences of up to 128 behind 500 73, 48; D = 256 1200 337, 250; 17 of up to 28 behind 13484 1850, 1045; 2048, whose turns are full, 547 (in three parts 621).
 // As many as leave the stream's buffer within 256 MiB, sums and statistics (it grows to one and a half times what is asked for).
 constexpr int64_t kMostScratch = (1 << 28) / 3 * 2;
 int parts_by_turns(int64_t likely, int64_t most, int64_t tiles, int64_t rows, int d, int n_cus) { // (workgroups that have rows: the device knows)
@@ -830,10 +833,10 @@ hipError_t launch(PromptParams P, int64_t max_k, int device, int n_cus, hipStrea
             const int64_t likely = ((P.total_q * P.group + 32 * WR - 1) / (32 * WR) + (P.batch - 1) / 2) * P.kv_heads; // (the bound has a tile more a sequence)
             P.splits = parts_by_turns(likely, P.batch > 1 ? wgs : likely, (max_k + KS - 1) / KS, P.total_q * P.heads, D, n_cus);
         }
-    // Sequences of several tiles on a few workgroups a compute unit: by length (unsplit).  Us by the offsets and so: f32 six causal prompts up to 700 124,
-    // 82; bf16 D = 256 twelve up to 1000 139, 127; D = 64 five up to 2500 81, 76, four not causal up to 1500 42, 40; but where workgroups are many,
-    // the last ones matter less than that those of one sequence find its keys in the L2 (30 up to 1501 of 32 heads 460, 500), and many short
-    // sequences are over too soon (64 up to 100 20, 23.5).
+    // Sequences of several tiles on a few workgroups a compute unit: by length (unsplit).  Us by the offsets and so: f32 six causal prompts up to 700 85 to
+    // 96, 75; bf16 D = 256 twelve up to 1000 122, 112; D = 64 five up to 2500 67, 61, four not causal up to 1500 60, 59; 16 heads on 2 twelve up to 900 60, 54; but where
+    // workgroups are many, the last ones matter less than that those of one sequence find its keys in the L2 (30 up to 1501 of 32 heads 380, 401),
+    // and many short sequences are over too soon (64 up to 100 19.6, 21.4).
     P.by_length = P.splits == 1 && P.batch > 1 && P.batch <= 64 && wgs > n_cus && wgs <= 8 * (int64_t)n_cus && P.total_q * P.group >= 4 * 128 * (int64_t)P.batch;
     const int64_t rows = P.total_q * P.heads;
     if (P.splits > 1) {
@@ -870,17 +873,19 @@ hipError_t launch(PromptParams P, int64_t max_k, int device, int n_cus, hipStrea
 // Which workgroups.  f16 and bf16: four waves of 32 rows on 64 keys at a time (two on halves of the head each for D = 256, 32 keys), or where
 // those would not fill the compute units, two waves of rows on 32 keys and two on the 32 behind them (D = 256: half the rows): causal
 // prompts, whose workgroups are of unequal length, change over later.  16 bf16 heads on 8, us of the larger and the smaller workgroups: D = 128
-// causal 700 tokens 26, 15; 2600 51, 44.6; 3500 73, 70; not causal 700 26, 15; 1500 32, 34; 2000 42.6, 47; D = 64 causal 2600 37.7, 29.5; 3500
-// 49.5, 42; not causal 2600 51, 47; 3500 71, 77; D = 256 causal 2048 90, 77; 2600 112, 137; not causal 700 42, 27; 1500 67, 104.  More than
-// 64 rows on very many keys read them too often with the smaller ones (17 tokens of 32 heads behind 30011 31.5, 36.2; 250 of 16 behind 8000 34,
-// 40, behind 2000 24.7, 21).  Up to 64 keys the second pair would have few (37 tokens 5.9, 6.6).
+// causal 700 tokens 28, 15; 2600 63, 52; 3500 93, 90; not causal 700 27, 15; 1500 37, 39; 2000 53, 56; D = 64 causal 2600 45, 34; 3500
+// 62, 54; not causal 2600 66, 59; 3500 93, 101; D = 256 causal 2048 105, 84; 2600 134, 140; not causal 700 42, 29; 1500 75, 107 (of as many rows in 32 heads
+// on 8, 8 on 8 and 16 on 2, twenty-two of each, the side taken is the slower one by 3 % at most).  More than 64 rows on very many keys read them too
+// often with the smaller ones (17 tokens of 32 heads behind 30011 34, 38; 250 of 16 behind 8000 39, 42, behind 2000 25, 22).  Up to 64 keys the
+// second pair would have few (37 tokens 6.5, 7.1).
 // f32: the larger ones, whose next tile is taken apart beside the products, and the smaller where those leave compute units without work.  16
 // heads on 8, us of the larger and the smaller: D = 128 few rows and many tiles each (4 tokens behind 1087 of 10 sequences 46.7, 36.5), two to
 // four tiles (37 tokens 12.4, 11.6; 100 of 6 sequences 23, 16; one tile 8.8, 11.2; seven 28, 31), several causal prompts that are about as many
 // larger workgroups as compute units, of unequal length and not in parts (700 and 700 tokens 73, 52; four of 400 45, 41; 1000 and 900 101, 82; six of
-// 300 38.5, 40.6; of 8 heads on 8 and 16 on 2 alike, of 32 on 8 450, 150 and 250 50, 44; 500 and 450 55, 52), but neither one prompt nor those behind a
-// past, which come in parts (1100 tokens 64, 75; 2048 137, 144; 3500 332, 408; behind 3000 250, 393; four of 300 behind 1000 110, 152; not causal 1100 98,
-// 149; 8 heads on 8 2200 96, 137; 32 on 8 1024 86, 79); D = 64 causal 1200 tokens 64, 43; 3500 197, 174; 6000 433, 461; 100 of 30 15.7, 17.9; not causal
+// 300 38.5, 40.6; of 8 heads on 8 and 16 on 2 alike, of 32 on 8 450, 150 and 250 50, 44; 500 and 450 55, 52), but not those behind a
+// past and one prompt only where its tiles are few for its rows: these come in parts, whose join goes by the rows (1100 tokens 64, 75; 2048 137, 144; 3500
+// 332, 408; behind 3000 250, 393; four of 300 behind 1000 110, 152; not causal 1100 98, 149; 8 heads on 8 2200 99, 139; but of 32 on 8 550 45, 42.5; 1024
+// 86, 80); D = 64 causal 1200 tokens 64, 43; 3500 197, 174; 6000 433, 461; 100 of 30 15.7, 17.9; not causal
 // 1200 64, 62; 2048 113, 113; one tile (9 of 13) 5.6, 6.6.
 template <typename T, int D>
 hipError_t launch_of(const PromptParams& P, int64_t max_k, int device, int n_cus, hipStream_t stream) {
@@ -893,7 +898,7 @@ hipError_t launch_of(const PromptParams& P, int64_t max_k, int device, int n_cus
         const int64_t large = row_tiles(P, 128) * P.kv_heads; // workgroups
         const bool small = D == 64 ? tiles > 1 && large < (P.causal ? 2 : 1) * (int64_t)n_cus
                                    : (rows <= 64 && tiles >= 4 * splits_of<T>(wgs, max_k, 32, n_cus)) || (tiles > 1 && tiles <= 4 && 2 * large <= n_cus) ||
-                                         (P.causal && P.batch > 1 && P.total_k <= 2 * P.total_q && tiles >= 12 && 2 * large > n_cus && 4 * large <= 5 * n_cus);
+                                         (P.causal && (P.batch > 1 ? P.total_k <= 2 * P.total_q : large > 6 * tiles) && tiles >= 12 && 2 * large > n_cus && 4 * large <= 5 * n_cus);
         return small ? launch<T, D, 2, 2, DZ, 32>(P, max_k, device, n_cus, stream) : launch<T, D, 4, 1, DZ, 32>(P, max_k, device, n_cus, stream);
     } else {
         const int quarters = P.causal ? (D == 64 ? 8 : D == 128 ? 7 : 4) : (D == 64 ? 6 : 2); // of a workgroup per compute unit

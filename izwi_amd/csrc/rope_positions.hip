@@ -5,9 +5,9 @@
 // worked out in 64 bits, too: times the factor they are rounded to 32 bits once.  (As 32-bit functions of a fraction of a turn in 32 bits
 // they left f32 results 1.4 times as far off.  The f64 instructions are a few more and take no longer.)
 //
-// Bound by memory where there is much to do: 16384 tokens of 32 and 8 heads of 128, f32, 126 us, 5.3 TB/s (a copy of 1 GiB reaches 4.9; part of
-// this fits the last-level cache); 2051 tokens bf16 with the norm, parts of q|k|v rows, 12.5 us, 3.4 TB/s.  By the launch and one chain
-// of loads, angles (f64) and stores where there is little: one token 3.1 us, 777 of 24 heads of 64 3.4.
+// Bound by memory where there is much to do: 16384 tokens of 32 and 8 heads of 128, f32, 126 us, 5.3 TB/s (a copy of 1 GiB reaches 5.2; part of
+// this fits the last-level cache); 2051 tokens bf16 with the norm, parts of q|k|v rows, 12.0 us, 3.5 TB/s.  By the launch and one chain
+// of loads, angles (f64) and stores where there is little: one token 3.2 us, 777 of 24 heads of 64 4.3.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -100,8 +100,9 @@ __global__ __launch_bounds__(256) void rope_any_kernel(RopeParams P) {
 
 // The same in pieces of 16 bytes: a lane has two pieces of a head, those whose elements turn against each other (halves) or two neighbours
 // (interleaved, and what does not turn), LP lanes a head, 64 / LP heads at once; a wave has `passes` such sets of one token's heads, requests
-// kAtOnce of them ahead of working out the angles, and every angle once.  (Pairs of single elements, a workgroup a token: 2051 tokens 32 us
-// instead of 12.5.)
+// kAtOnce of them ahead of working out the angles, and every angle once (a token whose heads go to several waves has its angles worked out
+// by each).  (Pairs of single elements, a workgroup a token: 2051 tokens 32 us instead of 12.)  Reading the angles back has two lanes on a
+// bank (a lane's are 64 bytes on from its neighbour's): 44 % of the LDS's cycles in use, which are 4 % of a busy compute unit's.
 constexpr int kAtOnce = 4, kPiecePairs = 256;
 
 template <typename T, int V>
