@@ -266,8 +266,7 @@ int izwi_rope_positions_bf16(const uint16_t* q, int64_t q_stride, const uint16_t
  * (total_k at most), only decides how the work is shared out.
  * What a query does not see has no influence, whatever it holds.  A NaN that it sees in q or a key makes its row NaN, one in a
  * value that element; an infinity in a value makes the element that infinity, or in f32 NaN.  A score that f32 does not hold, (q . k) * scale *
- * log2(e) beyond 2^128, makes its row NaN.  (Weights stand up to 2^8 above 1 until they are divided by their sum: values above 2^120 over
- * the number of keys may leave f32 on their way to the mean.)
+ * log2(e) beyond 2^128, makes its row NaN.  Values may be as large as the type holds: their mean is right where their sum leaves f32.
  * The products run on the matrix cores with f32 sums: f16 and bf16 values as they are, weights as two numbers of the type (f16 2^-22,
  * bf16 2^-16 of each); f32 ones as three bf16 numbers each, all 24 bits down to 2^-100.  head_dim 64, 128 or 256; rows begin on 16 bytes; out
  * shares no memory with the inputs.  Uses the library's per-stream scratch where workgroups have parts of a row's

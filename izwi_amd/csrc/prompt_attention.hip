@@ -361,6 +361,9 @@ __global__ __launch_bounds__(64 * WR * WZ * DZ, Elem<T>::N == 1 || D == 64 ? 2 :
 #pragma unroll
         for (int r = 0; r < 16; r++) o[d][r] = 0.0f;
     float ref = -INFINITY, sum[2] = {}; // ref: base 2; sum: of this lane's positions, in two parts
+    constexpr bool kWide = E::kLift == 0; // values may be as large as f32 is
+    constexpr float kShrink = kWide ? 0x1p-32f : 1.0f;
+    [[maybe_unused]] float shrink = 1.0f; // of all weights, in the second pass (below)
     if (threadIdx.x == 0) *odd_values = 0;
 
     // Scores, weights and the weighted values of a tile that has landed.  MASKED: some row of the workgroup does not see all of its
@@ -461,6 +464,7 @@ __global__ __launch_bounds__(64 * WR * WZ * DZ, Elem<T>::N == 1 || D == 64 ? 2 :
                 float e = __builtin_fmaf(p[pt][r], P.scale, -from);
                 if constexpr (N == 3) e = p[pt][r] == -INFINITY ? e : __builtin_fmaf(p[pt][r], P.scale_rest, e); // (the rest may be negative)
                 p[pt][r] = __builtin_amdgcn_exp2f(e);
+                if constexpr (MASKED && kWide) p[pt][r] *= shrink;
                 sum[r & 1] += p[pt][r];
             }
 
@@ -526,7 +530,8 @@ __global__ __launch_bounds__(64 * WR * WZ * DZ, Elem<T>::N == 1 || D == 64 ? 2 :
     // A value that is no number must not reach the rows that do not see it, and a weight of zero would not keep it out; nor would what is left of a
     // weight, zero or below it, leave an infinity that a row does see what it is.  Results that hold one are worked out once more, with
     // care: the tile goes on with a zero in its place, and the rows that see such a value remember it, a bit for each of the lane's elements: up
-    // is an infinity, down a negative one, both NaN (f32: any).  (A look at the values of every tile that some row does not see all of took
+    // is an infinity, down a negative one, both NaN (f32: any).  And as finite values may have left f32 on their way, all weights are 2^-32 of what
+    // they were then: exact, but for those below 2^-94 of the reference.  (A look at the values of every tile that some row does not see all of took
     // 1200 of the 11600 cycles of 37 bf16 tokens.)
     uint64_t up = 0, down = 0;
     static_assert(DT * 16 <= 64);
@@ -592,7 +597,7 @@ __global__ __launch_bounds__(64 * WR * WZ * DZ, Elem<T>::N == 1 || D == 64 ? 2 :
         if (__any(zero != 0.0f) && lane == 0) *odd_values = 1;
         __syncthreads();
         if (*odd_values == 0) break;
-        care = true;
+        care = true, shrink = kShrink;
         if (first < end) request(first, 0);
 #pragma unroll
         for (int d = 0; d < DT; d++)
@@ -651,8 +656,11 @@ __global__ __launch_bounds__(64 * WR * WZ * DZ, Elem<T>::N == 1 || D == 64 ? 2 :
     const float total = qmm_add_lane32(sum[0]);
     const int64_t out_row = (s.q0 + token) * P.heads + head;
     if constexpr (SPLIT) {
-        // (a sum below zero: the split has no position that the row sees)
-        if (h == 0 && dz == 0) P.stats[out_row * P.splits + split] = float2{ref, first < end && limit >= first * KS ? total : -1.0f};
+        // (a sum below zero: the split has no position that the row sees; sums divided by it: their mean is no larger than the values are)
+        if (h == 0 && dz == 0) P.stats[out_row * P.splits + split] = float2{ref, first < end && limit >= first * KS ? total / shrink : -1.0f};
+        const float mean = total == 0.0f ? 1.0f : 1.0f / total;
+#pragma unroll
+        for (int d = 0; d < DT; d++) o[d] *= mean;
         float* to = P.sums + (out_row * P.splits + split) * D + dz * DW + 4 * h;
 #pragma unroll
         for (int d = 0; d < DT; d++)
@@ -709,7 +717,7 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(PromptParams P, int64_
         }
         if (!inside) return; // (the same in the whole workgroup)
     }
-    // (a reference of -infinity: no score is above it, the sums are zero or no number; a sum below zero: no position that the row sees)
+    // (a reference of -infinity: no score is above it, the sum is zero or no number; a sum below zero: no position that the row sees)
     vec v[A], a = 0.0f;
     float2 st[A];
     const auto take = [&](int i0) {
@@ -721,11 +729,15 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(PromptParams P, int64_
         }
     };
     take(mine);
-    float ref = -INFINITY, sum = 0.0f;
+    float ref = -INFINITY, sum = 0.0f; // of all parts
     bool any = false;
+    const auto weight = [&](float2 one) { return one.y * (one.x == -INFINITY ? 1.0f : rescale(one.x - ref)); };
     if constexpr (FEW) {
 #pragma unroll
         for (int j = 0; j < A; j++) ref = fmaxf(ref, st[j].y < 0.0f ? -INFINITY : st[j].x);
+#pragma unroll
+        for (int j = 0; j < A; j++)
+            if (j < P.splits && !(st[j].y < 0.0f)) any = true, sum += weight(st[j]);
     } else {
         for (int i = lane; i < P.splits; i += 64) {
             const float2 one = stats[i];
@@ -736,40 +748,33 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(PromptParams P, int64_
         ref = fmaxf(ref, dpp_f<0x124>(ref));
         ref = fmaxf(ref, dpp_f<0x4E>(ref));
         ref = fmaxf(ref, dpp_f<0xB1>(ref));
+        for (int i = lane; i < P.splits; i += 64) {
+            const float2 one = stats[i];
+            if (!(one.y < 0.0f)) any = true, sum += weight(one);
+        }
+        any = __any(any), sum = wave_sum(sum);
     }
     for (int i0 = mine; i0 < P.splits;) {
 #pragma unroll
-        for (int j = 0; j < A; j++) {
-            const bool there = i0 + j * step < P.splits && !(st[j].y < 0.0f);
-            const float by = st[j].x == -INFINITY ? 1.0f : rescale(st[j].x - ref);
-            any |= there;
-            sum += there ? st[j].y * by : 0.0f;
-            a += there ? rescaled(v[j], by) : vec(0.0f);
-        }
+        for (int j = 0; j < A; j++)
+            if (i0 + j * step < P.splits && !(st[j].y < 0.0f)) a += rescaled(v[j], weight(st[j]) / sum);
         i0 += A * step;
         if (i0 < P.splits) take(i0);
     }
     T* const to = static_cast<T*>(P.out) + token * P.out_stride + (row % P.heads) * D + at * E;
     if constexpr (FEW) {
 #pragma unroll
-        for (int e = 0; e < E; e++) to[e] = (T)(any ? a[e] / sum : 0.0f);
+        for (int e = 0; e < E; e++) to[e] = (T)(any ? a[e] : 0.0f);
     } else {
         __shared__ vec part[kPer][D / 4];
-        __shared__ float part_sum[kPer]; // below zero: nothing
         part[mine][at] = a;
-        if (at == 0) part_sum[mine] = any ? sum : -1.0f;
         __syncthreads();
         if (threadIdx.x >= D / 4) return;
-        any = false, sum = 0.0f, a = 0.0f;
+        a = 0.0f;
 #pragma unroll
-        for (int i = 0; i < kPer; i++) {
-            const float s = part_sum[i];
-            any |= !(s < 0.0f);
-            sum += s < 0.0f ? 0.0f : s;
-            a += part[i][at];
-        }
+        for (int i = 0; i < kPer; i++) a += part[i][at];
 #pragma unroll
-        for (int e = 0; e < E; e++) to[e] = (T)(any ? a[e] / sum : 0.0f);
+        for (int e = 0; e < E; e++) to[e] = (T)(any ? a[e] : 0.0f);
     }
 }
 

@@ -59,3 +59,26 @@ def test_infinities_under_no_weight(qa, dtype, d, n, keys, heads, kv, bad):
     assert (torch.isnan(got[..., 7]) if bad != bad else got[..., 7] == bad).all() and torch.isnan(got[..., 9]).all()
     rest = [i for i in range(d) if i not in (7, 9)]
     assert torch.equal(got[..., rest], want[..., rest])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("n,keys,heads,kv", CASES + [(9, 8400, 16, 8)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_means_of_the_largest_values(qa, dtype, d, n, keys, heads, kv, causal):
+    """Values near the largest number of the type, whose weighted sums leave it and whose mean does not, in one element of every sixteen; the others are
+    what they are beside ordinary values, to the bit (weights are scaled by a power of two)."""
+    q, k, v = (torch.randn(rows, g, d, device="cuda").to(dtype) for rows, g in ((n, heads), (keys, kv), (keys, kv)))
+    v[..., 3::16] = 1.0
+    want = qa.prompt_attention(q, k, v, causal=causal)
+    v[..., 3::16] = 3e38
+    got = qa.prompt_attention(q, k, v, causal=causal)
+    big = torch.arange(d, device="cuda") % 16 == 3
+    sees = torch.ones(n, dtype=torch.bool, device="cuda")
+    if causal and n > keys:
+        sees[:n - keys] = False
+    # a mean of equal values: what its products leave out (2^-22, bf16 weights 2^-16) and the sums of 17 and more terms at once, of f32 6 of each, 2^-24 an addition
+    tol = (6 * keys / 16 + 64) * 2.0 ** -24 + 2.0 ** -22 + (2.0 ** -16 + 2.0 ** -8 if dtype == torch.bfloat16 else 0)
+    off = (got[sees][..., big].double() / v[0, 0, 3].double() - 1).abs().max()
+    assert off <= tol, float(off)
+    assert torch.equal(got[..., ~big], want[..., ~big])
