@@ -352,7 +352,8 @@ inline void beam_select(const float* logits, int64_t prompts, int64_t beams, int
                                       lineage, lineage_capacity, lens, lineage_out, stream));
 }
 
-// Whole prompts, packed one behind the other (izwi_decode_ops.h), device pointers.  Frequencies (rotary_dim / 2 of them, on the host) of a model's
+// Whole prompts, packed one behind the other (izwi_decode_ops.h), device pointers; f32, as all of this mirror's activations are (the C entry points take
+// f16 and bf16, too).  Frequencies (rotary_dim / 2 of them, on the host) of a model's
 // rotary positions; `scaling` is one of IZWI_ROPE_*.  Returns the factor on cosine and sine.
 inline double rope_frequencies(int scaling, int64_t rotary_dim, double base, double factor, double original_len, double low, double high,
                                std::vector<double>& frequencies) {
